@@ -259,6 +259,72 @@ int tc_probe_mma_fp8(const uint8_t *a, const uint8_t *b, int64_t M, int64_t N, i
 int tc_probe_mma_fp4(const uint8_t *a, const uint8_t *b, const uint8_t *sfa, const uint8_t *sfb, int64_t M, int64_t N,
                      int64_t K, int32_t scale_fmt, float *out, int32_t *status, tc_stream stream);
 
+/* ---- Serving operators: entry points without a TriCast counterpart ---- */
+
+/* Root-mean-square norm with the residual's addition and an 8-bit output with scales: h = x + residual
+ * (x where residual is NULL), y = h / sqrt(mean(h^2) + eps) * weight (no product where weight is NULL),
+ * codes and scales as tc_quantize gives them for y in fp32. x and residual: [rows][K] of dtype with row
+ * strides in elements. codes: [rows][K] bytes. scale: per row or per group of the row ([rows][groups]),
+ * fp32, or one E8M0 byte each where the spec's scale format is E8M0. residual_out: NULL, or h [rows][K]
+ * in dtype. spec: fp8_e4m3, fp8_e5m2 or int8 elements rounded to nearest even and saturating; row or group
+ * granularity; fp32 absmax or E8M0 pow2_floor scales; anything else is TC_UNSUPPORTED. Only
+ * residual_out may alias x or residual, and only in whole. */
+int tc_rms_norm_quantize(const void *x, const void *residual, int32_t dtype, int64_t rows, int64_t K,
+                         int64_t x_stride, int64_t residual_stride, const void *weight, int32_t weight_dtype, float eps,
+                         const tc_quant_spec *spec, void *codes, void *scale, void *residual_out, tc_stream stream);
+
+/* How a paged cache holds a key or value row (one token, one head): as it is; E4M3 or INT8 codes with one
+ * fp32 absmax scale (the fp8_row / int8_row schemes of a [rows][head_dim] tensor); E2M1 codes, two a byte
+ * (low nibble first), with one E8M0 scale byte per 32 elements (mxfp4). */
+typedef enum tc_kv_scheme { TC_KV_NONE = 0, TC_KV_FP8_ROW = 1, TC_KV_INT8_ROW = 2, TC_KV_MXFP4 = 3 } tc_kv_scheme;
+
+/* A paged key / value cache the caller owns: k and v hold [num_pages][kv_heads][page_size] rows of codes,
+ * k_scale and v_scale the rows' scales in the same order (NULL for TC_KV_NONE). dtype is that of the keys,
+ * values and queries outside the cache. page_size: a power of two in [8, 256]; head_dim: a multiple of 16
+ * (TC_KV_MXFP4: 32) in [16, 256]. Slot s is token s % page_size of page s / page_size. */
+typedef struct tc_kv_cache {
+  void *k;
+  void *v;
+  void *k_scale;
+  void *v_scale;
+  int32_t scheme;
+  int32_t dtype;
+  int64_t num_pages;
+  int32_t page_size;
+  int32_t kv_heads;
+  int32_t head_dim;
+} tc_kv_cache;
+
+/* Quantize the keys and values of `tokens` tokens ([tokens][kv_heads][head_dim] with token and head
+ * strides in elements, head_dim contiguous) into their slots. Slots outside the cache (-1) are skipped;
+ * of two tokens with one slot, either may stay. */
+int tc_kv_write(const tc_kv_cache *cache, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
+                int64_t v_token_stride, int64_t v_head_stride, const int64_t *slots, int64_t tokens, tc_stream stream);
+
+/* Dequantize the tokens at `slots` into k and v, [tokens][kv_heads][head_dim] of the cache's dtype: code *
+ * scale in fp32, rounded once. Slots outside the cache read as zeros. */
+int tc_kv_read(const tc_kv_cache *cache, const int64_t *slots, int64_t tokens, void *k, void *v, tc_stream stream);
+
+/* Bytes of scratch tc_paged_attention needs for these sizes (0 when none). */
+size_t tc_paged_attention_workspace(const tc_kv_cache *cache, int32_t q_heads, int64_t total_q, int32_t batch,
+                                    int32_t max_q_len);
+
+/* out = softmax(scale * q k^T) v over each sequence's cached keys and values, for the last tokens of the
+ * sequence: q and out [total_q][q_heads][head_dim] of the cache's dtype (q with token and head strides in
+ * elements, out contiguous), query head h reading key / value head h / (q_heads / kv_heads). cu_q
+ * [batch + 1]: sequence b's new tokens are cu_q[b] .. cu_q[b + 1] - 1, at most max_q_len of them; NULL:
+ * one each. seq_lens [batch]: its context, the new tokens (already written) included; token i of n sits
+ * at position seq_lens[b] - n + i. block_table [batch][max_pages] (row stride table_stride): the page of
+ * each page_size positions; keys on a page outside the cache count as absent. causal: a token sees itself
+ * and earlier positions, the last `window` of them where window > 0; otherwise the whole context. Scores,
+ * softmax and sums are fp32. A row that sees no key gives zeros, and -Inf in lse (NULL, or the fp32
+ * [total_q][q_heads] natural logarithms of the softmax sums). */
+int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64_t q_token_stride, int64_t q_head_stride,
+                       int64_t total_q, int32_t q_heads, const int32_t *block_table, int64_t table_stride,
+                       int32_t max_pages, const int32_t *seq_lens, const int32_t *cu_q, int32_t batch, int32_t max_q_len,
+                       float scale, int32_t causal, int32_t window, void *out, float *lse, void *workspace,
+                       size_t workspace_bytes, tc_stream stream);
+
 /* Library version string. */
 const char *tc_version(void);
 

@@ -6,6 +6,7 @@ cannot be loaded the import fails; there is no CPU fallback.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import threading
 from pathlib import Path
@@ -23,6 +24,7 @@ METHOD_CODES = {"absmax": 0, "pow2_floor": 1, "pow2_ceil": 2, "mse": 3, "percent
 ZERO_POINT_CODES = {"none": 0, "int": 1, "float": 2}
 ALGORITHM_CODES = {"cofda": 0, "gdfs": 1, "fp32_fma": 2, "fp64": 3, "int_exact": 4}
 APPLY_CODES = {"epilogue": 0, "product": 1, "group": 2, "promote": 3, "operand": 4}
+KV_SCHEME_CODES = {None: 0, "fp8_row": 1, "int8_row": 2, "mxfp4": 3}
 SCALE_KIND_CODES = {"none": 0, "tensor": 1, "row": 2, "k": 3}
 
 
@@ -60,6 +62,12 @@ class TcMmaSpec(C.Structure):
                 ("out_format", TcFormat), ("out_dtype", C.c_int32)]
 
 
+class TcKvCache(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("scheme", C.c_int32), ("dtype", C.c_int32), ("num_pages", C.c_int64), ("page_size", C.c_int32),
+                ("kv_heads", C.c_int32), ("head_dim", C.c_int32)]
+
+
 EXPORTS = {
     "tc_cast": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.POINTER(TcFormat), C.c_int32, C.c_int32,
                           C.c_int32, C.c_void_p]),
@@ -78,6 +86,17 @@ EXPORTS = {
                                   C.c_void_p, C.c_void_p]),
     "tc_any_nonfinite": (C.c_int, [C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p]),
     "tc_error_stats": (C.c_int, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_void_p]),
+    "tc_rms_norm_quantize": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int64, C.c_int64, C.c_int64,
+                                       C.c_void_p, C.c_int32, C.c_float, C.POINTER(TcQuantSpec), C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_void_p]),
+    "tc_kv_write": (C.c_int, [C.POINTER(TcKvCache), C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64,
+                              C.c_void_p, C.c_int64, C.c_void_p]),
+    "tc_kv_read": (C.c_int, [C.POINTER(TcKvCache), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "tc_paged_attention_workspace": (C.c_size_t, [C.POINTER(TcKvCache), C.c_int32, C.c_int64, C.c_int32, C.c_int32]),
+    "tc_paged_attention": (C.c_int, [C.POINTER(TcKvCache), C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int32,
+                                     C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                     C.c_float, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,
+                                     C.c_void_p]),
     "tc_last_error": (C.c_char_p, []),
     "tc_version": (C.c_char_p, []),
     "tc_launch_count": (C.c_uint64, []),
@@ -92,6 +111,7 @@ EXPORTS = {
                                    C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p]),
 }
 
+_NOTHING = contextlib.nullcontext()
 _lib = None
 _lock = threading.Lock()
 
@@ -162,8 +182,15 @@ def stream_of(device) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def on_device(device):
+    """A context in which ``device`` is current; nothing to enter where it already is."""
+    import torch
+
+    return _NOTHING if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
 def ptr(t) -> C.c_void_p:
     return C.c_void_p(0 if t is None else t.data_ptr())
 
 
-__all__ = ["lib", "check", "tc_format", "rounding_code", "dtype_code", "stream_of", "ptr"]
+__all__ = ["lib", "check", "tc_format", "rounding_code", "dtype_code", "stream_of", "on_device", "ptr"]

@@ -1,0 +1,75 @@
+"""Attention of a chunk of new tokens (a prefill chunk, drafted tokens or a decode step) over a
+:class:`PagedKVCache`, reading its codes."""
+
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _native as N
+
+
+def _index(t: torch.Tensor, shape, device, name: str) -> None:
+    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape:
+        raise ValueError(f"{name} must be an int32 tensor of shape {list(shape)} on the cache's device")
+
+
+def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens: torch.Tensor,
+                    cu_q: torch.Tensor | None = None, *, max_q_len: int | None = None, scale: float | None = None,
+                    causal: bool = True, window: int = 0, return_lse: bool = False):
+    """``softmax(scale * q k^T) v`` of each sequence's last tokens over its cached keys and values.
+
+    ``q`` ``[total_q, heads, head_dim]`` of the cache's dtype (any strides with contiguous elements), query head
+    ``h`` reading key / value head ``h // (heads // kv_heads)``. ``cu_q`` (int32 ``[batch + 1]``): sequence ``b``'s
+    new tokens are ``q[cu_q[b]:cu_q[b + 1]]``, at most ``max_q_len`` of them (default: ``total_q``); without it
+    every sequence has one. ``seq_lens`` (int32 ``[batch]``): the sequence's context, the new tokens, written
+    before this call, included. ``block_table`` (int32 ``[batch, max_pages]``): the page of each ``page_size``
+    positions; entries past the context are not read, and keys on a page outside the cache (``-1``) count as
+    absent. ``causal``: a token sees itself and what precedes it, the last ``window`` positions of that where
+    ``window > 0``. ``scale`` defaults to ``1 / sqrt(head_dim)``.
+
+    Returns ``[total_q, heads, head_dim]`` in the cache's dtype, and with ``return_lse`` the fp32 natural
+    logarithms of the softmax sums ``[total_q, heads]``. A token that sees no key gives zeros and ``-inf``."""
+    device = cache.device
+    if q.ndim != 3 or q.shape[2] != cache.head_dim or q.dtype != cache.dtype or q.device != device:
+        raise ValueError(f"q must be [tokens, heads, {cache.head_dim}] of {cache.dtype} on the cache's device")
+    total, heads, dim = q.shape
+    if heads == 0 or heads % cache.kv_heads:
+        raise ValueError("the number of query heads must be a multiple of the cache's")
+    if block_table.ndim != 2 or block_table.dtype != torch.int32 or block_table.device != device:
+        raise ValueError("block_table must be an int32 tensor [batch, max_pages] on the cache's device")
+    batch, max_pages = block_table.shape
+    _index(seq_lens, (batch,), device, "seq_lens")
+    if cu_q is not None:
+        _index(cu_q, (batch + 1,), device, "cu_q")
+        cu_q = cu_q.contiguous()
+    elif total != batch:
+        raise ValueError("without cu_q every sequence has one new token: q needs as many tokens as block_table rows")
+    if window < 0 or (window and not causal):
+        raise ValueError("window must be positive and needs causal=True")
+    if max_q_len is None:
+        max_q_len = max(total, 1)
+    elif max_q_len < 1:
+        raise ValueError("max_q_len must be positive")
+    if q.stride(2) != 1:
+        q = q.contiguous()
+    if max_pages and block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    seq_lens = seq_lens.contiguous()
+    out = torch.empty((total, heads, dim), dtype=q.dtype, device=device)
+    lse = torch.empty((total, heads), dtype=torch.float32, device=device) if return_lse else None
+    lib = N.lib()
+    with N.on_device(device):
+        nbytes = lib.tc_paged_attention_workspace(cache._ref, heads, total, batch, max_q_len)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        N.check(lib.tc_paged_attention(
+            cache._ref, q.data_ptr(), q.stride(0), q.stride(1), total, heads, block_table.data_ptr(),
+            block_table.stride(0), max_pages, seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch,
+            max_q_len, 1.0 / math.sqrt(dim) if scale is None else scale, causal, window, out.data_ptr(),
+            None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
+            N.stream_of(device)), "tc_paged_attention")
+    return (out, lse) if return_lse else out
+
+
+__all__ = ["paged_attention"]

@@ -51,6 +51,8 @@ class Operand:
 
 def expand_scale(t: torch.Tensor, spec, rows: int, K: int) -> torch.Tensor:
     """One scale (or zero point) per element, from the domain layout of ``spec``."""
+    if t.dtype == torch.float8_e8m0fnu:
+        t = t.float()
     if spec.granularity in ("tensor", "row"):
         return t.expand(rows, K)
     if spec.granularity == "group":
@@ -110,7 +112,7 @@ class QTensor:
             return Operand(values, spec.dequant_format)
         if self.scale is None:
             return Operand(self.values.float(), spec.format)
-        scale, kind, width = self.scale, spec.granularity, 0
+        scale, kind, width = self.scale.to(torch.float32), spec.granularity, 0
         if kind == "group":
             kind, width = "k", spec.group_size
         elif kind == "block":
