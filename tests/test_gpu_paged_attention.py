@@ -1,9 +1,10 @@
 """Attention over the quantized paged cache against the formula in 64 bits on the cache's own values.
 
-Tolerance, by the arithmetic: weights may be rounded to bf16 before their product with the values (2**-9 of
-each weight), the result is rounded to its type (at most 2**-9 of it), and fp32 scores, exponentials and sums
-add less than 1e-4: |error| <= (2**-8 + 1e-4) * sum_j p_j |v_j| for 16-bit types. In fp32 nothing is rounded
-below 32 bits: scores of magnitude up to 100 carry 1e-5, so 4e-5 * sum_j p_j |v_j|."""
+Tolerance, by the arithmetic (``_bound``, in units of sum_j p_j |v_j|): a weight is rounded once to the 16-bit
+type of its product with the values (fp16 over quantized caches, the cache's own type otherwise) and the
+result once to its type; rounding to nearest is off by at most 2**-8 of a bf16 value (8 significant bits) and
+2**-11 of an fp16 value. fp32 scores, exponentials and sums add less than 1e-4. In fp32 nothing is rounded below
+32 bits: scores of magnitude up to 100 carry 1e-5, so 4e-5."""
 
 from __future__ import annotations
 
@@ -18,6 +19,15 @@ from tricast_b200 import PagedKVCache, paged_attention
 pytestmark = pytest.mark.gpu
 
 SCHEMES = [None, "fp8_row", "int8_row", "mxfp4"]
+
+
+UNIT = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+
+
+def _bound(dtype, scheme):
+    if dtype == torch.float32:
+        return 4e-5
+    return UNIT[dtype if scheme is None else torch.float16] + UNIT[dtype] + 1e-4
 
 
 class Batch:
@@ -96,7 +106,7 @@ class Batch:
     def check(self, **kw):
         out, lse = self.run(return_lse=True, **kw)
         want, size, want_lse = self.exact(**kw)
-        tol = 4e-5 if self.q.dtype == torch.float32 else 2.0 ** -8 + 1e-4
+        tol = _bound(self.q.dtype, self.cache.scheme)
         assert out.dtype == self.q.dtype and out.shape == self.q.shape
         assert torch.isfinite(out).all()
         assert ((out.double() - want).abs() <= tol * size + 1e-30).all(), ((out.double() - want).abs() / (size + 1e-30)).max()
@@ -173,7 +183,7 @@ def test_large_and_extreme_scores(scheme):
         want, size, lse = b.exact(scale=20.0)
         # A score of magnitude s carries s * 64 * 2**-24 of error into its weight.
         top = lse.abs().max().item()
-        tol = 2.0 ** -8 + 1e-4 + 4 * top * 64 * 2.0 ** -24
+        tol = _bound(torch.bfloat16, scheme) + 4 * top * 64 * 2.0 ** -24
         assert torch.isfinite(out).all()
         assert ((out.double() - want).abs() <= tol * (size + b.v[0].abs().max())).all()
 
@@ -193,7 +203,7 @@ def test_absent_pages_count_as_masked(scheme):
         got, _ = b.run(return_lse=True, causal=False)
         b.k[0], b.v[0], b.total[0] = b.k[0][gone], b.v[0][gone], int(gone.sum())
         want, size, _ = b.exact(causal=False)
-        assert ((got.double() - want).abs() <= (2.0 ** -8 + 1e-4) * size).all()
+        assert ((got.double() - want).abs() <= _bound(torch.bfloat16, scheme) * size).all()
         assert not torch.equal(got, out)
 
 
@@ -244,7 +254,7 @@ def test_a_call_without_cu_q_and_in_a_graph():
     b.total = b.lens.tolist()
     b.k, b.v = [k[:t] for k, t in zip(b.k, b.total)], [v[:t] for v, t in zip(b.v, b.total)]
     exact, size, _ = b.exact()
-    assert ((out.double() - exact).abs() <= (2.0 ** -8 + 1e-4) * size).all()
+    assert ((out.double() - exact).abs() <= _bound(torch.bfloat16, "fp8_row") * size).all()
 
 
 def test_pool_offsets_beyond_32_bits():

@@ -89,12 +89,38 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(Args a) {
   }
 }
 
+int launch_split_none(const Args &a, float *parts, int most, cudaStream_t s);
+int launch_split_fp8(const Args &a, float *parts, int most, cudaStream_t s);
+int launch_split_int8(const Args &a, float *parts, int most, cudaStream_t s);
+int launch_split_mxfp4(const Args &a, float *parts, int most, cudaStream_t s);
+
+// Blocks of the split kernel: as many as run at once.
+static int split_blocks(const KvCache &c) {
+  return sm_count() * (c.scheme == KV_NONE && split_width(c.dim) == 256 ? 1 : 2);
+}
+
+static int launch_split(const Args &a, float *parts, cudaStream_t s) {
+  const int most = split_blocks(a.c);
+  const int st = a.c.scheme == KV_NONE       ? launch_split_none(a, parts, most, s)
+                 : a.c.scheme == KV_FP8_ROW  ? launch_split_fp8(a, parts, most, s)
+                 : a.c.scheme == KV_INT8_ROW ? launch_split_int8(a, parts, most, s)
+                                             : launch_split_mxfp4(a, parts, most, s);
+  if (st != TC_OK) return st;
+  if (a.c.dtype == TC_BF16) join_kernel<__nv_bfloat16, 16, 64><<<most - 1, 256, 0, s>>>(a, parts, split_width(a.c.dim), most);
+  else join_kernel<__half, 16, 64><<<most - 1, 256, 0, s>>>(a, parts, split_width(a.c.dim), most);
+  count_launch();
+  return TC_OK;
+}
+
 }  // namespace attn
 }  // namespace tc
 
 extern "C" size_t tc_paged_attention_workspace(const tc_kv_cache *cache, int32_t q_heads, int64_t total_q, int32_t batch,
                                                int32_t max_q_len) {
-  return 0;
+  using namespace tc;
+  KvCache c;
+  if (kv_cache_check(cache, c) != TC_OK || c.dtype == TC_F32) return 0;
+  return 2 * (size_t)attn::split_blocks(c) * attn::partial_floats(16, attn::split_width(c.dim)) * sizeof(float);
 }
 
 extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64_t q_token_stride, int64_t q_head_stride,
@@ -114,7 +140,8 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
   if (q_heads < 1 || q_heads % cache->kv_heads) return bad("query heads must be a multiple of the cache's");
   if (!std::isfinite(scale)) return bad("scale must be finite");
   if (window < 0 || (window && !causal)) return bad("a window must be positive and needs causal");
-  if (((int64_t)max_pages << a.c.page_shift) > 0x7FFFFFFFll) return bad("contexts are limited to 2**31 - 1 tokens");
+  if (((int64_t)max_pages << a.c.page_shift) > (1ll << 30)) return bad("contexts are limited to 2**30 tokens");
+  if (total_q * q_heads > 0x7FFFFFFFll) return bad("queries are limited to 2**31 - 1 rows");
   a.q = q;
   a.q_tok = q_token_stride;
   a.q_head = q_head_stride;
@@ -134,12 +161,16 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
   a.out = out;
   a.lse = lse;
   cudaStream_t s = (cudaStream_t)stream;
-  const int64_t want = (total_q * q_heads + 7) / 8, most = (int64_t)sm_count() * 8;
-  const unsigned grid = (unsigned)(want < most ? want : most);
-  if (a.c.dtype == TC_F32) attn::plain_kernel<float><<<grid, attn::kThreads, 0, s>>>(a);
-  else if (a.c.dtype == TC_BF16) attn::plain_kernel<__nv_bfloat16><<<grid, attn::kThreads, 0, s>>>(a);
-  else attn::plain_kernel<__half><<<grid, attn::kThreads, 0, s>>>(a);
-  count_launch();
+  if (a.c.dtype == TC_F32) {
+    const int64_t want = (total_q * q_heads + 7) / 8, most = (int64_t)sm_count() * 8;
+    attn::plain_kernel<float><<<(unsigned)(want < most ? want : most), attn::kThreads, 0, s>>>(a);
+    count_launch();
+  } else {
+    if (!workspace || workspace_bytes < tc_paged_attention_workspace(cache, q_heads, total_q, batch, max_q_len))
+      return set_error("tc_paged_attention: workspace too small"), TC_WORKSPACE_TOO_SMALL;
+    const int r = attn::launch_split(a, static_cast<float *>(workspace), s);
+    if (r != TC_OK) return r;
+  }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
   return TC_OK;

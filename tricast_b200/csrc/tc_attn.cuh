@@ -1,6 +1,7 @@
 // Attention of new tokens over a paged cache: the call's arguments and what the kernels share.
 #pragma once
 
+#include "tc_mma16.cuh"
 #include "tc_serve.cuh"
 
 namespace tc {
@@ -48,6 +49,229 @@ __device__ __forceinline__ void visible(const Args &a, const Seq &s, int i, int 
   hi = a.causal ? max(at + 1, 0) : s.len;
   lo = a.window > 0 ? max(at + 1 - a.window, 0) : 0;
 }
+
+// ---------------------------------------------------------------- work split
+// The tensor-core kernels cut the call into items, one per (sequence, key / value head, tile of kRows query
+// rows), and an item into units of kKeys keys. A query row is a (new token, head of the group) pair, tokens
+// outermost, so the heads that share keys share their reads. All units form one line, sequences outermost,
+// then heads, then row tiles; each of the blocks that run takes an equal stretch of it, whatever the lengths.
+// An item that lies inside one block's stretch is finished there. The others leave partial results (the
+// running maximum and sum of each row and its unnormalised output, fp32), at most two a block: slot
+// 2 c for the stretch's first item when it began before the stretch, 2 c + 1 for its last when it goes
+// on after it; the join kernel merges them in block order, so results do not depend on timing.
+struct Item {
+  int b, head, tile;  // sequence, key / value head, row tile
+  int units;          // of the item, at least 1 (an item without keys still writes its rows)
+  int at, n;          // the stretch's part: units [at, at + n)
+  int64_t left;       // units of the stretch after this part
+};
+
+template <int kRows, int kKeys>
+struct Work {
+  // Keys [lo, hi) that any row of the tile sees, lo rounded down to a whole unit.
+  static __device__ __forceinline__ void keys(const Args &a, const Seq &s, int tile, int &lo, int &hi) {
+    const int first = tile * kRows / a.group;
+    const int last = min((tile + 1) * kRows - 1, s.n * a.group - 1) / a.group;
+    int unused;
+    visible(a, s, first, lo, unused);
+    visible(a, s, last, unused, hi);
+    lo = min(lo, hi) / kKeys * kKeys;
+  }
+  static __device__ __forceinline__ int tiles(const Args &a, const Seq &s) {
+    return (int)(((int64_t)s.n * a.group + kRows - 1) / kRows);
+  }
+  static __device__ __forceinline__ int units(const Args &a, const Seq &s, int tile) {
+    int lo, hi;
+    keys(a, s, tile, lo, hi);
+    return max((hi - lo + kKeys - 1) / kKeys, 1);
+  }
+  // Units of one head of a sequence, by a whole warp; every lane gets the sum.
+  static __device__ __forceinline__ int64_t head_units(const Args &a, const Seq &s) {
+    const int n = tiles(a, s);
+    int64_t sum = 0;
+    for (int t = threadIdx.x & 31; t < n; t += 32) sum += units(a, s, t);
+    for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, m);
+    return sum;
+  }
+  // Calls visit(b, units of one head) for every sequence in order, by a whole warp, until it returns false.
+  template <typename F>
+  static __device__ __forceinline__ void scan(const Args &a, F visit) {
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      Seq s{0, 0, 0};
+      int one = 0;
+      if (b0 + lane < a.batch) {
+        s = sequence(a, b0 + lane);
+        const int n = tiles(a, s);
+        one = n == 0 ? 0 : n == 1 ? units(a, s, 0) : -1;
+      }
+      for (int i = 0; i < 32 && b0 + i < a.batch; ++i) {
+        int64_t u = __shfl_sync(0xFFFFFFFFu, one, i);
+        if (u < 0) {
+          Seq t;
+          t.q0 = __shfl_sync(0xFFFFFFFFu, s.q0, i);
+          t.n = __shfl_sync(0xFFFFFFFFu, s.n, i);
+          t.len = __shfl_sync(0xFFFFFFFFu, s.len, i);
+          u = head_units(a, t);
+        }
+        if (!visit(b0 + i, u)) return;
+      }
+    }
+  }
+  // Units of the whole call, by a whole warp.
+  static __device__ __forceinline__ int64_t total(const Args &a) {
+    int64_t sum = 0;
+    const int lane = threadIdx.x & 31;
+    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+      Seq s{0, 0, 0};
+      int n = 0;
+      if (b0 + lane < a.batch) {
+        s = sequence(a, b0 + lane);
+        n = tiles(a, s);
+      }
+      if (n == 1) sum += units(a, s, 0);
+      uint32_t more = __ballot_sync(0xFFFFFFFFu, n > 1);
+      while (more) {
+        const int i = __ffs(more) - 1;
+        more &= more - 1;
+        Seq t;
+        t.q0 = 0;
+        t.n = __shfl_sync(0xFFFFFFFFu, s.n, i);
+        t.len = __shfl_sync(0xFFFFFFFFu, s.len, i);
+        const int nt = tiles(a, t);
+        for (int k = lane; k < nt; k += 32) sum += units(a, t, k);
+      }
+    }
+    for (int m = 16; m; m >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, m);
+    return sum * a.c.heads;
+  }
+  // The item that unit u of the line lies in, with at = u's place in it (n and left are not set).
+  static __device__ __forceinline__ Item find(const Args &a, int64_t u) {
+    Item it{0, 0, 0, 1, 0, 0, 0};
+    int64_t per = 0;
+    scan(a, [&](int b, int64_t n) {
+      it.b = b;
+      per = n;
+      if (u < n * a.c.heads) return false;
+      u -= n * a.c.heads;
+      return true;
+    });
+    it.head = (int)(u / per);
+    u -= it.head * per;
+    const Seq s = sequence(a, it.b);
+    const int nt = tiles(a, s), lane = threadIdx.x & 31;
+    for (int t0 = 0; t0 < nt; t0 += 32) {
+      const int mine = t0 + lane < nt ? units(a, s, t0 + lane) : 0;
+      int64_t upto = mine;
+      for (int m = 1; m < 32; m <<= 1) {
+        const int64_t o = __shfl_up_sync(0xFFFFFFFFu, upto, m);
+        if (lane >= m) upto += o;
+      }
+      const uint32_t past = __ballot_sync(0xFFFFFFFFu, u < upto);
+      if (past) {
+        const int i = __ffs(past) - 1;
+        it.tile = t0 + i;
+        it.units = __shfl_sync(0xFFFFFFFFu, mine, i);
+        it.at = (int)(u - (__shfl_sync(0xFFFFFFFFu, upto, i) - it.units));
+        return it;
+      }
+      u -= __shfl_sync(0xFFFFFFFFu, upto, 31);
+    }
+    return it;
+  }
+  // The next item of the line (any thread by itself); only called while units are left.
+  static __device__ __forceinline__ void next(const Args &a, Item &it) {
+    Seq s = sequence(a, it.b);
+    if (++it.tile >= tiles(a, s)) {
+      it.tile = 0;
+      if (++it.head >= a.c.heads) {
+        it.head = 0;
+        do s = sequence(a, ++it.b);
+        while (s.n == 0);
+      }
+    }
+    it.units = units(a, s, it.tile);
+    it.at = 0;
+    it.n = (int)min((int64_t)it.units, it.left);
+    it.left -= it.n;
+  }
+  // Blocks that share `total` units, at most `most`.
+  static __device__ __forceinline__ int blocks(int64_t total, int most) { return (int)min(total, (int64_t)most); }
+  static __device__ __forceinline__ int64_t start(int64_t total, int c, int n) { return total * c / n; }
+};
+
+// One partial result: kRows maxima (base-2 logarithms), kRows sums, then [dim][kRows] outputs.
+__host__ __device__ constexpr size_t partial_floats(int rows, int dim) { return (size_t)rows * (dim + 2); }
+
+// Merges the partial results of the items that several blocks share. One block for each border between two
+// stretches; it acts if the border is the first inside its item. Elements [dim][row] of an item are spread
+// over the threads.
+template <typename T, int kRows, int kKeys>
+__global__ void __launch_bounds__(256) join_kernel(Args a, const float *parts, int dim_pad, int most) {
+  using W = Work<kRows, kKeys>;
+  __shared__ Item item;
+  __shared__ int from, upto;
+  __shared__ float top[kRows], scale[kRows];
+  const int c = blockIdx.x + 1;
+  if (threadIdx.x < 32) {
+    const int64_t total = W::total(a);
+    const int n = W::blocks(total, most);
+    if (c >= n) {
+      if (threadIdx.x == 0) upto = 0;
+    } else {
+      const int64_t u = W::start(total, c, n);
+      const Item it = W::find(a, u);
+      const int64_t begin = u - it.at, end = begin + it.units;
+      if (threadIdx.x == 0) {
+        item = it;
+        from = c - 1;
+        upto = 0;
+        if (it.at > 0 && W::start(total, c - 1, n) <= begin) {
+          // Blocks whose stretch starts before the item's end; starts grow by at least one unit a block.
+          int64_t k = end * n / total;
+          while (k < n && W::start(total, (int)k, n) < end) ++k;
+          while (k > 0 && W::start(total, (int)k - 1, n) >= end) --k;
+          upto = (int)min(k, (int64_t)n);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  if (upto == 0) return;
+  const size_t size = partial_floats(kRows, dim_pad);
+  // The first block left it in its last slot, the others in their first.
+  auto slot = [&](int k) { return parts + (size_t)(2 * k + (k == from ? 1 : 0)) * size; };
+  const Seq s = sequence(a, item.b);
+  for (int r = threadIdx.x; r < kRows; r += 256) {
+    float m = -INFINITY, sum = 0.0f;
+    for (int k = from; k < upto; ++k) m = fmaxf(m, slot(k)[r]);
+    for (int k = from; k < upto; ++k) {
+      const float t = slot(k)[r], l = slot(k)[kRows + r];
+      sum += t == -INFINITY && l == 0.0f ? 0.0f : l * exp2_fast(t - m);
+    }
+    top[r] = m;
+    scale[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
+    const int row = item.tile * kRows + r;
+    if (a.lse && row < s.n * a.group)
+      a.lse[(s.q0 + row / a.group) * a.heads + item.head * a.group + row % a.group] =
+          sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.69314718055994531f;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < kRows * a.c.dim; e += 256) {
+    const int r = e % kRows, d = e / kRows, row = item.tile * kRows + r;
+    if (row >= s.n * a.group) continue;
+    float v = 0.0f;
+    for (int k = from; k < upto; ++k) {
+      const float t = slot(k)[r];
+      if (t != -INFINITY) v += slot(k)[(2 + d) * kRows + r] * exp2_fast(t - top[r]);
+    }
+    const int64_t out = (s.q0 + row / a.group) * a.heads + item.head * a.group + row % a.group;
+    static_cast<T *>(a.out)[out * a.c.dim + d] = Io<T>::put(v * scale[r]);
+  }
+}
+
+// Blocks per multiprocessor of the split kernel, and its width of a head.
+inline int split_width(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 }  // namespace attn
 }  // namespace tc

@@ -1,0 +1,10 @@
+// The split attention kernel for one cache scheme (compiled on its own to build in parallel).
+#include "tc_attn_split.cuh"
+
+namespace tc {
+namespace attn {
+int launch_split_fp8(const Args &a, float *parts, int most, cudaStream_t s) {
+  return split::launch_scheme<KV_FP8_ROW>(a, parts, most, s);
+}
+}  // namespace attn
+}  // namespace tc

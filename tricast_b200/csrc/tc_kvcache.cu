@@ -33,7 +33,7 @@ int kv_cache_check(const tc_kv_cache *c, KvCache &o) {
   o.row_bytes = c->scheme == KV_NONE ? o.dim * (c->dtype == TC_F32 ? 4 : 2) : c->scheme == KV_MXFP4 ? o.dim / 2 : o.dim;
   o.scale_bytes = c->scheme == KV_NONE ? 0 : c->scheme == KV_MXFP4 ? o.dim / 32 : 4;
   if (((uintptr_t)o.k | (uintptr_t)o.v) % 16) return bad("codes must be 16-byte aligned");
-  if ((c->scheme == KV_FP8_ROW || c->scheme == KV_INT8_ROW) && ((uintptr_t)o.ks | (uintptr_t)o.vs) % 4)
+  if (c->scheme != KV_NONE && ((uintptr_t)o.ks | (uintptr_t)o.vs) % 4)
     return bad("scales must be 4-byte aligned");
   return TC_OK;
 }
