@@ -15,6 +15,7 @@ import pytest
 import torch
 
 from tricast_b200 import PagedKVCache, paged_attention
+from tricast_b200 import _native as N
 
 pytestmark = pytest.mark.gpu
 
@@ -281,6 +282,20 @@ def test_lengths_beyond_the_table_are_clamped():
     b.table = b.table[:, :40].contiguous()
     b.lens[1] = 1 << 30
     assert torch.equal(b.run()[1:], want[1:])
+
+
+@pytest.mark.parametrize("polls", [0, 1])
+@pytest.mark.parametrize("scheme", SCHEMES)
+def test_a_wait_that_runs_out_still_gives_the_result(scheme, polls):
+    """With the pipeline waits limited to none or one poll the chunk kernel gives up; what runs after it
+    computes the call again."""
+    b = Batch([130, 1, 300], [300, 40, 300], 4, 2, 128, 16, scheme, torch.bfloat16)
+    N.lib().tc_set_wait_limit(polls)
+    try:
+        b.check()
+    finally:
+        N.lib().tc_set_wait_limit(-1)
+    b.check()
 
 
 def test_no_tokens_and_refusals():

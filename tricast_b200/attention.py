@@ -52,6 +52,8 @@ def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens:
         max_q_len = max(total, 1)
     elif max_q_len < 1:
         raise ValueError("max_q_len must be positive")
+    if cu_q is None:
+        max_q_len = 1
     if q.stride(2) != 1:
         q = q.contiguous()
     if max_pages and block_table.stride(1) != 1:

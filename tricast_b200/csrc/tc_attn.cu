@@ -9,90 +9,20 @@ namespace attn {
 
 constexpr int kThreads = 256;
 
-// Element d of a cached row, in fp32.
-template <typename T>
-__device__ __forceinline__ float cached(const KvCache &c, const unsigned char *codes, const unsigned char *scales, int d) {
-  if (c.scheme == KV_NONE) return Io<T>::get(reinterpret_cast<const T *>(codes)[d]);
-  if (c.scheme == KV_MXFP4) return __fmul_rn(decode_e2m1((codes[d >> 1] >> (4 * (d & 1))) & 15u), pow2_value(scales[d >> 5]));
-  const float s = *reinterpret_cast<const float *>(scales);
-  return __fmul_rn(c.scheme == KV_FP8_ROW ? decode_e4m3(codes[d]) : (float)(signed char)codes[d], s);
-}
-
-// A warp a (new token, query head): lanes over the head's elements, one key at a time, with the running
-// maximum and sum of the softmax. Every type, scheme and head size; all arithmetic in fp32.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) plain_kernel(Args a) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = a.total_q * a.heads;
-  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < rows;
-       r += (int64_t)gridDim.x * (kThreads / 32)) {
-    const int64_t token = r / a.heads;
-    const int head = (int)(r % a.heads);
-    // The last sequence whose first token is not after this one (idle sequences share their start with
-    // the next one).
-    int b = 0;
-    if (a.cu) {
-      int hi = a.batch;
-      while (b + 1 < hi) {
-        const int mid = (b + hi) >> 1;
-        if (a.cu[mid] <= token) b = mid;
-        else hi = mid;
-      }
-    } else {
-      b = (int)token;
-    }
-    const Seq s = sequence(a, b);
-    if (token < s.q0 || token >= s.q0 + s.n) continue;
-    int lo, hi;
-    visible(a, s, (int)(token - s.q0), lo, hi);
-    const T *qp = static_cast<const T *>(a.q) + token * a.q_tok + head * a.q_head;
-    float q[8], o[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = lane + 32 * i;
-      q[i] = d < a.c.dim ? Io<T>::get(qp[d]) : 0.0f;
-      o[i] = 0.0f;
-    }
-    float top = -INFINITY, total = 0.0f;
-    const int kvh = head / a.group;
-    for (int p = lo; p < hi; ++p) {
-      const int page = a.table[b * a.table_stride + (p >> a.c.page_shift)];
-      if (page < 0 || page >= a.c.pages) continue;
-      const int64_t row = (((int64_t)page * a.c.heads + kvh) << a.c.page_shift) + (p & (a.c.page_size - 1));
-      const unsigned char *kc = a.c.k + row * a.c.row_bytes, *ks = a.c.ks + row * a.c.scale_bytes;
-      const unsigned char *vc = a.c.v + row * a.c.row_bytes, *vs = a.c.vs + row * a.c.scale_bytes;
-      float dot = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        if (d < a.c.dim) dot = __fmaf_rn(q[i], cached<T>(a.c, kc, ks, d), dot);
-      }
-      for (int m = 16; m; m >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, m);
-      dot *= a.scale;
-      if (dot == -INFINITY) continue;  // exp2 of it is 0 whatever the maximum
-      const float now = fmaxf(top, dot), keep = exp2f(top - now), w = exp2f(dot - now);
-      top = now;
-      total = __fmaf_rn(total, keep, w);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int d = lane + 32 * i;
-        if (d < a.c.dim) o[i] = __fmaf_rn(w, cached<T>(a.c, vc, vs, d), o[i] * keep);
-      }
-    }
-    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int d = lane + 32 * i;
-      if (d < a.c.dim) static_cast<T *>(a.out)[r * a.c.dim + d] = Io<T>::put(o[i] * inv);
-    }
-    if (a.lse && lane == 0) a.lse[r] = total == 0.0f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f;
-  }
+  plain_rows<T>(a, (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), (int64_t)gridDim.x * (kThreads / 32));
 }
 
 int launch_split_none(const Args &a, float *parts, int most, cudaStream_t s);
 int launch_split_fp8(const Args &a, float *parts, int most, cudaStream_t s);
 int launch_split_int8(const Args &a, float *parts, int most, cudaStream_t s);
 int launch_split_mxfp4(const Args &a, float *parts, int most, cudaStream_t s);
+
+int launch_chunk_none(const Args &a, float *parts, int *status, int most, cudaStream_t s);
+int launch_chunk_fp8(const Args &a, float *parts, int *status, int most, cudaStream_t s);
+int launch_chunk_int8(const Args &a, float *parts, int *status, int most, cudaStream_t s);
+int launch_chunk_mxfp4(const Args &a, float *parts, int *status, int most, cudaStream_t s);
 
 // Blocks of the split kernel: as many as run at once.
 static int split_blocks(const KvCache &c) {
@@ -106,8 +36,35 @@ static int launch_split(const Args &a, float *parts, cudaStream_t s) {
                  : a.c.scheme == KV_INT8_ROW ? launch_split_int8(a, parts, most, s)
                                              : launch_split_mxfp4(a, parts, most, s);
   if (st != TC_OK) return st;
-  if (a.c.dtype == TC_BF16) join_kernel<__nv_bfloat16, 16, 64><<<most - 1, 256, 0, s>>>(a, parts, split_width(a.c.dim), most);
-  else join_kernel<__half, 16, 64><<<most - 1, 256, 0, s>>>(a, parts, split_width(a.c.dim), most);
+  if (a.c.dtype == TC_BF16) join_kernel<__nv_bfloat16, 16, 64><<<most - 1, 256, 0, s>>>(a, parts, split_width(a.c.dim), most, nullptr);
+  else join_kernel<__half, 16, 64><<<most - 1, 256, 0, s>>>(a, parts, split_width(a.c.dim), most, nullptr);
+  count_launch();
+  return TC_OK;
+}
+
+// Query rows of one key / value head from which the chunk kernel's tiles of 128 rows pay.
+constexpr int64_t kChunkRows = 65;
+static bool use_chunk(const KvCache &c, int group, int64_t max_q) { return c.dim <= 128 && max_q * group >= kChunkRows; }
+
+static size_t split_bytes(const KvCache &c) {
+  return 2 * (size_t)split_blocks(c) * partial_floats(16, split_width(c.dim)) * sizeof(float);
+}
+static size_t chunk_bytes(const KvCache &c) {
+  return 2 * (size_t)sm_count() * partial_floats(256, split_width(c.dim)) * sizeof(float);
+}
+
+static int launch_chunk(const Args &a, void *workspace, cudaStream_t s) {
+  const int most = sm_count();
+  float *parts = static_cast<float *>(workspace);
+  int *status = reinterpret_cast<int *>(static_cast<char *>(workspace) + chunk_bytes(a.c));
+  const int st = a.c.scheme == KV_NONE       ? launch_chunk_none(a, parts, status, most, s)
+                 : a.c.scheme == KV_FP8_ROW  ? launch_chunk_fp8(a, parts, status, most, s)
+                 : a.c.scheme == KV_INT8_ROW ? launch_chunk_int8(a, parts, status, most, s)
+                                             : launch_chunk_mxfp4(a, parts, status, most, s);
+  if (st != TC_OK) return st;
+  const dim3 grid(most > 1 ? most - 1 : 1, 8);
+  if (a.c.dtype == TC_BF16) join_kernel<__nv_bfloat16, 256, 128><<<grid, 256, 0, s>>>(a, parts, split_width(a.c.dim), most, status);
+  else join_kernel<__half, 256, 128><<<grid, 256, 0, s>>>(a, parts, split_width(a.c.dim), most, status);
   count_launch();
   return TC_OK;
 }
@@ -120,7 +77,9 @@ extern "C" size_t tc_paged_attention_workspace(const tc_kv_cache *cache, int32_t
   using namespace tc;
   KvCache c;
   if (kv_cache_check(cache, c) != TC_OK || c.dtype == TC_F32) return 0;
-  return 2 * (size_t)attn::split_blocks(c) * attn::partial_floats(16, attn::split_width(c.dim)) * sizeof(float);
+  if (q_heads < c.heads || q_heads % c.heads) return 0;
+  if (attn::use_chunk(c, q_heads / c.heads, max_q_len)) return attn::chunk_bytes(c) + sm_count() * sizeof(int);
+  return attn::split_bytes(c);
 }
 
 extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64_t q_token_stride, int64_t q_head_stride,
@@ -135,6 +94,7 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
   auto bad = [](const char *m) { return set_error(std::string("tc_paged_attention: ") + m), (int)TC_INVALID_ARGUMENT; };
   if (total_q == 0 || batch == 0) return TC_OK;
   if (!q || !block_table || !seq_lens || !out) return bad("null pointer");
+  if ((uintptr_t)out % 16 || (uintptr_t)workspace % 16) return bad("out and workspace must be 16-byte aligned");
   if (total_q < 0 || total_q > 0x7FFFFFFFll || batch < 0 || max_pages < 0 || max_q_len < 1) return bad("sizes out of range");
   if (!cu_q && total_q != batch) return bad("without cu_q every sequence has one new token");
   if (q_heads < 1 || q_heads % cache->kv_heads) return bad("query heads must be a multiple of the cache's");
@@ -166,9 +126,10 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
     attn::plain_kernel<float><<<(unsigned)(want < most ? want : most), attn::kThreads, 0, s>>>(a);
     count_launch();
   } else {
-    if (!workspace || workspace_bytes < tc_paged_attention_workspace(cache, q_heads, total_q, batch, max_q_len))
+    if (!workspace || workspace_bytes < tc_paged_attention_workspace(cache, q_heads, total_q, batch, a.max_q))
       return set_error("tc_paged_attention: workspace too small"), TC_WORKSPACE_TOO_SMALL;
-    const int r = attn::launch_split(a, static_cast<float *>(workspace), s);
+    const int r = attn::use_chunk(a.c, a.group, a.max_q) ? attn::launch_chunk(a, workspace, s)
+                                                         : attn::launch_split(a, static_cast<float *>(workspace), s);
     if (r != TC_OK) return r;
   }
   const cudaError_t e = cudaGetLastError();

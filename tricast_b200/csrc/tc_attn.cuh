@@ -203,12 +203,101 @@ struct Work {
 // One partial result: kRows maxima (base-2 logarithms), kRows sums, then [dim][kRows] outputs.
 __host__ __device__ constexpr size_t partial_floats(int rows, int dim) { return (size_t)rows * (dim + 2); }
 
+// Element d of a cached row, in fp32.
+template <typename T>
+__device__ __forceinline__ float cached(const KvCache &c, const unsigned char *codes, const unsigned char *scales, int d) {
+  if (c.scheme == KV_NONE) return Io<T>::get(reinterpret_cast<const T *>(codes)[d]);
+  if (c.scheme == KV_MXFP4) return __fmul_rn(decode_e2m1((codes[d >> 1] >> (4 * (d & 1))) & 15u), pow2_value(scales[d >> 5]));
+  const float s = *reinterpret_cast<const float *>(scales);
+  return __fmul_rn(c.scheme == KV_FP8_ROW ? decode_e4m3(codes[d]) : (float)(signed char)codes[d], s);
+}
+
+// A warp a (new token, query head): lanes over the head's elements, one key at a time, with the running
+// maximum and sum of the softmax. Every type, scheme and head size; all arithmetic in fp32.
+template <typename T>
+__device__ __noinline__ void plain_rows(const Args &a, int64_t warp, int64_t warps) {
+  const int lane = threadIdx.x & 31;
+  const int64_t rows = a.total_q * a.heads;
+  for (int64_t r = warp; r < rows; r += warps) {
+    const int64_t token = r / a.heads;
+    const int head = (int)(r % a.heads);
+    // The last sequence whose first token is not after this one (idle sequences share their start with
+    // the next one).
+    int b = 0;
+    if (a.cu) {
+      int hi = a.batch;
+      while (b + 1 < hi) {
+        const int mid = (b + hi) >> 1;
+        if (a.cu[mid] <= token) b = mid;
+        else hi = mid;
+      }
+    } else {
+      b = (int)token;
+    }
+    const Seq s = sequence(a, b);
+    if (token < s.q0 || token >= s.q0 + s.n) continue;
+    int lo, hi;
+    visible(a, s, (int)(token - s.q0), lo, hi);
+    const T *qp = static_cast<const T *>(a.q) + token * a.q_tok + head * a.q_head;
+    float q[8], o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = lane + 32 * i;
+      q[i] = d < a.c.dim ? Io<T>::get(qp[d]) : 0.0f;
+      o[i] = 0.0f;
+    }
+    float top = -INFINITY, total = 0.0f;
+    const int kvh = head / a.group;
+    for (int p = lo; p < hi; ++p) {
+      const int page = a.table[b * a.table_stride + (p >> a.c.page_shift)];
+      if (page < 0 || page >= a.c.pages) continue;
+      const int64_t row = (((int64_t)page * a.c.heads + kvh) << a.c.page_shift) + (p & (a.c.page_size - 1));
+      const unsigned char *kc = a.c.k + row * a.c.row_bytes, *ks = a.c.ks + row * a.c.scale_bytes;
+      const unsigned char *vc = a.c.v + row * a.c.row_bytes, *vs = a.c.vs + row * a.c.scale_bytes;
+      float dot = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = lane + 32 * i;
+        if (d < a.c.dim) dot = __fmaf_rn(q[i], cached<T>(a.c, kc, ks, d), dot);
+      }
+      for (int m = 16; m; m >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, m);
+      dot *= a.scale;
+      if (dot == -INFINITY) continue;  // exp2 of it is 0 whatever the maximum
+      const float now = fmaxf(top, dot), keep = exp2f(top - now), w = exp2f(dot - now);
+      top = now;
+      total = __fmaf_rn(total, keep, w);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int d = lane + 32 * i;
+        if (d < a.c.dim) o[i] = __fmaf_rn(w, cached<T>(a.c, vc, vs, d), o[i] * keep);
+      }
+    }
+    const float inv = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int d = lane + 32 * i;
+      if (d < a.c.dim) static_cast<T *>(a.out)[r * a.c.dim + d] = Io<T>::put(o[i] * inv);
+    }
+    if (a.lse && lane == 0) a.lse[r] = total == 0.0f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f;
+  }
+}
+
 // Merges the partial results of the items that several blocks share. One block for each border between two
 // stretches; it acts if the border is the first inside its item. Elements [dim][row] of an item are spread
-// over the threads.
+// over the threads and over gridDim.y. Where `status` is given and a block of the kernel before gave up a
+// wait (which takes a fault elsewhere, or a test), everything is computed again by the plain rows.
 template <typename T, int kRows, int kKeys>
-__global__ void __launch_bounds__(256) join_kernel(Args a, const float *parts, int dim_pad, int most) {
+__global__ void __launch_bounds__(256) join_kernel(Args a, const float *parts, int dim_pad, int most, const int *status) {
   using W = Work<kRows, kKeys>;
+  if (status) {
+    int bad = 0;
+    for (int i = threadIdx.x; i < most; i += 256) bad |= status[i];
+    if (__syncthreads_or(bad)) {
+      const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+      plain_rows<T>(a, block * 8 + (threadIdx.x >> 5), (int64_t)gridDim.x * gridDim.y * 8);
+      return;
+    }
+  }
   __shared__ Item item;
   __shared__ int from, upto;
   __shared__ float top[kRows], scale[kRows];
@@ -252,12 +341,12 @@ __global__ void __launch_bounds__(256) join_kernel(Args a, const float *parts, i
     top[r] = m;
     scale[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
     const int row = item.tile * kRows + r;
-    if (a.lse && row < s.n * a.group)
+    if (a.lse && blockIdx.y == 0 && row < s.n * a.group)
       a.lse[(s.q0 + row / a.group) * a.heads + item.head * a.group + row % a.group] =
           sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.69314718055994531f;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < kRows * a.c.dim; e += 256) {
+  for (int e = blockIdx.y * 256 + threadIdx.x; e < kRows * a.c.dim; e += 256 * gridDim.y) {
     const int r = e % kRows, d = e / kRows, row = item.tile * kRows + r;
     if (row >= s.n * a.group) continue;
     float v = 0.0f;

@@ -1,0 +1,10 @@
+// The chunk attention kernel for one cache scheme (compiled on its own to build in parallel).
+#include "tc_attn_chunk.cuh"
+
+namespace tc {
+namespace attn {
+int launch_chunk_int8(const Args &a, float *parts, int *status, int most, cudaStream_t s) {
+  return chunk::launch_scheme<KV_INT8_ROW>(a, parts, status, most, s);
+}
+}  // namespace attn
+}  // namespace tc
