@@ -3,11 +3,12 @@
 //
 // A block takes a stretch of the work line (tc_attn.cuh) in items of 256 query rows, two tiles of 128, and
 // units of 128 keys. Its warps have roles, joined by mbarriers:
-//  - producers (4 warps) read the codes of a unit, a step ahead in registers, and write them as 16-bit
-//    operands into swizzled shared memory (K and V, two stages each), with the keys' scales beside them;
+//  - producers (7 warps) take the quarters of K and V tiles in turn: the codes of 32 keys, fetched into registers
+//    a turn ahead, become 16-bit operands in swizzled shared memory (K and V, two stages each), with the
+//    keys' scales beside them;
 //  - one thread issues the tcgen05 MMAs: S = Q K^T of each tile into TMEM, O += P V with P read from TMEM;
-//  - two groups of 4 warps, one a tile, a thread a row: S to P by the running softmax, P over the
-//    columns of S it has read. One tile's softmax runs under the other's MMAs.
+//  - two groups of 4 warps, one a tile, a warp 32 rows: S to P by the running softmax, P over the columns
+//    of S it has read, half a unit at a time. One tile's softmax runs under the other's MMAs.
 // TMEM: S of the two tiles (128 columns each, P over their first 64), O of the two (DP columns each).
 //
 // Codes are exact in fp16 and their scales stay out of the products, as in the split kernel: a key's scale
@@ -29,7 +30,9 @@ namespace attn {
 namespace chunk {
 
 constexpr int kTile = 128, kRows = 2 * kTile, kKeys = 128, kSlots = 4;
-constexpr int kSoftmaxWarps = 8, kProducerWarps = 4, kThreads = (kSoftmaxWarps + kProducerWarps + 1) * 32;
+constexpr int kSoftmaxWarps = 8, kProducerWarps = 7, kThreads = 512;  // and one warp for the MMA thread
+// Registers a thread: 128 at launch; 256 * 160 + 256 * 96 = 512 * 128.
+constexpr int kSoftmaxRegs = 160, kOtherRegs = 96;
 using W = Work<kRows, kKeys>;
 
 template <int DP>
@@ -42,8 +45,10 @@ struct Shape {
 // What the softmax needs of a unit's keys.
 struct __align__(16) KeySlot {
   float k[kKeys], v[kKeys];
-  uint32_t valid[4];
-  int vfield[4];  // largest exponent field of the value scales, by quarter
+  uint32_t valid[4];  // keys that are there
+  uint32_t dead[4];   // keys whose rows of scores or values are not numbers: their scales here are 1, their V
+                      // is 0, and the rows that see them become NaN
+  int vfield[4];      // largest exponent field of the value scales, by quarter
 };
 
 // 16 bytes (8 elements) of row r, granule q of a tile: 128-byte rows in blocks of 128, swizzled.
@@ -59,26 +64,39 @@ __device__ __forceinline__ uint64_t desc_sw128(uint32_t addr, uint32_t lbo) {
          (1ull << 46) | (2ull << 61);
 }
 
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t r;
+// Pairs of fp32: one instruction where two would issue.
+using F2 = uint64_t;
+__device__ __forceinline__ F2 pack2(float a, float b) {
+  F2 r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
   return r;
 }
-__device__ __forceinline__ void unpack2(uint64_t v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
+__device__ __forceinline__ void unpack2(F2 v, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
   return r;
+}
+
+// 16 bytes that L1 need not keep: what shared memory leaves of it holds the few spilled registers.
+__device__ __forceinline__ uint4 load_once(const unsigned char *p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ void st_shared16(uint32_t at, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 __device__ __forceinline__ void fence_async_proxy() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -91,8 +109,15 @@ __device__ __forceinline__ uint32_t range_bits(int lo, int hi, int part) {
   return below_h & ~below_l;
 }
 
+// One arrival for the warp, after what its threads have done: every thread's arrival costs about 20 cycles, one
+// after the other.
+__device__ __forceinline__ void warp_arrive(uint64_t *bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
+}
+
 struct Barriers {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], slot[kSlots], qfull[2], sfull[2], pfull[2], ofull[2], drain;
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], slot[kSlots], qfull[2], sfull[2], pfull[2][2], phalf[2], ofull[2], drain;
 };
 
 // Bounds of an item that every role derives alike.
@@ -100,7 +125,7 @@ struct Part {
   Seq s;
   int rows;            // of the sequence's heads on this key head
   bool two;            // the second tile has rows
-  int64_t key0, key1;  // keys of the part
+  int key0, key1;      // keys of the part
   int steps;
   int all_lo, all_hi;  // keys that every row sees
 };
@@ -111,8 +136,8 @@ __device__ __forceinline__ Part part_of(const Args &a, const Item &it) {
   p.two = p.rows > it.tile * kRows + kTile;
   int lo, hi, unused;
   W::keys(a, p.s, it.tile, lo, hi);
-  p.key0 = (int64_t)lo + (int64_t)it.at * kKeys;
-  p.key1 = min((int64_t)lo + (int64_t)(it.at + it.n) * kKeys, (int64_t)hi);
+  p.key0 = lo + it.at * kKeys;
+  p.key1 = min(lo + (it.at + it.n) * kKeys, hi);
   p.steps = it.n;
   visible(a, p.s, it.tile * kRows / a.group, unused, p.all_hi);
   visible(a, p.s, (min((it.tile + 1) * kRows, p.rows) - 1) / a.group, p.all_lo, unused);
@@ -120,222 +145,274 @@ __device__ __forceinline__ Part part_of(const Args &a, const Item &it) {
 }
 
 // ---------------------------------------------------------------- producers
+// A job is 32 keys (a quarter) of a unit's K or V: job 8 u + 4 side + quarter of the block's unit u. A warp
+// takes every seventh.
+struct Job {
+  int page;    // of this lane's key, -1 for a key that is not there
+  int at;      // its position
+  int head;
+  bool mixed;  // the item's rows differ in which of the unit's keys they see
+};
+
 template <typename T, int S, int DP>
 __device__ __forceinline__ bool produce(const Args &a, Item it, unsigned char *ks, unsigned char *vs, KeySlot *slots,
                                         Barriers &bar, int polls) {
   constexpr int kRowBytes = S == KV_NONE ? 2 * DP : S == KV_MXFP4 ? DP / 2 : DP;
-  constexpr int kCpr = kRowBytes / 16;                      // 16-byte chunks of a row
-  constexpr int kOwn = kCpr * kKeys / (kProducerWarps * 32);  // chunks a thread and side
+  constexpr int kCpr = kRowBytes / 16;                            // 16-byte chunks of a row
+  constexpr int kOwn = kCpr;                                      // chunks a lane and job
   constexpr int kOut = S == KV_NONE ? 1 : S == KV_MXFP4 ? 4 : 2;  // granules of a chunk
+  // A job is four blocks of 8 rows; a warp's access covers 8 rows by 64 bytes (16 by 32 where a row has no
+  // more), so that neither the reads nor the swizzled writes collide.
+  constexpr int kBlocks = kCpr >= 4 ? 4 : 2;  // that a lane has chunks in
   const KvCache &c = a.c;
-  const int warp = (threadIdx.x >> 5) - kSoftmaxWarps, lane = threadIdx.x & 31, key = warp * 32 + lane;
-  uint32_t step = 0;
+  const int warp = (threadIdx.x >> 5) - kSoftmaxWarps, lane = threadIdx.x & 31;
+  const int chunk0 = kCpr >= 4 ? lane >> 3 : (lane >> 3) & 1;
+  const bool fits = c.dim == DP;
 
-  // A warp's chunks lie in its 32 keys, in four blocks of 8 rows: chunk i of a lane.
-  auto block_of = [&](int i) { return kCpr >= 4 ? i / (kCpr / 4) : 2 * i + (lane >> 4); };
-  auto chunk_of = [&](int i) { return kCpr >= 4 ? (i % (kCpr / 4)) * 4 + (lane >> 3) : (lane >> 3) & 1; };
-
-  while (true) {
-    const Part p = part_of(a, it);
-    const int *table = a.table + (int64_t)it.b * a.table_stride;
-    // Page of this lane's key, and with it the row: -1 for a key that is not there.
-    auto page_at = [&](int j) {
-      const int64_t at = p.key0 + (int64_t)j * kKeys + key;
-      return j < p.steps && at < p.key1 ? table[at >> c.page_shift] : -1;
-    };
-    auto row_at = [&](int j, int pg) -> int64_t {
-      if (pg < 0 || pg >= c.pages) return -1;
-      const int64_t at = p.key0 + (int64_t)j * kKeys + key;
-      return (((int64_t)pg * c.heads + it.head) << c.page_shift) + (at & (c.page_size - 1));
-    };
-    // Row of lane 8 i's key, as every lane of the warp needs it: rows of a block of 8 are adjacent.
-    auto block_row = [&](int64_t row, int blk) { return __shfl_sync(0xFFFFFFFFu, row, 8 * blk + (lane & 7)); };
-
-    uint4 kreg[S == KV_NONE ? 1 : kOwn], vreg[S == KV_NONE ? 1 : kOwn];
-    uint32_t kword[2] = {0u, 0u}, vword[2] = {0u, 0u};  // this key's scales as they are stored
-    auto load = [&](const unsigned char *codes, int64_t row, uint4 *reg) {
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        const int64_t r = block_row(row, block_of(i));
-        const int ch = chunk_of(i);
-        reg[S == KV_NONE ? 0 : i] = r >= 0 && ch * 16 < c.row_bytes
-                                        ? __ldg(reinterpret_cast<const uint4 *>(codes + r * c.row_bytes + ch * 16))
-                                        : make_uint4(0, 0, 0, 0);
+  // The item that the jobs being looked up belong to, and its first unit in the block's count.
+  Part p = part_of(a, it);
+  uint32_t base = 0;
+  bool over = false;
+  auto look = [&](uint32_t job) {
+    Job r{-1, 0, 0, false};
+    const uint32_t unit = job >> 3;
+    while (!over && unit >= base + (uint32_t)p.steps) {
+      base += (uint32_t)p.steps;
+      if (it.left == 0) {
+        over = true;
+      } else {
+        W::next(a, it);
+        p = part_of(a, it);
       }
-    };
-    auto load_scale = [&](const unsigned char *scales, int64_t row, uint32_t (&w)[2]) {
-      w[0] = w[1] = 0u;
-      if (row < 0) return;
+    }
+    if (over) return r;
+    const int p0 = p.key0 + (int)(unit - base) * kKeys, at = p0 + 32 * (int)(job & 3) + lane;
+    if (at < p.key1) {
+      const int pg = a.table[(int64_t)it.b * a.table_stride + (at >> c.page_shift)];
+      r.page = pg < c.pages ? pg : -1;
+    }
+    r.at = at;
+    r.head = it.head;
+    r.mixed = !(p0 >= p.all_lo && p0 + kKeys <= p.all_hi);
+    return r;
+  };
+  // Row of key `in` of the job, whose page is pg >= 0.
+  auto row_at = [&](const Job &r, int pg, int in) -> int64_t {
+    return (((int64_t)pg * c.heads + r.head) << c.page_shift) + ((r.at - lane + in) & (c.page_size - 1));
+  };
+  auto key_of = [&](int blk) { return 8 * (kCpr >= 4 ? blk : 2 * blk + (lane >> 4)) + (lane & 7); };
+  // Chunk i is chunk chunk0 + cstep(i) of key key_of(bstep(i)).
+  auto bstep = [&](int i) { return kCpr >= 4 ? i / (kCpr / 4) : i; };
+  auto cstep = [&](int i) { return kCpr >= 4 ? (i % (kCpr / 4)) * 4 : 0; };
+  auto load_scale = [&](const unsigned char *scales, const Job &r) {
+    uint32_t w = 0u;
+    if (r.page >= 0) {
+      const int64_t row = row_at(r, r.page, lane);
       if (S == KV_MXFP4) {
 #pragma unroll
         for (int q = 0; q < DP / 32; ++q)
-          if (q < c.scale_bytes) w[0] |= (uint32_t)scales[row * c.scale_bytes + q] << (8 * q);
+          if (q < c.scale_bytes) w |= (uint32_t)scales[row * c.scale_bytes + q] << (8 * q);
       } else if (S != KV_NONE) {
-        w[0] = *reinterpret_cast<const uint32_t *>(scales + row * 4);
+        w = *reinterpret_cast<const uint32_t *>(scales + row * 4);
+      }
+    }
+    return w;
+  };
+  // Largest group exponent of a key (mxfp4).
+  auto biggest = [&](uint32_t w) {
+    int big = 0;
+#pragma unroll
+    for (int q = 0; q < DP / 32; ++q) big = max(big, (int)((w >> (8 * q)) & 0xFFu));
+    return big;
+  };
+  // Where rows of a job differ in what they see, a V row of an unquantized cache that is not finite must not
+  // reach the others: the whole row counts as 0 and the weights of the rows that see it become NaN.
+  auto not_finite = [&](const Job &r) {
+    bool bad = false;
+    if (r.mixed && r.page >= 0) {
+      const uint32_t m = Same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
+      const uint32_t *v = reinterpret_cast<const uint32_t *>(c.v + row_at(r, r.page, lane) * c.row_bytes);
+      for (int d = 0; d < c.row_bytes / 4; ++d) bad |= (v[d] & m) == m || ((v[d] >> 16) & m) == m;
+    }
+    return bad;
+  };
+  // The keys' entries of the unit's slot.
+  auto put_slot = [&](uint32_t job, const Job &r, uint32_t kw, uint32_t vw) {
+    KeySlot &sl = slots[(job >> 3) % kSlots];
+    const int quarter = job & 3;
+    float k = 1.0f, v = 1.0f;
+    bool dead = false;
+    if (S == KV_MXFP4) {
+      k = pow2_value((uint32_t)biggest(kw)) * (1.0f / (1 << kGroupShift));
+      v = pow2_value((uint32_t)biggest(vw)) * (1.0f / (1 << kGroupShift));
+    } else if (S != KV_NONE) {
+      k = u2f(kw);
+      v = u2f(vw);
+    } else {
+      dead = not_finite(r);
+    }
+    dead |= k != k || v != v;
+    if (r.page < 0 || dead) k = v = 1.0f;
+    sl.k[32 * quarter + lane] = k;
+    sl.v[32 * quarter + lane] = v;
+    const uint32_t valid = __ballot_sync(0xFFFFFFFFu, r.page >= 0), dead_keys = __ballot_sync(0xFFFFFFFFu, r.page >= 0 && dead);
+    const int top = (int)__reduce_max_sync(0xFFFFFFFFu, r.page >= 0 && !dead ? f2u(v) >> 23 : 0u);
+    if (lane == 0) {
+      sl.valid[quarter] = valid;
+      sl.dead[quarter] = dead_keys;
+      sl.vfield[quarter] = top;
+    }
+  };
+  auto wait_empty = [&](uint32_t job) {
+    const uint32_t unit = job >> 3, st = unit & 1, parity = ((unit >> 1) & 1) ^ 1;
+    return mbar_wait_sleep((job & 4) ? &bar.vempty[st] : &bar.kempty[st], parity, polls);
+  };
+  auto arrive_full = [&](uint32_t job) {
+    const uint32_t unit = job >> 3, st = unit & 1;
+    fence_async_proxy();
+    warp_arrive((job & 4) ? &bar.vfull[st] : &bar.kfull[st]);
+    if (!(job & 4) && (threadIdx.x & 31) == 0) mbar_arrive(&bar.slot[unit % kSlots]);
+  };
+
+  uint32_t job = (uint32_t)warp;
+  Job now = look(job);
+  if (over) return true;  // a stretch of one unit has a job for every warp: not taken
+  if constexpr (S != KV_NONE) {
+    uint4 buf[kOwn];
+    int64_t off[kBlocks];
+    uint32_t kword = 0u, vword = 0u;
+    // Where the lane's chunks of a job begin; -1 for a key that is not there.
+    auto find_rows = [&](const Job &r) {
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b) {
+        const int pg = __shfl_sync(0xFFFFFFFFu, r.page, key_of(b));
+        off[b] = pg >= 0 ? row_at(r, pg, key_of(b)) * c.row_bytes + chunk0 * 16 : -1;
       }
     };
-    // Largest group exponent of a key (mxfp4).
-    auto biggest = [&](uint32_t w) {
-      int big = 0;
-#pragma unroll
-      for (int q = 0; q < DP / 32; ++q) big = max(big, (int)((w >> (8 * q)) & 0xFFu));
-      return big;
+    // Chunk i: 16 bytes of codes. `full`: every key of the job is there, and heads fill the rows.
+    auto load = [&](const unsigned char *codes, bool full, int i) {
+      const int64_t at = off[bstep(i)];
+      if (full) return load_once(codes + at + 16 * cstep(i));
+      uint4 v = make_uint4(0, 0, 0, 0);
+      if (at >= 0 && 16 * (chunk0 + cstep(i)) < c.row_bytes) v = load_once(codes + at + 16 * cstep(i));
+      return v;
     };
-    auto convert = [&](const uint4 *reg, uint32_t scale_word, bool dead, unsigned char *dst) {
+    // Chunk i as 16-bit granules into a tile (a shared-memory address).
+    auto convert = [&](const uint4 in, uint32_t scale_word, uint32_t dead_keys, uint32_t dst, int i) {
+      const int key = key_of(bstep(i));
+      const uint32_t w[4] = {in.x, in.y, in.z, in.w};
+      uint32_t mul = 0u;
+      if (S == KV_MXFP4) {
+        const uint32_t sw = __shfl_sync(0xFFFFFFFFu, scale_word, key);
+        mul = half_pow2((int)((sw >> (8 * chunk0)) & 0xFFu) - biggest(sw) + kGroupShift) * 0x10001u;
+      }
 #pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        const int blk = block_of(i), ch = chunk_of(i), r = warp * 32 + blk * 8 + (lane & 7);
-        const uint4 in = reg[S == KV_NONE ? 0 : i];
-        const uint32_t w[4] = {in.x, in.y, in.z, in.w};
-        uint32_t h[4 * kOut];
+      for (int g = 0; g < kOut; ++g) {
+        uint32_t h[4];
         if (S == KV_MXFP4) {
-          const uint32_t sw = __shfl_sync(0xFFFFFFFFu, scale_word, 8 * blk + (lane & 7));
-          const uint32_t mul = half_pow2((int)((sw >> (8 * ch)) & 0xFFu) - biggest(sw) + kGroupShift) * 0x10001u;
+          e2m1x8_half2(w[g % 4], h);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t e[4];
-            e2m1x8_half2(w[q], e);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) h[(4 * q + k) % (4 * kOut)] = mul_half2(e[k], mul);
-          }
+          for (int k = 0; k < 4; ++k) h[k] = mul_half2(h[k], mul);
         } else {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int k = 0; k < 2; ++k) {
+            const uint32_t v = w[(2 * g + k) % 4];
             if (S == KV_FP8_ROW) {
-              h[(2 * q) % (4 * kOut)] = e4m3x2_half2(w[q] & 0xFFFFu);
-              h[(2 * q + 1) % (4 * kOut)] = e4m3x2_half2(w[q] >> 16);
+              e4m3x4_half2(v, h[2 * k], h[2 * k + 1]);
             } else {
-              h[(2 * q) % (4 * kOut)] = int8x2_half2<0x4140>(w[q] ^ 0x80808080u);
-              h[(2 * q + 1) % (4 * kOut)] = int8x2_half2<0x4342>(w[q] ^ 0x80808080u);
+              h[2 * k] = int8x2_half2<0x4140>(v ^ 0x80808080u);
+              h[2 * k + 1] = int8x2_half2<0x4342>(v ^ 0x80808080u);
             }
           }
         }
-        // A key with a NaN scale has NaN codes, which would reach rows that do not see it as 0 * NaN: they
-        // count as 0, and the scale carries the NaN.
-        const bool zero = S == KV_FP8_ROW && __shfl_sync(0xFFFFFFFFu, (int)dead, 8 * blk + (lane & 7));
-#pragma unroll
-        for (int g = 0; g < kOut; ++g)
-          *reinterpret_cast<uint4 *>(dst + tile_at(r, ch * kOut + g)) =
-              zero ? make_uint4(0, 0, 0, 0)
-                   : make_uint4(h[(4 * g) % (4 * kOut)], h[(4 * g + 1) % (4 * kOut)], h[(4 * g + 2) % (4 * kOut)],
-                                h[(4 * g + 3) % (4 * kOut)]);
+        // A key with a NaN value scale has NaN codes, which would reach rows that do not see it as 0 * NaN:
+        // they count as 0.
+        if (S == KV_FP8_ROW && dead_keys && ((dead_keys >> key) & 1u)) h[0] = h[1] = h[2] = h[3] = 0u;
+        // Granule q of the key's row, what depends on the lane apart from what depends on i.
+        const int q0 = chunk0 * kOut + g, qi = cstep(i) * kOut;
+        st_shared16(dst + (uint32_t)(((qi >> 3) + (q0 >> 3)) * (kTile * 128) + key * 128 + (((q0 & 7) ^ (lane & 7)) << 4)), h[0],
+                    h[1], h[2], h[3]);
       }
-    };
-    // Unquantized rows go straight to shared memory.
-    auto copy = [&](const unsigned char *codes, int64_t row, bool skip, unsigned char *dst) {
-#pragma unroll
-      for (int i = 0; i < kOwn; ++i) {
-        const int blk = block_of(i), ch = chunk_of(i), r = warp * 32 + blk * 8 + (lane & 7);
-        const int64_t from = block_row(skip ? -1 : row, blk);
-        const bool use = from >= 0 && ch * 16 < c.row_bytes;
-        cp_async16_or_zero(dst + tile_at(r, ch), codes + (use ? from : 0) * c.row_bytes + (use ? ch * 16 : 0), use);
-      }
-    };
-    // The key's entry of the unit's slot; true where its V row must count as zeros.
-    auto put_slot = [&](int j, int64_t row) {
-      KeySlot &sl = slots[(step + j) % kSlots];
-      float k = 1.0f, v = 1.0f;
-      bool dead = false;
-      if (S == KV_MXFP4) {
-        k = pow2_value((uint32_t)biggest(kword[0])) * (1.0f / (1 << kGroupShift));
-        v = pow2_value((uint32_t)biggest(vword[0])) * (1.0f / (1 << kGroupShift));
-      } else if (S != KV_NONE) {
-        k = u2f(kword[0]);
-        v = u2f(vword[0]);
-        dead = v != v;
-      } else {
-        const int64_t p0 = p.key0 + (int64_t)j * kKeys;
-        if (row >= 0 && !(p0 >= p.all_lo && p0 + kKeys <= p.all_hi)) {
-          // Rows differ in what they see: a value that is not finite must not reach the others. The whole
-          // V row counts as 0 and the weights of the rows that see it become NaN.
-          const uint32_t m = Same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
-          for (int d = 0; d < c.row_bytes / 4; ++d) {
-            const uint32_t w = reinterpret_cast<const uint32_t *>(c.v + row * c.row_bytes)[d];
-            dead |= (w & m) == m || ((w >> 16) & m) == m;
-          }
-          if (dead) v = u2f(kQNaN);
-        }
-      }
-      if (row < 0) k = v = 0.0f;
-      sl.k[key] = k;
-      sl.v[key] = v;
-      const uint32_t valid = __ballot_sync(0xFFFFFFFFu, row >= 0);
-      const int f = (int)((f2u(v) >> 23) & 0xFFu);
-      const int top = (int)__reduce_max_sync(0xFFFFFFFFu, (uint32_t)(f == 255 ? 0 : f));
-      if (lane == 0) {
-        sl.valid[warp] = valid;
-        sl.vfield[warp] = top;
-      }
-      return dead;
     };
 
-    int64_t row = row_at(0, page_at(0));
-    int page = page_at(1);
-    if (S != KV_NONE) {
-      load_scale(c.ks, row, kword);
-      load_scale(c.vs, row, vword);
-      load(c.k, row, kreg);
-      load(c.v, row, vreg);
-      for (int j = 0; j < p.steps; ++j) {
-        const uint32_t n = step + j, st = n & 1, ph = (n >> 1) & 1;
-        const int64_t next = row_at(j + 1, page);
-        page = page_at(j + 2);
-        if (!mbar_wait_sleep(&bar.kempty[st], ph ^ 1, polls)) return false;
-        const bool dead = put_slot(j, row);
-        convert(kreg, kword[0], false, ks + st * Shape<DP>::kOperand);
-        fence_async_proxy();
-        mbar_arrive(&bar.kfull[st]);
-        mbar_arrive(&bar.slot[n % kSlots]);
-        const uint32_t vw = vword[0];
-        load(c.k, next, kreg);
-        load_scale(c.ks, next, kword);
-        load_scale(c.vs, next, vword);
-        if (!mbar_wait_sleep(&bar.vempty[st], ph ^ 1, polls)) return false;
-        convert(vreg, vw, dead, vs + st * Shape<DP>::kOperand);
-        fence_async_proxy();
-        mbar_arrive(&bar.vfull[st]);
-        load(c.v, next, vreg);
-        row = next;
-      }
-    } else {
-      bool dead = false;
-      if (!mbar_wait_sleep(&bar.kempty[step & 1], ((step >> 1) & 1) ^ 1, polls)) return false;
-      copy(c.k, row, false, ks + (step & 1) * Shape<DP>::kOperand);
-      cp_async_commit();
-      dead = put_slot(0, row);
-      if (!mbar_wait_sleep(&bar.vempty[step & 1], ((step >> 1) & 1) ^ 1, polls)) return false;
-      copy(c.v, row, dead, vs + (step & 1) * Shape<DP>::kOperand);
-      cp_async_commit();
-      for (int j = 0; j < p.steps; ++j) {
-        const uint32_t n = step + j, st = n & 1, nst = (n + 1) & 1, nph = ((n + 1) >> 1) & 1;
-        const int64_t next = row_at(j + 1, page);
-        page = page_at(j + 2);
-        const bool more = j + 1 < p.steps;
-        if (more) {
-          if (!mbar_wait_sleep(&bar.kempty[nst], nph ^ 1, polls)) return false;
-          copy(c.k, next, false, ks + nst * Shape<DP>::kOperand);
-        }
-        cp_async_commit();
-        cp_async_wait<2>();
-        fence_async_proxy();
-        mbar_arrive(&bar.kfull[st]);
-        mbar_arrive(&bar.slot[n % kSlots]);
-        if (more) {
-          dead = put_slot(j + 1, next);
-          if (!mbar_wait_sleep(&bar.vempty[nst], nph ^ 1, polls)) return false;
-          copy(c.v, next, dead, vs + nst * Shape<DP>::kOperand);
-        }
-        cp_async_commit();
-        cp_async_wait<2>();
-        fence_async_proxy();
-        mbar_arrive(&bar.vfull[st]);
-        row = next;
-      }
-      cp_async_wait_all();
+    Job next = look(job + kProducerWarps);
+    bool over1 = over;
+    find_rows(now);
+    {
+      const bool full = fits && __all_sync(0xFFFFFFFFu, now.page >= 0);
+      if (!(job & 4)) kword = load_scale(c.ks, now);
+      vword = load_scale(c.vs, now);
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) buf[i] = load((job & 4) ? c.v : c.k, full, i);
     }
-    step += (uint32_t)p.steps;
-    if (it.left == 0) return true;
-    W::next(a, it);
+    while (true) {
+      // now: its codes arrive in buf; next: its page arrives.
+      if (!wait_empty(job)) return false;
+      const uint32_t kw = kword, vw = vword;
+      if (!(job & 4)) put_slot(job, now, kw, vw);
+      const uint32_t dead = S == KV_FP8_ROW && (job & 4) ? __ballot_sync(0xFFFFFFFFu, (vw & 0x7FFFFFFFu) > kInf) : 0u;
+      const uint32_t st = (job >> 3) & 1, ahead = job + kProducerWarps;
+      const uint32_t dst = smem_addr((job & 4) ? vs : ks) + st * Shape<DP>::kOperand + (job & 3) * 32 * 128;
+      const unsigned char *codes = (ahead & 4) ? c.v : c.k;
+      const bool full = fits && __all_sync(0xFFFFFFFFu, next.page >= 0);
+      if (!over1) {
+        find_rows(next);
+        if (!(ahead & 4)) kword = load_scale(c.ks, next);
+        vword = load_scale(c.vs, next);
+      }
+      const uint32_t word = (job & 4) ? vw : kw;
+      if (!over1 && full) {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          convert(buf[i], word, dead, dst, i);
+          buf[i] = load(codes, true, i);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kOwn; ++i) {
+          convert(buf[i], word, dead, dst, i);
+          if (!over1) buf[i] = load(codes, false, i);
+        }
+      }
+      arrive_full(job);
+      if (over1) return true;
+      now = next;
+      job = ahead;
+      next = look(job + kProducerWarps);
+      over1 = over;
+    }
+  } else {
+    // Unquantized rows go straight to shared memory.
+    auto copy = [&](uint32_t j, const Job &r) {
+      if (!(j & 4)) put_slot(j, r, 0u, 0u);
+      const int use_page = (j & 4) && not_finite(r) ? -1 : r.page;
+      const unsigned char *codes = (j & 4) ? c.v : c.k;
+      unsigned char *dst = ((j & 4) ? vs : ks) + ((j >> 3) & 1) * Shape<DP>::kOperand;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const int key = key_of(bstep(i)), ch = chunk0 + cstep(i);
+        const int pg = __shfl_sync(0xFFFFFFFFu, use_page, key);
+        const bool use = pg >= 0 && ch * 16 < c.row_bytes;
+        cp_async16_or_zero(dst + tile_at(32 * (j & 3) + key, ch), use ? codes + row_at(r, pg, key) * c.row_bytes + ch * 16 : codes, use);
+      }
+      cp_async_commit();
+    };
+    if (!wait_empty(job)) return false;
+    copy(job, now);
+    while (true) {
+      const uint32_t ahead = job + kProducerWarps;
+      now = look(ahead);
+      if (!over) {
+        if (!wait_empty(ahead)) return false;
+        copy(ahead, now);
+        cp_async_wait<1>();
+      } else {
+        cp_async_wait<0>();
+      }
+      arrive_full(job);
+      if (over) return true;
+      job = ahead;
+    }
   }
 }
 
@@ -370,14 +447,20 @@ __device__ __forceinline__ bool multiply(const Args &a, Item it, uint32_t qs, ui
       const uint32_t n = step + j;
       const bool more = j + 1 < p.steps;
       for (int t = 0; t < tiles; ++t) {
-        if (!mbar_wait(&bar.pfull[t], psteps[t]++ & 1, polls)) return false;
-        if (t == 0 && !mbar_wait(&bar.vfull[n & 1], (n >> 1) & 1, polls)) return false;
-        tc5::fence_after_sync();
         const uint32_t v0 = vs + (n & 1) * Shape<DP>::kOperand;
+        for (int half = 0; half < 2; ++half) {
+          if (!mbar_wait(&bar.pfull[t][half], psteps[t] & 1, polls)) return false;
+          if (t == 0 && half == 0 && !mbar_wait(&bar.vfull[n & 1], (n >> 1) & 1, polls)) return false;
+          tc5::fence_after_sync();
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          tc5::mma_f16_ts(tmem + 256 + t * DP, tmem + t * 128 + k * 8, desc_sw128(v0 + k * 2048, kTile * 128), kPv,
-                          j > 0 || k > 0);
+          for (int k = 0; k < kKeys / 32; ++k) {
+            const int kk = half * (kKeys / 32) + k;
+            tc5::mma_f16_ts(tmem + 256 + t * DP, tmem + t * 128 + kk * 8, desc_sw128(v0 + kk * 2048, kTile * 128), kPv,
+                            j > 0 || kk > 0);
+          }
+          if (half == 0) tc5::mma_commit(&bar.phalf[t]);
+        }
+        ++psteps[t];
         if (t == tiles - 1) tc5::mma_commit(&bar.vempty[n & 1]);
         if (more) {
           if (t == 0) {
@@ -398,26 +481,123 @@ __device__ __forceinline__ bool multiply(const Args &a, Item it, uint32_t qs, ui
 }
 
 // ---------------------------------------------------------------- softmax (a thread a row)
+// A step of the softmax covers half a unit. A warp's 32 rows are held as MMA fragments: thread (g, t) has columns
+// 8 j + 2 t, + 1 of rows 16 h + 8 e + g, rows 2 h + e of its four. A key's scale then serves four rows: what the
+// scales take of shared memory's bandwidth, which the MMAs need, is a quarter of a thread a row's.
+constexpr int kHalf = kKeys / 2, kPairs = kHalf / 8;
+using Rows = F2[4][kPairs];  // [row][j]: two neighbouring columns
+
+__device__ __forceinline__ void load_rows(uint32_t ts, Rows &x) {
+  uint32_t a[kHalf / 2], b[kHalf / 2];
+  tc5::tmem_ld_frag64(ts, a);
+  tc5::tmem_ld_frag64(ts + (16u << 16), b);
+  tc5::tmem_wait_ld_frag(a);
+  tc5::tmem_wait_ld_frag(b);
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) {
+    x[0][j] = pack2(u2f(a[4 * j]), u2f(a[4 * j + 1]));
+    x[1][j] = pack2(u2f(a[4 * j + 2]), u2f(a[4 * j + 3]));
+    x[2][j] = pack2(u2f(b[4 * j]), u2f(b[4 * j + 1]));
+    x[3][j] = pack2(u2f(b[4 * j + 2]), u2f(b[4 * j + 3]));
+  }
+}
+
+// Scores that a row does not see become -Inf, those of keys that are not numbers NaN. Rows see keys [lo, hi)
+// of the half; there and dead are its keys' bits.
+__device__ __forceinline__ void mask_rows(Rows &x, const uint32_t *there, const uint32_t *dead, int t, const int (&lo)[4],
+                                          const int (&hi)[4]) {
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) {
+    const int key = 8 * j + 2 * t;
+    const uint32_t in = there[j >> 2] >> (key & 31), bad = dead[j >> 2] >> (key & 31);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float v[2];
+      unpack2(x[r][j], v[0], v[1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        if ((bad >> e) & 1u) v[e] = u2f(kQNaN);
+        if (!((in >> e) & 1u) || key + e < lo[r] || key + e >= hi[r]) v[e] = -INFINITY;
+      }
+      x[r][j] = pack2(v[0], v[1]);
+    }
+  }
+}
+
+// P = exp2(score * key scale * qmul - ref) * value scale as packed pairs, this thread's sums of P before the
+// value's scale, and its largest scores (before qmul). Everything in one pass: the products and maxima issue
+// under the exponentials, which bound it (16 a cycle and SM).
+template <int S, bool BF16>
+__device__ __forceinline__ void weights(const Rows &x, const float *ks, const float *vs, int t, const float (&qmul)[4],
+                                        const float (&ref)[4], uint32_t (&p)[2][kHalf / 4], F2 (&sum2)[4], float (&m)[4]) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) m[r] = -INFINITY;
+#pragma unroll
+  for (int j = 0; j < kPairs; ++j) {
+    F2 k2, v2;
+    if (S != KV_NONE) {
+      k2 = *reinterpret_cast<const F2 *>(ks + 8 * j + 2 * t);
+      v2 = *reinterpret_cast<const F2 *>(vs + 8 * j + 2 * t);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      F2 y = x[r][j];
+      if (S != KV_NONE) y = mul2(y, k2);
+      float v0, v1;
+      unpack2(y, v0, v1);
+      m[r] = fmaxf(fmaxf(m[r], v0), v1);
+      unpack2(fma2(y, pack2(qmul[r], qmul[r]), pack2(-ref[r], -ref[r])), v0, v1);
+      y = pack2(exp2_fast(v0), exp2_fast(v1));
+      sum2[r] = j ? add2(sum2[r], y) : y;
+      if (S != KV_NONE) y = mul2(y, v2);
+      unpack2(y, v0, v1);
+      p[r >> 1][2 * j + (r & 1)] = BF16 ? pack_bf16(v0, v1) : pack_half(v0, v1);
+    }
+  }
+}
+
+// Multiplies the outputs so far by a power of two a row.
+template <int DP>
+__device__ __forceinline__ void rescale(const float (&keep)[4], uint32_t to) {
+#pragma unroll 1
+  for (int i = 0; i < 2 * (DP / 32); ++i) {
+    const int h = i & 1;
+    const float k0 = h ? keep[2] : keep[0], k1 = h ? keep[3] : keep[1];
+    const uint32_t at = to + (h ? 16u << 16 : 0u) + 32 * (i >> 1);
+    uint32_t o[16];
+    tc5::tmem_ld_frag32(at, o);
+    tc5::tmem_wait_ld_frag(o);
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = f2u(u2f(o[e]) * ((e & 2) ? k1 : k0));
+    tc5::tmem_st_frag32(at, o);
+  }
+}
+
+// How far a row's reference stays below its maximum: exp2(x - ref) <= 2**(8 + 6) / T, at most 2**(8 + 100), for T
+// of this exponent field.
+__device__ __forceinline__ float room(int field) { return fminf(6.0f + (127.0f - (float)field), 100.0f); }
+
 template <typename T, int S, int DP>
 __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *qs, const KeySlot *slots, uint32_t tmem,
                                         Barriers &bar, int polls, float *parts) {
   constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
-  const int t = threadIdx.x >> 7, row = threadIdx.x & 127;
-  const uint32_t lanes = (uint32_t)((threadIdx.x >> 5) & 3) << 21;  // this warp's 32 lanes of TMEM, bits 16 up
-  const uint32_t ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * DP;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
+  const int t = warp >> 2, row0 = 32 * (warp & 3);  // a warp reaches the 32 TMEM lanes of its index
+  const uint32_t ts = tmem + ((uint32_t)row0 << 16) + t * 128, to = tmem + ((uint32_t)row0 << 16) + 256 + t * DP;
   unsigned char *q0 = qs + t * Shape<DP>::kOperand;
   const bool qvec = ((uintptr_t)a.q | (uintptr_t)(a.q_tok * 2) | (uintptr_t)(a.q_head * 2)) % 16 == 0;
   uint32_t step = 0, ssteps = 0, items = 0;
   while (true) {
     const Part p = part_of(a, it);
     if (t == 0 || p.two) {
-      const int r = it.tile * kRows + t * kTile + row;
-      const int tok = min(r, p.rows - 1) / a.group;
-      const int head = it.head * a.group + r % a.group;
-      // Q: the row as 16-bit operand; over quantized caches scaled by a power of two into fp16.
-      float qmul = a.scale;
+      const int first = it.tile * kRows + t * kTile + row0;  // the warp's first row
+      // Q: a thread a row, as 16-bit operand; over quantized caches scaled by a power of two into fp16. The
+      // sign of the scale goes into Q; a scale of 0 is replaced by one whose scores vanish but keep -Inf.
+      float qmul = a.scale == 0.0f ? 1.1754943508222875e-38f : fabsf(a.scale);
       {
-        const T *qp = static_cast<const T *>(a.q) + (p.s.q0 + tok) * a.q_tok + head * a.q_head;
+        const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        const int r = first + lane, tok = min(r, p.rows - 1) / a.group;
+        const T *qp = static_cast<const T *>(a.q) + (p.s.q0 + tok) * a.q_tok + (it.head * a.group + r % a.group) * a.q_head;
         uint32_t w[DP / 2];
 #pragma unroll
         for (int g = 0; g < DP / 8; ++g) {
@@ -432,7 +612,7 @@ __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *q
             }
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) w[4 * g + k] = x[k];
+          for (int k = 0; k < 4; ++k) w[4 * g + k] = x[k] ^ flip;
         }
         if (S != KV_NONE) {
           float big = 0.0f;
@@ -447,17 +627,22 @@ __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *q
         }
 #pragma unroll
         for (int g = 0; g < DP / 8; ++g)
-          *reinterpret_cast<uint4 *>(q0 + tile_at(row, g)) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
+          *reinterpret_cast<uint4 *>(q0 + tile_at(row0 + lane, g)) = make_uint4(w[4 * g], w[4 * g + 1], w[4 * g + 2], w[4 * g + 3]);
         fence_async_proxy();
         tc5::fence_before_sync();
-        mbar_arrive(&bar.qfull[t]);
+        warp_arrive(&bar.qfull[t]);
       }
-      int see_lo, see_hi;
-      visible(a, p.s, tok, see_lo, see_hi);
-      const uint64_t qmul2 = pack2(qmul, qmul);
-      float top = -INFINITY;  // maximum that ref follows
-      float ref = 0.0f;       // base-2 logarithm that weights are relative to
-      uint64_t sum2 = 0ull;
+      // From here on a thread works for rows 8 i + g of the warp's 32.
+      // ref: the base-2 logarithm that weights are relative to, `above` below a row's maximum; far below
+      // everything before the row has seen a key (the first one then moves it).
+      float qm[4], ref[4];
+      F2 sum2[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        qm[i] = __shfl_sync(0xFFFFFFFFu, qmul, 8 * i + g4);
+        ref[i] = -3e38f;
+        sum2[i] = pack2(0.0f, 0.0f);
+      }
       int vfield = kBf16 ? 127 : 0;  // exponent field of T
       for (int j = 0; j < p.steps; ++j) {
         const uint32_t n = step + j;
@@ -465,144 +650,118 @@ __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *q
         if (!mbar_wait_sleep(&bar.slot[n % kSlots], (n / kSlots) & 1, polls)) return false;
         if (!mbar_wait(&bar.sfull[t], ssteps++ & 1, polls)) return false;
         tc5::fence_after_sync();
-        const int64_t p0 = p.key0 + (int64_t)j * kKeys;
+        const int p0 = p.key0 + j * kKeys;
         const bool whole = p0 >= p.all_lo && p0 + kKeys <= p.all_hi &&
-                           (sl.valid[0] & sl.valid[1] & sl.valid[2] & sl.valid[3]) == 0xFFFFFFFFu;
-        const int lo = (int)max(min((int64_t)see_lo - p0, (int64_t)kKeys), (int64_t)0);
-        const int hi = (int)max(min((int64_t)see_hi - p0, (int64_t)kKeys), (int64_t)0);
-
-        // The maximum of the row's scores.
-        float m = -INFINITY;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t x[32];
-          tc5::tmem_ld32(ts + 32 * q, x);
-          const uint32_t bits = whole ? 0xFFFFFFFFu : sl.valid[q] & range_bits(lo, hi, q);
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float v[4] = {u2f(x[i]), u2f(x[i + 1]), u2f(x[i + 2]), u2f(x[i + 3])};
-            if (S != KV_NONE) {
-              const float4 k4 = *reinterpret_cast<const float4 *>(&sl.k[32 * q + i]);
-              unpack2(mul2(pack2(v[0], v[1]), pack2(k4.x, k4.y)), v[0], v[1]);
-              unpack2(mul2(pack2(v[2], v[3]), pack2(k4.z, k4.w)), v[2], v[3]);
-            }
-            if (!whole) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (!((bits >> (i + e)) & 1u)) v[e] = qmul >= 0.0f ? -INFINITY : INFINITY;
-            }
-            if (qmul >= 0.0f) m = fmaxf(m, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])));
-            else m = fmaxf(m, -fminf(fminf(v[0], v[1]), fminf(v[2], v[3])));
-          }
-        }
-        m = m == -INFINITY ? m : m * fabsf(qmul);
-        // The reference moves when the maximum has risen by more than 2**8 (or from nothing), and when
-        // a larger value scale comes.
+                           ((sl.valid[0] & ~sl.dead[0]) & (sl.valid[1] & ~sl.dead[1]) & (sl.valid[2] & ~sl.dead[2]) &
+                            (sl.valid[3] & ~sl.dead[3])) == 0xFFFFFFFFu;
         int field = vfield;
         if (!kBf16) field = max(max(field, max(sl.vfield[0], sl.vfield[1])), max(sl.vfield[2], sl.vfield[3]));
-        const bool up = m > top + 8.0f || (top == -INFINITY && m != -INFINITY);
-        if (__any_sync(0xFFFFFFFFu, up) || field != vfield) {
-          const float now = up ? m : top;
-          // exp2(x - ref) <= 2**(8 + 6) / T, at most 2**(8 + 100).
-          const float next = (now == -INFINITY ? 0.0f : now) - fminf(6.0f + (127.0f - (float)field), 100.0f);
-          const float keep = top == -INFINITY ? 0.0f : exp2_fast(ref - next);
-          top = now;
-          ref = next;
-          vfield = field;
-          sum2 = mul2(sum2, pack2(keep, keep));
-          if (j > 0) {
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          // With the reference as it is. It moves when a row's maximum has risen by more than 2**8 (or from
+          // nothing), and when a larger value scale comes, by whole powers of two, so that what it scales
+          // stays exact; the half is then computed again.
+          uint32_t pw[2][kHalf / 4];
+          F2 part2[4];
+          while (true) {
+            Rows x;
+            load_rows(ts + kHalf * half, x);
+            if (!whole) {
+              int lo[4], hi[4];
 #pragma unroll
-            for (int q = 0; q < DP / 32; ++q) {
-              uint32_t x[32];
-              tc5::tmem_ld32(to + 32 * q, x);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) x[i] = f2u(u2f(x[i]) * keep);
-              tc5::tmem_st32(to + 32 * q, x);
-            }
-          }
-        }
-        const uint64_t nref2 = pack2(-ref, -ref);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          uint32_t x[32], w[16];
-          tc5::tmem_ld32(ts + 32 * q, x);
-          const uint32_t bits = whole ? 0xFFFFFFFFu : sl.valid[q] & range_bits(lo, hi, q);
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            uint64_t y0 = pack2(u2f(x[i]), u2f(x[i + 1])), y1 = pack2(u2f(x[i + 2]), u2f(x[i + 3]));
-            if (S != KV_NONE) {
-              const float4 k4 = *reinterpret_cast<const float4 *>(&sl.k[32 * q + i]);
-              y0 = mul2(y0, pack2(k4.x, k4.y));
-              y1 = mul2(y1, pack2(k4.z, k4.w));
-            }
-            y0 = fma2(y0, qmul2, nref2);
-            y1 = fma2(y1, qmul2, nref2);
-            float v[4];
-            unpack2(y0, v[0], v[1]);
-            unpack2(y1, v[2], v[3]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[e] = exp2_fast(v[e]);
-              if (!whole && !((bits >> (i + e)) & 1u)) v[e] = 0.0f;
-            }
-            y0 = pack2(v[0], v[1]);
-            y1 = pack2(v[2], v[3]);
-            sum2 = add2(sum2, add2(y0, y1));
-            if (S != KV_NONE || !whole) {
-              const float4 v4 = *reinterpret_cast<const float4 *>(&sl.v[32 * q + i]);
-              unpack2(mul2(y0, pack2(v4.x, v4.y)), v[0], v[1]);
-              unpack2(mul2(y1, pack2(v4.z, v4.w)), v[2], v[3]);
-              if (!whole) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if (!((bits >> (i + e)) & 1u)) v[e] = 0.0f;  // whatever the scale
+              for (int i = 0; i < 4; ++i) {
+                visible(a, p.s, min(first + 8 * i + g4, p.rows - 1) / a.group, lo[i], hi[i]);
+                lo[i] -= p0 + kHalf * half;
+                hi[i] -= p0 + kHalf * half;
               }
+              mask_rows(x, sl.valid + 2 * half, sl.dead + 2 * half, t4, lo, hi);
             }
-            w[i / 2] = kBf16 ? pack_bf16(v[0], v[1]) : pack_half(v[0], v[1]);
-            w[i / 2 + 1] = kBf16 ? pack_bf16(v[2], v[3]) : pack_half(v[2], v[3]);
+            float m[4];
+            weights<S, kBf16>(x, sl.k + kHalf * half, sl.v + kHalf * half, t4, qm, ref, pw, part2, m);
+            const float above = room(vfield);
+            bool any = field != vfield;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any |= m[i] * qm[i] > ref[i] + (above + 8.0f);
+            if (!__any_sync(0xFFFFFFFFu, any)) break;
+            float keep[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              m[i] = fmaxf(m[i], __shfl_xor_sync(0xFFFFFFFFu, m[i], 1));
+              m[i] = fmaxf(m[i], __shfl_xor_sync(0xFFFFFFFFu, m[i], 2));
+              const float now = m[i] * qm[i] > ref[i] + (above + 8.0f) ? ceilf(m[i] * qm[i]) : ref[i] + above;
+              const float next = now - room(field);
+              keep[i] = exp2_fast(ref[i] - next);
+              ref[i] = next;
+              sum2[i] = mul2(sum2[i], pack2(keep[i], keep[i]));
+            }
+            vfield = field;
+            // Before the second half the first half's products must be in: the next S of the tile, which the
+            // steps above waited for, comes after all of them, but this half does not wait for that.
+            if (half && !mbar_wait(&bar.phalf[t], (ssteps - 1) & 1, polls)) return false;
+            if (half) tc5::fence_after_sync();
+            if (j > 0 || half) rescale<DP>(keep, to);
           }
-          tc5::tmem_st16(ts + 16 * q, w);
+          tc5::tmem_st_pairs64(ts + 32 * half, pw[0]);
+          tc5::tmem_st_pairs64(ts + (16u << 16) + 32 * half, pw[1]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum2[i] = add2(sum2[i], part2[i]);
+          tc5::tmem_wait_st();
+          tc5::fence_before_sync();
+          warp_arrive(&bar.pfull[t][half]);
         }
-        tc5::tmem_wait_st();
-        tc5::fence_before_sync();
-        mbar_arrive(&bar.pfull[t]);
       }
       // The item's part is done.
       if (!mbar_wait_sleep(&bar.ofull[t], items++ & 1, polls)) return false;
       tc5::fence_after_sync();
-      float sum, s1;
-      unpack2(sum2, sum, s1);
-      sum += s1;
       const bool done = it.at == 0 && it.n == it.units;
-      float *part = parts + (size_t)(2 * blockIdx.x + (it.at > 0 ? 0 : 1)) * partial_floats(kRows, DP) + t * kTile + row;
-      const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-      const int64_t out_row = (p.s.q0 + tok) * a.heads + head;
+      float *part = parts + (size_t)(2 * blockIdx.x + (it.at > 0 ? 0 : 1)) * partial_floats(kRows, DP) + t * kTile + row0 + g4;
+#pragma unroll 1
+      for (int h = 0; h < 2; ++h) {
+        float sum[2], inv[2];
+        int64_t out_row[2];
+        bool real[2];
 #pragma unroll
-      for (int q = 0; q < DP / 32; ++q) {
-        uint32_t x[32];
-        tc5::tmem_ld32(to + 32 * q, x);
-        if (!done) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) part[(2 + 32 * q + i) * kRows] = u2f(x[i]);
-        } else if (r < p.rows) {
-          T *o = static_cast<T *>(a.out) + out_row * a.c.dim + 32 * q;
-#pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            if (32 * q + i < a.c.dim) {
-              uint32_t w[4];
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                w[k] = sum == 0.0f ? 0u : pack16<T>(u2f(x[i + 2 * k]) * inv, u2f(x[i + 2 * k + 1]) * inv);
-              *reinterpret_cast<uint4 *>(o + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int i = 0; i < 2; ++i) {
+          float s1;
+          unpack2(h ? sum2[2 + i] : sum2[i], sum[i], s1);
+          const float last = h ? ref[2 + i] : ref[i];
+          sum[i] += s1;
+          sum[i] += __shfl_xor_sync(0xFFFFFFFFu, sum[i], 1);
+          sum[i] += __shfl_xor_sync(0xFFFFFFFFu, sum[i], 2);
+          inv[i] = sum[i] == 0.0f ? 0.0f : 1.0f / sum[i];
+          const int r = first + 16 * h + 8 * i + g4;
+          real[i] = r < p.rows;
+          out_row[i] = (p.s.q0 + min(r, p.rows - 1) / a.group) * a.heads + it.head * a.group + r % a.group;
+          if (t4 == 0) {
+            if (!done) {
+              part[16 * h + 8 * i] = sum[i] == 0.0f ? -INFINITY : last;
+              part[kRows + 16 * h + 8 * i] = sum[i];
+            } else if (a.lse && real[i]) {
+              a.lse[out_row[i]] = sum[i] == 0.0f ? -INFINITY : (last + log2f(sum[i])) * 0.69314718055994531f;
             }
           }
         }
-      }
-      if (!done) {
-        part[0] = sum == 0.0f ? -INFINITY : ref;
-        part[kRows] = sum;
-      } else if (a.lse && r < p.rows) {
-        a.lse[out_row] = sum == 0.0f ? -INFINITY : (ref + log2f(sum)) * 0.69314718055994531f;
+#pragma unroll 1
+        for (int q = 0; q < DP / 32; ++q) {
+          uint32_t o[16];
+          tc5::tmem_ld_frag32(to + (h ? 16u << 16 : 0u) + 32 * q, o);
+          tc5::tmem_wait_ld_frag(o);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int d = 32 * q + 8 * k + 2 * t4;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float v0 = u2f(o[4 * k + 2 * i]), v1 = u2f(o[4 * k + 2 * i + 1]);
+              if (!done) {
+                part[(2 + d) * kRows + 16 * h + 8 * i] = v0;
+                part[(3 + d) * kRows + 16 * h + 8 * i] = v1;
+              } else if (real[i] && d < a.c.dim) {
+                *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out_row[i] * a.c.dim + d) =
+                    sum[i] == 0.0f ? 0u : pack16<T>(v0 * inv[i], v1 * inv[i]);
+              }
+            }
+          }
+        }
       }
       tc5::fence_before_sync();
     }
@@ -641,16 +800,18 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.kfull[i], kProducerWarps * 32);
-      mbar_init(&bar.vfull[i], kProducerWarps * 32);
+      mbar_init(&bar.kfull[i], 4);
+      mbar_init(&bar.vfull[i], 4);
       mbar_init(&bar.kempty[i], 1);
       mbar_init(&bar.vempty[i], 1);
-      mbar_init(&bar.qfull[i], kTile);
-      mbar_init(&bar.pfull[i], kTile);
+      mbar_init(&bar.qfull[i], 4);
+      mbar_init(&bar.pfull[i][0], 4);
+      mbar_init(&bar.pfull[i][1], 4);
       mbar_init(&bar.sfull[i], 1);
+      mbar_init(&bar.phalf[i], 1);
       mbar_init(&bar.ofull[i], 1);
     }
-    for (int i = 0; i < kSlots; ++i) mbar_init(&bar.slot[i], kProducerWarps * 32);
+    for (int i = 0; i < kSlots; ++i) mbar_init(&bar.slot[i], 4);
     mbar_init(&bar.drain, 1);
     fence_barrier_init();
   }
@@ -663,18 +824,23 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
   if (it.n > 0) {
     bool ok = true;
     if (warp < kSoftmaxWarps) {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
       ok = softmax<T, S, DP>(a, it, qs, slots, tmem, bar, polls, parts);
-    } else if (warp < kSoftmaxWarps + kProducerWarps) {
-      ok = produce<T, S, DP>(a, it, ks, vs, slots, bar, polls);
-      cp_async_wait_all();
-    } else if (lane == 0) {
-      bool issued = false;
-      ok = multiply<kBf16, DP>(a, it, smem_addr(qs), smem_addr(ks), smem_addr(vs), tmem, bar, polls, issued);
-      if (issued) {
-        // No MMA may be in flight when the block's shared memory and TMEM go.
-        tc5::mma_commit(&bar.drain);
-        mbar_wait_sleep(&bar.drain, 0);
+    } else {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+      if (warp < kSoftmaxWarps + kProducerWarps) {
+        ok = produce<T, S, DP>(a, it, ks, vs, slots, bar, polls);
+        cp_async_wait_all();
+      } else if (lane == 0) {
+        bool issued = false;
+        ok = multiply<kBf16, DP>(a, it, smem_addr(qs), smem_addr(ks), smem_addr(vs), tmem, bar, polls, issued);
+        if (issued) {
+          // No MMA may be in flight when the block's shared memory and TMEM go.
+          tc5::mma_commit(&bar.drain);
+          mbar_wait_sleep(&bar.drain, 0);
+        }
       }
+      __syncwarp();
     }
     if (!ok) failed = 1;
   }

@@ -76,6 +76,11 @@ __device__ __forceinline__ uint32_t e4m3x2_half2(uint32_t two) {
   asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(r) : "r"(two));
   return r;
 }
+__device__ __forceinline__ void e4m3x4_half2(uint32_t w, uint32_t &lo, uint32_t &hi) {
+  asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
+}
 // Eight codes (code 0 in the low nibble) to four pairs.
 __device__ __forceinline__ void e2m1x8_half2(uint32_t w, uint32_t (&h)[4]) {
   asm("{\n.reg .b8 a, b, c, d;\nmov.b32 {a, b, c, d}, %4;\n"
