@@ -182,15 +182,24 @@ def stream_of(device) -> C.c_void_p:
     return C.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
-def on_device(device):
-    """A context in which ``device`` is current; nothing to enter where it already is."""
+def raw_stream(index: int) -> int:
+    """The current stream of a device as an integer handle, without building a torch Stream object (3 us of a
+    call that takes 20)."""
     import torch
 
-    return _NOTHING if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    fast = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return fast(index) if fast is not None else torch.cuda.current_stream(index).cuda_stream
+
+
+def on_device(index: int):
+    """A context in which the device is current; nothing to enter where it already is."""
+    import torch
+
+    return _NOTHING if torch.cuda.current_device() == index else torch.cuda.device(index)
 
 
 def ptr(t) -> C.c_void_p:
     return C.c_void_p(0 if t is None else t.data_ptr())
 
 
-__all__ = ["lib", "check", "tc_format", "rounding_code", "dtype_code", "stream_of", "on_device", "ptr"]
+__all__ = ["lib", "check", "tc_format", "rounding_code", "dtype_code", "stream_of", "raw_stream", "on_device", "ptr"]

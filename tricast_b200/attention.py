@@ -3,15 +3,13 @@
 
 from __future__ import annotations
 
-import math
-
 import torch
 
 from . import _native as N
 
 
 def _index(t: torch.Tensor, shape, device, name: str) -> None:
-    if t.dtype != torch.int32 or t.device != device or tuple(t.shape) != shape:
+    if t.dtype != torch.int32 or t.device != device or t.shape != shape:
         raise ValueError(f"{name} must be an int32 tensor of shape {list(shape)} on the cache's device")
 
 
@@ -43,7 +41,8 @@ def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens:
     _index(seq_lens, (batch,), device, "seq_lens")
     if cu_q is not None:
         _index(cu_q, (batch + 1,), device, "cu_q")
-        cu_q = cu_q.contiguous()
+        if cu_q.stride(0) != 1:
+            cu_q = cu_q.contiguous()
     elif total != batch:
         raise ValueError("without cu_q every sequence has one new token: q needs as many tokens as block_table rows")
     if window < 0 or (window and not causal):
@@ -56,21 +55,28 @@ def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens:
         max_q_len = 1
     if q.stride(2) != 1:
         q = q.contiguous()
-    if max_pages and block_table.stride(1) != 1:
+    table_stride, one = block_table.stride()
+    if one != 1 and max_pages > 1:
         block_table = block_table.contiguous()
-    seq_lens = seq_lens.contiguous()
+        table_stride = max_pages
+    if seq_lens.stride(0) != 1:
+        seq_lens = seq_lens.contiguous()
     out = torch.empty((total, heads, dim), dtype=q.dtype, device=device)
     lse = torch.empty((total, heads), dtype=torch.float32, device=device) if return_lse else None
     lib = N.lib()
-    with N.on_device(device):
+    index = device.index
+    token_stride, head_stride, _ = q.stride()
+    with N.on_device(index):
         nbytes = lib.tc_paged_attention_workspace(cache._ref, heads, total, batch, max_q_len)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-        N.check(lib.tc_paged_attention(
-            cache._ref, q.data_ptr(), q.stride(0), q.stride(1), total, heads, block_table.data_ptr(),
-            block_table.stride(0), max_pages, seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch,
-            max_q_len, 1.0 / math.sqrt(dim) if scale is None else scale, causal, window, out.data_ptr(),
+        status = lib.tc_paged_attention(
+            cache._ref, q.data_ptr(), token_stride, head_stride, total, heads, block_table.data_ptr(), table_stride,
+            max_pages, seq_lens.data_ptr(), None if cu_q is None else cu_q.data_ptr(), batch, max_q_len,
+            dim ** -0.5 if scale is None else scale, causal, window, out.data_ptr(),
             None if lse is None else lse.data_ptr(), None if ws is None else ws.data_ptr(), nbytes,
-            N.stream_of(device)), "tc_paged_attention")
+            N.raw_stream(index))
+    if status:
+        N.check(status, "tc_paged_attention")
     return (out, lse) if return_lse else out
 
 

@@ -71,6 +71,24 @@ __device__ __forceinline__ float decode_e4m3(uint32_t c) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw((__nv_fp8_storage_t)c, __NV_E4M3)));
 }
 
+// RN(x / s) for finite x without a division: with r = RN(1 / s) a quotient within an ulp or two is corrected
+// twice by its exact remainder (Markstein's theorem: the second step rounds correctly). s in
+// [2**-100, 2**100]; quotients below 2**-60, which every format here rounds to 0, may lose bits.
+__device__ __forceinline__ bool divides_fast(float s) { return s >= 7.888609052210118e-31f && s <= 1.2676506002282294e30f; }
+__device__ __forceinline__ float divide_fast(float x, float s, float r) {
+  float q = __fmul_rn(x, r);
+  q = __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
+  return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
+}
+
+// Codes of two values of magnitude at most a hair above the format's largest (finite): low byte first.
+template <int E>
+__device__ __forceinline__ uint32_t encode8x2(float a, float b) {
+  if (E == E8_INT8)  // the integer in the low bits of a + 1.5 * 2**23, rounded to nearest even by the addition
+    return __byte_perm(f2u(__fadd_rn(a, 12582912.0f)), f2u(__fadd_rn(b, 12582912.0f)), 0x0040) & 0xFFFFu;
+  return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, E == E8_E4M3 ? __NV_E4M3 : __NV_E5M2);
+}
+
 template <typename T>
 struct Io;
 template <>

@@ -36,7 +36,7 @@ class PagedKVCache:
         if num_pages < 1 or not 1 <= kv_heads <= 65535:
             raise ValueError("num_pages and kv_heads must be positive")
         self.num_pages, self.page_size, self.kv_heads, self.head_dim = num_pages, page_size, kv_heads, head_dim
-        self.scheme, self.dtype = scheme, dtype
+        self.scheme, self.dtype, self._row = scheme, dtype, (kv_heads, head_dim)
         device = torch.device(device)
         if device.type != "cuda":
             raise ValueError("the B200 backend requires a CUDA device")
@@ -76,7 +76,7 @@ class PagedKVCache:
         return slots if slots.is_contiguous() else slots.contiguous()
 
     def _rows(self, x: torch.Tensor, tokens: int, name: str) -> torch.Tensor:
-        if x.shape != (tokens, self.kv_heads, self.head_dim) or x.dtype != self.dtype or x.device != self.device:
+        if x.shape != (tokens, *self._row) or x.dtype != self.dtype or x.device != self.device:
             raise ValueError(f"{name} must be [tokens, {self.kv_heads}, {self.head_dim}] of {self.dtype} on the cache's device")
         return x if x.stride(2) == 1 else x.contiguous()
 
@@ -87,9 +87,12 @@ class PagedKVCache:
         slots = self._slots(slots)
         tokens = slots.shape[0]
         k, v = self._rows(k, tokens, "k"), self._rows(v, tokens, "v")
-        with N.on_device(self.device):
-            N.check(N.lib().tc_kv_write(self._ref, k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-                                        v.stride(1), slots.data_ptr(), tokens, N.stream_of(self.device)), "tc_kv_write")
+        ks, vs, index = k.stride(), v.stride(), self.device.index
+        with N.on_device(index):
+            status = N.lib().tc_kv_write(self._ref, k.data_ptr(), ks[0], ks[1], v.data_ptr(), vs[0], vs[1],
+                                         slots.data_ptr(), tokens, N.raw_stream(index))
+        if status:
+            N.check(status, "tc_kv_write")
 
     def read(self, slots: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """The keys and values at ``slots``, dequantized to the cache's dtype: ``[tokens, kv_heads, head_dim]``
@@ -98,9 +101,12 @@ class PagedKVCache:
         tokens = slots.shape[0]
         k = torch.empty((tokens, self.kv_heads, self.head_dim), dtype=self.dtype, device=self.device)
         v = torch.empty_like(k)
-        with N.on_device(self.device):
-            N.check(N.lib().tc_kv_read(self._ref, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(),
-                                       N.stream_of(self.device)), "tc_kv_read")
+        index = self.device.index
+        with N.on_device(index):
+            status = N.lib().tc_kv_read(self._ref, slots.data_ptr(), tokens, k.data_ptr(), v.data_ptr(),
+                                        N.raw_stream(index))
+        if status:
+            N.check(status, "tc_kv_read")
         return k, v
 
 

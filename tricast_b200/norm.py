@@ -11,7 +11,7 @@ from .operand import QTensor
 from .quantize import _qspec
 
 _CODE_DTYPES = {("float", 4): torch.float8_e4m3fn, ("float", 5): torch.float8_e5m2}
-_PREPARED: dict = {}  # spec object -> (it, its C descriptor, code dtype, group size, whether scales are E8M0)
+_PREPARED: dict = {}  # spec object -> (it, its C descriptor, code dtype, group size, scale dtype)
 
 
 def _prepared(spec):
@@ -24,8 +24,20 @@ def _prepared(spec):
         group = spec.group_size if spec.granularity == "group" else 0
         if len(_PREPARED) >= 64:
             _PREPARED.clear()
-        hit = _PREPARED[id(spec)] = (spec, _qspec(spec), code, group, spec.scale.format.kind == "pow2")
+        hit = _PREPARED[id(spec)] = (
+            spec, _qspec(spec), code, group, torch.float8_e8m0fnu if spec.scale.format.kind == "pow2" else torch.float32)
     return hit
+
+
+def _rows(x: torch.Tensor, K: int) -> tuple:
+    """``x`` as rows of K contiguous elements, and their stride."""
+    if x.ndim != 2:
+        x = x.reshape(-1, K)
+    step, one = x.stride()
+    if (one != 1 and K > 1) or step < K:
+        x = x.contiguous()
+        step = K
+    return x, step
 
 
 def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None, spec, *, residual: torch.Tensor | None = None,
@@ -42,42 +54,41 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None, spec, *, res
         from .spec import get_scheme
 
         spec = get_scheme(spec)
-    _, qs, code_dtype, group, e8m0 = _prepared(spec)
+    _, qs, code_dtype, group, scale_dtype = _prepared(spec)
     if not x.is_cuda:
         raise ValueError("the B200 backend requires a CUDA tensor")
-    if x.ndim == 0 or x.numel() == 0:
+    shape = x.shape
+    if not shape or x.numel() == 0:
         raise ValueError("rms_norm_quantize needs a nonempty tensor of shape [..., K]")
     dtype = N.dtype_code(x.dtype)
-    K = x.shape[-1]
+    K = shape[-1]
     device = x.device
-    x2 = x.reshape(-1, K)
-    if x2.stride(1) != 1 and K > 1 or x2.stride(0) < K:
-        x2 = x2.contiguous()
-    rows = x2.shape[0]
-    r2 = None
+    x2, stride = _rows(x, K)
+    r2, rstride = None, K
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != device:
+        if residual.shape != shape or residual.dtype != x.dtype or residual.device != device:
             raise ValueError("residual must have x's shape, dtype and device")
-        r2 = residual.reshape(-1, K)
-        if r2.stride(1) != 1 and K > 1 or r2.stride(0) < K:
-            r2 = r2.contiguous()
+        r2, rstride = _rows(residual, K)
     wdt = 0
     if weight is not None:
         if weight.shape != (K,) or weight.device != device:
             raise ValueError("weight must have shape [K] on x's device")
         wdt = N.dtype_code(weight.dtype)
-        weight = weight.contiguous()
+        if weight.stride(0) != 1:
+            weight = weight.contiguous()
+    rows = x2.shape[0]
     values = torch.empty((rows, K), device=device, dtype=code_dtype)
-    groups = -(-K // group) if group else 1
-    scale = torch.empty((rows, groups), device=device, dtype=torch.float8_e8m0fnu if e8m0 else torch.float32)
-    h = None if r2 is None else torch.empty(x.shape, device=device, dtype=x.dtype)
-    with N.on_device(device):
-        N.check(N.lib().tc_rms_norm_quantize(
-            x2.data_ptr(), None if r2 is None else r2.data_ptr(), dtype, rows, K, x2.stride(0),
-            K if r2 is None else r2.stride(0), None if weight is None else weight.data_ptr(), wdt, eps, qs,
-            values.data_ptr(), scale.data_ptr(), None if h is None else h.data_ptr(), N.stream_of(device)),
-            "tc_rms_norm_quantize")
-    return QTensor(values, scale, None, None, spec, tuple(x.shape)), h
+    scale = torch.empty((rows, -(-K // group) if group else 1), device=device, dtype=scale_dtype)
+    h = None if r2 is None else torch.empty(shape, device=device, dtype=x.dtype)
+    index = device.index
+    with N.on_device(index):
+        status = N.lib().tc_rms_norm_quantize(
+            x2.data_ptr(), None if r2 is None else r2.data_ptr(), dtype, rows, K, stride, rstride,
+            None if weight is None else weight.data_ptr(), wdt, eps, qs, values.data_ptr(), scale.data_ptr(),
+            None if h is None else h.data_ptr(), N.raw_stream(index))
+    if status:
+        N.check(status, "tc_rms_norm_quantize")
+    return QTensor(values, scale, None, None, spec, tuple(shape)), h
 
 
 __all__ = ["rms_norm_quantize"]
