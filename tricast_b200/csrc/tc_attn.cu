@@ -36,10 +36,8 @@ static int launch_split(const Args &a, float *parts, cudaStream_t s) {
                  : a.c.scheme == KV_INT8_ROW ? launch_split_int8(a, parts, most, s)
                                              : launch_split_mxfp4(a, parts, most, s);
   if (st != TC_OK) return st;
-  if (a.c.dtype == TC_BF16) join_kernel<__nv_bfloat16, 16, 64><<<most - 1, 256, 0, s>>>(a, parts, split_width(a.c.dim), most, nullptr);
-  else join_kernel<__half, 16, 64><<<most - 1, 256, 0, s>>>(a, parts, split_width(a.c.dim), most, nullptr);
-  count_launch();
-  return TC_OK;
+  return a.c.dtype == TC_BF16 ? launch_join<__nv_bfloat16, 16, 64>(a, parts, most, nullptr, s)
+                              : launch_join<__half, 16, 64>(a, parts, most, nullptr, s);
 }
 
 // Query rows of one key / value head from which the chunk kernel's tiles of 128 rows pay.
@@ -62,11 +60,8 @@ static int launch_chunk(const Args &a, void *workspace, cudaStream_t s) {
                  : a.c.scheme == KV_INT8_ROW ? launch_chunk_int8(a, parts, status, most, s)
                                              : launch_chunk_mxfp4(a, parts, status, most, s);
   if (st != TC_OK) return st;
-  const dim3 grid(most > 1 ? most - 1 : 1, 8);
-  if (a.c.dtype == TC_BF16) join_kernel<__nv_bfloat16, 256, 128><<<grid, 256, 0, s>>>(a, parts, split_width(a.c.dim), most, status);
-  else join_kernel<__half, 256, 128><<<grid, 256, 0, s>>>(a, parts, split_width(a.c.dim), most, status);
-  count_launch();
-  return TC_OK;
+  return a.c.dtype == TC_BF16 ? launch_join<__nv_bfloat16, 256, 128>(a, parts, most, status, s)
+                              : launch_join<__half, 256, 128>(a, parts, most, status, s);
 }
 
 }  // namespace attn

@@ -282,81 +282,153 @@ __device__ __noinline__ void plain_rows(const Args &a, int64_t warp, int64_t war
   }
 }
 
+// Lets the kernel queued behind this one start (it waits for this one's end before it reads results), and that
+// wait. Without the launch attribute both do nothing.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Merges the partial results of the items that several blocks share. One block for each border between two
-// stretches; it acts if the border is the first inside its item. Elements [dim][row] of an item are spread
-// over the threads and over gridDim.y. Where `status` is given and a block of the kernel before gave up a
-// wait (which takes a fault elsewhere, or a test), everything is computed again by the plain rows.
+// stretches and kJoinRows rows of the item; it acts if the border is the first inside its item. It looks its item
+// up while the kernel before it ends. A row's maxima and sums are read side by side into shared memory (as many
+// parts at a time as it holds), its outputs [dim][row] by four rows a thread. Where `status` is given and a block
+// of the kernel before gave up a wait (which takes a fault elsewhere, or a test), everything is computed again by
+// the plain rows.
+constexpr int kJoinRows = 16, kJoinParts = 128, kJoinThreads = 256;
 template <typename T, int kRows, int kKeys>
-__global__ void __launch_bounds__(256) join_kernel(Args a, const float *parts, int dim_pad, int most, const int *status) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float *parts, int dim_pad, int most, const int *status) {
   using W = Work<kRows, kKeys>;
-  if (status) {
-    int bad = 0;
-    for (int i = threadIdx.x; i < most; i += 256) bad |= status[i];
-    if (__syncthreads_or(bad)) {
-      const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-      plain_rows<T>(a, block * 8 + (threadIdx.x >> 5), (int64_t)gridDim.x * gridDim.y * 8);
-      return;
-    }
-  }
   __shared__ Item item;
   __shared__ int from, upto;
-  __shared__ float top[kRows], scale[kRows];
-  const int c = blockIdx.x + 1;
-  if (threadIdx.x < 32) {
+  __shared__ float part_top[kJoinParts][kJoinRows], part_sum[kJoinParts][kJoinRows];
+  __shared__ float top[kJoinRows], sum[kJoinRows], keep[kJoinRows];
+  const int c = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
     const int64_t total = W::total(a);
     const int n = W::blocks(total, most);
-    if (c >= n) {
-      if (threadIdx.x == 0) upto = 0;
-    } else {
+    if (lane == 0) upto = 0;
+    if (c < n) {
       const int64_t u = W::start(total, c, n);
       const Item it = W::find(a, u);
       const int64_t begin = u - it.at, end = begin + it.units;
-      if (threadIdx.x == 0) {
+      if (lane == 0 && it.at > 0 && W::start(total, c - 1, n) <= begin) {
+        // Blocks whose stretch starts before the item's end; starts grow by at least one unit a block.
+        int64_t k = end * n / total;
+        while (k < n && W::start(total, (int)k, n) < end) ++k;
+        while (k > 0 && W::start(total, (int)k - 1, n) >= end) --k;
         item = it;
         from = c - 1;
-        upto = 0;
-        if (it.at > 0 && W::start(total, c - 1, n) <= begin) {
-          // Blocks whose stretch starts before the item's end; starts grow by at least one unit a block.
-          int64_t k = end * n / total;
-          while (k < n && W::start(total, (int)k, n) < end) ++k;
-          while (k > 0 && W::start(total, (int)k - 1, n) >= end) --k;
-          upto = (int)min(k, (int64_t)n);
-        }
+        upto = (int)min(k, (int64_t)n);
       }
+    }
+  }
+  wait_for_previous();
+  if (status) {
+    int bad = 0;
+    for (int i = threadIdx.x; i < most; i += kJoinThreads) bad |= status[i];
+    if (__syncthreads_or(bad)) {
+      const int64_t block = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
+      plain_rows<T>(a, block * (kJoinThreads / 32) + warp, (int64_t)gridDim.x * gridDim.y * (kJoinThreads / 32));
+      return;
     }
   }
   __syncthreads();
   if (upto == 0) return;
+  const Seq s = sequence(a, item.b);
+  const int row0 = blockIdx.y * kJoinRows, first = item.tile * kRows + row0, rows = s.n * a.group;
+  if (first >= rows) return;
   const size_t size = partial_floats(kRows, dim_pad);
   // The first block left it in its last slot, the others in their first.
-  auto slot = [&](int k) { return parts + (size_t)(2 * k + (k == from ? 1 : 0)) * size; };
-  const Seq s = sequence(a, item.b);
-  for (int r = threadIdx.x; r < kRows; r += 256) {
-    float m = -INFINITY, sum = 0.0f;
-    for (int k = from; k < upto; ++k) m = fmaxf(m, slot(k)[r]);
-    for (int k = from; k < upto; ++k) {
-      const float t = slot(k)[r], l = slot(k)[kRows + r];
-      sum += t == -INFINITY && l == 0.0f ? 0.0f : l * exp2_fast(t - m);
-    }
-    top[r] = m;
-    scale[r] = sum == 0.0f ? 0.0f : 1.0f / sum;
-    const int row = item.tile * kRows + r;
-    if (a.lse && blockIdx.y == 0 && row < s.n * a.group)
-      a.lse[(s.q0 + row / a.group) * a.heads + item.head * a.group + row % a.group] =
-          sum == 0.0f ? -INFINITY : (m + log2f(sum)) * 0.69314718055994531f;
+  auto slot = [&](int k) { return parts + (size_t)(2 * k + (k == from ? 1 : 0)) * size + row0; };
+  if (threadIdx.x < kJoinRows) {
+    top[threadIdx.x] = -INFINITY;
+    sum[threadIdx.x] = 0.0f;
   }
-  __syncthreads();
-  for (int e = blockIdx.y * 256 + threadIdx.x; e < kRows * a.c.dim; e += 256 * gridDim.y) {
-    const int r = e % kRows, d = e / kRows, row = item.tile * kRows + r;
-    if (row >= s.n * a.group) continue;
-    float v = 0.0f;
-    for (int k = from; k < upto; ++k) {
-      const float t = slot(k)[r];
-      if (t != -INFINITY) v += slot(k)[(2 + d) * kRows + r] * exp2_fast(t - top[r]);
+  constexpr int kQuads = kJoinRows / 4, kLanesD = kJoinThreads / kQuads;  // a thread: four rows of every 64th dim
+  const int quad = threadIdx.x % kQuads, d0 = threadIdx.x / kQuads;
+  float4 acc[256 / kLanesD];
+#pragma unroll
+  for (int i = 0; i < 256 / kLanesD; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int k0 = from; k0 < upto; k0 += kJoinParts) {
+    const int n = min(kJoinParts, upto - k0);
+    __syncthreads();
+    for (int i = threadIdx.x; i < n * kJoinRows; i += kJoinThreads) {
+      part_top[i / kJoinRows][i % kJoinRows] = slot(k0 + i / kJoinRows)[i % kJoinRows];
+      part_sum[i / kJoinRows][i % kJoinRows] = slot(k0 + i / kJoinRows)[kRows + i % kJoinRows];
     }
+    __syncthreads();
+    for (int r = warp; r < kJoinRows; r += kJoinThreads / 32) {
+      const float old = top[r];
+      float m = old;
+      for (int k = lane; k < n; k += 32) m = fmaxf(m, part_top[k][r]);
+      for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
+      float l = 0.0f;
+      for (int k = lane; k < n; k += 32) {
+        const float w = part_top[k][r] == -INFINITY ? 0.0f : exp2_fast(part_top[k][r] - m);
+        // A part that saw no key has no weight; one whose scores were all NaN has a NaN sum that stays.
+        l += part_sum[k][r] == 0.0f ? 0.0f : w == 0.0f && part_sum[k][r] == part_sum[k][r] ? 0.0f : part_sum[k][r] * (part_sum[k][r] == part_sum[k][r] ? w : 1.0f);
+        part_top[k][r] = w;
+      }
+      for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
+      if (lane == 0) {
+        const float f = old == -INFINITY ? 0.0f : exp2_fast(old - m);
+        keep[r] = f;
+        sum[r] = sum[r] * f + l;
+        top[r] = m;
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 256 / kLanesD; ++i) {
+      const int d = d0 + i * kLanesD;
+      if (d >= a.c.dim) break;
+      float4 v = acc[i];
+      v.x *= keep[4 * quad], v.y *= keep[4 * quad + 1], v.z *= keep[4 * quad + 2], v.w *= keep[4 * quad + 3];
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) {
+        const float4 o = *reinterpret_cast<const float4 *>(slot(k0 + k) + (size_t)(2 + d) * kRows + 4 * quad);
+        const float *w = &part_top[k][4 * quad];
+        if (w[0] != 0.0f) v.x += o.x * w[0];
+        if (w[1] != 0.0f) v.y += o.y * w[1];
+        if (w[2] != 0.0f) v.z += o.z * w[2];
+        if (w[3] != 0.0f) v.w += o.w * w[3];
+      }
+      acc[i] = v;
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int in = 4 * quad + r, row = first + in;
+    if (row >= rows) continue;
+    const float l = sum[in], inv = l == 0.0f ? 0.0f : 1.0f / l;
     const int64_t out = (s.q0 + row / a.group) * a.heads + item.head * a.group + row % a.group;
-    static_cast<T *>(a.out)[out * a.c.dim + d] = Io<T>::put(v * scale[r]);
+    if (a.lse && d0 == 0) a.lse[out] = l == 0.0f ? -INFINITY : (top[in] + log2f(l)) * 0.69314718055994531f;
+#pragma unroll
+    for (int i = 0; i < 256 / kLanesD; ++i) {
+      const int d = d0 + i * kLanesD;
+      if (d >= a.c.dim) break;
+      const float v = r == 0 ? acc[i].x : r == 1 ? acc[i].y : r == 2 ? acc[i].z : acc[i].w;
+      static_cast<T *>(a.out)[out * a.c.dim + d] = Io<T>::put(v * inv);
+    }
   }
+}
+
+// Queues the join behind the kernel before it, to start as that one ends.
+template <typename T, int kRows, int kKeys>
+inline int launch_join(const Args &a, const float *parts, int most, const int *status, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(most > 1 ? most - 1 : 1, kRows / kJoinRows);
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  const int pad = a.c.dim <= 64 ? 64 : a.c.dim <= 128 ? 128 : 256;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<T, kRows, kKeys>, a, parts, pad, most, status);
+  if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
+  count_launch();
+  return TC_OK;
 }
 
 // Blocks per multiprocessor of the split kernel, and its width of a head.

@@ -819,6 +819,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
   tc5::fence_before_sync();
   __syncthreads();
   tc5::fence_after_sync();
+  let_next_start();
   const Item it = first;
   const uint32_t tmem = tmem_base;
   if (it.n > 0) {

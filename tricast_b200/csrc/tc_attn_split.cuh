@@ -95,6 +95,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
   }
   if (padded) clear();
   __syncthreads();
+  let_next_start();
   Item it = first;
   if (it.n == 0) return;
   const int cpr = c.row_bytes / 16;
