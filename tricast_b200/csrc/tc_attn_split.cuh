@@ -64,7 +64,8 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
   return (w & m) == m || ((w >> 16) & m) == m;
 }
 
-template <typename T, int S, int DP>
+// PAD: head_dim is below DP (the general, slower addressing).
+template <typename T, int S, int DP, bool PAD>
 __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(Args a, float *parts, int most) {
   using P = Shape<S, DP>;
   constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
@@ -74,7 +75,6 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
   __shared__ uint4 qfrag[DP == 256 ? P::kKSteps * 32 : 1];  // Q of wide heads does not fit the registers
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const KvCache &c = a.c;
-  const bool padded = c.dim != DP;
   unsigned char *ring = smem + warp * P::kStages * P::kStage;
   // Columns past head_dim are never copied to: they are zeros.
   auto clear = [&]() {
@@ -93,63 +93,101 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
     }
     if (lane == 0) first = it;
   }
-  if (padded) clear();
+  if (PAD) clear();
   __syncthreads();
   let_next_start();
   Item it = first;
   if (it.n == 0) return;
-  const int cpr = c.row_bytes / 16;
+  const int cpr = c.row_bytes / 16, dim = PAD ? c.dim : DP, row_bytes = PAD ? c.row_bytes : P::kRowBytes;
+  const int scale_bytes = PAD ? c.scale_bytes : P::kScaleBytes;
+  // Where this lane's operands lie in a stage side (the swizzle makes a table of it; rows 8 further are a constant
+  // away where 8 rows are whole swizzle periods).
+  constexpr bool kWide = P::kRowBytes >= 128;
+  auto k_at = [&](int nt, int ch) {
+    const int at = ((kWide ? 0 : nt * 8) + g) * P::kRowBytes + (ch * 4 + t) * P::kLaneBytes;
+    return 16 * granule(at / 16) + at % 16 + (kWide ? nt * 8 * P::kRowBytes : 0);
+  };
+  auto v_at = [&](int k, int part) {
+    const int at = (2 * t + (k & 1) + (kWide ? 0 : 8 * (k >> 1))) * P::kRowBytes + g * P::kVBytes + part * 16;
+    return 16 * granule(at / 16) + at % 16 + (kWide ? 8 * (k >> 1) * P::kRowBytes : 0);
+  };
+  int koff[kWide ? 1 : 2][P::kChunks], voff[kWide ? 2 : 4][P::kVBytes / P::kVPart];
+#pragma unroll
+  for (int nt = 0; nt < (kWide ? 1 : 2); ++nt)
+#pragma unroll
+    for (int ch = 0; ch < P::kChunks; ++ch) koff[nt][ch] = k_at(nt, ch);
+#pragma unroll
+  for (int k = 0; k < (kWide ? 2 : 4); ++k)
+#pragma unroll
+    for (int part = 0; part < P::kVBytes / P::kVPart; ++part) voff[k][part] = v_at(k, part);
   const bool qvec = ((uintptr_t)a.q | (uintptr_t)(a.q_tok * 2) | (uintptr_t)(a.q_head * 2)) % 16 == 0;
 
   while (true) {
     const Seq s = sequence(a, it.b);
     int lo, hi;
     W::keys(a, s, it.tile, lo, hi);
-    const int64_t key0 = (int64_t)lo + (int64_t)it.at * kKeys + warp * kStep;
-    const int64_t key1 = min((int64_t)lo + (int64_t)(it.at + it.n) * kKeys, (int64_t)hi);
-    const int steps = key1 > key0 ? (int)((key1 - key0 + kKeys - 1) / kKeys) : 0;
+    const int key0 = lo + it.at * kKeys + warp * kStep;
+    const int key1 = min(lo + (it.at + it.n) * kKeys, hi);
+    const int steps = key1 > key0 ? (key1 - key0 + kKeys - 1) / kKeys : 0;
     const int *table = a.table + (int64_t)it.b * a.table_stride;
 
     // Page of the half (8 keys: a page's least) of step i, -1 past the keys.
     auto page_at = [&](int i, int half) {
-      const int64_t p = key0 + (int64_t)i * kKeys + 8 * half;
+      const int p = key0 + i * kKeys + 8 * half;
       return p < key1 ? table[p >> c.page_shift] : -1;
     };
-    auto issue = [&](int i, int pg0, int pg1) {
-      unsigned char *st = ring + (i % P::kStages) * P::kStage;
-      const int64_t p0 = key0 + (int64_t)i * kKeys;
-      const int n = (int)min((int64_t)kStep, key1 - p0);
-      int64_t row[2];
-      uint32_t valid = 0;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int pg = half ? pg1 : pg0;
-        const bool ok = pg >= 0 && pg < c.pages;
-        row[half] = ok ? ((((int64_t)pg * c.heads + it.head) << c.page_shift) + ((p0 + 8 * half) & (c.page_size - 1))) : 0;
-        const int here = max(0, min(8, n - 8 * half));
-        if (ok) valid |= ((1u << here) - 1u) << (8 * half);
-      }
+    auto issue = [&](int i, int slot, int pg0, int pg1) {
+      unsigned char *st = ring + slot * P::kStage;
+      const int p0 = key0 + i * kKeys;
+      const int n = min(kStep, key1 - p0);
+      const bool ok0 = pg0 >= 0 && pg0 < c.pages, ok1 = pg1 >= 0 && pg1 < c.pages;
+      const int64_t row0 = ok0 ? (((int64_t)pg0 * c.heads + it.head) << c.page_shift) + (p0 & (c.page_size - 1)) : 0;
+      const int64_t row1 = ok1 ? (((int64_t)pg1 * c.heads + it.head) << c.page_shift) + ((p0 + 8) & (c.page_size - 1)) : 0;
+      const uint32_t valid = (ok0 ? (1u << min(n, 8)) - 1u : 0u) | (ok1 ? ((1u << max(n - 8, 0)) - 1u) << 8 : 0u);
+      const bool all = valid == 0xFFFFu;
 #pragma unroll
       for (int side = 0; side < 2; ++side) {
         const unsigned char *src = side ? c.v : c.k;
         unsigned char *dst = st + side * P::kSide;
+        // Granule lane + 32 j of the 16 rows, which are contiguous by halves.
+        constexpr int kCount = P::kSide / 16, kHalf = kCount / 2;
+        if (!PAD) {
+          const unsigned char *s0 = src + row0 * row_bytes + lane * 16, *s1 = src + (row1 - 8) * row_bytes + lane * 16;
+          unsigned char *d = dst + 16 * granule(lane), *dx = dst + 16 * (granule(lane) ^ 4);
+          if (all) {
 #pragma unroll
-        for (int j = 0; j < (P::kSide / 16 + 31) / 32; ++j) {
-          const int i16 = lane + 32 * j;
-          const int r = padded ? i16 / cpr : i16 / (P::kRowBytes / 16);
-          const int ch = padded ? i16 - r * cpr : i16 % (P::kRowBytes / 16);
-          if (r < kStep)
+            for (int j = 0; j < (kCount + 31) / 32; ++j) {
+              const bool second = kHalf >= 32 ? 32 * j >= kHalf : lane + 32 * j >= kHalf;
+              if (kCount >= 32 || lane < kCount) cp_async16((j & 1 ? dx : d) + 512 * j, (second ? s1 : s0) + 512 * j);
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < (kCount + 31) / 32; ++j) {
+              const bool second = kHalf >= 32 ? 32 * j >= kHalf : lane + 32 * j >= kHalf;
+              const int r = (lane + 32 * j) / (P::kRowBytes / 16);
+              if (kCount >= 32 || lane < kCount) {
+                const bool use = (valid >> r) & 1u;
+                cp_async16_or_zero((j & 1 ? dx : d) + 512 * j, use ? (second ? s1 : s0) + 512 * j : src, use);
+              }
+            }
+          }
+        } else {
+          for (int i16 = lane; i16 < kStep * cpr; i16 += 32) {
+            const int r = i16 / cpr, ch = i16 - r * cpr;
+            const bool use = (valid >> r) & 1u;
             cp_async16_or_zero(dst + 16 * granule(r * (P::kRowBytes / 16) + ch),
-                               src + ((r >> 3 ? row[1] : row[0]) + (r & 7)) * c.row_bytes + 16 * ch, (valid >> r) & 1u);
+                               use ? src + ((r >> 3 ? row1 : row0) + (r & 7)) * row_bytes + 16 * ch : src, use);
+          }
         }
         if (S != KV_NONE) {
           // The scales of 8 rows are contiguous and 4-byte aligned, whatever one row's count.
           const unsigned char *ss = side ? c.vs : c.ks;
           unsigned char *sd = st + 2 * P::kSide + side * P::kScales;
-          const int words = 2 * c.scale_bytes;
+          const int words = 2 * scale_bytes;
+#pragma unroll
           for (int w = lane; w < 2 * words; w += 32) {
-            const int half = w >= words;
-            cp_async4_or_zero(sd + 4 * w, ss + (half ? row[1] : row[0]) * c.scale_bytes + 4 * (w - half * words), (valid >> (8 * half)) & 1u);
+            const bool half = w >= words, use = half ? ok1 && n > 8 : ok0;
+            cp_async4_or_zero(sd + 4 * w, use ? ss + (half ? row1 : row0) * scale_bytes + 4 * (w - (half ? words : 0)) : ss, use);
           }
         }
       }
@@ -158,7 +196,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
 
     int pre0 = -1, pre1 = -1;  // the pages of the next step to issue, fetched a step before they are needed
     for (int i = 0; i < P::kStages - 1; ++i) {
-      if (i < steps) issue(i, page_at(i, 0), page_at(i, 1));
+      if (i < steps) issue(i, i, page_at(i, 0), page_at(i, 1));
       cp_async_commit();
     }
     if (P::kStages - 1 < steps) {
@@ -183,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
         for (int e = 0; e < P::kLaneDims; e += 8) {
           const int d = (ch * 4 + t) * P::kLaneDims + e;
           uint32_t w[4] = {0u, 0u, 0u, 0u};
-          if (r < rows && d < c.dim) {
+          if (r < rows && d < dim) {
             if (qvec) {
               load_words<4>(reinterpret_cast<const unsigned char *>(qp + d), w);
             } else {
@@ -234,19 +272,19 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
     float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
     int vfield = 254;  // exponent field of 2**14 / T (what the weights are multiplied by)
 
-    for (int i = 0; i < steps; ++i) {
+    for (int i = 0, slot = 0; i < steps; ++i, slot = slot + 1 == P::kStages ? 0 : slot + 1) {
       if (i + P::kStages - 1 < steps) {
-        issue(i + P::kStages - 1, pre0, pre1);
+        issue(i + P::kStages - 1, slot == 0 ? P::kStages - 1 : slot - 1, pre0, pre1);
         pre0 = page_at(i + P::kStages, 0);
         pre1 = page_at(i + P::kStages, 1);
       }
       cp_async_commit();
       cp_async_wait<P::kStages - 1>();
       __syncwarp();
-      const unsigned char *st = ring + (i % P::kStages) * P::kStage;
+      const unsigned char *st = ring + slot * P::kStage;
       const unsigned char *kscales = st + 2 * P::kSide, *vscales = kscales + P::kScales;
       const uint32_t valid = *reinterpret_cast<const uint32_t *>(st + P::kStage - 16);
-      const int64_t p0 = key0 + (int64_t)i * kKeys;
+      const int p0 = key0 + i * kKeys;
 
       // Scores: x[nt][e] is key nt * 8 + 2 t + (e & 1), row g + 8 (e >> 1).
       float x[2][4], vscale[2][2];
@@ -259,16 +297,15 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
         if (S == KV_MXFP4) {
 #pragma unroll
           for (int q = 0; q < P::kScaleBytes; ++q)
-            if (q < c.scale_bytes) big = max(big, (int)kscales[r * c.scale_bytes + q]);
+            if (q < scale_bytes) big = max(big, (int)kscales[r * scale_bytes + q]);
         }
 #pragma unroll
         for (int ch = 0; ch < P::kChunks; ++ch) {
           uint32_t w[P::kLaneBytes / 4], gmul = 0u;
-          const int at = r * P::kRowBytes + (ch * 4 + t) * P::kLaneBytes;
-          load_words<P::kLaneBytes / 4>(st + 16 * granule(at / 16) + at % 16, w);
+          load_words<P::kLaneBytes / 4>(st + koff[kWide ? 0 : nt][ch] + (kWide ? nt * 8 * P::kRowBytes : 0), w);
           if (S == KV_MXFP4) {
             const int grp = (ch * 4 + t) * P::kLaneDims / 32;
-            if (grp < c.scale_bytes) gmul = half_pow2((int)kscales[r * c.scale_bytes + grp] - big + kGroupShift) * 0x10001u;
+            if (grp < scale_bytes) gmul = half_pow2((int)kscales[r * scale_bytes + grp] - big + kGroupShift) * 0x10001u;
           }
 #pragma unroll
           for (int k = 0; k < P::kLaneDims / 4; ++k) {
@@ -281,8 +318,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
               b0 = mul_half2(h[2 * (k & 1)], gmul);
               b1 = mul_half2(h[2 * (k & 1) + 1], gmul);
             } else if (S == KV_FP8_ROW) {
-              b0 = e4m3x2_half2(w[k % (P::kLaneBytes / 4)] & 0xFFFFu);
-              b1 = e4m3x2_half2(w[k % (P::kLaneBytes / 4)] >> 16);
+              e4m3x4_half2(w[k % (P::kLaneBytes / 4)], b0, b1);
             } else {
               const uint32_t u = w[k % (P::kLaneBytes / 4)] ^ 0x80808080u;
               b0 = int8x2_half2<0x4140>(u);
@@ -307,9 +343,9 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
             int bk = 0, bv = 0;
 #pragma unroll
             for (int q = 0; q < P::kScaleBytes; ++q)
-              if (q < c.scale_bytes) {
-                bk = max(bk, (int)kscales[key * c.scale_bytes + q]);
-                bv = max(bv, (int)vscales[key * c.scale_bytes + q]);
+              if (q < scale_bytes) {
+                bk = max(bk, (int)kscales[key * scale_bytes + q]);
+                bv = max(bv, (int)vscales[key * scale_bytes + q]);
               }
             ks = pow2_value(bk) * (1.0f / (1 << kGroupShift));
             vscale[nt][e] = pow2_value(bv);
@@ -429,13 +465,13 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
       uint32_t vm0 = 0u, vm1 = 0u;
       if (S == KV_MXFP4) {
         const int grp = g * (DP / 8) / 32;
-        if (grp < c.scale_bytes) {
+        if (grp < scale_bytes) {
           uint32_t m[2][2];
 #pragma unroll
           for (int nt = 0; nt < 2; ++nt)
 #pragma unroll
             for (int e = 0; e < 2; ++e)
-              m[nt][e] = half_pow2((int)vscales[(nt * 8 + 2 * t + e) * c.scale_bytes + grp] - vbig[nt][e] + kGroupShift);
+              m[nt][e] = half_pow2((int)vscales[(nt * 8 + 2 * t + e) * scale_bytes + grp] - vbig[nt][e] + kGroupShift);
           vm0 = m[0][0] | (m[0][1] << 16);
           vm1 = m[1][0] | (m[1][1] << 16);
         }
@@ -446,8 +482,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const int key = 2 * t + (k & 1) + 8 * (k >> 1);
-          const int at = key * P::kRowBytes + g * P::kVBytes + part * 16;
-          load_words<P::kVPart / 4>(st + P::kSide + 16 * granule(at / 16) + at % 16, w[k]);
+          load_words<P::kVPart / 4>(st + P::kSide + voff[kWide ? k & 1 : k][part] + (kWide ? 8 * (k >> 1) * P::kRowBytes : 0), w[k]);
           if (nan_keys)
 #pragma unroll
             for (int q = 0; q < P::kVPart / 4; ++q)
@@ -482,8 +517,11 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
               const uint32_t ab = __byte_perm(w[0][q], w[1][q], k ? 0x7362 : 0x5140);
               const uint32_t cd = __byte_perm(w[2][q], w[3][q], k ? 0x7362 : 0x5140);
               if (S == KV_FP8_ROW) {
-                mma16<false>(o[j + 2 * k], pf, e4m3x2_half2(ab & 0xFFFFu), e4m3x2_half2(cd & 0xFFFFu));
-                mma16<false>(o[j + 2 * k + 1], pf, e4m3x2_half2(ab >> 16), e4m3x2_half2(cd >> 16));
+                uint32_t h[4];
+                e4m3x4_half2(ab, h[0], h[1]);
+                e4m3x4_half2(cd, h[2], h[3]);
+                mma16<false>(o[j + 2 * k], pf, h[0], h[2]);
+                mma16<false>(o[j + 2 * k + 1], pf, h[1], h[3]);
               } else {
                 const uint32_t u0 = ab ^ 0x80808080u, u1 = cd ^ 0x80808080u;
                 mma16<false>(o[j + 2 * k], pf, int8x2_half2<0x4140>(u0), int8x2_half2<0x4140>(u1));
@@ -531,13 +569,13 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
     const int r = it.tile * kRows + row;
     const int64_t out_row = (s.q0 + r / a.group) * a.heads + it.head * a.group + r % a.group;
     const float inv = total == 0.0f ? 0.0f : 1.0f / total;
-    for (int d = threadIdx.x / kRows; d < c.dim; d += kThreads / kRows) {
+    for (int d = threadIdx.x / kRows; d < dim; d += kThreads / kRows) {
       float v = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w)
         if (weight[w] != 0.0f) v += reinterpret_cast<const float *>(smem)[(w * DP + d) * kRows + row] * weight[w];
       if (!done) part[(2 + d) * kRows + row] = v;
-      else if (r < rows) static_cast<T *>(a.out)[out_row * c.dim + d] = Io<T>::put(v * inv);
+      else if (r < rows) static_cast<T *>(a.out)[out_row * dim + d] = Io<T>::put(v * inv);
     }
     if (threadIdx.x < kRows) {
       if (!done) {
@@ -549,15 +587,15 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
     }
     __syncthreads();
     if (it.left == 0) return;
-    if (padded) clear();
+    if (PAD) clear();
     W::next(a, it);
   }
 }
 
-template <typename T, int S, int DP>
-int launch(const Args &a, float *parts, int most, cudaStream_t s) {
+template <typename T, int S, int DP, bool PAD>
+int launch_pad(const Args &a, float *parts, int most, cudaStream_t s) {
   using P = Shape<S, DP>;
-  auto kern = split_kernel<T, S, DP>;
+  auto kern = split_kernel<T, S, DP, PAD>;
   static std::atomic<uint64_t> ready[2];  // devices whose shared-memory limit is raised
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -570,6 +608,11 @@ int launch(const Args &a, float *parts, int most, cudaStream_t s) {
   kern<<<most, kThreads, P::kSmem, s>>>(a, parts, most);
   count_launch();
   return TC_OK;
+}
+
+template <typename T, int S, int DP>
+int launch(const Args &a, float *parts, int most, cudaStream_t s) {
+  return a.c.dim == DP ? launch_pad<T, S, DP, false>(a, parts, most, s) : launch_pad<T, S, DP, true>(a, parts, most, s);
 }
 
 template <int S>

@@ -70,12 +70,7 @@ __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Two codes to two fp16 values, exactly; the low code to the low half.
-__device__ __forceinline__ uint32_t e4m3x2_half2(uint32_t two) {
-  uint32_t r;
-  asm("{\n.reg .b16 t;\ncvt.u16.u32 t, %1;\ncvt.rn.f16x2.e4m3x2 %0, t;\n}" : "=r"(r) : "r"(two));
-  return r;
-}
+// Four codes to two pairs of fp16 values, exactly; the low code to the low half of the first.
 __device__ __forceinline__ void e4m3x4_half2(uint32_t w, uint32_t &lo, uint32_t &hi) {
   asm("{\n.reg .b16 a, b;\nmov.b32 {a, b}, %2;\ncvt.rn.f16x2.e4m3x2 %0, a;\ncvt.rn.f16x2.e4m3x2 %1, b;\n}"
       : "=r"(lo), "=r"(hi)
