@@ -14,9 +14,9 @@ __global__ void __launch_bounds__(kThreads) plain_kernel(Args a) {
   plain_rows<T>(a, (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5), (int64_t)gridDim.x * (kThreads / 32));
 }
 
-int launch_split_none(const Args &a, float *parts, int most, cudaStream_t s);
-int launch_split_fp8(const Args &a, float *parts, int most, cudaStream_t s);
-int launch_split_int8(const Args &a, float *parts, int most, cudaStream_t s);
+int launch_split_none(const Args &a, float *parts, int sms, cudaStream_t s);
+int launch_split_fp8(const Args &a, float *parts, int sms, cudaStream_t s);
+int launch_split_int8(const Args &a, float *parts, int sms, cudaStream_t s);
 int launch_split_mxfp4(const Args &a, float *parts, int most, cudaStream_t s);
 
 int launch_chunk_none(const Args &a, float *parts, int *status, int most, cudaStream_t s);
@@ -24,20 +24,12 @@ int launch_chunk_fp8(const Args &a, float *parts, int *status, int most, cudaStr
 int launch_chunk_int8(const Args &a, float *parts, int *status, int most, cudaStream_t s);
 int launch_chunk_mxfp4(const Args &a, float *parts, int *status, int most, cudaStream_t s);
 
-// Blocks of the split kernel: as many as run at once.
-static int split_blocks(const KvCache &c) {
-  return sm_count() * (c.scheme == KV_NONE && split_width(c.dim) == 256 ? 1 : 2);
-}
-
 static int launch_split(const Args &a, float *parts, cudaStream_t s) {
-  const int most = split_blocks(a.c);
-  const int st = a.c.scheme == KV_NONE       ? launch_split_none(a, parts, most, s)
-                 : a.c.scheme == KV_FP8_ROW  ? launch_split_fp8(a, parts, most, s)
-                 : a.c.scheme == KV_INT8_ROW ? launch_split_int8(a, parts, most, s)
-                                             : launch_split_mxfp4(a, parts, most, s);
-  if (st != TC_OK) return st;
-  return a.c.dtype == TC_BF16 ? launch_join<__nv_bfloat16, 16, 64>(a, parts, most, nullptr, s)
-                              : launch_join<__half, 16, 64>(a, parts, most, nullptr, s);
+  const int sms = sm_count();
+  return a.c.scheme == KV_NONE       ? launch_split_none(a, parts, sms, s)
+         : a.c.scheme == KV_FP8_ROW  ? launch_split_fp8(a, parts, sms, s)
+         : a.c.scheme == KV_INT8_ROW ? launch_split_int8(a, parts, sms, s)
+                                     : launch_split_mxfp4(a, parts, sms, s);
 }
 
 // Query rows of one key / value head from which the chunk kernel's tiles of 128 rows pay.
@@ -45,7 +37,8 @@ constexpr int64_t kChunkRows = 65;
 static bool use_chunk(const KvCache &c, int group, int64_t max_q) { return c.dim <= 128 && max_q * group >= kChunkRows; }
 
 static size_t split_bytes(const KvCache &c) {
-  return 2 * (size_t)split_blocks(c) * partial_floats(16, split_width(c.dim)) * sizeof(float);
+  // At most four blocks an SM of 8 rows, or as many rows in fewer blocks (split::Shape).
+  return 2 * (size_t)sm_count() * 4 * partial_floats(16, split_width(c.dim)) * sizeof(float);
 }
 static size_t chunk_bytes(const KvCache &c) {
   return 2 * (size_t)sm_count() * partial_floats(256, split_width(c.dim)) * sizeof(float);

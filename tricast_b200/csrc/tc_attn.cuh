@@ -200,6 +200,10 @@ struct Work {
   static __device__ __forceinline__ int64_t start(int64_t total, int c, int n) { return total * c / n; }
 };
 
+// How far a row's reference stays below its maximum: exp2(x - ref) <= 2**(8 + 6) / T, at most 2**(8 + 100), for T
+// of this exponent field.
+__device__ __forceinline__ float room(int field) { return fminf(6.0f + (127.0f - (float)field), 100.0f); }
+
 // One partial result: kRows maxima (base-2 logarithms), kRows sums, then [dim][kRows] outputs.
 __host__ __device__ constexpr size_t partial_floats(int rows, int dim) { return (size_t)rows * (dim + 2); }
 
@@ -288,15 +292,17 @@ __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Merges the partial results of the items that several blocks share. One block for each border between two
-// stretches and kJoinRows rows of the item; it acts if the border is the first inside its item. It looks its item
+// stretches and 8 or 16 rows of the item; it acts if the border is the first inside its item. It looks its item
 // up while the kernel before it ends. A row's maxima and sums are read side by side into shared memory (as many
 // parts at a time as it holds), its outputs [dim][row] by four rows a thread. Where `status` is given and a block
 // of the kernel before gave up a wait (which takes a fault elsewhere, or a test), everything is computed again by
 // the plain rows.
-constexpr int kJoinRows = 16, kJoinParts = 128, kJoinThreads = 256;
+constexpr int kJoinParts = 128, kJoinThreads = 256;
+constexpr int join_rows(int rows) { return rows < 16 ? rows : 16; }  // of an item, a block
 template <typename T, int kRows, int kKeys>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float *parts, int dim_pad, int most, const int *status) {
   using W = Work<kRows, kKeys>;
+  constexpr int kJoinRows = join_rows(kRows);
   __shared__ Item item;
   __shared__ int from, upto;
   __shared__ float part_top[kJoinParts][kJoinRows], part_sum[kJoinParts][kJoinRows];
@@ -345,9 +351,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
   }
   constexpr int kQuads = kJoinRows / 4, kLanesD = kJoinThreads / kQuads;  // a thread: four rows of every 64th dim
   const int quad = threadIdx.x % kQuads, d0 = threadIdx.x / kQuads;
-  float4 acc[256 / kLanesD];
+  constexpr int kDims = (256 + kLanesD - 1) / kLanesD;
+  float4 acc[kDims];
 #pragma unroll
-  for (int i = 0; i < 256 / kLanesD; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i = 0; i < kDims; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int k0 = from; k0 < upto; k0 += kJoinParts) {
     const int n = min(kJoinParts, upto - k0);
     __syncthreads();
@@ -378,7 +385,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 256 / kLanesD; ++i) {
+    for (int i = 0; i < kDims; ++i) {
       const int d = d0 + i * kLanesD;
       if (d >= a.c.dim) break;
       float4 v = acc[i];
@@ -403,7 +410,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
     const int64_t out = (s.q0 + row / a.group) * a.heads + item.head * a.group + row % a.group;
     if (a.lse && d0 == 0) a.lse[out] = l == 0.0f ? -INFINITY : (top[in] + log2f(l)) * 0.69314718055994531f;
 #pragma unroll
-    for (int i = 0; i < 256 / kLanesD; ++i) {
+    for (int i = 0; i < kDims; ++i) {
       const int d = d0 + i * kLanesD;
       if (d >= a.c.dim) break;
       const float v = r == 0 ? acc[i].x : r == 1 ? acc[i].y : r == 2 ? acc[i].z : acc[i].w;
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
 template <typename T, int kRows, int kKeys>
 inline int launch_join(const Args &a, const float *parts, int most, const int *status, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(most > 1 ? most - 1 : 1, kRows / kJoinRows);
+  cfg.gridDim = dim3(most > 1 ? most - 1 : 1, kRows / join_rows(kRows));
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = s;
   cudaLaunchAttribute at[1];

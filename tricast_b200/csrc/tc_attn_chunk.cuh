@@ -573,10 +573,6 @@ __device__ __forceinline__ void rescale(const float (&keep)[4], uint32_t to) {
   }
 }
 
-// How far a row's reference stays below its maximum: exp2(x - ref) <= 2**(8 + 6) / T, at most 2**(8 + 100), for T
-// of this exponent field.
-__device__ __forceinline__ float room(int field) { return fminf(6.0f + (127.0f - (float)field), 100.0f); }
-
 template <typename T, int S, int DP>
 __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *qs, const KeySlot *slots, uint32_t tmem,
                                         Barriers &bar, int polls, float *parts) {

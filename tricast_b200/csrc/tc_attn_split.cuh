@@ -1,21 +1,22 @@
 // Attention of few query rows over a long paged cache (decode steps, drafted tokens): bound by the bytes of
 // the codes, which are read once.
 //
-// A block takes a stretch of the work line (tc_attn.cuh) in items of 16 query rows, one tensor-core tile,
-// and units of 64 keys, 16 for each of its four warps. A warp runs alone through its keys: asynchronous
-// copies bring 16 rows of K and V codes into its own ring of shared-memory stages, several steps ahead, and
-// codes go from there to registers as the operands of m16n8k16 MMAs. No step needs another warp or a
-// transposed copy:
-//  - K is the MMA's B operand with one key a column. The order of the summed index is free as long as Q has
-//    the same, so lane t of a quad reads 16 contiguous bytes of its key and Q is laid out to match.
-//  - V is the B operand with the keys summed over: a register holds one element of two keys. Lane g reads
-//    the same bytes of four keys and interleaves them; the order of V's columns is free too, so its bytes
-//    are contiguous again (column n of MMA tile j is dim n * DP / 8 + j).
-// Codes are exact in fp16 (E4M3, INT8, E2M1 times a power of two), so scales stay out of the products: a
-// key's scale multiplies its score, a value's scale its weight. Q is scaled per row by a power of two into
-// fp16's range. Weights are fp16 too, as p * scale * 2**14 / T with T the power of two of the largest scale
-// so far: 11 bits down to 2**-28 of the largest product. Unquantized rows use their own type; bf16 ones get
-// bf16 weights.
+// A block takes a stretch of the work line (tc_attn.cuh) in items of 8 or 16 query rows and units of 64 keys,
+// 16 for each of its four warps. A warp runs alone through its keys: asynchronous copies bring 16 rows of K and V
+// codes into its own ring of shared-memory stages, several steps ahead, and codes go from there to registers as
+// the left operands of m16n8k16 MMAs, keys and elements in rows and queries in columns, so that 8 query rows fill
+// them: S^T = K Q^T and O^T = V^T P^T. No step needs another warp or a transposed copy:
+//  - K has one key a row. The order of the summed index is free as long as Q has the same, so lane t of a quad
+//    reads 16 contiguous bytes of its key and Q is laid out to match.
+//  - V^T has one element a row, the keys summed over: a register holds one element of two keys. Lane g reads the
+//    same bytes of four keys and interleaves them; the order of V's elements is free too, so its bytes are
+//    contiguous again (rows g and g + 8 of MMA i are elements g * DP / 8 + 2 i and + 1).
+//  - P^T is S^T transposed by 8 x 8 (movmatrix).
+// Codes are exact in fp16 (E4M3, INT8, E2M1 times a power of two), so scales stay out of the products: a key's
+// scale multiplies its score, a value's scale its weight. Q is scaled per row by a power of two into fp16's
+// range. Weights are relative to a reference that follows a row's maximum only when it has risen by more than
+// 2**8, and the largest value scale so far, as in the chunk kernel (tc_attn_chunk.cuh), so a step votes once and
+// reduces nothing. Unquantized rows use their own type; bf16 ones get bf16 weights.
 #pragma once
 
 #include <atomic>
@@ -29,19 +30,22 @@ namespace tc {
 namespace attn {
 namespace split {
 
-constexpr int kRows = 16, kStep = 16, kWarps = 4, kKeys = kStep * kWarps, kThreads = kWarps * 32;
-using W = Work<kRows, kKeys>;
+constexpr int kStep = 16, kWarps = 4, kKeys = kStep * kWarps, kThreads = kWarps * 32;
 
-template <int S, int DP>
+template <int S, int DP, int NR>
 struct Shape {
+  static constexpr int kRows = 8 * NR;
   static constexpr int kRowBytes = S == KV_NONE ? 2 * DP : S == KV_MXFP4 ? DP / 2 : DP;  // a row in a stage
   static constexpr int kScaleBytes = S == KV_NONE ? 0 : S == KV_MXFP4 ? DP / 32 : 4;
   static constexpr int kSide = kStep * kRowBytes;
   static constexpr int kScales = (kStep * kScaleBytes + 15) / 16 * 16;
   static constexpr int kStage = 2 * kSide + 2 * kScales + 16;  // K codes, V codes, K scales, V scales, key mask
-  // As deep as two blocks fit an SM with (one for unquantized rows of 256): the ring covers HBM's latency.
-  static constexpr int kBlocks = S == KV_NONE && DP == 256 ? 1 : 2;
-  static constexpr int kFit = (kBlocks == 1 ? 200 : 104) * 1024 / (kWarps * kStage);
+  // Blocks an SM: as many as the registers allow (outputs and queries take DP / 2 * NR of a thread's), and the
+  // ring as deep as they fit its 227 KB: it covers HBM's latency.
+  static constexpr int kRegs = DP * NR <= 64 ? 4 : DP * NR <= 128 ? 4 : DP * NR <= 256 ? 2 : 1;
+  static constexpr int kRoom = kRowBytes <= 128 ? 4 : kRowBytes <= 256 ? 2 : 1;
+  static constexpr int kBlocks = kRegs < kRoom ? kRegs : kRoom;
+  static constexpr int kFit = (kBlocks == 4 ? 54 : kBlocks == 2 ? 108 : 200) * 1024 / (kWarps * kStage);
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kMerge = kWarps * kRows * DP * 4;  // the warps' outputs, over the ring
@@ -65,14 +69,23 @@ __device__ __forceinline__ bool not_finite2(uint32_t w) {
 }
 
 // PAD: head_dim is below DP (the general, slower addressing).
-template <typename T, int S, int DP, bool PAD>
-__global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(Args a, float *parts, int most) {
-  using P = Shape<S, DP>;
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+  return r;
+}
+
+template <typename T, int S, int DP, int NR, bool PAD>
+__global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_kernel(Args a, float *parts, int most) {
+  using P = Shape<S, DP, NR>;
+  constexpr int kRows = P::kRows;
+  using W = Work<kRows, kKeys>;
   constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Item first;
   __shared__ float merge_top[kWarps][kRows], merge_sum[kWarps][kRows];
-  __shared__ uint4 qfrag[DP == 256 ? P::kKSteps * 32 : 1];  // Q of wide heads does not fit the registers
+  constexpr bool kSharedQ = DP * NR > 256;  // Q does not fit the registers
+  __shared__ uint4 qfrag[kSharedQ ? P::kKSteps * 32 : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const KvCache &c = a.c;
   unsigned char *ring = smem + warp * P::kStages * P::kStage;
@@ -120,6 +133,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
   for (int k = 0; k < (kWide ? 2 : 4); ++k)
 #pragma unroll
     for (int part = 0; part < P::kVBytes / P::kVPart; ++part) voff[k][part] = v_at(k, part);
+  const uint32_t flip_q = a.scale < 0.0f ? 0x80008000u : 0u;  // the scale's sign goes into Q
   const bool qvec = ((uintptr_t)a.q | (uintptr_t)(a.q_tok * 2) | (uintptr_t)(a.q_head * 2)) % 16 == 0;
 
   while (true) {
@@ -204,16 +218,14 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
       pre1 = page_at(P::kStages - 1, 1);
     }
 
-    // Q: lane (g, t) holds rows g and g + 8 at the dims its K bytes cover; rows past the last are zero.
+    // Q: lane (g, t) holds rows g (and g + 8) at the dims its K bytes cover; rows past the last are zero.
     const int rows = s.n * a.group;
-    uint32_t qf[P::kKSteps][4];
-    float qmul[2];
-    int tok[2];
+    uint32_t qf[P::kKSteps][2 * NR];
+    float qmul[NR][2];  // of rows 8 r + 2 t and + 1, whose scores this lane gets
 #pragma unroll
-    for (int hrow = 0; hrow < 2; ++hrow) {
-      const int r = it.tile * kRows + g + 8 * hrow;
-      tok[hrow] = min(r, rows - 1) / a.group;
-      const T *qp = static_cast<const T *>(a.q) + (s.q0 + tok[hrow]) * a.q_tok + (it.head * a.group + r % a.group) * a.q_head;
+    for (int nr = 0; nr < NR; ++nr) {
+      const int r = it.tile * kRows + g + 8 * nr, tok = min(r, rows - 1) / a.group;
+      const T *qp = static_cast<const T *>(a.q) + (s.q0 + tok) * a.q_tok + (it.head * a.group + r % a.group) * a.q_head;
       float big = 0.0f;
 #pragma unroll
       for (int ch = 0; ch < P::kChunks; ++ch)
@@ -232,45 +244,56 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
           }
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            qf[(ch * P::kLaneDims + e) / 4 + (k >> 1)][hrow + 2 * (k & 1)] = w[k];
+            qf[(ch * P::kLaneDims + e) / 4 + (k >> 1)][2 * nr + (k & 1)] = w[k] ^ flip_q;
             big = fmaxf(big, fmaxf(fabsf(half_bits_to_float<T>(w[k] & 0xFFFFu)), fabsf(half_bits_to_float<T>(w[k] >> 16))));
           }
         }
-      qmul[hrow] = a.scale;
+      float mul = a.scale == 0.0f ? 1.1754943508222875e-38f : fabsf(a.scale);  // scores vanish but keep -Inf
       if (S != KV_NONE) {
         big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 1));
         big = fmaxf(big, __shfl_xor_sync(0xFFFFFFFFu, big, 2));
         const Pow2 f = fp16_shift(big);
-        qmul[hrow] = a.scale * f.inverse;
+        mul *= f.inverse;
 #pragma unroll
         for (int k = 0; k < P::kKSteps; ++k)
 #pragma unroll
-          for (int e = 0; e < 4; e += 2) {
-            const uint32_t w = qf[k][hrow + e];
-            qf[k][hrow + e] = pack_half(half_bits_to_float<T>(w & 0xFFFFu) * f.factor, half_bits_to_float<T>(w >> 16) * f.factor);
+          for (int e = 0; e < 2; ++e) {
+            const uint32_t w = qf[k][2 * nr + e];
+            qf[k][2 * nr + e] = pack_half(half_bits_to_float<T>(w & 0xFFFFu) * f.factor, half_bits_to_float<T>(w >> 16) * f.factor);
           }
       }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) qmul[nr][e] = __shfl_sync(0xFFFFFFFFu, mul, 4 * (2 * t + e));
     }
-    if (DP == 256) {  // the last item's readers passed its closing barrier
+    if constexpr (kSharedQ) {  // the last item's readers passed its closing barrier
       if (warp == 0)
 #pragma unroll
-        for (int k = 0; k < P::kKSteps; ++k) qfrag[DP == 256 ? k * 32 + lane : 0] = make_uint4(qf[k][0], qf[k][1], qf[k][2], qf[k][3]);
+        for (int k = 0; k < P::kKSteps; ++k) qfrag[k * 32 + lane] = make_uint4(qf[k][0], qf[k][1], qf[k][2], qf[k][3]);
       __syncthreads();
     }
-    // Keys that rows g and g + 8 see, and those that every row of the tile sees.
-    int see_lo[2], see_hi[2], all_lo, all_hi, unused;
-#pragma unroll
-    for (int hrow = 0; hrow < 2; ++hrow) visible(a, s, tok[hrow], see_lo[hrow], see_hi[hrow]);
+    // Keys that the lane's rows see, and those that every row of the tile sees.
+    int all_lo, all_hi, unused;
     visible(a, s, it.tile * kRows / a.group, unused, all_hi);
     visible(a, s, (min((it.tile + 1) * kRows, rows) - 1) / a.group, all_lo, unused);
 
-    float o[DP / 8][4];
+    float o[DP / 16][NR][4];  // elements g * DP / 8 + 2 i + (e >> 1), rows 8 nr + 2 t + (e & 1)
 #pragma unroll
-    for (int j = 0; j < DP / 8; ++j)
+    for (int i = 0; i < DP / 16; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[j][e] = 0.0f;
-    float top[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-    int vfield = 254;  // exponent field of 2**14 / T (what the weights are multiplied by)
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][nr][e] = 0.0f;
+    // ref: the base-2 logarithm that a row's weights are relative to, room(vfield) below its maximum, far below
+    // everything before the first key; sum: of this lane's weights. vfield: exponent field of T.
+    float ref[NR][2], sum[NR][2];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        ref[nr][e] = -3e38f;
+        sum[nr][e] = 0.0f;
+      }
+    int vfield = kBf16 ? 127 : 0;
 
     for (int i = 0, slot = 0; i < steps; ++i, slot = slot + 1 == P::kStages ? 0 : slot + 1) {
       if (i + P::kStages - 1 < steps) {
@@ -286,139 +309,102 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
       const uint32_t valid = *reinterpret_cast<const uint32_t *>(st + P::kStage - 16);
       const int p0 = key0 + i * kKeys;
 
-      // Scores: x[nt][e] is key nt * 8 + 2 t + (e & 1), row g + 8 (e >> 1).
-      float x[2][4], vscale[2][2];
-      int vbig[2][2];
+      // Scores: x[nr][e] is key g + 8 (e >> 1), row 8 nr + 2 t + (e & 1).
+      float x[NR][4], vscale[2] = {1.0f, 1.0f};
+      int vbig[2] = {0, 0};
 #pragma unroll
-      for (int nt = 0; nt < 2; ++nt) {
-        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int r = nt * 8 + g;
-        int big = 0;
-        if (S == KV_MXFP4) {
+      for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-          for (int q = 0; q < P::kScaleBytes; ++q)
-            if (q < scale_bytes) big = max(big, (int)kscales[r * scale_bytes + q]);
-        }
+        for (int e = 0; e < 4; ++e) x[nr][e] = 0.0f;
+      {
+        int kbig[2] = {0, 0};
+        float kscale[2] = {1.0f, 1.0f};
 #pragma unroll
-        for (int ch = 0; ch < P::kChunks; ++ch) {
-          uint32_t w[P::kLaneBytes / 4], gmul = 0u;
-          load_words<P::kLaneBytes / 4>(st + koff[kWide ? 0 : nt][ch] + (kWide ? nt * 8 * P::kRowBytes : 0), w);
+        for (int h = 0; h < 2; ++h) {
+          const int key = g + 8 * h;
           if (S == KV_MXFP4) {
-            const int grp = (ch * 4 + t) * P::kLaneDims / 32;
-            if (grp < scale_bytes) gmul = half_pow2((int)kscales[r * scale_bytes + grp] - big + kGroupShift) * 0x10001u;
-          }
-#pragma unroll
-          for (int k = 0; k < P::kLaneDims / 4; ++k) {
-            uint32_t b0, b1, h[4];
-            if (S == KV_NONE) {
-              b0 = w[(2 * k) % (P::kLaneBytes / 4)];
-              b1 = w[(2 * k + 1) % (P::kLaneBytes / 4)];
-            } else if (S == KV_MXFP4) {
-              e2m1x8_half2(w[(k >> 1) % (P::kLaneBytes / 4)], h);
-              b0 = mul_half2(h[2 * (k & 1)], gmul);
-              b1 = mul_half2(h[2 * (k & 1) + 1], gmul);
-            } else if (S == KV_FP8_ROW) {
-              e4m3x4_half2(w[k % (P::kLaneBytes / 4)], b0, b1);
-            } else {
-              const uint32_t u = w[k % (P::kLaneBytes / 4)] ^ 0x80808080u;
-              b0 = int8x2_half2<0x4140>(u);
-              b1 = int8x2_half2<0x4342>(u);
-            }
-            const int ks = ch * (P::kLaneDims / 4) + k;
-            if (DP == 256) {
-              const uint4 q4 = qfrag[DP == 256 ? ks * 32 + lane : 0];
-              const uint32_t qa[4] = {q4.x, q4.y, q4.z, q4.w};
-              mma16<kBf16>(acc, qa, b0, b1);
-            } else {
-              mma16<kBf16>(acc, qf[ks], b0, b1);
-            }
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = nt * 8 + 2 * t + e;
-          float ks = 1.0f;
-          vscale[nt][e] = 1.0f;
-          if (S == KV_MXFP4) {
-            int bk = 0, bv = 0;
 #pragma unroll
             for (int q = 0; q < P::kScaleBytes; ++q)
               if (q < scale_bytes) {
-                bk = max(bk, (int)kscales[key * scale_bytes + q]);
-                bv = max(bv, (int)vscales[key * scale_bytes + q]);
+                kbig[h] = max(kbig[h], (int)kscales[key * scale_bytes + q]);
+                vbig[h] = max(vbig[h], (int)vscales[key * scale_bytes + q]);
               }
-            ks = pow2_value(bk) * (1.0f / (1 << kGroupShift));
-            vscale[nt][e] = pow2_value(bv);
-            vbig[nt][e] = bv;
+            kscale[h] = pow2_value(kbig[h]) * (1.0f / (1 << kGroupShift));
+            vscale[h] = pow2_value(vbig[h]) * (1.0f / (1 << kGroupShift));
           } else if (S != KV_NONE) {
-            ks = reinterpret_cast<const float *>(kscales)[key];
-            vscale[nt][e] = reinterpret_cast<const float *>(vscales)[key];
+            kscale[h] = reinterpret_cast<const float *>(kscales)[key];
+            vscale[h] = reinterpret_cast<const float *>(vscales)[key];
           }
-          x[nt][e] = acc[e] * ks * qmul[0];
-          x[nt][e + 2] = acc[e + 2] * ks * qmul[1];
         }
+#pragma unroll
+        for (int ch = 0; ch < P::kChunks; ++ch) {
+          uint32_t w[2][P::kLaneBytes / 4], gmul[2] = {0u, 0u};
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            load_words<P::kLaneBytes / 4>(st + koff[kWide ? 0 : h][ch] + (kWide ? h * 8 * P::kRowBytes : 0), w[h]);
+            if (S == KV_MXFP4) {
+              const int grp = (ch * 4 + t) * P::kLaneDims / 32;
+              if (grp < scale_bytes)
+                gmul[h] = half_pow2((int)kscales[(g + 8 * h) * scale_bytes + grp] - kbig[h] + kGroupShift) * 0x10001u;
+            }
+          }
+#pragma unroll
+          for (int k = 0; k < P::kLaneDims / 4; ++k) {
+            uint32_t ka[4];  // key g, key g + 8 at the first two elements, then at the next two
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (S == KV_NONE) {
+                ka[h] = w[h][(2 * k) % (P::kLaneBytes / 4)];
+                ka[2 + h] = w[h][(2 * k + 1) % (P::kLaneBytes / 4)];
+              } else if (S == KV_MXFP4) {
+                uint32_t v[4];
+                e2m1x8_half2(w[h][(k >> 1) % (P::kLaneBytes / 4)], v);
+                ka[h] = mul_half2(v[2 * (k & 1)], gmul[h]);
+                ka[2 + h] = mul_half2(v[2 * (k & 1) + 1], gmul[h]);
+              } else if (S == KV_FP8_ROW) {
+                e4m3x4_half2(w[h][k % (P::kLaneBytes / 4)], ka[h], ka[2 + h]);
+              } else {
+                const uint32_t u = w[h][k % (P::kLaneBytes / 4)] ^ 0x80808080u;
+                ka[h] = int8x2_half2<0x4140>(u);
+                ka[2 + h] = int8x2_half2<0x4342>(u);
+              }
+            }
+            const int ks = ch * (P::kLaneDims / 4) + k;
+            if constexpr (kSharedQ) {
+              const uint4 q4 = qfrag[ks * 32 + lane];
+              mma16<kBf16>(x[0], ka, q4.x, q4.y);
+              mma16<kBf16>(x[NR - 1], ka, q4.z, q4.w);
+            } else {
+#pragma unroll
+              for (int nr = 0; nr < NR; ++nr) mma16<kBf16>(x[nr], ka, qf[ks][2 * nr], qf[ks][2 * nr + 1]);
+            }
+          }
+        }
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[nr][e] = x[nr][e] * kscale[e >> 1] * qmul[nr][e & 1];
       }
       const bool whole = valid == 0xFFFFu && p0 >= all_lo && p0 + kStep <= all_hi;
       if (!whole) {
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
+        for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int key = nt * 8 + 2 * t + (e & 1);
-            const bool there = (valid >> key) & 1u;
-            if (!there || p0 + key < see_lo[e >> 1] || p0 + key >= see_hi[e >> 1]) x[nt][e] = -INFINITY;
-            if (e < 2 && !there) vscale[nt][e] = 0.0f;
+          for (int r = 0; r < 2; ++r) {
+            int lo_r, hi_r;
+            visible(a, s, min(it.tile * kRows + 8 * nr + 2 * t + r, rows - 1) / a.group, lo_r, hi_r);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const int key = g + 8 * h;
+              if (!((valid >> key) & 1u) || p0 + key < lo_r || p0 + key >= hi_r) x[nr][2 * h + r] = -INFINITY;
+            }
           }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (!((valid >> (g + 8 * h)) & 1u)) vscale[h] = 0.0f;
       }
-
-      // Running maxima and sums; keep[] scales what the sums hold, okeep[] what the outputs hold.
-      float keep[2], okeep[2];
-      bool moved = false;
-#pragma unroll
-      for (int hrow = 0; hrow < 2; ++hrow) {
-        float m = fmaxf(fmaxf(x[0][2 * hrow], x[0][2 * hrow + 1]), fmaxf(x[1][2 * hrow], x[1][2 * hrow + 1]));
-        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
-        m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-        m = fmaxf(m, top[hrow]);
-        keep[hrow] = okeep[hrow] = m == top[hrow] ? 1.0f : exp2_fast(top[hrow] - m);
-        moved |= m != top[hrow];
-        top[hrow] = m;
-      }
-      uint32_t nan_keys = 0u;  // keys whose V scale is NaN
-      float vmul = 16384.0f;
-      if (S != KV_NONE) {
-        int f = 0;
-        bool nan = false;
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int v = (int)(f2u(vscale[nt][e]) >> 23);
-            nan |= v >= 255;
-            f = max(f, v >= 255 ? 0 : v);
-          }
-        f = max(f, __shfl_xor_sync(0xFFFFFFFFu, f, 1));
-        f = max(f, __shfl_xor_sync(0xFFFFFFFFu, f, 2));
-        const int field = min(vfield, 268 - f);  // 2**(14 - (f - 127)), at most 2**127
-        if (field != vfield) {
-          const float down = u2f((uint32_t)max(127 + field - vfield, 0) << 23);
-          okeep[0] *= down;
-          okeep[1] *= down;
-          moved = true;
-          vfield = field;
-        }
-        vmul = u2f((uint32_t)vfield << 23);
-        if (__any_sync(0xFFFFFFFFu, nan)) {
-          // Rare. A NaN scale comes with NaN codes, which would reach rows that do not see the key as
-          // 0 * NaN: such codes count as 0 below, and the weight carries the NaN.
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              if ((f2u(vscale[nt][e]) >> 23) >= 255) nan_keys |= 1u << (nt * 8 + 2 * t + e);
-          nan_keys = __reduce_or_sync(0xFFFFFFFFu, nan_keys);
-        }
-      } else if (!whole) {
+      uint32_t nan_keys = 0u;  // keys whose values are not numbers
+      if (S == KV_NONE && !whole) {
         // Rows of the step differ in what they see: a value that is not finite must not reach the others.
         // Its whole row counts as 0 and the weights of the rows that see it become NaN.
         for (int r = 0; r < kStep; ++r) {
@@ -430,51 +416,90 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
           if (__any_sync(0xFFFFFFFFu, bad)) nan_keys |= 1u << r;
         }
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int e = 0; e < 2; ++e)
-            if ((nan_keys >> (nt * 8 + 2 * t + e)) & 1u) vscale[nt][e] = u2f(kQNaN);
-      }
-      uint32_t pf[4];
-#pragma unroll
-      for (int hrow = 0; hrow < 2; ++hrow) {
-        const float ref = top[hrow] == -INFINITY ? 0.0f : top[hrow];
-        sum[hrow] *= keep[hrow];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          float p[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            p[e] = exp2_fast(x[nt][2 * hrow + e] - ref);
-            sum[hrow] += p[e];
-            if (S != KV_NONE) p[e] = p[e] == 0.0f ? 0.0f : p[e] * (vscale[nt][e] * vmul);
-            else if (!kBf16) p[e] *= vmul;
-            if (S == KV_NONE && nan_keys && p[e] != 0.0f) p[e] *= vscale[nt][e];
-          }
-          pf[2 * nt + hrow] = kBf16 ? pack_bf16(p[0], p[1]) : pack_half(p[0], p[1]);
-        }
-      }
-      if (__any_sync(0xFFFFFFFFu, moved)) {
-#pragma unroll
-        for (int j = 0; j < DP / 8; ++j)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) o[j][e] *= okeep[e >> 1];
+        for (int h = 0; h < 2; ++h)
+          if ((nan_keys >> (g + 8 * h)) & 1u) vscale[h] = u2f(kQNaN);
       }
 
-      // O += P V. Keys of the operand: 2 t, 2 t + 1 (b0), 2 t + 8, 2 t + 9 (b1).
+      // Does a row's reference, or T, have to move?
+      float m[NR][2];
+      bool any = false;
+      const float above = room(vfield);
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          m[nr][r] = fmaxf(x[nr][r], x[nr][2 + r]);
+          any |= m[nr][r] > ref[nr][r] + (above + 8.0f);
+        }
+      if (!kBf16) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) any |= (int)(f2u(vscale[h]) >> 23) > vfield;  // NaN too
+      }
+      if (__any_sync(0xFFFFFFFFu, any)) {
+        int field = vfield;
+        if (!kBf16) {
+          uint32_t f = 0u;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t v = f2u(vscale[h]) >> 23;
+            // A NaN scale comes with NaN codes, which would reach rows that do not see the key as 0 * NaN: such
+            // codes count as 0 below, and the weight carries the NaN.
+            if (v >= 255u) nan_keys |= 1u << (g + 8 * h);
+            else f = max(f, v);
+          }
+          nan_keys = __reduce_or_sync(0xFFFFFFFFu, nan_keys);
+          field = max(field, (int)warp_max(f));
+        }
+        float keep[NR][2];
+#pragma unroll
+        for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            float top = m[nr][r];
+#pragma unroll
+            for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
+            const float now = top > ref[nr][r] + (above + 8.0f) ? ceilf(top) : ref[nr][r] + above;
+            const float next = now - room(field);
+            keep[nr][r] = exp2_fast(ref[nr][r] - next);
+            ref[nr][r] = next;
+            sum[nr][r] *= keep[nr][r];
+          }
+        vfield = field;
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k)
+#pragma unroll
+          for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[k][nr][e] *= keep[nr][e & 1];
+      }
+      uint32_t pf[NR][2];  // P^T: keys 2 t, 2 t + 1 (and + 8) of row g
+#pragma unroll
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float p[2];
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            p[r] = exp2_fast(x[nr][2 * h + r] - ref[nr][r]);
+            sum[nr][r] += p[r];
+            if (S != KV_NONE || nan_keys) p[r] = nan_keys && p[r] == 0.0f ? 0.0f : p[r] * vscale[h];
+          }
+          pf[nr][h] = transpose8x8(kBf16 ? pack_bf16(p[0], p[1]) : pack_half(p[0], p[1]));
+        }
+
+      // O^T += V^T P^T. Keys of the operand: 2 t, 2 t + 1, then 2 t + 8, 2 t + 9.
       uint32_t vm0 = 0u, vm1 = 0u;
       if (S == KV_MXFP4) {
         const int grp = g * (DP / 8) / 32;
-        if (grp < scale_bytes) {
-          uint32_t m[2][2];
+        uint32_t mul[4];
 #pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-              m[nt][e] = half_pow2((int)vscales[(nt * 8 + 2 * t + e) * scale_bytes + grp] - vbig[nt][e] + kGroupShift);
-          vm0 = m[0][0] | (m[0][1] << 16);
-          vm1 = m[1][0] | (m[1][1] << 16);
+        for (int k = 0; k < 4; ++k) {
+          const int key = 2 * t + (k & 1) + 8 * (k >> 1);
+          const int big = __shfl_sync(0xFFFFFFFFu, k >> 1 ? vbig[1] : vbig[0], 4 * (2 * t + (k & 1)));
+          mul[k] = grp < scale_bytes ? half_pow2((int)vscales[key * scale_bytes + grp] - big + kGroupShift) : 0u;
         }
+        vm0 = mul[0] | (mul[1] << 16);
+        vm1 = mul[2] | (mul[3] << 16);
       }
 #pragma unroll
       for (int part = 0; part < P::kVBytes / P::kVPart; ++part) {
@@ -490,43 +515,41 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
         }
 #pragma unroll
         for (int q = 0; q < P::kVPart / 4; ++q) {
+          auto add = [&](int i, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3) {
+            const uint32_t va[4] = {a0, a1, a2, a3};
+#pragma unroll
+            for (int nr = 0; nr < NR; ++nr) mma16<kBf16>(o[i][nr], va, pf[nr][0], pf[nr][1]);
+          };
           if (S == KV_NONE) {
-            const int j = (part * 16 + q * 4) / 2;
-            mma16<kBf16>(o[j], pf, __byte_perm(w[0][q], w[1][q], 0x5410), __byte_perm(w[2][q], w[3][q], 0x5410));
-            mma16<kBf16>(o[j + 1], pf, __byte_perm(w[0][q], w[1][q], 0x7632), __byte_perm(w[2][q], w[3][q], 0x7632));
+            add((part * 16 + q * 4) / 4, __byte_perm(w[0][q], w[1][q], 0x5410), __byte_perm(w[0][q], w[1][q], 0x7632),
+                __byte_perm(w[2][q], w[3][q], 0x5410), __byte_perm(w[2][q], w[3][q], 0x7632));
           } else if (S == KV_MXFP4) {
-            const int j = (part * 16 + q * 4) * 2;
             // Bytes of one nibble from each of two keys: even elements, odd elements.
-            const uint32_t e0 = (w[0][q] & 0x0F0F0F0Fu) | ((w[1][q] & 0x0F0F0F0Fu) << 4);
-            const uint32_t d0 = ((w[0][q] >> 4) & 0x0F0F0F0Fu) | (w[1][q] & 0xF0F0F0F0u);
-            const uint32_t e1 = (w[2][q] & 0x0F0F0F0Fu) | ((w[3][q] & 0x0F0F0F0Fu) << 4);
-            const uint32_t d1 = ((w[2][q] >> 4) & 0x0F0F0F0Fu) | (w[3][q] & 0xF0F0F0F0u);
-            uint32_t h0[4], h1[4];
-            e2m1x8_half2(e0, h0);
-            e2m1x8_half2(e1, h1);
+            uint32_t e0[4], d0[4], e1[4], d1[4];
+            e2m1x8_half2((w[0][q] & 0x0F0F0F0Fu) | ((w[1][q] & 0x0F0F0F0Fu) << 4), e0);
+            e2m1x8_half2(((w[0][q] >> 4) & 0x0F0F0F0Fu) | (w[1][q] & 0xF0F0F0F0u), d0);
+            e2m1x8_half2((w[2][q] & 0x0F0F0F0Fu) | ((w[3][q] & 0x0F0F0F0Fu) << 4), e1);
+            e2m1x8_half2(((w[2][q] >> 4) & 0x0F0F0F0Fu) | (w[3][q] & 0xF0F0F0F0u), d1);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) mma16<false>(o[j + 2 * k], pf, mul_half2(h0[k], vm0), mul_half2(h1[k], vm1));
-            e2m1x8_half2(d0, h0);
-            e2m1x8_half2(d1, h1);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) mma16<false>(o[j + 2 * k + 1], pf, mul_half2(h0[k], vm0), mul_half2(h1[k], vm1));
+            for (int k = 0; k < 4; ++k)
+              add(part * 16 + q * 4 + k, mul_half2(e0[k], vm0), mul_half2(d0[k], vm0), mul_half2(e1[k], vm1), mul_half2(d1[k], vm1));
           } else {
-            const int j = part * 16 + q * 4;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
               const uint32_t ab = __byte_perm(w[0][q], w[1][q], k ? 0x7362 : 0x5140);
               const uint32_t cd = __byte_perm(w[2][q], w[3][q], k ? 0x7362 : 0x5140);
+              uint32_t h[4];
               if (S == KV_FP8_ROW) {
-                uint32_t h[4];
                 e4m3x4_half2(ab, h[0], h[1]);
                 e4m3x4_half2(cd, h[2], h[3]);
-                mma16<false>(o[j + 2 * k], pf, h[0], h[2]);
-                mma16<false>(o[j + 2 * k + 1], pf, h[1], h[3]);
               } else {
                 const uint32_t u0 = ab ^ 0x80808080u, u1 = cd ^ 0x80808080u;
-                mma16<false>(o[j + 2 * k], pf, int8x2_half2<0x4140>(u0), int8x2_half2<0x4140>(u1));
-                mma16<false>(o[j + 2 * k + 1], pf, int8x2_half2<0x4342>(u0), int8x2_half2<0x4342>(u1));
+                h[0] = int8x2_half2<0x4140>(u0);
+                h[1] = int8x2_half2<0x4342>(u0);
+                h[2] = int8x2_half2<0x4140>(u1);
+                h[3] = int8x2_half2<0x4342>(u1);
               }
+              add((part * 16 + q * 4) / 2 + k, h[0], h[1], h[2], h[3]);
             }
           }
         }
@@ -537,22 +560,25 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
     // The warps' results become one.
     cp_async_wait_all();
     __syncthreads();
-    float undo = S == KV_NONE ? (kBf16 ? 1.0f : 1.0f / 16384.0f) : 1.0f / u2f((uint32_t)vfield << 23);
-    if (S == KV_MXFP4) undo *= 1.0f / (1 << kGroupShift);
     float *mo = reinterpret_cast<float *>(smem) + warp * kRows * DP;
 #pragma unroll
-    for (int hrow = 0; hrow < 2; ++hrow) {
-      sum[hrow] += __shfl_xor_sync(0xFFFFFFFFu, sum[hrow], 1);
-      sum[hrow] += __shfl_xor_sync(0xFFFFFFFFu, sum[hrow], 2);
-      if (t == 0) {
-        merge_top[warp][g + 8 * hrow] = top[hrow];
-        merge_sum[warp][g + 8 * hrow] = sum[hrow];
+    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int k = 4; k < 32; k <<= 1) sum[nr][r] += __shfl_xor_sync(0xFFFFFFFFu, sum[nr][r], k);
+        if (g == 0) {
+          merge_top[warp][8 * nr + 2 * t + r] = sum[nr][r] == 0.0f ? -INFINITY : ref[nr][r];
+          merge_sum[warp][8 * nr + 2 * t + r] = sum[nr][r];
+        }
       }
-    }
 #pragma unroll
-    for (int j = 0; j < DP / 8; ++j)
+    for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) mo[((2 * t + (e & 1)) * (DP / 8) + j) * kRows + g + 8 * (e >> 1)] = o[j][e] * undo;
+      for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          mo[(g * (DP / 8) + 2 * k + (e >> 1)) * kRows + 8 * nr + 2 * t + (e & 1)] = o[k][nr][e];
     __syncthreads();
     const bool done = it.at == 0 && it.n == it.units;
     float *part = parts + (size_t)(2 * blockIdx.x + (it.at > 0 ? 0 : 1)) * partial_floats(kRows, DP);
@@ -563,7 +589,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
     float weight[kWarps], total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      weight[w] = merge_top[w][row] == -INFINITY && merge_sum[w][row] == 0.0f ? 0.0f : exp2_fast(merge_top[w][row] - m);
+      weight[w] = merge_top[w][row] == -INFINITY ? 0.0f : exp2_fast(merge_top[w][row] - m);
       total += merge_sum[w][row] * weight[w];
     }
     const int r = it.tile * kRows + row;
@@ -592,10 +618,11 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP>::kBlocks) split_kernel(
   }
 }
 
-template <typename T, int S, int DP, bool PAD>
-int launch_pad(const Args &a, float *parts, int most, cudaStream_t s) {
-  using P = Shape<S, DP>;
-  auto kern = split_kernel<T, S, DP, PAD>;
+template <typename T, int S, int DP, int NR, bool PAD>
+int launch(const Args &a, float *parts, int sms, cudaStream_t s) {
+  using P = Shape<S, DP, NR>;
+  static_assert(P::kStages >= 2, "the ring holds the step at hand and the next");
+  auto kern = split_kernel<T, S, DP, NR, PAD>;
   static std::atomic<uint64_t> ready[2];  // devices whose shared-memory limit is raised
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -605,22 +632,26 @@ int launch_pad(const Args &a, float *parts, int most, cudaStream_t s) {
     if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
     if (dev < 128) ready[dev >> 6].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
   }
+  const int most = sms * P::kBlocks;
   kern<<<most, kThreads, P::kSmem, s>>>(a, parts, most);
   count_launch();
-  return TC_OK;
+  return launch_join<T, 8 * NR, kKeys>(a, parts, most, nullptr, s);
 }
 
 template <typename T, int S, int DP>
-int launch(const Args &a, float *parts, int most, cudaStream_t s) {
-  return a.c.dim == DP ? launch_pad<T, S, DP, false>(a, parts, most, s) : launch_pad<T, S, DP, true>(a, parts, most, s);
+int launch_rows(const Args &a, float *parts, int sms, cudaStream_t s) {
+  const bool pad = a.c.dim != DP;
+  if ((int64_t)a.max_q * a.group <= 8)
+    return pad ? launch<T, S, DP, 1, true>(a, parts, sms, s) : launch<T, S, DP, 1, false>(a, parts, sms, s);
+  return pad ? launch<T, S, DP, 2, true>(a, parts, sms, s) : launch<T, S, DP, 2, false>(a, parts, sms, s);
 }
 
 template <int S>
-int launch_scheme(const Args &a, float *parts, int most, cudaStream_t s) {
+int launch_scheme(const Args &a, float *parts, int sms, cudaStream_t s) {
   const bool bf16 = a.c.dtype == TC_BF16;
-  if (a.c.dim <= 64) return bf16 ? launch<__nv_bfloat16, S, 64>(a, parts, most, s) : launch<__half, S, 64>(a, parts, most, s);
-  if (a.c.dim <= 128) return bf16 ? launch<__nv_bfloat16, S, 128>(a, parts, most, s) : launch<__half, S, 128>(a, parts, most, s);
-  return bf16 ? launch<__nv_bfloat16, S, 256>(a, parts, most, s) : launch<__half, S, 256>(a, parts, most, s);
+  if (a.c.dim <= 64) return bf16 ? launch_rows<__nv_bfloat16, S, 64>(a, parts, sms, s) : launch_rows<__half, S, 64>(a, parts, sms, s);
+  if (a.c.dim <= 128) return bf16 ? launch_rows<__nv_bfloat16, S, 128>(a, parts, sms, s) : launch_rows<__half, S, 128>(a, parts, sms, s);
+  return bf16 ? launch_rows<__nv_bfloat16, S, 256>(a, parts, sms, s) : launch_rows<__half, S, 256>(a, parts, sms, s);
 }
 
 }  // namespace split

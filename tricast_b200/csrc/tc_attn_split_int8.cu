@@ -3,8 +3,8 @@
 
 namespace tc {
 namespace attn {
-int launch_split_int8(const Args &a, float *parts, int most, cudaStream_t s) {
-  return split::launch_scheme<KV_INT8_ROW>(a, parts, most, s);
+int launch_split_int8(const Args &a, float *parts, int sms, cudaStream_t s) {
+  return split::launch_scheme<KV_INT8_ROW>(a, parts, sms, s);
 }
 }  // namespace attn
 }  // namespace tc
