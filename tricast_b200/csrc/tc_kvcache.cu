@@ -2,6 +2,7 @@
 // scales) per token and head, so that a token is written without touching its neighbours.
 #include <string>
 
+#include "tc_mma16.cuh"
 #include "tc_serve.cuh"
 
 namespace tc {
@@ -46,6 +47,7 @@ struct Move {
   int64_t k_tok, k_head, v_tok, v_head;
   const int64_t *slots;
   int64_t tokens;
+  uint32_t rows;  // tokens * heads * 2
 };
 
 constexpr int kThreads = 256;
@@ -56,78 +58,263 @@ __device__ __forceinline__ int64_t pool_row(const KvCache &c, int64_t slot, int 
   return (((slot >> c.page_shift) * c.heads + head) << c.page_shift) + (slot & (c.page_size - 1));
 }
 
-// A warp a row (token, head, side).
-template <typename T, int S>
+constexpr int kOwn = 16;  // elements a lane: what finding a row costs is shared by them
+
+// A lane's elements as they are stored; whole 16-byte words where rows start at such boundaries (VEC).
+template <typename T>
+struct Held {
+  uint32_t w[kOwn * sizeof(T) / 4];
+};
+template <typename T, bool VEC>
+__device__ __forceinline__ void fetch(const T *x, Held<T> &h) {
+  if (VEC) {
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(Held<T>) / 16; ++k) {
+      const uint4 v = reinterpret_cast<const uint4 *>(x)[k];
+      h.w[4 * k] = v.x, h.w[4 * k + 1] = v.y, h.w[4 * k + 2] = v.z, h.w[4 * k + 3] = v.w;
+    }
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) h.w[k] = reinterpret_cast<const uint32_t *>(x)[k];
+  } else {
+    const unsigned short *u = reinterpret_cast<const unsigned short *>(x);
+#pragma unroll
+    for (int k = 0; k < kOwn / 2; ++k) h.w[k] = (uint32_t)u[2 * k] | ((uint32_t)u[2 * k + 1] << 16);
+  }
+}
+template <typename T, bool VEC>
+__device__ __forceinline__ void store(T *x, const Held<T> &h) {
+  if (VEC) {
+#pragma unroll
+    for (int k = 0; k < (int)sizeof(Held<T>) / 16; ++k)
+      reinterpret_cast<uint4 *>(x)[k] = make_uint4(h.w[4 * k], h.w[4 * k + 1], h.w[4 * k + 2], h.w[4 * k + 3]);
+  } else if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) reinterpret_cast<uint32_t *>(x)[k] = h.w[k];
+  } else {
+    unsigned short *u = reinterpret_cast<unsigned short *>(x);
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) u[k] = (unsigned short)(h.w[k >> 1] >> (16 * (k & 1)));
+  }
+}
+template <typename T>
+__device__ __forceinline__ float element_of(const Held<T> &h, int e) {
+  if constexpr (sizeof(T) == 4) return u2f(h.w[e]);
+  else if constexpr (Same<T, __nv_bfloat16>::value) return u2f(e & 1 ? h.w[e >> 1] & 0xFFFF0000u : h.w[e >> 1] << 16);
+  else return __half2float(__ushort_as_half((unsigned short)(h.w[e >> 1] >> (16 * (e & 1)))));
+}
+// Bits of the largest magnitude as fp32: the order of the bits is that of the magnitudes in every type, NaN on
+// top, so 16-bit ones are compared two at a time as they are.
+template <typename T>
+__device__ __forceinline__ uint32_t top_of(const Held<T> &h) {
+  uint32_t m = 0u;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int k = 0; k < kOwn; ++k) m = max(m, h.w[k] & 0x7FFFFFFFu);
+    return m;
+  } else {
+#pragma unroll
+    for (int k = 0; k < kOwn / 2; ++k) m = __vmaxu2(m, h.w[k] & 0x7FFF7FFFu);
+    m = max(m & 0xFFFFu, m >> 16);
+    if constexpr (Same<T, __nv_bfloat16>::value) return m << 16;
+    else return f2u(__half2float(__ushort_as_half((unsigned short)m))) & 0x7FFFFFFFu;
+  }
+}
+
+// The item (token, head, side) of a group of lanes that hold a row, 16 elements each. Rows follow one another by
+// head within a token and side, so a warp's reads are whole lines.
+struct RowOf {
+  int64_t row;  // in the pool, -1 for none
+  uint32_t token;
+  int head, side;
+};
+__device__ __forceinline__ RowOf row_of(const Move &m, uint32_t i) {
+  RowOf r{-1, 0u, 0, 0};
+  if (i >= m.rows) return r;
+  const uint32_t rest = i / (uint32_t)m.c.heads;
+  r.head = (int)(i - rest * m.c.heads);
+  r.side = (int)(rest & 1u);
+  r.token = rest >> 1;
+  r.row = pool_row(m.c, m.slots[r.token], r.head);
+  return r;
+}
+
+// LANES (a power of two, at most 16) lanes a row of at most 16 LANES elements; VEC: rows start at 16-byte
+// boundaries. Bound by HBM: a row is read once and written once, kFlight rows a group of lanes in flight.
+template <typename T>
+constexpr int flight() {
+  return sizeof(T) == 4 ? 2 : 4;
+}
+template <typename T, int S, int LANES, bool VEC>
 __global__ void __launch_bounds__(kThreads) write_kernel(Move m) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = m.tokens * m.c.heads * 2;
-  for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < rows;
-       i += (int64_t)gridDim.x * (kThreads / 32)) {
-    const int side = (int)(i & 1);
-    const int64_t token = (i >> 1) / m.c.heads;
-    const int head = (int)((i >> 1) % m.c.heads);
-    const int64_t row = pool_row(m.c, m.slots[token], head);
-    if (row < 0) continue;
-    const T *x = side ? static_cast<const T *>(m.v) + token * m.v_tok + head * m.v_head
-                      : static_cast<const T *>(m.k) + token * m.k_tok + head * m.k_head;
-    unsigned char *codes = (side ? m.c.v : m.c.k) + row * m.c.row_bytes;
-    unsigned char *scales = (side ? m.c.vs : m.c.ks) + row * m.c.scale_bytes;
-    if (S == KV_NONE) {
-      for (int d = lane; d < m.c.dim; d += 32) reinterpret_cast<T *>(codes)[d] = x[d];
-    } else if (S == KV_MXFP4) {
-      for (int d = lane; d < m.c.dim; d += 32) {
-        const float v = Io<T>::get(x[d]);
-        const uint32_t sc = pow2_code(warp_max(abs_bits(v)), 2);
-        const uint32_t c = encode_e2m1(__fmul_rn(v, pow2_inverse(sc)));
-        const uint32_t next = __shfl_down_sync(0xFFFFFFFFu, c, 1);
-        if (!(lane & 1)) codes[d >> 1] = (unsigned char)(c | (next << 4));
-        if (lane == 0) scales[d >> 5] = (unsigned char)sc;
+  constexpr int kFlight = flight<T>();
+  const int lane = threadIdx.x % LANES, d0 = lane * kOwn;
+  const uint32_t groups = gridDim.x * (kThreads / LANES), first = blockIdx.x * (kThreads / LANES);
+  const bool have = d0 < m.c.dim;
+  // Every lane of a block goes round equally often: the lanes of a row exchange values.
+  for (uint32_t b0 = first; b0 < m.rows; b0 += groups * kFlight) {
+    const uint32_t i0 = b0 + threadIdx.x / LANES;
+    RowOf r[kFlight];
+    Held<T> h[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      r[f] = row_of(m, i0 + f * groups);
+      if (!have) r[f].row = -1;
+#pragma unroll
+      for (int k = 0; k < (int)sizeof(Held<T>) / 4; ++k) h[f].w[k] = 0u;
+      if (r[f].row >= 0)
+        fetch<T, VEC>((r[f].side ? static_cast<const T *>(m.v) + r[f].token * m.v_tok + r[f].head * m.v_head
+                                 : static_cast<const T *>(m.k) + r[f].token * m.k_tok + r[f].head * m.k_head) + d0, h[f]);
+    }
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      unsigned char *codes = (r[f].side ? m.c.v : m.c.k) + r[f].row * m.c.row_bytes;
+      unsigned char *scales = (r[f].side ? m.c.vs : m.c.ks) + r[f].row * m.c.scale_bytes;
+      const bool live = r[f].row >= 0;
+      if (S == KV_NONE) {
+        if (live) store<T, true>(reinterpret_cast<T *>(codes) + d0, h[f]);
+        continue;
       }
-    } else {
-      uint32_t top = 0u;
-      for (int d = lane; d < m.c.dim; d += 32) top = max(top, abs_bits(Io<T>::get(x[d])));
-      const float s = absmax_scale(warp_max(top), S == KV_FP8_ROW ? 448.0f : 127.0f);
-      if (lane == 0) *reinterpret_cast<float *>(scales) = s;
-      for (int d = lane; d < m.c.dim; d += 32)
-        codes[d] = (unsigned char)encode8<S == KV_FP8_ROW ? E8_E4M3 : E8_INT8>(__fdiv_rn(Io<T>::get(x[d]), s));
+      uint32_t top = top_of<T>(h[f]);
+      // A row's lanes, or the two that share 32 elements.
+#pragma unroll
+      for (int k = 1; k < (S == KV_MXFP4 ? 2 : LANES); k <<= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
+      if (S == KV_MXFP4) {
+        const uint32_t sc = pow2_code(top, 2);
+        const float inv = pow2_inverse(sc);
+        uint32_t w[2] = {0u, 0u};
+#pragma unroll
+        for (int e = 0; e < kOwn; ++e) w[e >> 3] |= encode_e2m1(__fmul_rn(element_of<T>(h[f], e), inv)) << (4 * (e & 7));
+        if (live) {
+          *reinterpret_cast<uint2 *>(codes + d0 / 2) = make_uint2(w[0], w[1]);
+          if ((lane & 1) == 0) scales[d0 / 32] = (unsigned char)sc;
+        }
+      } else {
+        constexpr int E = S == KV_FP8_ROW ? E8_E4M3 : E8_INT8;
+        const float s = absmax_scale(top, E == E8_E4M3 ? 448.0f : 127.0f);
+        uint32_t q[4];
+        if (divides_fast(s)) {
+          const float rs = __frcp_rn(s);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = divide_fast(element_of<T>(h[f], 4 * k + e), s, rs);
+            q[k] = encode8x2<E>(v[0], v[1]) | (encode8x2<E>(v[2], v[3]) << 16);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            q[k] = 0u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) q[k] |= encode8<E>(__fdiv_rn(element_of<T>(h[f], 4 * k + e), s)) << (8 * e);
+          }
+        }
+        if (live) {
+          *reinterpret_cast<uint4 *>(codes + d0) = make_uint4(q[0], q[1], q[2], q[3]);
+          if (lane == 0) *reinterpret_cast<float *>(scales) = s;
+        }
+      }
     }
   }
 }
 
-// Value of element d of a pool row, in fp32: code * scale with one rounding (exact for mxfp4).
-template <typename T, int S>
-__device__ __forceinline__ float element(const unsigned char *codes, const unsigned char *scales, int d) {
-  if (S == KV_NONE) return Io<T>::get(reinterpret_cast<const T *>(codes)[d]);
-  if (S == KV_MXFP4) return __fmul_rn(decode_e2m1((codes[d >> 1] >> (4 * (d & 1))) & 15u), pow2_value(scales[d >> 5]));
-  const float s = *reinterpret_cast<const float *>(scales);
-  return __fmul_rn(S == KV_FP8_ROW ? decode_e4m3(codes[d]) : (float)(signed char)codes[d], s);
+// The same lanes: code * scale in fp32, rounded once to T (exact for mxfp4 in fp32 and bf16).
+template <typename T, int S, int LANES, bool VEC>
+__global__ void __launch_bounds__(kThreads) read_kernel(Move m) {
+  constexpr int kFlight = flight<T>();
+  const int lane = threadIdx.x % LANES, d0 = lane * kOwn;
+  const uint32_t groups = gridDim.x * (kThreads / LANES);
+  if (d0 >= m.c.dim) return;
+  for (uint32_t i0 = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES; i0 < m.rows; i0 += groups * kFlight) {
+    RowOf r[kFlight];
+    Held<T> h[kFlight];
+    uint4 c[kFlight];
+    float sc[kFlight];
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      r[f] = row_of(m, i0 + f * groups);
+      c[f] = make_uint4(0, 0, 0, 0);
+      sc[f] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < (int)sizeof(Held<T>) / 4; ++k) h[f].w[k] = 0u;
+      if (r[f].row >= 0) {
+        const unsigned char *codes = (r[f].side ? m.c.v : m.c.k) + r[f].row * m.c.row_bytes;
+        const unsigned char *scales = (r[f].side ? m.c.vs : m.c.ks) + r[f].row * m.c.scale_bytes;
+        if (S == KV_NONE) {
+          fetch<T, true>(reinterpret_cast<const T *>(codes) + d0, h[f]);
+        } else if (S == KV_MXFP4) {
+          const uint2 w = *reinterpret_cast<const uint2 *>(codes + d0 / 2);
+          c[f].x = w.x, c[f].y = w.y;
+          sc[f] = pow2_value(scales[d0 / 32]);
+        } else {
+          c[f] = *reinterpret_cast<const uint4 *>(codes + d0);
+          sc[f] = *reinterpret_cast<const float *>(scales);
+        }
+      }
+    }
+#pragma unroll
+    for (int f = 0; f < kFlight; ++f) {
+      if (i0 + f * groups >= m.rows) continue;
+      T *x = (r[f].side ? static_cast<T *>(m.v) + r[f].token * m.v_tok + r[f].head * m.v_head
+                        : static_cast<T *>(m.k) + r[f].token * m.k_tok + r[f].head * m.k_head) + d0;
+      if (S != KV_NONE && r[f].row >= 0) {
+        const uint32_t w[4] = {c[f].x, c[f].y, c[f].z, c[f].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          float v[4];
+          if (S == KV_MXFP4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = decode_e2m1((w[k >> 1] >> (4 * (4 * (k & 1) + e))) & 15u);
+          } else if (S == KV_FP8_ROW) {
+            uint32_t lo, hi;
+            e4m3x4_half2(w[k], lo, hi);
+            v[0] = half_bits_to_float<__half>(lo & 0xFFFFu), v[1] = half_bits_to_float<__half>(lo >> 16);
+            v[2] = half_bits_to_float<__half>(hi & 0xFFFFu), v[3] = half_bits_to_float<__half>(hi >> 16);
+          } else {
+            // 2**23 + (v + 128) from the byte, less 2**23 + 128.
+            const uint32_t u = w[k] ^ 0x80808080u;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __fsub_rn(u2f(__byte_perm(u, 0x4B000000u, 0x7440 + e)), 8388736.0f);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = __fmul_rn(v[e], sc[f]);
+          if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) h[f].w[4 * k + e] = f2u(v[e]);
+          } else {
+            h[f].w[2 * k] = pack16<T>(v[0], v[1]);
+            h[f].w[2 * k + 1] = pack16<T>(v[2], v[3]);
+          }
+        }
+      }
+      store<T, VEC>(x, h[f]);
+    }
+  }
 }
 
-template <typename T, int S>
-__global__ void __launch_bounds__(kThreads) read_kernel(Move m) {
-  const int lane = threadIdx.x & 31;
-  const int64_t rows = m.tokens * m.c.heads * 2;
-  for (int64_t i = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); i < rows;
-       i += (int64_t)gridDim.x * (kThreads / 32)) {
-    const int side = (int)(i & 1);
-    const int64_t token = (i >> 1) / m.c.heads;
-    const int head = (int)((i >> 1) % m.c.heads);
-    const int64_t row = pool_row(m.c, m.slots[token], head);
-    T *x = side ? static_cast<T *>(m.v) + token * m.v_tok + head * m.v_head
-                : static_cast<T *>(m.k) + token * m.k_tok + head * m.k_head;
-    const unsigned char *codes = (side ? m.c.v : m.c.k) + (row < 0 ? 0 : row) * m.c.row_bytes;
-    const unsigned char *scales = (side ? m.c.vs : m.c.ks) + (row < 0 ? 0 : row) * m.c.scale_bytes;
-    for (int d = lane; d < m.c.dim; d += 32) x[d] = Io<T>::put(row < 0 ? 0.0f : element<T, S>(codes, scales, d));
+template <typename T, int S, int LANES>
+static void launch_lanes(const Move &m, bool write, cudaStream_t s) {
+  const int64_t per = kThreads / LANES, want = (m.rows + per - 1) / per, most = (int64_t)sm_count() * 8;
+  const unsigned grid = (unsigned)(want < most ? want : most);
+  const int64_t strides = m.k_tok | m.k_head | m.v_tok | m.v_head;
+  const bool vec = ((uintptr_t)m.k | (uintptr_t)m.v) % 16 == 0 && (strides * (int64_t)sizeof(T)) % 16 == 0;
+  if (write) {
+    if (vec) write_kernel<T, S, LANES, true><<<grid, kThreads, 0, s>>>(m);
+    else write_kernel<T, S, LANES, false><<<grid, kThreads, 0, s>>>(m);
+  } else {
+    if (vec) read_kernel<T, S, LANES, true><<<grid, kThreads, 0, s>>>(m);
+    else read_kernel<T, S, LANES, false><<<grid, kThreads, 0, s>>>(m);
   }
+  count_launch();
 }
 
 template <typename T, int S>
 static void launch(const Move &m, bool write, cudaStream_t s) {
-  const int64_t want = (m.tokens * m.c.heads * 2 + kThreads / 32 - 1) / (kThreads / 32), most = (int64_t)sm_count() * 8;
-  const unsigned grid = (unsigned)(want < most ? want : most);
-  if (write) write_kernel<T, S><<<grid, kThreads, 0, s>>>(m);
-  else read_kernel<T, S><<<grid, kThreads, 0, s>>>(m);
-  count_launch();
+  if (m.c.dim <= 32) launch_lanes<T, S, 2>(m, write, s);
+  else if (m.c.dim <= 64) launch_lanes<T, S, 4>(m, write, s);
+  else if (m.c.dim <= 128) launch_lanes<T, S, 8>(m, write, s);
+  else launch_lanes<T, S, 16>(m, write, s);
 }
 
 template <typename T>
@@ -137,6 +324,8 @@ static void by_scheme(const Move &m, bool write, cudaStream_t s) {
   else if (m.c.scheme == KV_INT8_ROW) launch<T, KV_INT8_ROW>(m, write, s);
   else launch<T, KV_MXFP4>(m, write, s);
 }
+
+static int64_t c_size(int dtype) { return dtype == TC_F32 ? 4 : 2; }
 
 static int move(const char *what, const tc_kv_cache *cache, const int64_t *slots, int64_t tokens, void *k, int64_t k_tok,
                 int64_t k_head, void *v, int64_t v_tok, int64_t v_head, bool write, tc_stream stream) {
@@ -148,18 +337,23 @@ static int move(const char *what, const tc_kv_cache *cache, const int64_t *slots
     set_error(std::string(what) + ": bad argument");
     return TC_INVALID_ARGUMENT;
   }
-  m.k = k;
-  m.v = v;
   m.k_tok = k_tok;
   m.k_head = k_head;
   m.v_tok = v_tok;
   m.v_head = v_head;
-  m.slots = slots;
-  m.tokens = tokens;
   cudaStream_t s = (cudaStream_t)stream;
-  if (m.c.dtype == TC_F32) by_scheme<float>(m, write, s);
-  else if (m.c.dtype == TC_BF16) by_scheme<__nv_bfloat16>(m, write, s);
-  else by_scheme<__half>(m, write, s);
+  // Rows are counted in 32 bits: calls of more than 2**30 take several launches.
+  const int64_t most = (1ll << 30) / (2 * m.c.heads), size = c_size(m.c.dtype);
+  for (int64_t at = 0; at < tokens; at += most) {
+    m.k = static_cast<char *>(k) + at * k_tok * size;
+    m.v = static_cast<char *>(v) + at * v_tok * size;
+    m.slots = slots + at;
+    m.tokens = tokens - at < most ? tokens - at : most;
+    m.rows = (uint32_t)(m.tokens * m.c.heads * 2);
+    if (m.c.dtype == TC_F32) by_scheme<float>(m, write, s);
+    else if (m.c.dtype == TC_BF16) by_scheme<__nv_bfloat16>(m, write, s);
+    else by_scheme<__half>(m, write, s);
+  }
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_error(std::string(what) + ": " + cudaGetErrorString(e)), TC_CUDA_ERROR;
   return TC_OK;
