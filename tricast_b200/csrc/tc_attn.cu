@@ -19,10 +19,10 @@ int launch_split_fp8(const Args &a, float *parts, int sms, cudaStream_t s);
 int launch_split_int8(const Args &a, float *parts, int sms, cudaStream_t s);
 int launch_split_mxfp4(const Args &a, float *parts, int most, cudaStream_t s);
 
-int launch_chunk_none(const Args &a, float *parts, int *status, int most, cudaStream_t s);
-int launch_chunk_fp8(const Args &a, float *parts, int *status, int most, cudaStream_t s);
-int launch_chunk_int8(const Args &a, float *parts, int *status, int most, cudaStream_t s);
-int launch_chunk_mxfp4(const Args &a, float *parts, int *status, int most, cudaStream_t s);
+int launch_chunk_none(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s);
+int launch_chunk_fp8(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s);
+int launch_chunk_int8(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s);
+int launch_chunk_mxfp4(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s);
 
 static int launch_split(const Args &a, float *parts, cudaStream_t s) {
   const int sms = sm_count();
@@ -38,23 +38,27 @@ static bool use_chunk(const KvCache &c, int group, int64_t max_q) { return c.dim
 
 static size_t split_bytes(const KvCache &c) {
   // At most four blocks an SM of 8 rows, or as many rows in fewer blocks (split::Shape).
-  return 2 * (size_t)sm_count() * 4 * partial_floats(16, split_width(c.dim)) * sizeof(float);
+  return 2 * (size_t)sm_count() * 4 * partial_floats(16, split_width(c.dim)) * sizeof(float) + (size_t)sm_count() * 4 * sizeof(Stretch);
+}
+static size_t chunk_parts(const KvCache &c) {
+  return 2 * (size_t)sm_count() * partial_floats(256, split_width(c.dim)) * sizeof(float);
 }
 static size_t chunk_bytes(const KvCache &c) {
-  return 2 * (size_t)sm_count() * partial_floats(256, split_width(c.dim)) * sizeof(float);
+  return chunk_parts(c) + (size_t)sm_count() * (sizeof(Stretch) + sizeof(int));
 }
 
 static int launch_chunk(const Args &a, void *workspace, cudaStream_t s) {
   const int most = sm_count();
   float *parts = static_cast<float *>(workspace);
-  int *status = reinterpret_cast<int *>(static_cast<char *>(workspace) + chunk_bytes(a.c));
-  const int st = a.c.scheme == KV_NONE       ? launch_chunk_none(a, parts, status, most, s)
-                 : a.c.scheme == KV_FP8_ROW  ? launch_chunk_fp8(a, parts, status, most, s)
-                 : a.c.scheme == KV_INT8_ROW ? launch_chunk_int8(a, parts, status, most, s)
-                                             : launch_chunk_mxfp4(a, parts, status, most, s);
+  Stretch *stretches = reinterpret_cast<Stretch *>(static_cast<char *>(workspace) + chunk_parts(a.c));
+  int *status = reinterpret_cast<int *>(stretches + most);
+  const int st = a.c.scheme == KV_NONE       ? launch_chunk_none(a, parts, stretches, status, most, s)
+                 : a.c.scheme == KV_FP8_ROW  ? launch_chunk_fp8(a, parts, stretches, status, most, s)
+                 : a.c.scheme == KV_INT8_ROW ? launch_chunk_int8(a, parts, stretches, status, most, s)
+                                             : launch_chunk_mxfp4(a, parts, stretches, status, most, s);
   if (st != TC_OK) return st;
-  return a.c.dtype == TC_BF16 ? launch_join<__nv_bfloat16, 256, 128>(a, parts, most, status, s)
-                              : launch_join<__half, 256, 128>(a, parts, most, status, s);
+  return a.c.dtype == TC_BF16 ? launch_join<__nv_bfloat16, 256>(a, parts, stretches, most, status, s)
+                              : launch_join<__half, 256>(a, parts, stretches, most, status, s);
 }
 
 }  // namespace attn
@@ -66,7 +70,7 @@ extern "C" size_t tc_paged_attention_workspace(const tc_kv_cache *cache, int32_t
   KvCache c;
   if (kv_cache_check(cache, c) != TC_OK || c.dtype == TC_F32) return 0;
   if (q_heads < c.heads || q_heads % c.heads) return 0;
-  if (attn::use_chunk(c, q_heads / c.heads, max_q_len)) return attn::chunk_bytes(c) + sm_count() * sizeof(int);
+  if (attn::use_chunk(c, q_heads / c.heads, max_q_len)) return attn::chunk_bytes(c);
   return attn::split_bytes(c);
 }
 

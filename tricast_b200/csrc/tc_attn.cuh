@@ -66,6 +66,12 @@ struct Item {
   int64_t left;       // units of the stretch after this part
 };
 
+// What a block leaves for the join: where its stretch starts and in which item (n 0: it has none).
+struct Stretch {
+  Item first;
+  int64_t start;
+};
+
 template <int kRows, int kKeys>
 struct Work {
   // Keys [lo, hi) that any row of the tile sees, lo rounded down to a whole unit.
@@ -195,6 +201,20 @@ struct Work {
     it.n = (int)min((int64_t)it.units, it.left);
     it.left -= it.n;
   }
+  // The stretch of block c of `most`, by a whole warp.
+  static __device__ __forceinline__ Stretch stretch(const Args &a, int c, int most) {
+    const int64_t sum = total(a);
+    const int n = blocks(sum, most);
+    Stretch s{{0, 0, 0, 0, 0, 0, 0}, sum};
+    if (c < n) {
+      const int64_t u0 = start(sum, c, n), u1 = start(sum, c + 1, n);
+      s.first = find(a, u0);
+      s.first.n = (int)min((int64_t)(s.first.units - s.first.at), u1 - u0);
+      s.first.left = u1 - u0 - s.first.n;
+      s.start = u0;
+    }
+    return s;
+  }
   // Blocks that share `total` units, at most `most`.
   static __device__ __forceinline__ int blocks(int64_t total, int most) { return (int)min(total, (int64_t)most); }
   static __device__ __forceinline__ int64_t start(int64_t total, int c, int n) { return total * c / n; }
@@ -292,41 +312,20 @@ __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Merges the partial results of the items that several blocks share. One block for each border between two
-// stretches and 8 or 16 rows of the item; it acts if the border is the first inside its item. It looks its item
-// up while the kernel before it ends. A row's maxima and sums are read side by side into shared memory (as many
+// stretches and 8 or 16 rows of the item; it acts if the border is the first inside its item. A row's maxima and sums are read side by side into shared memory (as many
 // parts at a time as it holds), its outputs [dim][row] by four rows a thread. Where `status` is given and a block
 // of the kernel before gave up a wait (which takes a fault elsewhere, or a test), everything is computed again by
 // the plain rows.
 constexpr int kJoinParts = 128, kJoinThreads = 256;
 constexpr int join_rows(int rows) { return rows < 16 ? rows : 16; }  // of an item, a block
-template <typename T, int kRows, int kKeys>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float *parts, int dim_pad, int most, const int *status) {
-  using W = Work<kRows, kKeys>;
+template <typename T, int kRows>
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float *parts, const Stretch *stretches, int dim_pad, int most, const int *status) {
   constexpr int kJoinRows = join_rows(kRows);
   __shared__ Item item;
   __shared__ int from, upto;
   __shared__ float part_top[kJoinParts][kJoinRows], part_sum[kJoinParts][kJoinRows];
   __shared__ float top[kJoinRows], sum[kJoinRows], keep[kJoinRows];
   const int c = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warp == 0) {
-    const int64_t total = W::total(a);
-    const int n = W::blocks(total, most);
-    if (lane == 0) upto = 0;
-    if (c < n) {
-      const int64_t u = W::start(total, c, n);
-      const Item it = W::find(a, u);
-      const int64_t begin = u - it.at, end = begin + it.units;
-      if (lane == 0 && it.at > 0 && W::start(total, c - 1, n) <= begin) {
-        // Blocks whose stretch starts before the item's end; starts grow by at least one unit a block.
-        int64_t k = end * n / total;
-        while (k < n && W::start(total, (int)k, n) < end) ++k;
-        while (k > 0 && W::start(total, (int)k - 1, n) >= end) --k;
-        item = it;
-        from = c - 1;
-        upto = (int)min(k, (int64_t)n);
-      }
-    }
-  }
   wait_for_previous();
   if (status) {
     int bad = 0;
@@ -336,6 +335,29 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
       plain_rows<T>(a, block * (kJoinThreads / 32) + warp, (int64_t)gridDim.x * gridDim.y * (kJoinThreads / 32));
       return;
     }
+  }
+  if (warp == 0) {
+    int end = 0;
+    if (c < most) {
+      const Stretch mine = stretches[c], before = stretches[c - 1];
+      const int64_t begin = mine.start - mine.first.at;
+      if (mine.first.n > 0 && mine.first.at > 0 && before.start <= begin) {
+        // The blocks from here on whose stretch starts inside the item.
+        end = c + 1;
+        while (true) {
+          const int k = end + lane;
+          const bool in = k < most && stretches[k].first.n > 0 && stretches[k].start < begin + mine.first.units;
+          const int n = __popc(__ballot_sync(0xFFFFFFFFu, in));
+          end += n;
+          if (n < 32) break;
+        }
+        if (lane == 0) {
+          item = mine.first;
+          from = c - 1;
+        }
+      }
+    }
+    if (lane == 0) upto = end;
   }
   __syncthreads();
   if (upto == 0) return;
@@ -420,8 +442,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
 }
 
 // Queues the join behind the kernel before it, to start as that one ends.
-template <typename T, int kRows, int kKeys>
-inline int launch_join(const Args &a, const float *parts, int most, const int *status, cudaStream_t s) {
+template <typename T, int kRows>
+inline int launch_join(const Args &a, const float *parts, const Stretch *stretches, int most, const int *status, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(most > 1 ? most - 1 : 1, kRows / join_rows(kRows));
   cfg.blockDim = dim3(kJoinThreads);
@@ -432,7 +454,7 @@ inline int launch_join(const Args &a, const float *parts, int most, const int *s
   cfg.attrs = at;
   cfg.numAttrs = 1;
   const int pad = a.c.dim <= 64 ? 64 : a.c.dim <= 128 ? 128 : 256;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<T, kRows, kKeys>, a, parts, pad, most, status);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<T, kRows>, a, parts, stretches, pad, most, status);
   if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
   count_launch();
   return TC_OK;

@@ -768,7 +768,7 @@ __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *q
 }
 
 template <typename T, int S, int DP>
-__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts, int *status, int most, int polls) {
+__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts, Stretch *stretches, int *status, int most, int polls) {
   constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char raw[];
   __shared__ KeySlot slots[kSlots];
@@ -780,17 +780,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
   unsigned char *qs = smem, *ks = qs + 2 * Shape<DP>::kOperand, *vs = ks + 2 * Shape<DP>::kOperand;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == kSoftmaxWarps) {
-    const int64_t total = W::total(a);
-    const int n = W::blocks(total, most);
-    Item it{0, 0, 0, 0, 0, 0, 0};
-    if ((int)blockIdx.x < n) {
-      const int64_t u0 = W::start(total, blockIdx.x, n), u1 = W::start(total, blockIdx.x + 1, n);
-      it = W::find(a, u0);
-      it.n = (int)min((int64_t)(it.units - it.at), u1 - u0);
-      it.left = u1 - u0 - it.n;
-    }
+    const Stretch mine = W::stretch(a, blockIdx.x, most);
     if (lane == 0) {
-      first = it;
+      first = mine.first;
+      stretches[blockIdx.x] = mine;
       failed = 0;
     }
   }
@@ -849,7 +842,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
 }
 
 template <typename T, int S, int DP>
-int launch(const Args &a, float *parts, int *status, int most, cudaStream_t s) {
+int launch(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s) {
   auto kern = chunk_kernel<T, S, DP>;
   static std::atomic<uint64_t> ready[2];  // devices whose shared-memory limit is raised
   int dev = 0;
@@ -860,17 +853,17 @@ int launch(const Args &a, float *parts, int *status, int most, cudaStream_t s) {
     if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
     if (dev < 128) ready[dev >> 6].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
   }
-  kern<<<most, kThreads, Shape<DP>::kSmem, s>>>(a, parts, status, most, wait_polls());
+  kern<<<most, kThreads, Shape<DP>::kSmem, s>>>(a, parts, stretches, status, most, wait_polls());
   count_launch();
   return TC_OK;
 }
 
 template <int S>
-int launch_scheme(const Args &a, float *parts, int *status, int most, cudaStream_t s) {
+int launch_scheme(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s) {
   const bool bf16 = a.c.dtype == TC_BF16;
   if (a.c.dim <= 64)
-    return bf16 ? launch<__nv_bfloat16, S, 64>(a, parts, status, most, s) : launch<__half, S, 64>(a, parts, status, most, s);
-  return bf16 ? launch<__nv_bfloat16, S, 128>(a, parts, status, most, s) : launch<__half, S, 128>(a, parts, status, most, s);
+    return bf16 ? launch<__nv_bfloat16, S, 64>(a, parts, stretches, status, most, s) : launch<__half, S, 64>(a, parts, stretches, status, most, s);
+  return bf16 ? launch<__nv_bfloat16, S, 128>(a, parts, stretches, status, most, s) : launch<__half, S, 128>(a, parts, stretches, status, most, s);
 }
 
 }  // namespace chunk

@@ -3,8 +3,8 @@
 
 namespace tc {
 namespace attn {
-int launch_chunk_int8(const Args &a, float *parts, int *status, int most, cudaStream_t s) {
-  return chunk::launch_scheme<KV_INT8_ROW>(a, parts, status, most, s);
+int launch_chunk_int8(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s) {
+  return chunk::launch_scheme<KV_INT8_ROW>(a, parts, stretches, status, most, s);
 }
 }  // namespace attn
 }  // namespace tc

@@ -76,7 +76,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
 }
 
 template <typename T, int S, int DP, int NR, bool PAD>
-__global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_kernel(Args a, float *parts, int most) {
+__global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_kernel(Args a, float *parts, Stretch *stretches, int most) {
   using P = Shape<S, DP, NR>;
   constexpr int kRows = P::kRows;
   using W = Work<kRows, kKeys>;
@@ -95,16 +95,11 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
     __syncwarp();
   };
   if (warp == 0) {
-    const int64_t total = W::total(a);
-    const int n = W::blocks(total, most);
-    Item it{0, 0, 0, 0, 0, 0, 0};
-    if ((int)blockIdx.x < n) {
-      const int64_t u0 = W::start(total, blockIdx.x, n), u1 = W::start(total, blockIdx.x + 1, n);
-      it = W::find(a, u0);
-      it.n = (int)min((int64_t)(it.units - it.at), u1 - u0);
-      it.left = u1 - u0 - it.n;
+    const Stretch mine = W::stretch(a, blockIdx.x, most);
+    if (lane == 0) {
+      first = mine.first;
+      stretches[blockIdx.x] = mine;
     }
-    if (lane == 0) first = it;
   }
   if (PAD) clear();
   __syncthreads();
@@ -633,9 +628,10 @@ int launch(const Args &a, float *parts, int sms, cudaStream_t s) {
     if (dev < 128) ready[dev >> 6].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
   }
   const int most = sms * P::kBlocks;
-  kern<<<most, kThreads, P::kSmem, s>>>(a, parts, most);
+  Stretch *stretches = reinterpret_cast<Stretch *>(parts + 2 * (size_t)most * partial_floats(8 * NR, DP));
+  kern<<<most, kThreads, P::kSmem, s>>>(a, parts, stretches, most);
   count_launch();
-  return launch_join<T, 8 * NR, kKeys>(a, parts, most, nullptr, s);
+  return launch_join<T, 8 * NR>(a, parts, stretches, most, nullptr, s);
 }
 
 template <typename T, int S, int DP>
