@@ -26,7 +26,7 @@ NVCC_FLAGS = [
     "-O3", "-std=c++17", "-Xcompiler", "-fPIC", "-lineinfo",
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-ftz=false", "-prec-div=true", "-prec-sqrt=true", "-fmad=false",
-    "--expt-relaxed-constexpr", "-Xptxas", "-O3",
+    "--expt-relaxed-constexpr", "-Xptxas", "-O3", "-Xfatbin=-compress-all",
 ]
 
 
