@@ -144,6 +144,21 @@ __device__ __forceinline__ Part part_of(const Args &a, const Item &it) {
   return p;
 }
 
+// What a warp knows of its item, kept in shared memory: registers are for what every step needs.
+struct Stash {
+  Item it;
+  Part p;
+};
+// The stash is written by one lane and read by all; the barriers keep the compiler from holding copies.
+__device__ __forceinline__ void put(Stash &st, const Item &it, const Part &p) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) {
+    st.it = it;
+    st.p = p;
+  }
+  __syncwarp();
+}
+
 // ---------------------------------------------------------------- producers
 // A job is 32 keys (a quarter) of a unit's K or V: job 8 u + 4 side + quarter of the block's unit u. A warp
 // takes every seventh.
@@ -155,7 +170,7 @@ struct Job {
 };
 
 template <typename T, int S, int DP>
-__device__ __forceinline__ bool produce(const Args &a, Item it, unsigned char *ks, unsigned char *vs, KeySlot *slots,
+__device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsigned char *vs, KeySlot *slots, Stash &mine,
                                         Barriers &bar, int polls) {
   constexpr int kRowBytes = S == KV_NONE ? 2 * DP : S == KV_MXFP4 ? DP / 2 : DP;
   constexpr int kCpr = kRowBytes / 16;                            // 16-byte chunks of a row
@@ -169,31 +184,31 @@ __device__ __forceinline__ bool produce(const Args &a, Item it, unsigned char *k
   const int chunk0 = kCpr >= 4 ? lane >> 3 : (lane >> 3) & 1;
   const bool fits = c.dim == DP;
 
-  // The item that the jobs being looked up belong to, and its first unit in the block's count.
-  Part p = part_of(a, it);
+  // The stash holds the item that the jobs being looked up belong to; base is its first unit in the block's count.
   uint32_t base = 0;
   bool over = false;
   auto look = [&](uint32_t job) {
     Job r{-1, 0, 0, false};
     const uint32_t unit = job >> 3;
-    while (!over && unit >= base + (uint32_t)p.steps) {
-      base += (uint32_t)p.steps;
+    while (!over && unit >= base + (uint32_t)mine.p.steps) {
+      base += (uint32_t)mine.p.steps;
+      Item it = mine.it;
       if (it.left == 0) {
         over = true;
       } else {
         W::next(a, it);
-        p = part_of(a, it);
+        put(mine, it, part_of(a, it));
       }
     }
     if (over) return r;
-    const int p0 = p.key0 + (int)(unit - base) * kKeys, at = p0 + 32 * (int)(job & 3) + lane;
-    if (at < p.key1) {
-      const int pg = a.table[(int64_t)it.b * a.table_stride + (at >> c.page_shift)];
+    const int p0 = mine.p.key0 + (int)(unit - base) * kKeys, at = p0 + 32 * (int)(job & 3) + lane;
+    if (at < mine.p.key1) {
+      const int pg = a.table[(int64_t)mine.it.b * a.table_stride + (at >> c.page_shift)];
       r.page = pg < c.pages ? pg : -1;
     }
     r.at = at;
-    r.head = it.head;
-    r.mixed = !(p0 >= p.all_lo && p0 + kKeys <= p.all_hi);
+    r.head = mine.it.head;
+    r.mixed = !(p0 >= mine.p.all_lo && p0 + kKeys <= mine.p.all_hi);
     return r;
   };
   // Row of key `in` of the job, whose page is pg >= 0.
@@ -574,7 +589,7 @@ __device__ __forceinline__ void rescale(const float (&keep)[4], uint32_t to) {
 }
 
 template <typename T, int S, int DP>
-__device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *qs, const KeySlot *slots, uint32_t tmem,
+__device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const KeySlot *slots, Stash &mine, uint32_t tmem,
                                         Barriers &bar, int polls, float *parts) {
   constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
@@ -584,14 +599,15 @@ __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *q
   const bool qvec = ((uintptr_t)a.q | (uintptr_t)(a.q_tok * 2) | (uintptr_t)(a.q_head * 2)) % 16 == 0;
   uint32_t step = 0, ssteps = 0, items = 0;
   while (true) {
-    const Part p = part_of(a, it);
-    if (t == 0 || p.two) {
-      const int first = it.tile * kRows + t * kTile + row0;  // the warp's first row
+    if (t == 0 || mine.p.two) {
       // Q: a thread a row, as 16-bit operand; over quantized caches scaled by a power of two into fp16. The
       // sign of the scale goes into Q; a scale of 0 is replaced by one whose scores vanish but keep -Inf.
       float qmul = a.scale == 0.0f ? 1.1754943508222875e-38f : fabsf(a.scale);
       {
         const uint32_t flip = a.scale < 0.0f ? 0x80008000u : 0u;
+        const Part p = mine.p;
+        const Item it = mine.it;
+        const int first = it.tile * kRows + t * kTile + row0;  // the warp's first row
         const int r = first + lane, tok = min(r, p.rows - 1) / a.group;
         const T *qp = static_cast<const T *>(a.q) + (p.s.q0 + tok) * a.q_tok + (it.head * a.group + r % a.group) * a.q_head;
         uint32_t w[DP / 2];
@@ -640,14 +656,16 @@ __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *q
         sum2[i] = pack2(0.0f, 0.0f);
       }
       int vfield = kBf16 ? 127 : 0;  // exponent field of T
-      for (int j = 0; j < p.steps; ++j) {
+      const int steps = mine.p.steps, key0 = mine.p.key0, all_lo = mine.p.all_lo, all_hi = mine.p.all_hi;
+      __syncwarp();
+      for (int j = 0; j < steps; ++j) {
         const uint32_t n = step + j;
         const KeySlot &sl = slots[n % kSlots];
         if (!mbar_wait_sleep(&bar.slot[n % kSlots], (n / kSlots) & 1, polls)) return false;
         if (!mbar_wait(&bar.sfull[t], ssteps++ & 1, polls)) return false;
         tc5::fence_after_sync();
-        const int p0 = p.key0 + j * kKeys;
-        const bool whole = p0 >= p.all_lo && p0 + kKeys <= p.all_hi &&
+        const int p0 = key0 + j * kKeys;
+        const bool whole = p0 >= all_lo && p0 + kKeys <= all_hi &&
                            ((sl.valid[0] & ~sl.dead[0]) & (sl.valid[1] & ~sl.dead[1]) & (sl.valid[2] & ~sl.dead[2]) &
                             (sl.valid[3] & ~sl.dead[3])) == 0xFFFFFFFFu;
         int field = vfield;
@@ -666,7 +684,7 @@ __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *q
               int lo[4], hi[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                visible(a, p.s, min(first + 8 * i + g4, p.rows - 1) / a.group, lo[i], hi[i]);
+                visible(a, mine.p.s, min(mine.it.tile * kRows + t * kTile + row0 + 8 * i + g4, mine.p.rows - 1) / a.group, lo[i], hi[i]);
                 lo[i] -= p0 + kHalf * half;
                 hi[i] -= p0 + kHalf * half;
               }
@@ -709,6 +727,10 @@ __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *q
       // The item's part is done.
       if (!mbar_wait_sleep(&bar.ofull[t], items++ & 1, polls)) return false;
       tc5::fence_after_sync();
+      __syncwarp();
+      const Part p = mine.p;
+      const Item it = mine.it;
+      const int first = it.tile * kRows + t * kTile + row0;
       const bool done = it.at == 0 && it.n == it.units;
       float *part = parts + (size_t)(2 * blockIdx.x + (it.at > 0 ? 0 : 1)) * partial_floats(kRows, DP) + t * kTile + row0 + g4;
 #pragma unroll 1
@@ -761,9 +783,11 @@ __device__ __forceinline__ bool softmax(const Args &a, Item it, unsigned char *q
       }
       tc5::fence_before_sync();
     }
-    step += (uint32_t)p.steps;
+    step += (uint32_t)mine.p.steps;
+    Item it = mine.it;
     if (it.left == 0) return true;
     W::next(a, it);
+    put(mine, it, part_of(a, it));
   }
 }
 
@@ -772,6 +796,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
   constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char raw[];
   __shared__ KeySlot slots[kSlots];
+  __shared__ Stash stash[kSoftmaxWarps + kProducerWarps];
   __shared__ __align__(8) Barriers bar;
   __shared__ Item first;
   __shared__ uint32_t tmem_base;
@@ -815,11 +840,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
     bool ok = true;
     if (warp < kSoftmaxWarps) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-      ok = softmax<T, S, DP>(a, it, qs, slots, tmem, bar, polls, parts);
+      put(stash[warp], it, part_of(a, it));
+      ok = softmax<T, S, DP>(a, qs, slots, stash[warp], tmem, bar, polls, parts);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
       if (warp < kSoftmaxWarps + kProducerWarps) {
-        ok = produce<T, S, DP>(a, it, ks, vs, slots, bar, polls);
+        put(stash[warp], it, part_of(a, it));
+        ok = produce<T, S, DP>(a, ks, vs, slots, stash[warp], bar, polls);
         cp_async_wait_all();
       } else if (lane == 0) {
         bool issued = false;
