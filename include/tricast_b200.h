@@ -307,7 +307,7 @@ int tc_kv_read(const tc_kv_cache *cache, const int64_t *slots, int64_t tokens, v
 
 /* Bytes of scratch tc_paged_attention needs for these sizes (0 when none). */
 size_t tc_paged_attention_workspace(const tc_kv_cache *cache, int32_t q_heads, int64_t total_q, int32_t batch,
-                                    int32_t max_q_len);
+                                    int32_t max_q_len, int32_t max_pages);
 
 /* out = softmax(scale * q k^T) v over each sequence's cached keys and values, for the last tokens of the
  * sequence: q and out [total_q][q_heads][head_dim] of the cache's dtype (q with token and head strides in

@@ -92,7 +92,7 @@ EXPORTS = {
     "tc_kv_write": (C.c_int, [C.POINTER(TcKvCache), C.c_void_p, C.c_int64, C.c_int64, C.c_void_p, C.c_int64, C.c_int64,
                               C.c_void_p, C.c_int64, C.c_void_p]),
     "tc_kv_read": (C.c_int, [C.POINTER(TcKvCache), C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_void_p]),
-    "tc_paged_attention_workspace": (C.c_size_t, [C.POINTER(TcKvCache), C.c_int32, C.c_int64, C.c_int32, C.c_int32]),
+    "tc_paged_attention_workspace": (C.c_size_t, [C.POINTER(TcKvCache), C.c_int32, C.c_int64, C.c_int32, C.c_int32, C.c_int32]),
     "tc_paged_attention": (C.c_int, [C.POINTER(TcKvCache), C.c_void_p, C.c_int64, C.c_int64, C.c_int64, C.c_int32,
                                      C.c_void_p, C.c_int64, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
                                      C.c_float, C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t,

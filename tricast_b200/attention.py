@@ -67,7 +67,7 @@ def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens:
     index = device.index
     token_stride, head_stride, _ = q.stride()
     with N.on_device(index):
-        nbytes = lib.tc_paged_attention_workspace(cache._ref, heads, total, batch, max_q_len)
+        nbytes = lib.tc_paged_attention_workspace(cache._ref, heads, total, batch, max_q_len, max_pages)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
         status = lib.tc_paged_attention(
             cache._ref, q.data_ptr(), token_stride, head_stride, total, heads, block_table.data_ptr(), table_stride,

@@ -24,6 +24,10 @@ int launch_chunk_fp8(const Args &a, float *parts, Stretch *stretches, int *statu
 int launch_chunk_int8(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s);
 int launch_chunk_mxfp4(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s);
 
+int launch_packed(const Args &a, float *parts, Stretch *stretches, int *status, int most, unsigned char *packed, int max_units,
+                  cudaStream_t s);
+size_t packed_unit_bytes(int dim);
+
 static int launch_split(const Args &a, float *parts, cudaStream_t s) {
   const int sms = sm_count();
   return a.c.scheme == KV_NONE       ? launch_split_none(a, parts, sms, s)
@@ -44,7 +48,23 @@ static size_t chunk_parts(const KvCache &c) {
   return 2 * (size_t)sm_count() * partial_floats(256, split_width(c.dim)) * sizeof(float);
 }
 static size_t chunk_bytes(const KvCache &c) {
-  return chunk_parts(c) + (size_t)sm_count() * (sizeof(Stretch) + sizeof(int));
+  const size_t n = chunk_parts(c) + (size_t)sm_count() * (sizeof(Stretch) + sizeof(int));
+  return (n + 127) / 128 * 128;
+}
+
+// Whether the chunk kernel's operands are laid out once, before it, and not by every row tile again: for quantized
+// caches (the others need no conversion), from kPackRows query rows of a key / value head on, while the tables'
+// width bounds the room it takes by kPackBytes.
+constexpr int64_t kPackRows = 257;
+constexpr size_t kPackBytes = (size_t)1 << 29;
+static int pack_units(const KvCache &c, int max_pages) {
+  const int64_t n = (((int64_t)max_pages << c.page_shift) + 127) / 128;
+  return (int)(n < 1 ? 1 : n);
+}
+static size_t pack_bytes(const KvCache &c, int group, int batch, int64_t max_q, int max_pages) {
+  if (c.scheme == KV_NONE || max_q * group < kPackRows) return 0;
+  const double n = (double)batch * c.heads * pack_units(c, max_pages) * (double)packed_unit_bytes(c.dim);
+  return n <= (double)kPackBytes ? (size_t)n : 0;
 }
 
 static int launch_chunk(const Args &a, void *workspace, cudaStream_t s) {
@@ -52,7 +72,10 @@ static int launch_chunk(const Args &a, void *workspace, cudaStream_t s) {
   float *parts = static_cast<float *>(workspace);
   Stretch *stretches = reinterpret_cast<Stretch *>(static_cast<char *>(workspace) + chunk_parts(a.c));
   int *status = reinterpret_cast<int *>(stretches + most);
-  const int st = a.c.scheme == KV_NONE       ? launch_chunk_none(a, parts, stretches, status, most, s)
+  const int st = pack_bytes(a.c, a.group, a.batch, a.max_q, a.max_pages)
+                     ? launch_packed(a, parts, stretches, status, most, static_cast<unsigned char *>(workspace) + chunk_bytes(a.c),
+                                     pack_units(a.c, a.max_pages), s)
+                 : a.c.scheme == KV_NONE     ? launch_chunk_none(a, parts, stretches, status, most, s)
                  : a.c.scheme == KV_FP8_ROW  ? launch_chunk_fp8(a, parts, stretches, status, most, s)
                  : a.c.scheme == KV_INT8_ROW ? launch_chunk_int8(a, parts, stretches, status, most, s)
                                              : launch_chunk_mxfp4(a, parts, stretches, status, most, s);
@@ -65,12 +88,13 @@ static int launch_chunk(const Args &a, void *workspace, cudaStream_t s) {
 }  // namespace tc
 
 extern "C" size_t tc_paged_attention_workspace(const tc_kv_cache *cache, int32_t q_heads, int64_t total_q, int32_t batch,
-                                               int32_t max_q_len) {
+                                               int32_t max_q_len, int32_t max_pages) {
   using namespace tc;
   KvCache c;
   if (kv_cache_check(cache, c) != TC_OK || c.dtype == TC_F32) return 0;
   if (q_heads < c.heads || q_heads % c.heads) return 0;
-  if (attn::use_chunk(c, q_heads / c.heads, max_q_len)) return attn::chunk_bytes(c);
+  const int group = q_heads / c.heads;
+  if (attn::use_chunk(c, group, max_q_len)) return attn::chunk_bytes(c) + attn::pack_bytes(c, group, batch, max_q_len, max_pages);
   return attn::split_bytes(c);
 }
 
@@ -118,7 +142,7 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
     attn::plain_kernel<float><<<(unsigned)(want < most ? want : most), attn::kThreads, 0, s>>>(a);
     count_launch();
   } else {
-    if (!workspace || workspace_bytes < tc_paged_attention_workspace(cache, q_heads, total_q, batch, a.max_q))
+    if (!workspace || workspace_bytes < tc_paged_attention_workspace(cache, q_heads, total_q, batch, a.max_q, max_pages))
       return set_error("tc_paged_attention: workspace too small"), TC_WORKSPACE_TOO_SMALL;
     const int r = attn::use_chunk(a.c, a.group, a.max_q) ? attn::launch_chunk(a, workspace, s)
                                                          : attn::launch_split(a, static_cast<float *>(workspace), s);

@@ -31,8 +31,11 @@ namespace chunk {
 
 constexpr int kTile = 128, kRows = 2 * kTile, kKeys = 128, kSlots = 4;
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 7, kThreads = 512;  // and one warp for the MMA thread
-// Registers a thread: 128 at launch; 256 * 160 + 256 * 96 = 512 * 128.
-constexpr int kSoftmaxRegs = 160, kOtherRegs = 96;
+// Registers a thread: 128 at launch; 256 * 160 + 256 * 96 = 512 * 128. Over packed units one warp stands in for the
+// producers, in a group of four with the MMA thread's: 168 at launch; 256 * 216 + 128 * 72 = 384 * 168.
+constexpr int kPackedThreads = 384;
+constexpr int softmax_regs(bool packed) { return packed ? 216 : 160; }
+constexpr int other_regs(bool packed) { return packed ? 72 : 96; }
 using W = Work<kRows, kKeys>;
 
 template <int DP>
@@ -49,6 +52,14 @@ struct __align__(16) KeySlot {
   uint32_t dead[4];   // keys whose rows of scores or values are not numbers: their scales here are 1, their V
                       // is 0, and the rows that see them become NaN
   int vfield[4];      // largest exponent field of the value scales, by quarter
+};
+
+// What pack_kernel leaves of a unit: the K and V tiles as they lie in shared memory, then the slot.
+constexpr int KV_PACKED = 100;  // in place of a scheme: the kernel over such units
+template <int DP>
+struct Packed {
+  static constexpr int kSlot = 2 * Shape<DP>::kOperand;
+  static constexpr int kBytes = kSlot + (int)(sizeof(KeySlot) + 127) / 128 * 128;
 };
 
 // 16 bytes (8 elements) of row r, granule q of a tile: 128-byte rows in blocks of 128, swizzled.
@@ -159,6 +170,78 @@ __device__ __forceinline__ void put(Stash &st, const Item &it, const Part &p) {
   __syncwarp();
 }
 
+// ---------------------------------------------------------------- codes to operands
+// Largest group exponent of a key (mxfp4), whose scales are the bytes of a word.
+template <int DP>
+__device__ __forceinline__ int biggest(uint32_t w) {
+  int big = 0;
+#pragma unroll
+  for (int q = 0; q < DP / 32; ++q) big = max(big, (int)((w >> (8 * q)) & 0xFFu));
+  return big;
+}
+// What a group's elements are multiplied by, twice, for a key of this largest exponent.
+__device__ __forceinline__ uint32_t group_mul(uint32_t exponent, int big) {
+  return half_pow2((int)exponent - big + kGroupShift) * 0x10001u;
+}
+// Eight 16-bit elements: granule g of 16 bytes of codes.
+template <int S>
+__device__ __forceinline__ void granule(const uint32_t (&w)[4], int g, uint32_t mul, uint32_t (&h)[4]) {
+  if (S == KV_MXFP4) {
+    e2m1x8_half2(w[g % 4], h);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = mul_half2(h[k], mul);
+  } else {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const uint32_t v = w[(2 * g + k) % 4];
+      if (S == KV_FP8_ROW) {
+        e4m3x4_half2(v, h[2 * k], h[2 * k + 1]);
+      } else {
+        h[2 * k] = int8x2_half2<0x4140>(v ^ 0x80808080u);
+        h[2 * k + 1] = int8x2_half2<0x4342>(v ^ 0x80808080u);
+      }
+    }
+  }
+}
+// A quarter's entries of its unit's slot, a lane a key: its scales' words, whether it is there, and whether its
+// rows of an unquantized cache are not numbers.
+template <int S, int DP>
+__device__ __forceinline__ void put_keys(KeySlot &sl, int quarter, bool there, uint32_t kw, uint32_t vw, bool dead) {
+  const int lane = threadIdx.x & 31;
+  float k = 1.0f, v = 1.0f;
+  if (S == KV_MXFP4) {
+    k = pow2_value((uint32_t)biggest<DP>(kw)) * (1.0f / (1 << kGroupShift));
+    v = pow2_value((uint32_t)biggest<DP>(vw)) * (1.0f / (1 << kGroupShift));
+  } else if (S != KV_NONE) {
+    k = u2f(kw);
+    v = u2f(vw);
+  }
+  dead |= k != k || v != v;
+  if (!there || dead) k = v = 1.0f;
+  sl.k[32 * quarter + lane] = k;
+  sl.v[32 * quarter + lane] = v;
+  const uint32_t valid = __ballot_sync(0xFFFFFFFFu, there), dead_keys = __ballot_sync(0xFFFFFFFFu, there && dead);
+  const int top = (int)__reduce_max_sync(0xFFFFFFFFu, there && !dead ? f2u(v) >> 23 : 0u);
+  if (lane == 0) {
+    sl.valid[quarter] = valid;
+    sl.dead[quarter] = dead_keys;
+    sl.vfield[quarter] = top;
+  }
+}
+// The word of a row's scales.
+template <int S, int DP>
+__device__ __forceinline__ uint32_t scale_word(const KvCache &c, const unsigned char *scales, int64_t row) {
+  uint32_t w = 0u;
+  if (S == KV_MXFP4) {
+#pragma unroll
+    for (int q = 0; q < DP / 32; ++q)
+      if (q < c.scale_bytes) w |= (uint32_t)scales[row * c.scale_bytes + q] << (8 * q);
+  } else if (S != KV_NONE) {
+    w = *reinterpret_cast<const uint32_t *>(scales + row * 4);
+  }
+  return w;
+}
+
 // ---------------------------------------------------------------- producers
 // A job is 32 keys (a quarter) of a unit's K or V: job 8 u + 4 side + quarter of the block's unit u. A warp
 // takes every seventh.
@@ -220,25 +303,7 @@ __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsign
   auto bstep = [&](int i) { return kCpr >= 4 ? i / (kCpr / 4) : i; };
   auto cstep = [&](int i) { return kCpr >= 4 ? (i % (kCpr / 4)) * 4 : 0; };
   auto load_scale = [&](const unsigned char *scales, const Job &r) {
-    uint32_t w = 0u;
-    if (r.page >= 0) {
-      const int64_t row = row_at(r, r.page, lane);
-      if (S == KV_MXFP4) {
-#pragma unroll
-        for (int q = 0; q < DP / 32; ++q)
-          if (q < c.scale_bytes) w |= (uint32_t)scales[row * c.scale_bytes + q] << (8 * q);
-      } else if (S != KV_NONE) {
-        w = *reinterpret_cast<const uint32_t *>(scales + row * 4);
-      }
-    }
-    return w;
-  };
-  // Largest group exponent of a key (mxfp4).
-  auto biggest = [&](uint32_t w) {
-    int big = 0;
-#pragma unroll
-    for (int q = 0; q < DP / 32; ++q) big = max(big, (int)((w >> (8 * q)) & 0xFFu));
-    return big;
+    return r.page >= 0 ? scale_word<S, DP>(c, scales, row_at(r, r.page, lane)) : 0u;
   };
   // Where rows of a job differ in what they see, a V row of an unquantized cache that is not finite must not
   // reach the others: the whole row counts as 0 and the weights of the rows that see it become NaN.
@@ -253,30 +318,7 @@ __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsign
   };
   // The keys' entries of the unit's slot.
   auto put_slot = [&](uint32_t job, const Job &r, uint32_t kw, uint32_t vw) {
-    KeySlot &sl = slots[(job >> 3) % kSlots];
-    const int quarter = job & 3;
-    float k = 1.0f, v = 1.0f;
-    bool dead = false;
-    if (S == KV_MXFP4) {
-      k = pow2_value((uint32_t)biggest(kw)) * (1.0f / (1 << kGroupShift));
-      v = pow2_value((uint32_t)biggest(vw)) * (1.0f / (1 << kGroupShift));
-    } else if (S != KV_NONE) {
-      k = u2f(kw);
-      v = u2f(vw);
-    } else {
-      dead = not_finite(r);
-    }
-    dead |= k != k || v != v;
-    if (r.page < 0 || dead) k = v = 1.0f;
-    sl.k[32 * quarter + lane] = k;
-    sl.v[32 * quarter + lane] = v;
-    const uint32_t valid = __ballot_sync(0xFFFFFFFFu, r.page >= 0), dead_keys = __ballot_sync(0xFFFFFFFFu, r.page >= 0 && dead);
-    const int top = (int)__reduce_max_sync(0xFFFFFFFFu, r.page >= 0 && !dead ? f2u(v) >> 23 : 0u);
-    if (lane == 0) {
-      sl.valid[quarter] = valid;
-      sl.dead[quarter] = dead_keys;
-      sl.vfield[quarter] = top;
-    }
+    put_keys<S, DP>(slots[(job >> 3) % kSlots], job & 3, r.page >= 0, kw, vw, S == KV_NONE && not_finite(r));
   };
   auto wait_empty = [&](uint32_t job) {
     const uint32_t unit = job >> 3, st = unit & 1, parity = ((unit >> 1) & 1) ^ 1;
@@ -313,33 +355,18 @@ __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsign
       return v;
     };
     // Chunk i as 16-bit granules into a tile (a shared-memory address).
-    auto convert = [&](const uint4 in, uint32_t scale_word, uint32_t dead_keys, uint32_t dst, int i) {
+    auto convert = [&](const uint4 in, uint32_t word, uint32_t dead_keys, uint32_t dst, int i) {
       const int key = key_of(bstep(i));
       const uint32_t w[4] = {in.x, in.y, in.z, in.w};
       uint32_t mul = 0u;
       if (S == KV_MXFP4) {
-        const uint32_t sw = __shfl_sync(0xFFFFFFFFu, scale_word, key);
-        mul = half_pow2((int)((sw >> (8 * chunk0)) & 0xFFu) - biggest(sw) + kGroupShift) * 0x10001u;
+        const uint32_t sw = __shfl_sync(0xFFFFFFFFu, word, key);
+        mul = group_mul((sw >> (8 * chunk0)) & 0xFFu, biggest<DP>(sw));
       }
 #pragma unroll
       for (int g = 0; g < kOut; ++g) {
         uint32_t h[4];
-        if (S == KV_MXFP4) {
-          e2m1x8_half2(w[g % 4], h);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) h[k] = mul_half2(h[k], mul);
-        } else {
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const uint32_t v = w[(2 * g + k) % 4];
-            if (S == KV_FP8_ROW) {
-              e4m3x4_half2(v, h[2 * k], h[2 * k + 1]);
-            } else {
-              h[2 * k] = int8x2_half2<0x4140>(v ^ 0x80808080u);
-              h[2 * k + 1] = int8x2_half2<0x4342>(v ^ 0x80808080u);
-            }
-          }
-        }
+        granule<S>(w, g, mul, h);
         // A key with a NaN value scale has NaN codes, which would reach rows that do not see it as 0 * NaN:
         // they count as 0.
         if (S == KV_FP8_ROW && dead_keys && ((dead_keys >> key) & 1u)) h[0] = h[1] = h[2] = h[3] = 0u;
@@ -429,6 +456,42 @@ __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsign
       job = ahead;
     }
   }
+}
+
+// ---------------------------------------------------------------- packed units (one thread)
+// Brings the units that pack_kernel has laid out: what the producers make, three bulk copies a unit.
+template <int DP>
+__device__ __forceinline__ bool fetch(const Args &a, Item it, const unsigned char *packed, int max_units, unsigned char *ks,
+                                      unsigned char *vs, KeySlot *slots, Barriers &bar, int polls) {
+  uint32_t step = 0, nk = 0, nv = 0;  // units whose K (and slot), whose V copies are on their way
+  bool ok = true;
+  while (ok) {
+    const Part p = part_of(a, it);
+    const unsigned char *from = packed + ((int64_t)(it.b * a.c.heads + it.head) * max_units + p.key0 / kKeys) * Packed<DP>::kBytes;
+    for (uint32_t n = step; n < step + (uint32_t)p.steps; ++n, from += Packed<DP>::kBytes) {
+      const uint32_t st = n & 1, parity = ((n >> 1) & 1) ^ 1;
+      if (!(ok = mbar_wait_sleep(&bar.kempty[st], parity, polls))) break;
+      mbar_expect_tx(&bar.kfull[st], Shape<DP>::kOperand);
+      bulk_g2s(ks + st * Shape<DP>::kOperand, from, Shape<DP>::kOperand, &bar.kfull[st]);
+      mbar_expect_tx(&bar.slot[n % kSlots], sizeof(KeySlot));
+      bulk_g2s(&slots[n % kSlots], from + Packed<DP>::kSlot, sizeof(KeySlot), &bar.slot[n % kSlots]);
+      ++nk;
+      if (!(ok = mbar_wait_sleep(&bar.vempty[st], parity, polls))) break;
+      mbar_expect_tx(&bar.vfull[st], Shape<DP>::kOperand);
+      bulk_g2s(vs + st * Shape<DP>::kOperand, from + Shape<DP>::kOperand, Shape<DP>::kOperand, &bar.vfull[st]);
+      ++nv;
+    }
+    step += (uint32_t)p.steps;
+    if (it.left == 0) break;
+    W::next(a, it);
+  }
+  // The block's shared memory stays until the copies are in.
+  for (uint32_t k = nk > 2 ? nk - 2 : 0; k < nk; ++k) {
+    mbar_wait_sleep(&bar.kfull[k & 1], (k >> 1) & 1);
+    mbar_wait_sleep(&bar.slot[k % kSlots], (k / kSlots) & 1);
+  }
+  for (uint32_t k = nv > 2 ? nv - 2 : 0; k < nv; ++k) mbar_wait_sleep(&bar.vfull[k & 1], (k >> 1) & 1);
+  return ok;
 }
 
 // ---------------------------------------------------------------- MMA issue (one thread)
@@ -792,11 +855,14 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
 }
 
 template <typename T, int S, int DP>
-__global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts, Stretch *stretches, int *status, int most, int polls) {
+__global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 1) chunk_kernel(Args a, float *parts, Stretch *stretches, int *status, int most, int polls,
+                                                                 const unsigned char *packed, int max_units) {
+  constexpr bool kPacked = S == KV_PACKED;
+  constexpr int kFullArrivals = kPacked ? 1 : 4, kFeeders = kPacked ? 1 : kProducerWarps;
   constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
   extern __shared__ unsigned char raw[];
   __shared__ KeySlot slots[kSlots];
-  __shared__ Stash stash[kSoftmaxWarps + kProducerWarps];
+  __shared__ Stash stash[kSoftmaxWarps + (kPacked ? 0 : kProducerWarps)];
   __shared__ __align__(8) Barriers bar;
   __shared__ Item first;
   __shared__ uint32_t tmem_base;
@@ -814,8 +880,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
   }
   if (threadIdx.x == 0) {
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&bar.kfull[i], 4);
-      mbar_init(&bar.vfull[i], 4);
+      mbar_init(&bar.kfull[i], kFullArrivals);
+      mbar_init(&bar.vfull[i], kFullArrivals);
       mbar_init(&bar.kempty[i], 1);
       mbar_init(&bar.vempty[i], 1);
       mbar_init(&bar.qfull[i], 4);
@@ -825,7 +891,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
       mbar_init(&bar.phalf[i], 1);
       mbar_init(&bar.ofull[i], 1);
     }
-    for (int i = 0; i < kSlots; ++i) mbar_init(&bar.slot[i], 4);
+    for (int i = 0; i < kSlots; ++i) mbar_init(&bar.slot[i], kFullArrivals);
     mbar_init(&bar.drain, 1);
     fence_barrier_init();
   }
@@ -834,21 +900,26 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
   __syncthreads();
   tc5::fence_after_sync();
   let_next_start();
+  if (kPacked) wait_for_previous();
   const Item it = first;
   const uint32_t tmem = tmem_base;
   if (it.n > 0) {
     bool ok = true;
     if (warp < kSoftmaxWarps) {
-      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(softmax_regs(kPacked)));
       put(stash[warp], it, part_of(a, it));
       ok = softmax<T, S, DP>(a, qs, slots, stash[warp], tmem, bar, polls, parts);
     } else {
-      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-      if (warp < kSoftmaxWarps + kProducerWarps) {
-        put(stash[warp], it, part_of(a, it));
-        ok = produce<T, S, DP>(a, ks, vs, slots, stash[warp], bar, polls);
-        cp_async_wait_all();
-      } else if (lane == 0) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(other_regs(kPacked)));
+      if (warp < kSoftmaxWarps + kFeeders) {
+        if constexpr (kPacked) {
+          if (lane == 0) ok = fetch<DP>(a, it, packed, max_units, ks, vs, slots, bar, polls);
+        } else {
+          put(stash[warp], it, part_of(a, it));
+          ok = produce<T, S, DP>(a, ks, vs, slots, stash[warp], bar, polls);
+          cp_async_wait_all();
+        }
+      } else if (warp == kSoftmaxWarps + kFeeders && lane == 0) {
         bool issued = false;
         ok = multiply<kBf16, DP>(a, it, smem_addr(qs), smem_addr(ks), smem_addr(vs), tmem, bar, polls, issued);
         if (issued) {
@@ -868,8 +939,75 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(Args a, float *parts
   if (threadIdx.x == 0) status[blockIdx.x] = failed;
 }
 
+// ---------------------------------------------------------------- packing
+// Lays units out as operands: a block one unit of a sequence's key / value head, a warp one of the jobs that the
+// producers would do for every row tile again. Bound by the memory it writes.
+template <int S, int DP>
+__global__ void __launch_bounds__(256) pack_kernel(Args a, unsigned char *packed, int max_units) {
+  constexpr int kRowBytes = S == KV_MXFP4 ? DP / 2 : DP, kCpr = kRowBytes / 16, kOut = S == KV_MXFP4 ? 4 : 2;
+  const KvCache &c = a.c;
+  const int unit = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
+  const int side = threadIdx.x >> 7, quarter = (threadIdx.x >> 5) & 3, lane = threadIdx.x & 31;
+  let_next_start();
+  const Seq s = sequence(a, b);
+  if (s.n == 0) return;
+  // Every unit that a row tile visits; the first one also where there are no keys.
+  int lo, hi, unused;
+  visible(a, s, 0, lo, hi);
+  lo = min(lo, hi);
+  visible(a, s, s.n - 1, unused, hi);
+  if (unit * kKeys >= max(hi, 1) || (unit + 1) * kKeys <= lo) return;
+  unsigned char *to = packed + ((int64_t)(b * c.heads + head) * max_units + unit) * Packed<DP>::kBytes;
+  const int at = unit * kKeys + 32 * quarter + lane;
+  int page = -1;
+  if (at < hi) {
+    const int pg = a.table[(int64_t)b * a.table_stride + (at >> c.page_shift)];
+    page = pg < c.pages ? pg : -1;
+  }
+  auto row_at = [&](int pg, int in) -> int64_t {
+    return (((int64_t)pg * c.heads + head) << c.page_shift) + ((at - lane + in) & (c.page_size - 1));
+  };
+  const uint32_t vw = page >= 0 ? scale_word<S, DP>(c, c.vs, row_at(page, lane)) : 0u;
+  uint32_t word = vw;
+  if (side == 0) {
+    word = page >= 0 ? scale_word<S, DP>(c, c.ks, row_at(page, lane)) : 0u;
+    put_keys<S, DP>(*reinterpret_cast<KeySlot *>(to + Packed<DP>::kSlot), quarter, page >= 0, word, vw, false);
+  }
+  // A key with a NaN value scale has NaN codes, which would reach rows that do not see it as 0 * NaN: they count
+  // as 0.
+  const uint32_t dead = S == KV_FP8_ROW && side ? __ballot_sync(0xFFFFFFFFu, (vw & 0x7FFFFFFFu) > kInf) : 0u;
+  const unsigned char *codes = side ? c.v : c.k;
+  to += side * Shape<DP>::kOperand;
+  uint4 buf[kCpr];
+  // Lane and step i: chunk n % kCpr of key n / kCpr for n = 32 i + lane.
+#pragma unroll
+  for (int i = 0; i < kCpr; ++i) {
+    const int key = (32 * i + lane) / kCpr, ch = lane % kCpr, pg = __shfl_sync(0xFFFFFFFFu, page, key);
+    buf[i] = make_uint4(0, 0, 0, 0);
+    if (pg >= 0 && 16 * ch < c.row_bytes) buf[i] = load_once(codes + row_at(pg, key) * c.row_bytes + 16 * ch);
+  }
+#pragma unroll
+  for (int i = 0; i < kCpr; ++i) {
+    const int key = (32 * i + lane) / kCpr, ch = lane % kCpr;
+    const uint32_t w[4] = {buf[i].x, buf[i].y, buf[i].z, buf[i].w};
+    uint32_t mul = 0u;
+    if (S == KV_MXFP4) {
+      const uint32_t sw = __shfl_sync(0xFFFFFFFFu, word, key);
+      mul = group_mul((sw >> (8 * ch)) & 0xFFu, biggest<DP>(sw));
+    }
+#pragma unroll
+    for (int g = 0; g < kOut; ++g) {
+      uint32_t h[4];
+      granule<S>(w, g, mul, h);
+      if (S == KV_FP8_ROW && ((dead >> key) & 1u)) h[0] = h[1] = h[2] = h[3] = 0u;
+      *reinterpret_cast<uint4 *>(to + tile_at(32 * quarter + key, ch * kOut + g)) = make_uint4(h[0], h[1], h[2], h[3]);
+    }
+  }
+}
+
 template <typename T, int S, int DP>
-int launch(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s) {
+int launch(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s, const unsigned char *packed = nullptr,
+           int max_units = 0) {
   auto kern = chunk_kernel<T, S, DP>;
   static std::atomic<uint64_t> ready[2];  // devices whose shared-memory limit is raised
   int dev = 0;
@@ -880,17 +1018,40 @@ int launch(const Args &a, float *parts, Stretch *stretches, int *status, int mos
     if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
     if (dev < 128) ready[dev >> 6].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
   }
-  kern<<<most, kThreads, Shape<DP>::kSmem, s>>>(a, parts, stretches, status, most, wait_polls());
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(most);
+  cfg.blockDim = dim3((S == KV_PACKED ? kPackedThreads : kThreads));
+  cfg.dynamicSmemBytes = Shape<DP>::kSmem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // over packed units: starts as pack_kernel ends
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = S == KV_PACKED ? 1 : 0;
+  e = cudaLaunchKernelEx(&cfg, kern, a, parts, stretches, status, most, wait_polls(), packed, max_units);
+  if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
   count_launch();
   return TC_OK;
 }
 
 template <int S>
-int launch_scheme(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s) {
+int launch_scheme(const Args &a, float *parts, Stretch *stretches, int *status, int most, cudaStream_t s,
+                  const unsigned char *packed = nullptr, int max_units = 0) {
   const bool bf16 = a.c.dtype == TC_BF16;
   if (a.c.dim <= 64)
-    return bf16 ? launch<__nv_bfloat16, S, 64>(a, parts, stretches, status, most, s) : launch<__half, S, 64>(a, parts, stretches, status, most, s);
-  return bf16 ? launch<__nv_bfloat16, S, 128>(a, parts, stretches, status, most, s) : launch<__half, S, 128>(a, parts, stretches, status, most, s);
+    return bf16 ? launch<__nv_bfloat16, S, 64>(a, parts, stretches, status, most, s, packed, max_units) : launch<__half, S, 64>(a, parts, stretches, status, most, s, packed, max_units);
+  return bf16 ? launch<__nv_bfloat16, S, 128>(a, parts, stretches, status, most, s, packed, max_units) : launch<__half, S, 128>(a, parts, stretches, status, most, s, packed, max_units);
+}
+
+// Packs the call's units, then runs the kernel over them.
+template <int S>
+int launch_packed(const Args &a, float *parts, Stretch *stretches, int *status, int most, unsigned char *packed, int max_units,
+                  cudaStream_t s) {
+  const dim3 grid((unsigned)max_units, (unsigned)a.c.heads, (unsigned)a.batch);
+  if (a.c.dim <= 64) pack_kernel<S, 64><<<grid, 256, 0, s>>>(a, packed, max_units);
+  else pack_kernel<S, 128><<<grid, 256, 0, s>>>(a, packed, max_units);
+  count_launch();
+  return launch_scheme<KV_PACKED>(a, parts, stretches, status, most, s, packed, max_units);
 }
 
 }  // namespace chunk
