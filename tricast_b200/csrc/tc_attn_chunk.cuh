@@ -32,10 +32,10 @@ namespace chunk {
 constexpr int kTile = 128, kRows = 2 * kTile, kKeys = 128, kSlots = 4;
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 7, kThreads = 512;  // and one warp for the MMA thread
 // Registers a thread: 128 at launch; 256 * 160 + 256 * 96 = 512 * 128. Over packed units one warp stands in for the
-// producers, in a group of four with the MMA thread's: 168 at launch; 256 * 216 + 128 * 72 = 384 * 168.
+// producers, in a group of four with the MMA thread's: 168 at launch; 256 * 200 + 128 * 104 = 384 * 168.
 constexpr int kPackedThreads = 384;
-constexpr int softmax_regs(bool packed) { return packed ? 216 : 160; }
-constexpr int other_regs(bool packed) { return packed ? 72 : 96; }
+constexpr int softmax_regs(bool packed) { return packed ? 200 : 160; }
+constexpr int other_regs(bool packed) { return packed ? 104 : 96; }
 using W = Work<kRows, kKeys>;
 
 template <int DP>
