@@ -312,15 +312,15 @@ __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Merges the partial results of the items that several blocks share. One block for each border between two
-// stretches and 8 or 16 rows of the item; it acts if the border is the first inside its item. A row's maxima and sums are read side by side into shared memory (as many
+// stretches and up to 64 rows of the item; it acts if the border is the first inside its item. A row's maxima and sums are read side by side into shared memory (as many
 // parts at a time as it holds), its outputs [dim][row] by four rows a thread. Where `status` is given and a block
 // of the kernel before gave up a wait (which takes a fault elsewhere, or a test), everything is computed again by
 // the plain rows.
-constexpr int kJoinParts = 128, kJoinThreads = 256;
-constexpr int join_rows(int rows) { return rows < 16 ? rows : 16; }  // of an item, a block
+constexpr int kJoinThreads = 256;
+constexpr int join_rows(int rows) { return rows < 64 ? rows : 64; }  // of an item, a block
 template <typename T, int kRows>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float *parts, const Stretch *stretches, int dim_pad, int most, const int *status) {
-  constexpr int kJoinRows = join_rows(kRows);
+  constexpr int kJoinRows = join_rows(kRows), kJoinParts = 2048 / kJoinRows;
   __shared__ Item item;
   __shared__ int from, upto;
   __shared__ float part_top[kJoinParts][kJoinRows], part_sum[kJoinParts][kJoinRows];
@@ -371,9 +371,9 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
     top[threadIdx.x] = -INFINITY;
     sum[threadIdx.x] = 0.0f;
   }
-  constexpr int kQuads = kJoinRows / 4, kLanesD = kJoinThreads / kQuads;  // a thread: four rows of every 64th dim
+  constexpr int kQuads = kJoinRows / 4, kLanesD = kJoinThreads / kQuads;  // a thread: four rows of every kLanesD-th dim
   const int quad = threadIdx.x % kQuads, d0 = threadIdx.x / kQuads;
-  constexpr int kDims = (256 + kLanesD - 1) / kLanesD;
+  constexpr int kDims = ((kRows > 16 ? 128 : 256) + kLanesD - 1) / kLanesD;  // the chunk kernel's heads end at 128
   float4 acc[kDims];
 #pragma unroll
   for (int i = 0; i < kDims; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

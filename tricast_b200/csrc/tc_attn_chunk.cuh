@@ -29,7 +29,7 @@ namespace tc {
 namespace attn {
 namespace chunk {
 
-constexpr int kTile = 128, kRows = 2 * kTile, kKeys = 128, kSlots = 4;
+constexpr int kTile = 128, kRows = 2 * kTile, kKeys = 128, kHalf = kKeys / 2, kSlots = 4;
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 7, kThreads = 512;  // and one warp for the MMA thread
 // Registers a thread: 128 at launch; 256 * 160 + 256 * 96 = 512 * 128. Over packed units one warp stands in for the
 // producers, in a group of four with the MMA thread's: 168 at launch; 256 * 200 + 128 * 104 = 384 * 168.
@@ -127,8 +127,19 @@ __device__ __forceinline__ void warp_arrive(uint64_t *bar) {
   if ((threadIdx.x & 31) == 0) mbar_arrive(bar);
 }
 
+// Waits by a whole warp, whose threads go on together or give up together.
+__device__ __forceinline__ bool warp_wait(uint64_t *bar, uint32_t parity, int polls) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait(bar, parity, polls));
+}
+__device__ __forceinline__ bool warp_wait_sleep(uint64_t *bar, uint32_t parity, int polls) {
+  return __all_sync(0xFFFFFFFFu, mbar_wait_sleep(bar, parity, polls));
+}
+
+// The same value in every thread of the warp, known to be.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xFFFFFFFFu, v, 0); }
+
 struct Barriers {
-  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], slot[kSlots], qfull[2], sfull[2], pfull[2][2], phalf[2], ofull[2], drain;
+  uint64_t kfull[2], kempty[2], vfull[2], vempty[2], slot[kSlots], qfull[2], sfull[2], pfull[2][2], pvdone[2], ofull[2], drain;
 };
 
 // Bounds of an item that every role derives alike.
@@ -322,7 +333,7 @@ __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsign
   };
   auto wait_empty = [&](uint32_t job) {
     const uint32_t unit = job >> 3, st = unit & 1, parity = ((unit >> 1) & 1) ^ 1;
-    return mbar_wait_sleep((job & 4) ? &bar.vempty[st] : &bar.kempty[st], parity, polls);
+    return warp_wait_sleep((job & 4) ? &bar.vempty[st] : &bar.kempty[st], parity, polls);
   };
   auto arrive_full = [&](uint32_t job) {
     const uint32_t unit = job >> 3, st = unit & 1;
@@ -494,7 +505,9 @@ __device__ __forceinline__ bool fetch(const Args &a, Item it, const unsigned cha
   return ok;
 }
 
-// ---------------------------------------------------------------- MMA issue (one thread)
+// ---------------------------------------------------------------- MMA issue (one warp)
+// The warp stays together and one of its threads issues: what the instructions take in uniform registers is then
+// prepared once. A lone thread in a branch of its own took about 110 cycles an MMA.
 template <bool BF16, int DP>
 __device__ __forceinline__ bool multiply(const Args &a, Item it, uint32_t qs, uint32_t ks, uint32_t vs, uint32_t tmem,
                                          Barriers &bar, int polls, bool &issued) {
@@ -504,55 +517,64 @@ __device__ __forceinline__ bool multiply(const Args &a, Item it, uint32_t qs, ui
   uint32_t step = 0, items[2] = {0u, 0u}, psteps[2] = {0u, 0u};
   while (true) {
     const Part p = part_of(a, it);
-    const int tiles = p.two ? 2 : 1;
-    auto qk = [&](int t, uint32_t n) {
-      const uint32_t k0 = ks + (n & 1) * Shape<DP>::kOperand, q0 = qs + t * Shape<DP>::kOperand;
-#pragma unroll
-      for (int k = 0; k < DP / 16; ++k) {
-        const uint32_t off = (k >> 2) * (kTile * 128) + (k & 3) * 32;
-        tc5::mma_f16_ss(tmem + t * 128, desc_sw128(q0 + off, 16), desc_sw128(k0 + off, 16), kQk, k > 0);
-      }
+    const int tiles = uniform(p.two ? 2 : 1), steps = uniform(p.steps);
+    // Scores of a unit; `then`: its keys are done with.
+    auto qk = [&](int t, uint32_t n, bool then) {
+      const uint64_t dk = desc_sw128(ks + (n & 1) * Shape<DP>::kOperand, 16);
+      const uint64_t dq = desc_sw128(qs + t * Shape<DP>::kOperand, 16);
+      const uint32_t d = tmem + t * 128;
       issued = true;
-      tc5::mma_commit(&bar.sfull[t]);
+      if (tc5::elect_one()) {
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint64_t off = ((k >> 2) * (kTile * 128) + (k & 3) * 32) >> 4;
+          tc5::mma_f16_ss(d, dq + off, dk + off, kQk, k > 0);
+        }
+        tc5::mma_commit(&bar.sfull[t]);
+        if (then) tc5::mma_commit(&bar.kempty[n & 1]);
+      }
+      __syncwarp();
     };
     for (int t = 0; t < tiles; ++t)
-      if (!mbar_wait_sleep(&bar.qfull[t], items[t]++ & 1, polls)) return false;
-    if (!mbar_wait(&bar.kfull[step & 1], (step >> 1) & 1, polls)) return false;
+      if (!warp_wait_sleep(&bar.qfull[t], items[t]++ & 1, polls)) return false;
+    if (!warp_wait(&bar.kfull[step & 1], (step >> 1) & 1, polls)) return false;
     tc5::fence_after_sync();
-    for (int t = 0; t < tiles; ++t) qk(t, step);
-    tc5::mma_commit(&bar.kempty[step & 1]);
-    for (int j = 0; j < p.steps; ++j) {
+    for (int t = 0; t < tiles; ++t) qk(t, step, t == tiles - 1);
+    for (int j = 0; j < steps; ++j) {
       const uint32_t n = step + j;
-      const bool more = j + 1 < p.steps;
-      for (int t = 0; t < tiles; ++t) {
-        const uint32_t v0 = vs + (n & 1) * Shape<DP>::kOperand;
-        for (int half = 0; half < 2; ++half) {
-          if (!mbar_wait(&bar.pfull[t][half], psteps[t] & 1, polls)) return false;
-          if (t == 0 && half == 0 && !mbar_wait(&bar.vfull[n & 1], (n >> 1) & 1, polls)) return false;
-          tc5::fence_after_sync();
+      const uint64_t dv = desc_sw128(vs + (n & 1) * Shape<DP>::kOperand, kTile * 128);
+      const bool more = j + 1 < steps;
 #pragma unroll
-          for (int k = 0; k < kKeys / 32; ++k) {
-            const int kk = half * (kKeys / 32) + k;
-            tc5::mma_f16_ts(tmem + 256 + t * DP, tmem + t * 128 + kk * 8, desc_sw128(v0 + kk * 2048, kTile * 128), kPv,
-                            j > 0 || kk > 0);
+      for (int t = 0; t < 2; ++t) {
+        if (t >= tiles) break;
+        const bool last = t == tiles - 1;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          if (!warp_wait(&bar.pfull[t][half], psteps[t] & 1, polls)) return false;
+          if (t == 0 && half == 0 && !warp_wait(&bar.vfull[n & 1], (n >> 1) & 1, polls)) return false;
+          tc5::fence_after_sync();
+          const uint32_t d = tmem + 256 + t * DP, w = tmem + t * 128 + half * kHalf;
+          if (tc5::elect_one()) {
+#pragma unroll
+            for (int k = 0; k < kHalf / 16; ++k)
+              tc5::mma_f16_ts(d, w + k * 8, dv + (half * (kHalf / 16) + k) * (2048 >> 4), kPv, j > 0 || half > 0 || k > 0);
+            tc5::mma_commit(&bar.pvdone[t]);
+            if (half && last) tc5::mma_commit(&bar.vempty[n & 1]);
+            if (half && !more) tc5::mma_commit(&bar.ofull[t]);
           }
-          if (half == 0) tc5::mma_commit(&bar.phalf[t]);
+          __syncwarp();
         }
         ++psteps[t];
-        if (t == tiles - 1) tc5::mma_commit(&bar.vempty[n & 1]);
         if (more) {
           if (t == 0) {
-            if (!mbar_wait(&bar.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1, polls)) return false;
+            if (!warp_wait(&bar.kfull[(n + 1) & 1], ((n + 1) >> 1) & 1, polls)) return false;
             tc5::fence_after_sync();
           }
-          qk(t, n + 1);
-          if (t == tiles - 1) tc5::mma_commit(&bar.kempty[(n + 1) & 1]);
-        } else {
-          tc5::mma_commit(&bar.ofull[t]);
+          qk(t, n + 1, last);
         }
       }
     }
-    step += (uint32_t)p.steps;
+    step += (uint32_t)steps;
     if (it.left == 0) return true;
     W::next(a, it);
   }
@@ -562,21 +584,28 @@ __device__ __forceinline__ bool multiply(const Args &a, Item it, uint32_t qs, ui
 // A step of the softmax covers half a unit. A warp's 32 rows are held as MMA fragments: thread (g, t) has columns
 // 8 j + 2 t, + 1 of rows 16 h + 8 e + g, rows 2 h + e of its four. A key's scale then serves four rows: what the
 // scales take of shared memory's bandwidth, which the MMAs need, is a quarter of a thread a row's.
-constexpr int kHalf = kKeys / 2, kPairs = kHalf / 8;
+constexpr int kPairs = kHalf / 8;
 using Rows = F2[4][kPairs];  // [row][j]: two neighbouring columns
 
-__device__ __forceinline__ void load_rows(uint32_t ts, Rows &x) {
+// As they come from TMEM: asked for, and there after `arrived`, through which they pass.
+struct Raw {
   uint32_t a[kHalf / 2], b[kHalf / 2];
-  tc5::tmem_ld_frag64(ts, a);
-  tc5::tmem_ld_frag64(ts + (16u << 16), b);
-  tc5::tmem_wait_ld_frag(a);
-  tc5::tmem_wait_ld_frag(b);
+};
+__device__ __forceinline__ void ask(uint32_t ts, Raw &r) {
+  tc5::tmem_ld_frag64(ts, r.a);
+  tc5::tmem_ld_frag64(ts + (16u << 16), r.b);
+}
+__device__ __forceinline__ void arrived(Raw &r) {
+  tc5::tmem_wait_ld_frag(r.a);
+  tc5::tmem_wait_ld_frag(r.b);
+}
+__device__ __forceinline__ void rows_of(const Raw &r, Rows &x) {
 #pragma unroll
   for (int j = 0; j < kPairs; ++j) {
-    x[0][j] = pack2(u2f(a[4 * j]), u2f(a[4 * j + 1]));
-    x[1][j] = pack2(u2f(a[4 * j + 2]), u2f(a[4 * j + 3]));
-    x[2][j] = pack2(u2f(b[4 * j]), u2f(b[4 * j + 1]));
-    x[3][j] = pack2(u2f(b[4 * j + 2]), u2f(b[4 * j + 3]));
+    x[0][j] = pack2(u2f(r.a[4 * j]), u2f(r.a[4 * j + 1]));
+    x[1][j] = pack2(u2f(r.a[4 * j + 2]), u2f(r.a[4 * j + 3]));
+    x[2][j] = pack2(u2f(r.b[4 * j]), u2f(r.b[4 * j + 1]));
+    x[3][j] = pack2(u2f(r.b[4 * j + 2]), u2f(r.b[4 * j + 3]));
   }
 }
 
@@ -724,25 +753,36 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
       for (int j = 0; j < steps; ++j) {
         const uint32_t n = step + j;
         const KeySlot &sl = slots[n % kSlots];
-        if (!mbar_wait_sleep(&bar.slot[n % kSlots], (n / kSlots) & 1, polls)) return false;
-        if (!mbar_wait(&bar.sfull[t], ssteps++ & 1, polls)) return false;
+        if (!warp_wait(&bar.sfull[t], ssteps & 1, polls)) return false;
         tc5::fence_after_sync();
+        Raw raw[2];
+        ask(ts, raw[0]);
+        // The slot after the scores, which a warp that had no rows for a while cannot be early for.
+        if (!warp_wait(&bar.slot[n % kSlots], (n / kSlots) & 1, polls)) return false;
         const int p0 = key0 + j * kKeys;
         const bool whole = p0 >= all_lo && p0 + kKeys <= all_hi &&
                            ((sl.valid[0] & ~sl.dead[0]) & (sl.valid[1] & ~sl.dead[1]) & (sl.valid[2] & ~sl.dead[2]) &
                             (sl.valid[3] & ~sl.dead[3])) == 0xFFFFFFFFu;
         int field = vfield;
-        if (!kBf16) field = max(max(field, max(sl.vfield[0], sl.vfield[1])), max(sl.vfield[2], sl.vfield[3]));
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
+        if (!kBf16) {
+          // With two binades to spare, so that slightly larger scales later on do not move it again.
+          const int top = max(max(sl.vfield[0], sl.vfield[1]), max(sl.vfield[2], sl.vfield[3]));
+          if (top > vfield) field = top + 2;
+        }
+        // Over packed units there are registers to ask for the second half before the first one's arithmetic.
+        constexpr bool kAhead = S == KV_PACKED;
+        auto step_half = [&](const int half) {
           // With the reference as it is. It moves when a row's maximum has risen by more than 2**8 (or from
           // nothing), and when a larger value scale comes, by whole powers of two, so that what it scales
           // stays exact; the half is then computed again.
           uint32_t pw[2][kHalf / 4];
           F2 part2[4];
+          if (half && !kAhead) ask(ts + kHalf, raw[half]);
+          arrived(raw[half]);
+          if (!half && kAhead) ask(ts + kHalf, raw[1]);
           while (true) {
             Rows x;
-            load_rows(ts + kHalf * half, x);
+            rows_of(raw[half], x);
             if (!whole) {
               int lo[4], hi[4];
 #pragma unroll
@@ -772,23 +812,29 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
               sum2[i] = mul2(sum2[i], pack2(keep[i], keep[i]));
             }
             vfield = field;
-            // Before the second half the first half's products must be in: the next S of the tile, which the
-            // steps above waited for, comes after all of them, but this half does not wait for that.
-            if (half && !mbar_wait(&bar.phalf[t], (ssteps - 1) & 1, polls)) return false;
-            if (half) tc5::fence_after_sync();
-            if (j > 0 || half) rescale<DP>(keep, to);
+            // The outputs so far: the products of the half before, which this half's scores did not wait for.
+            if (j > 0 || half) {
+              if (!warp_wait(&bar.pvdone[t], (half ^ 1) & 1, polls)) return false;
+              tc5::fence_after_sync();
+              rescale<DP>(keep, to);
+            }
+            ask(ts + kHalf * half, raw[half]);
+            arrived(raw[half]);
           }
-          tc5::tmem_st_pairs64(ts + 32 * half, pw[0]);
-          tc5::tmem_st_pairs64(ts + (16u << 16) + 32 * half, pw[1]);
+          tc5::tmem_st_pairs64(ts + kHalf * half, pw[0]);
+          tc5::tmem_st_pairs64(ts + (16u << 16) + kHalf * half, pw[1]);
 #pragma unroll
           for (int i = 0; i < 4; ++i) sum2[i] = add2(sum2[i], part2[i]);
           tc5::tmem_wait_st();
           tc5::fence_before_sync();
           warp_arrive(&bar.pfull[t][half]);
-        }
+          return true;
+        };
+        if (!step_half(0) || !step_half(1)) return false;
+        ++ssteps;
       }
       // The item's part is done.
-      if (!mbar_wait_sleep(&bar.ofull[t], items++ & 1, polls)) return false;
+      if (!warp_wait_sleep(&bar.ofull[t], items++ & 1, polls)) return false;
       tc5::fence_after_sync();
       __syncwarp();
       const Part p = mine.p;
@@ -869,7 +915,7 @@ __global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 
   __shared__ int failed;
   unsigned char *smem = raw + (1024 - (smem_addr(raw) & 1023)) % 1024;  // the swizzle is of address bits
   unsigned char *qs = smem, *ks = qs + 2 * Shape<DP>::kOperand, *vs = ks + 2 * Shape<DP>::kOperand;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   if (warp == kSoftmaxWarps) {
     const Stretch mine = W::stretch(a, blockIdx.x, most);
     if (lane == 0) {
@@ -888,7 +934,7 @@ __global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 
       mbar_init(&bar.pfull[i][0], 4);
       mbar_init(&bar.pfull[i][1], 4);
       mbar_init(&bar.sfull[i], 1);
-      mbar_init(&bar.phalf[i], 1);
+      mbar_init(&bar.pvdone[i], 1);
       mbar_init(&bar.ofull[i], 1);
     }
     for (int i = 0; i < kSlots; ++i) mbar_init(&bar.slot[i], kFullArrivals);
@@ -902,7 +948,7 @@ __global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 
   let_next_start();
   if (kPacked) wait_for_previous();
   const Item it = first;
-  const uint32_t tmem = tmem_base;
+  const uint32_t tmem = uniform(tmem_base);
   if (it.n > 0) {
     bool ok = true;
     if (warp < kSoftmaxWarps) {
@@ -919,12 +965,13 @@ __global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 
           ok = produce<T, S, DP>(a, ks, vs, slots, stash[warp], bar, polls);
           cp_async_wait_all();
         }
-      } else if (warp == kSoftmaxWarps + kFeeders && lane == 0) {
+      } else if (warp == kSoftmaxWarps + kFeeders) {
         bool issued = false;
         ok = multiply<kBf16, DP>(a, it, smem_addr(qs), smem_addr(ks), smem_addr(vs), tmem, bar, polls, issued);
         if (issued) {
           // No MMA may be in flight when the block's shared memory and TMEM go.
-          tc5::mma_commit(&bar.drain);
+          if (tc5::elect_one()) tc5::mma_commit(&bar.drain);
+          __syncwarp();
           mbar_wait_sleep(&bar.drain, 0);
         }
       }
