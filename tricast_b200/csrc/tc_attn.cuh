@@ -224,7 +224,8 @@ struct Work {
 // of this exponent field.
 __device__ __forceinline__ float room(int field) { return fminf(6.0f + (127.0f - (float)field), 100.0f); }
 
-// One partial result: kRows maxima (base-2 logarithms), kRows sums, then [dim][kRows] outputs.
+// One partial result: kRows maxima (base-2 logarithms), kRows sums, then the outputs as the kernel holds them:
+// [dim][kRows] of the split kernel (kRows 8 or 16), [kRows][dim] of the chunk kernel.
 __host__ __device__ constexpr size_t partial_floats(int rows, int dim) { return (size_t)rows * (dim + 2); }
 
 // Element d of a cached row, in fp32.
@@ -371,12 +372,15 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
     top[threadIdx.x] = -INFINITY;
     sum[threadIdx.x] = 0.0f;
   }
-  constexpr int kQuads = kJoinRows / 4, kLanesD = kJoinThreads / kQuads;  // a thread: four rows of every kLanesD-th dim
+  // Outputs of a thread, four at a time: rows of every kLanesD-th dim, or dims of a row of every kStep-th four.
+  constexpr bool kByRow = kRows > 16;
+  constexpr int kQuads = kJoinRows / 4, kLanesD = kJoinThreads / kQuads;
   const int quad = threadIdx.x % kQuads, d0 = threadIdx.x / kQuads;
-  constexpr int kDims = ((kRows > 16 ? 128 : 256) + kLanesD - 1) / kLanesD;  // the chunk kernel's heads end at 128
-  float4 acc[kDims];
+  constexpr int kFours = kByRow ? kJoinRows * (128 / 4) / kJoinThreads : (256 + kLanesD - 1) / kLanesD;
+  const int per_row = dim_pad / 4;
+  float4 acc[kFours];
 #pragma unroll
-  for (int i = 0; i < kDims; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  for (int i = 0; i < kFours; ++i) acc[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (int k0 = from; k0 < upto; k0 += kJoinParts) {
     const int n = min(kJoinParts, upto - k0);
     __syncthreads();
@@ -406,37 +410,69 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
       }
     }
     __syncthreads();
+    if constexpr (kByRow) {
 #pragma unroll
-    for (int i = 0; i < kDims; ++i) {
-      const int d = d0 + i * kLanesD;
-      if (d >= a.c.dim) break;
-      float4 v = acc[i];
-      v.x *= keep[4 * quad], v.y *= keep[4 * quad + 1], v.z *= keep[4 * quad + 2], v.w *= keep[4 * quad + 3];
-#pragma unroll 8
-      for (int k = 0; k < n; ++k) {
-        const float4 o = *reinterpret_cast<const float4 *>(slot(k0 + k) + (size_t)(2 + d) * kRows + 4 * quad);
-        const float *w = &part_top[k][4 * quad];
-        if (w[0] != 0.0f) v.x += o.x * w[0];
-        if (w[1] != 0.0f) v.y += o.y * w[1];
-        if (w[2] != 0.0f) v.z += o.z * w[2];
-        if (w[3] != 0.0f) v.w += o.w * w[3];
+      for (int i = 0; i < kFours; ++i) {
+        const int four = threadIdx.x + i * kJoinThreads, row = four / per_row, d = 4 * (four % per_row);
+        if (row >= kJoinRows) break;
+        const float f = keep[row];
+        float4 v = acc[i];
+        v.x *= f, v.y *= f, v.z *= f, v.w *= f;
+#pragma unroll 4
+        for (int k = 0; k < n; ++k) {
+          const float4 o = *reinterpret_cast<const float4 *>(slot(k0 + k) - row0 + 2 * kRows + (size_t)(row0 + row) * dim_pad + d);
+          const float w = part_top[k][row];
+          if (w != 0.0f) v.x += o.x * w, v.y += o.y * w, v.z += o.z * w, v.w += o.w * w;
+        }
+        acc[i] = v;
       }
-      acc[i] = v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kFours; ++i) {
+        const int d = d0 + i * kLanesD;
+        if (d >= a.c.dim) break;
+        float4 v = acc[i];
+        v.x *= keep[4 * quad], v.y *= keep[4 * quad + 1], v.z *= keep[4 * quad + 2], v.w *= keep[4 * quad + 3];
+#pragma unroll 8
+        for (int k = 0; k < n; ++k) {
+          const float4 o = *reinterpret_cast<const float4 *>(slot(k0 + k) + (size_t)(2 + d) * kRows + 4 * quad);
+          const float *w = &part_top[k][4 * quad];
+          if (w[0] != 0.0f) v.x += o.x * w[0];
+          if (w[1] != 0.0f) v.y += o.y * w[1];
+          if (w[2] != 0.0f) v.z += o.z * w[2];
+          if (w[3] != 0.0f) v.w += o.w * w[3];
+        }
+        acc[i] = v;
+      }
     }
   }
+  auto out_row = [&](int row) { return (s.q0 + row / a.group) * a.heads + item.head * a.group + row % a.group; };
+  for (int in = threadIdx.x; a.lse && in < kJoinRows && first + in < rows; in += kJoinThreads)
+    a.lse[out_row(first + in)] = sum[in] == 0.0f ? -INFINITY : (top[in] + log2f(sum[in])) * 0.69314718055994531f;
+  if constexpr (kByRow) {
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int in = 4 * quad + r, row = first + in;
-    if (row >= rows) continue;
-    const float l = sum[in], inv = l == 0.0f ? 0.0f : 1.0f / l;
-    const int64_t out = (s.q0 + row / a.group) * a.heads + item.head * a.group + row % a.group;
-    if (a.lse && d0 == 0) a.lse[out] = l == 0.0f ? -INFINITY : (top[in] + log2f(l)) * 0.69314718055994531f;
+    for (int i = 0; i < kFours; ++i) {
+      const int four = threadIdx.x + i * kJoinThreads, row = four / per_row, d = 4 * (four % per_row);
+      if (row >= kJoinRows || first + row >= rows) break;
+      if (d >= a.c.dim) continue;
+      const float l = sum[row], inv = l == 0.0f ? 0.0f : 1.0f / l;
+      *reinterpret_cast<uint2 *>(static_cast<T *>(a.out) + out_row(first + row) * a.c.dim + d) =
+          make_uint2(pack16<T>(acc[i].x * inv, acc[i].y * inv), pack16<T>(acc[i].z * inv, acc[i].w * inv));
+    }
+  } else {
 #pragma unroll
-    for (int i = 0; i < kDims; ++i) {
-      const int d = d0 + i * kLanesD;
-      if (d >= a.c.dim) break;
-      const float v = r == 0 ? acc[i].x : r == 1 ? acc[i].y : r == 2 ? acc[i].z : acc[i].w;
-      static_cast<T *>(a.out)[out * a.c.dim + d] = Io<T>::put(v * inv);
+    for (int r = 0; r < 4; ++r) {
+      const int in = 4 * quad + r, row = first + in;
+      if (row >= rows) continue;
+      const float l = sum[in], inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const int64_t out = out_row(row);
+#pragma unroll
+      for (int i = 0; i < kFours; ++i) {
+        const int d = d0 + i * kLanesD;
+        if (d >= a.c.dim) break;
+        const float v = r == 0 ? acc[i].x : r == 1 ? acc[i].y : r == 2 ? acc[i].z : acc[i].w;
+        static_cast<T *>(a.out)[out * a.c.dim + d] = Io<T>::put(v * inv);
+      }
     }
   }
 }

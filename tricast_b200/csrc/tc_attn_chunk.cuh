@@ -610,23 +610,26 @@ __device__ __forceinline__ void rows_of(const Raw &r, Rows &x) {
 }
 
 // Scores that a row does not see become -Inf, those of keys that are not numbers NaN. Rows see keys [lo, hi)
-// of the half; there and dead are its keys' bits.
+// of the half; there and dead are its keys' bits. A bit test and a select an element.
 __device__ __forceinline__ void mask_rows(Rows &x, const uint32_t *there, const uint32_t *dead, int t, const int (&lo)[4],
                                           const int (&hi)[4]) {
 #pragma unroll
-  for (int j = 0; j < kPairs; ++j) {
-    const int key = 8 * j + 2 * t;
-    const uint32_t in = there[j >> 2] >> (key & 31), bad = dead[j >> 2] >> (key & 31);
+  for (int part = 0; part < 2; ++part) {
+    const uint32_t keys = there[part], bad = dead[part] >> (2 * t);
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
-      float v[2];
-      unpack2(x[r][j], v[0], v[1]);
+      const uint32_t in = (keys & range_bits(lo[r], hi[r], part)) >> (2 * t);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        if ((bad >> e) & 1u) v[e] = u2f(kQNaN);
-        if (!((in >> e) & 1u) || key + e < lo[r] || key + e >= hi[r]) v[e] = -INFINITY;
+      for (int j = 0; j < kPairs / 2; ++j) {
+        float v0, v1;
+        F2 &pair = x[r][part * (kPairs / 2) + j];
+        unpack2(pair, v0, v1);
+        v0 = (bad & (1u << (8 * j))) ? u2f(kQNaN) : v0;
+        v1 = (bad & (2u << (8 * j))) ? u2f(kQNaN) : v1;
+        v0 = (in & (1u << (8 * j))) ? v0 : -INFINITY;
+        v1 = (in & (2u << (8 * j))) ? v1 : -INFINITY;
+        pair = pack2(v0, v1);
       }
-      x[r][j] = pack2(v[0], v[1]);
     }
   }
 }
@@ -841,7 +844,8 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
       const Item it = mine.it;
       const int first = it.tile * kRows + t * kTile + row0;
       const bool done = it.at == 0 && it.n == it.units;
-      float *part = parts + (size_t)(2 * blockIdx.x + (it.at > 0 ? 0 : 1)) * partial_floats(kRows, DP) + t * kTile + row0 + g4;
+      float *part = parts + (size_t)(2 * blockIdx.x + (it.at > 0 ? 0 : 1)) * partial_floats(kRows, DP);
+      const int prow = t * kTile + row0 + g4;
 #pragma unroll 1
       for (int h = 0; h < 2; ++h) {
         float sum[2], inv[2];
@@ -861,8 +865,8 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
           out_row[i] = (p.s.q0 + min(r, p.rows - 1) / a.group) * a.heads + it.head * a.group + r % a.group;
           if (t4 == 0) {
             if (!done) {
-              part[16 * h + 8 * i] = sum[i] == 0.0f ? -INFINITY : last;
-              part[kRows + 16 * h + 8 * i] = sum[i];
+              part[prow + 16 * h + 8 * i] = sum[i] == 0.0f ? -INFINITY : last;
+              part[kRows + prow + 16 * h + 8 * i] = sum[i];
             } else if (a.lse && real[i]) {
               a.lse[out_row[i]] = sum[i] == 0.0f ? -INFINITY : (last + log2f(sum[i])) * 0.69314718055994531f;
             }
@@ -880,8 +884,7 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
             for (int i = 0; i < 2; ++i) {
               const float v0 = u2f(o[4 * k + 2 * i]), v1 = u2f(o[4 * k + 2 * i + 1]);
               if (!done) {
-                part[(2 + d) * kRows + 16 * h + 8 * i] = v0;
-                part[(3 + d) * kRows + 16 * h + 8 * i] = v1;
+                *reinterpret_cast<float2 *>(part + 2 * kRows + (prow + 16 * h + 8 * i) * DP + d) = make_float2(v0, v1);
               } else if (real[i] && d < a.c.dim) {
                 *reinterpret_cast<uint32_t *>(static_cast<T *>(a.out) + out_row[i] * a.c.dim + d) =
                     sum[i] == 0.0f ? 0u : pack16<T>(v0 * inv[i], v1 * inv[i]);
