@@ -32,10 +32,10 @@ namespace chunk {
 constexpr int kTile = 128, kRows = 2 * kTile, kKeys = 128, kHalf = kKeys / 2, kSlots = 4;
 constexpr int kSoftmaxWarps = 8, kProducerWarps = 7, kThreads = 512;  // and one warp for the MMA thread
 // Registers a thread: 128 at launch; 256 * 160 + 256 * 96 = 512 * 128. Over packed units one warp stands in for the
-// producers, in a group of four with the MMA thread's: 168 at launch; 256 * 200 + 128 * 104 = 384 * 168.
+// producers, in a group of four with the MMA thread's: 168 at launch; 256 * 208 + 128 * 88 = 384 * 168.
 constexpr int kPackedThreads = 384;
-constexpr int softmax_regs(bool packed) { return packed ? 200 : 160; }
-constexpr int other_regs(bool packed) { return packed ? 104 : 96; }
+constexpr int softmax_regs(bool packed) { return packed ? 208 : 160; }
+constexpr int other_regs(bool packed) { return packed ? 88 : 96; }
 using W = Work<kRows, kKeys>;
 
 template <int DP>
@@ -772,17 +772,14 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
           const int top = max(max(sl.vfield[0], sl.vfield[1]), max(sl.vfield[2], sl.vfield[3]));
           if (top > vfield) field = top + 2;
         }
-        // Over packed units there are registers to ask for the second half before the first one's arithmetic.
-        constexpr bool kAhead = S == KV_PACKED;
         auto step_half = [&](const int half) {
           // With the reference as it is. It moves when a row's maximum has risen by more than 2**8 (or from
           // nothing), and when a larger value scale comes, by whole powers of two, so that what it scales
           // stays exact; the half is then computed again.
           uint32_t pw[2][kHalf / 4];
           F2 part2[4];
-          if (half && !kAhead) ask(ts + kHalf, raw[half]);
+          if (half) ask(ts + kHalf, raw[half]);  // (asked for before the first half's arithmetic it came out slower)
           arrived(raw[half]);
-          if (!half && kAhead) ask(ts + kHalf, raw[1]);
           while (true) {
             Rows x;
             rows_of(raw[half], x);
