@@ -36,9 +36,15 @@ static int launch_split(const Args &a, float *parts, cudaStream_t s) {
                                      : launch_split_mxfp4(a, parts, sms, s);
 }
 
-// Query rows of one key / value head from which the chunk kernel's tiles of 128 rows pay.
-constexpr int64_t kChunkRows = 65;
-static bool use_chunk(const KvCache &c, int group, int64_t max_q) { return c.dim <= 128 && max_q * group >= kChunkRows; }
+// From kChunkRows query rows of a key / value head the chunk kernel's tiles of 128 rows pay, unless the call is
+// small: its start and its join are some 25 us more. Split against chunk kernel, us, 8 heads of 128 over fp8: 16
+// sequences of 2048 keys 62 and 80 (32 rows), 97 and 82 (64 rows); 16 of 8192 145 and 195, 259 and 198; one of 16384
+// 79 and 84 (128 rows), 131 and 98 (256); one of 2048 37 and 58 (256), 83 and 61 (1024).
+constexpr int64_t kChunkRows = 65, kChunkTotalRows = 256;
+static bool use_chunk(const KvCache &c, int group, int batch, int64_t max_q) {
+  const int64_t rows = max_q * group;
+  return c.dim <= 128 && rows >= kChunkRows && rows * batch >= kChunkTotalRows;
+}
 
 static size_t split_bytes(const KvCache &c) {
   // At most four blocks an SM of 8 rows, or as many rows in fewer blocks (split::Shape).
@@ -54,8 +60,10 @@ static size_t chunk_bytes(const KvCache &c) {
 
 // Whether the chunk kernel's operands are laid out once, before it, and not by every row tile again: for quantized
 // caches (the others need no conversion), from kPackRows query rows of a key / value head on, while the tables'
-// width bounds the room it takes by kPackBytes.
-constexpr int64_t kPackRows = 257;
+// width bounds the room it takes by kPackBytes. Laid out by every tile against once (fp8, 8 heads of 128): 512 rows
+// over one sequence of 16384 keys 112 and 117 us, over sixteen of 2048 193 and 201; 1024 rows 150 and 139, 330 and
+// 287; 2048 rows 239 and 193, 529 and 439.
+constexpr int64_t kPackRows = 768;
 constexpr size_t kPackBytes = (size_t)1 << 29;
 static int pack_units(const KvCache &c, int max_pages) {
   const int64_t n = (((int64_t)max_pages << c.page_shift) + 127) / 128;
@@ -94,7 +102,7 @@ extern "C" size_t tc_paged_attention_workspace(const tc_kv_cache *cache, int32_t
   if (kv_cache_check(cache, c) != TC_OK || c.dtype == TC_F32) return 0;
   if (q_heads < c.heads || q_heads % c.heads) return 0;
   const int group = q_heads / c.heads;
-  if (attn::use_chunk(c, group, max_q_len)) return attn::chunk_bytes(c) + attn::pack_bytes(c, group, batch, max_q_len, max_pages);
+  if (attn::use_chunk(c, group, batch, max_q_len)) return attn::chunk_bytes(c) + attn::pack_bytes(c, group, batch, max_q_len, max_pages);
   return attn::split_bytes(c);
 }
 
@@ -144,7 +152,7 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
   } else {
     if (!workspace || workspace_bytes < tc_paged_attention_workspace(cache, q_heads, total_q, batch, a.max_q, max_pages))
       return set_error("tc_paged_attention: workspace too small"), TC_WORKSPACE_TOO_SMALL;
-    const int r = attn::use_chunk(a.c, a.group, a.max_q) ? attn::launch_chunk(a, workspace, s)
+    const int r = attn::use_chunk(a.c, a.group, a.batch, a.max_q) ? attn::launch_chunk(a, workspace, s)
                                                          : attn::launch_split(a, static_cast<float *>(workspace), s);
     if (r != TC_OK) return r;
   }

@@ -411,20 +411,23 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
     }
     __syncthreads();
     if constexpr (kByRow) {
+      // A part's outputs of the block's rows lie together: all of a thread's are asked for before the first is used.
+      const int fours = kJoinRows * per_row / kJoinThreads;
 #pragma unroll
       for (int i = 0; i < kFours; ++i) {
-        const int four = threadIdx.x + i * kJoinThreads, row = four / per_row, d = 4 * (four % per_row);
-        if (row >= kJoinRows) break;
-        const float f = keep[row];
-        float4 v = acc[i];
-        v.x *= f, v.y *= f, v.z *= f, v.w *= f;
-#pragma unroll 4
-        for (int k = 0; k < n; ++k) {
-          const float4 o = *reinterpret_cast<const float4 *>(slot(k0 + k) - row0 + 2 * kRows + (size_t)(row0 + row) * dim_pad + d);
-          const float w = part_top[k][row];
-          if (w != 0.0f) v.x += o.x * w, v.y += o.y * w, v.z += o.z * w, v.w += o.w * w;
+        const float f = keep[min((threadIdx.x + i * kJoinThreads) / per_row, kJoinRows - 1)];
+        acc[i].x *= f, acc[i].y *= f, acc[i].z *= f, acc[i].w *= f;
+      }
+      for (int k = 0; k < n; ++k) {
+        const float4 *from4 = reinterpret_cast<const float4 *>(slot(k0 + k) - row0 + 2 * kRows + (size_t)row0 * dim_pad) + threadIdx.x;
+        float4 o[kFours];
+#pragma unroll
+        for (int i = 0; i < kFours; ++i) o[i] = from4[(i < fours ? i : 0) * kJoinThreads];
+#pragma unroll
+        for (int i = 0; i < kFours; ++i) {
+          const float w = part_top[k][min((threadIdx.x + i * kJoinThreads) / per_row, kJoinRows - 1)];
+          if (w != 0.0f) acc[i].x += o[i].x * w, acc[i].y += o[i].y * w, acc[i].z += o[i].z * w, acc[i].w += o[i].w * w;
         }
-        acc[i] = v;
       }
     } else {
 #pragma unroll

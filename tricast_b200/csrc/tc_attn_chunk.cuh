@@ -704,23 +704,27 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
         const Item it = mine.it;
         const int first = it.tile * kRows + t * kTile + row0;  // the warp's first row
         const int r = first + lane, tok = min(r, p.rows - 1) / a.group;
-        const T *qp = static_cast<const T *>(a.q) + (p.s.q0 + tok) * a.q_tok + (it.head * a.group + r % a.group) * a.q_head;
+        const T *qp = static_cast<const T *>(a.q) + (p.s.q0 + tok) * a.q_tok + (it.head * a.group + min(r, p.rows - 1) % a.group) * a.q_head;
+        // Every thread reads, a row that is not there its neighbour's: without branches the loads go out together.
         uint32_t w[DP / 2];
 #pragma unroll
         for (int g = 0; g < DP / 8; ++g) {
-          uint32_t x[4] = {0u, 0u, 0u, 0u};
-          if (r < p.rows && 8 * g < a.c.dim) {
-            if (qvec) {
-              load_words<4>(reinterpret_cast<const unsigned char *>(qp + 8 * g), x);
-            } else {
-              const unsigned short *u = reinterpret_cast<const unsigned short *>(qp + 8 * g);
+          const int at = min(8 * g, a.c.dim - 8);
+          uint32_t x[4];
+          if (qvec) {
+            load_words<4>(reinterpret_cast<const unsigned char *>(qp + at), x);
+          } else {
+            const unsigned short *u = reinterpret_cast<const unsigned short *>(qp + at);
 #pragma unroll
-              for (int k = 0; k < 4; ++k) x[k] = (uint32_t)u[2 * k] | ((uint32_t)u[2 * k + 1] << 16);
-            }
+            for (int k = 0; k < 4; ++k) x[k] = (uint32_t)u[2 * k] | ((uint32_t)u[2 * k + 1] << 16);
           }
 #pragma unroll
-          for (int k = 0; k < 4; ++k) w[4 * g + k] = x[k] ^ flip;
+          for (int k = 0; k < 4; ++k) w[4 * g + k] = x[k];
         }
+#pragma unroll
+        for (int g = 0; g < DP / 8; ++g)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) w[4 * g + k] = r < p.rows && 8 * g < a.c.dim ? w[4 * g + k] ^ flip : 0u;
         if (S != KV_NONE) {
           float big = 0.0f;
 #pragma unroll
