@@ -88,8 +88,13 @@ static int launch_chunk(const Args &a, void *workspace, cudaStream_t s) {
                  : a.c.scheme == KV_INT8_ROW ? launch_chunk_int8(a, parts, stretches, status, most, s)
                                              : launch_chunk_mxfp4(a, parts, stretches, status, most, s);
   if (st != TC_OK) return st;
-  return a.c.dtype == TC_BF16 ? launch_join<__nv_bfloat16, 256>(a, parts, stretches, most, status, s)
-                              : launch_join<__half, 256>(a, parts, stretches, most, status, s);
+  // Few items are cut into many parts each (see join_kernel).
+  const double items = (double)a.batch * a.c.heads * (((double)a.max_q * a.group + 255) / 256);
+  if (items * 4 <= most)
+    return a.c.dtype == TC_BF16 ? launch_join<__nv_bfloat16, 256, 16>(a, parts, stretches, most, status, s)
+                                : launch_join<__half, 256, 16>(a, parts, stretches, most, status, s);
+  return a.c.dtype == TC_BF16 ? launch_join<__nv_bfloat16, 256, 64>(a, parts, stretches, most, status, s)
+                              : launch_join<__half, 256, 64>(a, parts, stretches, most, status, s);
 }
 
 }  // namespace attn

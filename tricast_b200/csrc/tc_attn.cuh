@@ -315,14 +315,15 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 // Merges the partial results of the items that several blocks share. One block for each border between two
 // stretches and up to 64 rows of the item; it acts if the border is the first inside its item. A row's maxima and
 // sums are read side by side into shared memory (as many parts at a time as it holds). 64 rows a block keep the
-// chunk kernel's join to one wave of blocks; the split kernel's items have 8 or 16. Where `status` is given and a
+// chunk kernel's join to one wave of blocks; where few items are cut into many parts, 16 rows a block have more
+// loads in flight (427 rows of one head over 13476 keys: 150 us a call with 64, 82 with 16). The split kernel's
+// items have 8 or 16. Where `status` is given and a
 // block of the kernel before gave up a wait (which takes a fault elsewhere, or a test), everything is computed again
 // by the plain rows.
 constexpr int kJoinThreads = 256;
-constexpr int join_rows(int rows) { return rows < 64 ? rows : 64; }  // of an item, a block
-template <typename T, int kRows>
+template <typename T, int kRows, int kJoinRows>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float *parts, const Stretch *stretches, int dim_pad, int most, const int *status) {
-  constexpr int kJoinRows = join_rows(kRows), kJoinParts = 2048 / kJoinRows;
+  constexpr int kJoinParts = 2048 / kJoinRows;
   __shared__ Item item;
   __shared__ int from, upto;
   __shared__ float part_top[kJoinParts][kJoinRows], part_sum[kJoinParts][kJoinRows];
@@ -419,15 +420,24 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
         const float f = keep[min((threadIdx.x + i * kJoinThreads) / per_row, kJoinRows - 1)];
         acc[i].x *= f, acc[i].y *= f, acc[i].z *= f, acc[i].w *= f;
       }
-      for (int k = 0; k < n; ++k) {
-        const float4 *from4 = reinterpret_cast<const float4 *>(slot(k0 + k) - row0 + 2 * kRows + (size_t)row0 * dim_pad) + threadIdx.x;
-        float4 o[kFours];
+      constexpr int kSide = 8 / kFours;  // parts side by side
+      for (int k = 0; k < n; k += kSide) {
+        float4 o[kSide][kFours];
 #pragma unroll
-        for (int i = 0; i < kFours; ++i) o[i] = from4[(i < fours ? i : 0) * kJoinThreads];
+        for (int u = 0; u < kSide; ++u) {
+          const float4 *from4 = reinterpret_cast<const float4 *>(slot(k0 + min(k + u, n - 1)) - row0 + 2 * kRows + (size_t)row0 * dim_pad) + threadIdx.x;
 #pragma unroll
-        for (int i = 0; i < kFours; ++i) {
-          const float w = part_top[k][min((threadIdx.x + i * kJoinThreads) / per_row, kJoinRows - 1)];
-          if (w != 0.0f) acc[i].x += o[i].x * w, acc[i].y += o[i].y * w, acc[i].z += o[i].z * w, acc[i].w += o[i].w * w;
+          for (int i = 0; i < kFours; ++i) o[u][i] = from4[(i < fours ? i : 0) * kJoinThreads];
+        }
+#pragma unroll
+        for (int u = 0; u < kSide; ++u) {
+          if (k + u >= n) break;
+#pragma unroll
+          for (int i = 0; i < kFours; ++i) {
+            const float w = part_top[k + u][min((threadIdx.x + i * kJoinThreads) / per_row, kJoinRows - 1)];
+            const float4 v = o[u][i];
+            if (w != 0.0f) acc[i].x += v.x * w, acc[i].y += v.y * w, acc[i].z += v.z * w, acc[i].w += v.w * w;
+          }
         }
       }
     } else {
@@ -482,10 +492,10 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
 }
 
 // Queues the join behind the kernel before it, to start as that one ends.
-template <typename T, int kRows>
+template <typename T, int kRows, int kJoinRows = kRows>
 inline int launch_join(const Args &a, const float *parts, const Stretch *stretches, int most, const int *status, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(most > 1 ? most - 1 : 1, kRows / join_rows(kRows));
+  cfg.gridDim = dim3(most > 1 ? most - 1 : 1, kRows / kJoinRows);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = s;
   cudaLaunchAttribute at[1];
@@ -494,7 +504,7 @@ inline int launch_join(const Args &a, const float *parts, const Stretch *stretch
   cfg.attrs = at;
   cfg.numAttrs = 1;
   const int pad = a.c.dim <= 64 ? 64 : a.c.dim <= 128 ? 128 : 256;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<T, kRows>, a, parts, stretches, pad, most, status);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, join_kernel<T, kRows, kJoinRows>, a, parts, stretches, pad, most, status);
   if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
   count_launch();
   return TC_OK;
