@@ -18,7 +18,8 @@
 // 2**8, and the largest value scale so far, as in the chunk kernel (tc_attn_chunk.cuh), so a step votes once and
 // reduces nothing. Unquantized rows use their own type; bf16 ones get bf16 weights. A weight is rounded once, to the
 // 16 bits of its product, and the sum it is divided by is taken before that in fp32: with the result's own rounding
-// an fp16 output is off by 1.4 times what rounding it alone would give.
+// an output over a cache of its own type (fp16 ones over any) is off by 1.4 to 1.6 times what rounding it alone would
+// give. Weights in two parts would undo that for twice the MMAs of the values.
 //
 // 64 sequences of 8192 keys, 8 heads of 128 over E4M3, 4 query heads each: 138 us, 4.8 TB/s of codes. 16 sequences
 // of 4000 keys and 4 new tokens over bf16: 46 us, 2.9 TB/s. One of 1025 keys: 15 us, start, one unit and join.
