@@ -220,9 +220,22 @@ struct Work {
   static __device__ __forceinline__ int64_t start(int64_t total, int c, int n) { return total * c / n; }
 };
 
-// How far a row's reference stays below its maximum: exp2(x - ref) <= 2**(8 + 6) / T, at most 2**(8 + 100), for T
-// of this exponent field.
-__device__ __forceinline__ float room(int field) { return fminf(6.0f + (127.0f - (float)field), 100.0f); }
+// Weights are kept relative to a row's reference: P = exp2(x - ref), and over quantized caches P * value scale is
+// what the products take in fp16. With lift = floor(log2(value scale)), the reference follows the largest x + lift of
+// the keys that the row sees, kBelow under it, and moves when one comes kHeadroom above it: products stay below
+// 2**15, and those within 2**20 of a row's largest keep fp16's 11 bits whatever the scales of other keys are. lift is
+// held at kLeastLift, so that P stays below 2**(kHeadroom - kLeastLift); a value scale above 2**kMostLift, or one that
+// is not a number, stays out of the fp16 products. What a part loses against another whose reference is 2**126
+// higher then had less than 2**(kMostLift - kLeastLift - 126) = 2**-26 of its weight.
+constexpr float kBelow = 6.0f, kHeadroom = 14.0f;
+constexpr int kLeastLift = -60, kMostLift = 40;
+// Lifts this close under the largest may count as the largest: the reference moves less often, and 16 of the 20 binades
+// remain.
+constexpr int kNarrow = 4;
+// For the exponent field of a scale.
+__device__ __forceinline__ float lift_of(int field) { return (float)max(field - 127, kLeastLift); }
+// A value scale (its bits) that the fp16 products do not take: beyond 2**kMostLift, infinite, NaN or negative.
+__device__ __forceinline__ bool odd_scale(uint32_t bits) { return bits > (uint32_t)(127 + kMostLift) << 23; }
 
 // One partial result: kRows maxima (base-2 logarithms), kRows sums, then the outputs as the kernel holds them:
 // [dim][kRows] of the split kernel (kRows 8 or 16), [kRows][dim] of the chunk kernel.
@@ -235,6 +248,16 @@ __device__ __forceinline__ float cached(const KvCache &c, const unsigned char *c
   if (c.scheme == KV_MXFP4) return __fmul_rn(decode_e2m1((codes[d >> 1] >> (4 * (d & 1))) & 15u), pow2_value(scales[d >> 5]));
   const float s = *reinterpret_cast<const float *>(scales);
   return __fmul_rn(c.scheme == KV_FP8_ROW ? decode_e4m3(codes[d]) : (float)(signed char)codes[d], s);
+}
+
+// Whether the products leave a row's values out. S: the scheme where it is known, KV_NONE for rows without scales.
+template <int S>
+__device__ __forceinline__ bool odd_values(const KvCache &c, int64_t row) {
+  if (S == KV_NONE) return false;
+  if (c.scheme != KV_MXFP4) return odd_scale(*reinterpret_cast<const uint32_t *>(c.vs + row * 4));
+  uint32_t big = 0u;
+  for (int q = 0; q < c.scale_bytes; ++q) big = max(big, (uint32_t)c.vs[row * c.scale_bytes + q]);
+  return odd_scale(f2u(pow2_value(big) * (1.0f / (1 << kGroupShift))));
 }
 
 // A warp a (new token, query head): lanes over the head's elements, one key at a time, with the running

@@ -21,9 +21,9 @@
 //
 // Codes are exact in fp16 and their scales stay out of the products, as in the split kernel: a key's scale
 // multiplies its score, a value's its weight. Weights are kept relative to a reference that follows a row's
-// maximum only when it has risen by more than 2**8 (O in TMEM is rescaled then, rarely), and to the largest
-// value scale so far, so that they stay below 2**15: P = exp2(x - ref) * scale with
-// ref = maximum - 6 + log2(T). The sum takes the weights before the value's scale and before their rounding.
+// largest product of weight and value scale (tc_attn.cuh) only when it has risen by more than 2**8 (O in TMEM is
+// rescaled then, rarely), so that the products stay below 2**15. The sum takes the weights before the value's scale
+// and before their rounding.
 #pragma once
 
 #include <atomic>
@@ -54,12 +54,15 @@ struct Shape {
 };
 
 // What the softmax needs of a unit's keys.
+constexpr int kOdd = 0x7FFFFFFF;
 struct __align__(16) KeySlot {
   float k[kKeys], v[kKeys];
   uint32_t valid[4];  // keys that are there
   uint32_t dead[4];   // keys whose rows of scores or values are not numbers: their scales here are 1, their V
                       // is 0, and the rows that see them become NaN
-  int vfield[4];      // largest exponent field of the value scales, by quarter
+  // Largest and least exponent field of the value scales, by quarter (0 and 255: none). A key whose values' scale is
+  // odd (tc_attn.cuh) has the scale 0 here, and makes its quarter's largest kOdd, which no reference is low enough for.
+  int top[4], low[4];
 };
 
 // What pack_kernel leaves of a unit: the K and V tiles as they lie in shared memory, then the slot.
@@ -178,6 +181,7 @@ __device__ __forceinline__ Part part_of(const Args &a, const Item &it) {
 struct Stash {
   Item it;
   Part p;
+  bool odd;  // the products left values out (of an item of the softmax)
 };
 // The stash is written by one lane and read by all; the barriers keep the compiler from holding copies.
 __device__ __forceinline__ void put(Stash &st, const Item &it, const Part &p) {
@@ -185,6 +189,7 @@ __device__ __forceinline__ void put(Stash &st, const Item &it, const Part &p) {
   if ((threadIdx.x & 31) == 0) {
     st.it = it;
     st.p = p;
+    st.odd = false;
   }
   __syncwarp();
 }
@@ -235,16 +240,21 @@ __device__ __forceinline__ void put_keys(KeySlot &sl, int quarter, bool there, u
     k = u2f(kw);
     v = u2f(vw);
   }
-  dead |= k != k || v != v;
-  if (!there || dead) k = v = 1.0f;
+  dead |= k != k;
+  const bool odd = there && odd_scale(f2u(v));
+  if (!there || dead) k = 1.0f;
+  if (!there) v = 1.0f;
+  if (odd) v = 0.0f;
   sl.k[32 * quarter + lane] = k;
   sl.v[32 * quarter + lane] = v;
   const uint32_t valid = __ballot_sync(0xFFFFFFFFu, there), dead_keys = __ballot_sync(0xFFFFFFFFu, there && dead);
-  const int top = (int)__reduce_max_sync(0xFFFFFFFFu, there && !dead ? f2u(v) >> 23 : 0u);
+  const int top = (int)__reduce_max_sync(0xFFFFFFFFu, odd ? (unsigned)kOdd : there ? f2u(v) >> 23 : 0u);
+  const int low = (int)__reduce_min_sync(0xFFFFFFFFu, there && !odd ? f2u(v) >> 23 : 255u);
   if (lane == 0) {
     sl.valid[quarter] = valid;
     sl.dead[quarter] = dead_keys;
-    sl.vfield[quarter] = top;
+    sl.top[quarter] = top;
+    sl.low[quarter] = low;
   }
 }
 // The word of a row's scales.
@@ -386,8 +396,7 @@ __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsign
       for (int g = 0; g < kOut; ++g) {
         uint32_t h[4];
         granule<S>(w, g, mul, h);
-        // A key with a NaN value scale has NaN codes, which would reach rows that do not see it as 0 * NaN:
-        // they count as 0.
+        // A key with a NaN value scale has NaN codes, which would be 0 * NaN for every row: they count as 0.
         if (S == KV_FP8_ROW && dead_keys && ((dead_keys >> key) & 1u)) h[0] = h[1] = h[2] = h[3] = 0u;
         // Granule q of the key's row, what depends on the lane apart from what depends on i.
         const int q0 = chunk0 * kOut + g, qi = cstep(i) * kOut;
@@ -674,6 +683,107 @@ __device__ __forceinline__ void weights(const Rows &x, const float *ks, const fl
   }
 }
 
+// This thread's largest x + lift of a half's keys that each of its rows sees, by every key's own lift: eight columns
+// of scores at a time, read again.
+__device__ __forceinline__ void highest(const Args &a, const Stash &mine, const KeySlot &sl, int half, int tile, int p0, bool whole,
+                                        uint32_t ts, const float (&qm)[4], float (&m)[4]) {
+  const int lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3, row0 = 32 * ((threadIdx.x >> 5) & 3);
+  int lo[4], hi[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    lo[i] = 0, hi[i] = kKeys;
+    if (!whole) {
+      visible(a, mine.p.s, min(mine.it.tile * kRows + tile * kTile + row0 + 8 * i + g4, mine.p.rows - 1) / a.group, lo[i], hi[i]);
+      lo[i] -= p0, hi[i] -= p0;
+    }
+    m[i] = -INFINITY;
+  }
+#pragma unroll 1
+  for (int j = 0; j < kPairs; ++j) {
+    uint32_t s[2][4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) tc5::tmem_ld_frag8(ts + (h ? 16u << 16 : 0u) + kHalf * half + 8 * j, s[h]);
+    tc5::tmem_wait_ld<4>(s[0]);
+    tc5::tmem_wait_ld<4>(s[1]);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int key = kHalf * half + 8 * j + 2 * t4 + e;
+      const bool there = ((sl.valid[key >> 5] & ~sl.dead[key >> 5]) >> (key & 31)) & 1u;
+      const float k = sl.k[key], lift = lift_of((int)(f2u(sl.v[key]) >> 23));
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (there && key >= lo[i] && key < hi[i]) m[i] = fmaxf(m[i], u2f(s[i >> 1][2 * (i & 1) + e]) * k * qm[i] + lift);
+    }
+  }
+}
+
+// Adds what the products left out: the values of odd keys, in fp32, to the outputs of the rows that see them. A thread
+// works out the scores of one row of its warp's 32 again, from Q as it lies in shared memory.
+template <typename T, int S, int DP>
+__device__ __noinline__ void add_odd(const Args &a, const Stash &mine, const unsigned char *q0, int tile, uint32_t to,
+                                        float4 qm4, float4 ref4) {
+  const float qm[4] = {qm4.x, qm4.y, qm4.z, qm4.w}, ref[4] = {ref4.x, ref4.y, ref4.z, ref4.w};
+  constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
+  const KvCache &c = a.c;
+  const int lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3, row0 = 32 * ((threadIdx.x >> 5) & 3);
+  const int *table = a.table + (int64_t)mine.it.b * a.table_stride;
+  auto row_of = [&](int at) -> int64_t {
+    const int page = table[at >> c.page_shift];
+    return page < 0 || page >= c.pages ? -1 : (((int64_t)page * c.heads + mine.it.head) << c.page_shift) + (at & (c.page_size - 1));
+  };
+  // Of this thread's row.
+  float qmul = 0.0f, below = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float q = __shfl_sync(0xFFFFFFFFu, qm[i], 4 * (lane & 7)), r = __shfl_sync(0xFFFFFFFFu, ref[i], 4 * (lane & 7));
+    if (lane >> 3 == i) qmul = q, below = r;
+  }
+  int lo, hi;
+  visible(a, mine.p.s, min(mine.it.tile * kRows + tile * kTile + row0 + lane, mine.p.rows - 1) / a.group, lo, hi);
+#pragma unroll 1
+  for (int at0 = mine.p.key0; at0 < mine.p.key1; at0 += 32) {
+    const int64_t own = at0 + lane < mine.p.key1 ? row_of(at0 + lane) : -1;
+    uint32_t odd = __ballot_sync(0xFFFFFFFFu, own >= 0 && odd_values<S>(c, own));
+#pragma unroll 1
+    for (; odd; odd &= odd - 1) {
+      const int at = at0 + __ffs(odd) - 1;
+      const int64_t row = __shfl_sync(0xFFFFFFFFu, own, at - at0);
+      float dot = 0.0f;
+#pragma unroll 1
+      for (int d = 0; d < c.dim; ++d) {
+        const unsigned char *q = q0 + tile_at(row0 + lane, d >> 3) + 2 * (d & 7);
+        const uint32_t bits = *reinterpret_cast<const unsigned short *>(q);
+        dot = __fmaf_rn(kBf16 ? half_bits_to_float<__nv_bfloat16>(bits) : half_bits_to_float<__half>(bits),
+                        cached<T>(c, c.k + row * c.row_bytes, c.ks + row * c.scale_bytes, d), dot);
+      }
+      const bool sees = at >= lo && at < hi;
+      const float weight = exp2_fast(dot * qmul - below);
+      const uint32_t who = __ballot_sync(0xFFFFFFFFu, sees);
+      float w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __shfl_sync(0xFFFFFFFFu, weight, 8 * i + g4);
+#pragma unroll 1
+      for (int i = 0; i < 2 * (DP / 32); ++i) {
+        const int h = i & 1;
+        const uint32_t out = to + (h ? 16u << 16 : 0u) + 32 * (i >> 1);
+        uint32_t o[16];
+        tc5::tmem_ld_frag32(out, o);
+        tc5::tmem_wait_ld_frag(o);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int d = 32 * (i >> 1) + 8 * (e >> 2) + 2 * t4 + (e & 1), r = 16 * h + (e & 2 ? 8 : 0) + g4;
+          const float mult = h ? (e & 2 ? w[3] : w[2]) : (e & 2 ? w[1] : w[0]);
+          if (d < c.dim && ((who >> r) & 1u))
+            o[e] = f2u(__fmaf_rn(mult, cached<T>(c, c.v + row * c.row_bytes, c.vs + row * c.scale_bytes, d), u2f(o[e])));
+        }
+        __syncwarp();
+        tc5::tmem_st_frag32(out, o);
+      }
+      tc5::tmem_wait_st();
+    }
+  }
+}
+
 // Multiplies the outputs so far by a power of two a row.
 template <int DP>
 __device__ __forceinline__ void rescale(const float (&keep)[4], uint32_t to) {
@@ -752,8 +862,8 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
         warp_arrive(&bar.qfull[t]);
       }
       // From here on a thread works for rows 8 i + g of the warp's 32.
-      // ref: the base-2 logarithm that weights are relative to, `above` below a row's maximum; far below
-      // everything before the row has seen a key (the first one then moves it).
+      // ref: the base-2 logarithm that weights are relative to; far below everything before the row has seen a key
+      // (the first one then moves it).
       float qm[4], ref[4];
       F2 sum2[4];
 #pragma unroll
@@ -762,7 +872,6 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
         ref[i] = -3e38f;
         sum2[i] = pack2(0.0f, 0.0f);
       }
-      int vfield = kBf16 ? 127 : 0;  // exponent field of T
       const int steps = mine.p.steps, key0 = mine.p.key0, all_lo = mine.p.all_lo, all_hi = mine.p.all_hi;
       __syncwarp();
       for (int j = 0; j < steps; ++j) {
@@ -778,16 +887,11 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
         const bool whole = p0 >= all_lo && p0 + kKeys <= all_hi &&
                            ((sl.valid[0] & ~sl.dead[0]) & (sl.valid[1] & ~sl.dead[1]) & (sl.valid[2] & ~sl.dead[2]) &
                             (sl.valid[3] & ~sl.dead[3])) == 0xFFFFFFFFu;
-        int field = vfield;
-        if (!kBf16) {
-          // With two binades to spare, so that slightly larger scales later on do not move it again.
-          const int top = max(max(sl.vfield[0], sl.vfield[1]), max(sl.vfield[2], sl.vfield[3]));
-          if (top > vfield) field = top + 2;
-        }
+        // The largest lift of the unit, seen or not: a score this far above the reference may have to move it.
+        const float lift = S == KV_NONE ? 0.0f : lift_of(max(max(sl.top[0], sl.top[1]), max(sl.top[2], sl.top[3])));
         auto step_half = [&](const int half) {
-          // With the reference as it is. It moves when a row's maximum has risen by more than 2**8 (or from
-          // nothing), and when a larger value scale comes, by whole powers of two, so that what it scales
-          // stays exact; the half is then computed again.
+          // With the reference as it is. It moves when a row's largest product has risen by more than 2**8 (or from
+          // nothing), by whole powers of two, so that what it scales stays exact; the half is then computed again.
           uint32_t pw[2][kHalf / 4];
           F2 part2[4];
           if (half) ask(ts + kHalf, raw[half]);  // (asked for before the first half's arithmetic it came out slower)
@@ -807,23 +911,30 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
             }
             float m[4];
             weights<S, kBf16>(x, sl.k + kHalf * half, sl.v + kHalf * half, t4, qm, ref, pw, part2, m);
-            const float above = room(vfield);
-            bool any = field != vfield;
+            bool any = false;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) any |= m[i] * qm[i] > ref[i] + (above + 8.0f);
+            for (int i = 0; i < 4; ++i) any |= m[i] * qm[i] > ref[i] + (kHeadroom - lift);
             if (!__any_sync(0xFFFFFFFFu, any)) break;
+            // Where the unit's lifts lie close together the largest score and lift will do; else every key by itself.
+            const bool narrow = S == KV_NONE || max(max(sl.top[0], sl.top[1]), max(sl.top[2], sl.top[3])) <=
+                                                    min(min(sl.low[0], sl.low[1]), min(sl.low[2], sl.low[3])) + kNarrow;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) m[i] = m[i] * qm[i] + lift;
+            if (!narrow) highest(a, mine, sl, half, t, p0, whole, ts, qm, m);
+            if (lift > (float)kMostLift) mine.odd = true;
             float keep[4];
+            any = false;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               m[i] = fmaxf(m[i], __shfl_xor_sync(0xFFFFFFFFu, m[i], 1));
               m[i] = fmaxf(m[i], __shfl_xor_sync(0xFFFFFFFFu, m[i], 2));
-              const float now = m[i] * qm[i] > ref[i] + (above + 8.0f) ? ceilf(m[i] * qm[i]) : ref[i] + above;
-              const float next = now - room(field);
+              const float next = m[i] > ref[i] + kHeadroom ? ceilf(m[i]) - kBelow : ref[i];
+              any |= next != ref[i];
               keep[i] = exp2_fast(ref[i] - next);
               ref[i] = next;
               sum2[i] = mul2(sum2[i], pack2(keep[i], keep[i]));
             }
-            vfield = field;
+            if (!__any_sync(0xFFFFFFFFu, any)) break;
             // The outputs so far: the products of the half before, which this half's scores did not wait for.
             if (j > 0 || half) {
               if (!warp_wait(&bar.pvdone[t], (half ^ 1) & 1, polls)) return false;
@@ -849,6 +960,7 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
       if (!warp_wait_sleep(&bar.ofull[t], items++ & 1, polls)) return false;
       tc5::fence_after_sync();
       __syncwarp();
+      if (mine.odd) add_odd<T, S, DP>(a, mine, q0, t, to, make_float4(qm[0], qm[1], qm[2], qm[3]), make_float4(ref[0], ref[1], ref[2], ref[3]));
       const Part p = mine.p;
       const Item it = mine.it;
       const int first = it.tile * kRows + t * kTile + row0;
@@ -913,7 +1025,7 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
 }
 
 template <typename T, int S, int DP>
-__global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 1) chunk_kernel(Args a, float *parts, Stretch *stretches, int *status, int most, int polls,
+__global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 1) chunk_kernel(const __grid_constant__ Args a, float *parts, Stretch *stretches, int *status, int most, int polls,
                                                                  const unsigned char *packed, int max_units) {
   constexpr bool kPacked = S == KV_PACKED;
   constexpr int kFullArrivals = kPacked ? 1 : 4, kFeeders = kPacked ? 1 : kProducerWarps;
@@ -1033,8 +1145,7 @@ __global__ void __launch_bounds__(256) pack_kernel(Args a, unsigned char *packed
     word = page >= 0 ? scale_word<S, DP>(c, c.ks, row_at(page, lane)) : 0u;
     put_keys<S, DP>(*reinterpret_cast<KeySlot *>(to + Packed<DP>::kSlot), quarter, page >= 0, word, vw, false);
   }
-  // A key with a NaN value scale has NaN codes, which would reach rows that do not see it as 0 * NaN: they count
-  // as 0.
+  // A key with a NaN value scale has NaN codes, which would be 0 * NaN for every row: they count as 0.
   const uint32_t dead = S == KV_FP8_ROW && side ? __ballot_sync(0xFFFFFFFFu, (vw & 0x7FFFFFFFu) > kInf) : 0u;
   const unsigned char *codes = side ? c.v : c.k;
   to += side * Shape<DP>::kOperand;

@@ -14,9 +14,8 @@
 //  - P^T is S^T transposed by 8 x 8 (movmatrix).
 // Codes are exact in fp16 (E4M3, INT8, E2M1 times a power of two), so scales stay out of the products: a key's
 // scale multiplies its score, a value's scale its weight. Q is scaled per row by a power of two into fp16's
-// range. Weights are relative to a reference that follows a row's maximum only when it has risen by more than
-// 2**8, and the largest value scale so far, as in the chunk kernel (tc_attn_chunk.cuh), so a step votes once and
-// reduces nothing. Unquantized rows use their own type; bf16 ones get bf16 weights. A weight is rounded once, to the
+// range. Weights are relative to a reference that follows a row's largest product of weight and value scale
+// (tc_attn.cuh) only when it has risen by more than 2**8, so a step votes once and reduces nothing. Unquantized rows use their own type; bf16 ones get bf16 weights. A weight is rounded once, to the
 // 16 bits of its product, and the sum it is divided by is taken before that in fp32: with the result's own rounding
 // an output over a cache of its own type (fp16 ones over any) is off by 1.4 to 1.6 times what rounding it alone would
 // give. Weights in two parts would undo that for twice the MMAs of the values.
@@ -90,6 +89,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ Item first;
   __shared__ float merge_top[kWarps][kRows], merge_sum[kWarps][kRows];
+  __shared__ int left_out[kWarps];  // whether the warp's products leave an odd key's values out
   constexpr bool kSharedQ = DP * NR > 256;  // Q does not fit the registers
   __shared__ uint4 qfrag[kSharedQ ? P::kKSteps * 32 : 1];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -284,8 +284,9 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
       for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][nr][e] = 0.0f;
-    // ref: the base-2 logarithm that a row's weights are relative to, room(vfield) below its maximum, far below
-    // everything before the first key; sum: of this lane's weights. vfield: exponent field of T.
+    // ref: the base-2 logarithm that a row's weights are relative to, far below everything before the first key; sum:
+    // of this lane's weights. vfield: the largest exponent field of a value scale so far, seen or not: it says when a
+    // reference may have to move, and the keys that the row sees say where to.
     float ref[NR][2], sum[NR][2];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
@@ -294,7 +295,8 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
         ref[nr][e] = -3e38f;
         sum[nr][e] = 0.0f;
       }
-    int vfield = kBf16 ? 127 : 0;
+    int vfield = S == KV_NONE ? 127 : 0;
+    if (lane == 0) left_out[warp] = 0;
 
     for (int i = 0, slot = 0; i < steps; ++i, slot = slot + 1 == P::kStages ? 0 : slot + 1) {
       if (i + P::kStages - 1 < steps) {
@@ -405,6 +407,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
           if (!((valid >> (g + 8 * h)) & 1u)) vscale[h] = 0.0f;
       }
       uint32_t nan_keys = 0u;  // keys whose values are not numbers
+      uint32_t odd_keys = 0u;  // keys whose values' scales are odd (tc_attn.cuh)
       if (S == KV_NONE && !whole) {
         // Rows of the step differ in what they see: a value that is not finite must not reach the others.
         // Its whole row counts as 0 and the weights of the rows that see it become NaN.
@@ -421,57 +424,61 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
           if ((nan_keys >> (g + 8 * h)) & 1u) vscale[h] = u2f(kQNaN);
       }
 
-      // Does a row's reference, or T, have to move?
-      float m[NR][2];
+      // May a row's reference have to move?
       bool any = false;
-      const float above = room(vfield);
+      const float above = kHeadroom - lift_of(vfield);
 #pragma unroll
       for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          m[nr][r] = fmaxf(x[nr][r], x[nr][2 + r]);
-          any |= m[nr][r] > ref[nr][r] + (above + 8.0f);
-        }
-      if (!kBf16) {
+        for (int r = 0; r < 2; ++r) any |= fmaxf(x[nr][r], x[nr][2 + r]) > ref[nr][r] + above;
+      if (S != KV_NONE) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) any |= (int)(f2u(vscale[h]) >> 23) > vfield;  // NaN too
+        for (int h = 0; h < 2; ++h) any |= (int)(f2u(vscale[h]) >> 23) > vfield;  // odd ones too
       }
       if (__any_sync(0xFFFFFFFFu, any)) {
-        int field = vfield;
-        if (!kBf16) {
+        float lift[2] = {0.0f, 0.0f};
+        if (S != KV_NONE) {
           uint32_t f = 0u;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const uint32_t v = f2u(vscale[h]) >> 23;
-            // A NaN scale comes with NaN codes, which would reach rows that do not see the key as 0 * NaN: such
-            // codes count as 0 below, and the weight carries the NaN.
-            if (v >= 255u) nan_keys |= 1u << (g + 8 * h);
-            else f = max(f, v);
+            const uint32_t v = f2u(vscale[h]);
+            // What rows see of an odd key's values is added at the end; in the products they count as 0 (where the
+            // scale is NaN so are the codes).
+            if (odd_scale(v)) {
+              odd_keys |= 1u << (g + 8 * h);
+              vscale[h] = 0.0f;
+              lift[h] = (float)kLeastLift;
+            } else {
+              f = max(f, v >> 23);
+              lift[h] = lift_of((int)(v >> 23));
+            }
           }
-          nan_keys = __reduce_or_sync(0xFFFFFFFFu, nan_keys);
-          field = max(field, (int)warp_max(f));
+          odd_keys = __reduce_or_sync(0xFFFFFFFFu, odd_keys);
+          vfield = max(vfield, (int)warp_max(f));
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            if (lift[h] >= lift_of(vfield) - kNarrow) lift[h] = lift_of(vfield);
         }
         float keep[NR][2];
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
           for (int r = 0; r < 2; ++r) {
-            float top = m[nr][r];
+            float top = fmaxf(x[nr][r] + lift[0], x[nr][2 + r] + lift[1]);
 #pragma unroll
             for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
-            const float now = top > ref[nr][r] + (above + 8.0f) ? ceilf(top) : ref[nr][r] + above;
-            const float next = now - room(field);
+            const float next = top > ref[nr][r] + kHeadroom ? ceilf(top) - kBelow : ref[nr][r];
             keep[nr][r] = exp2_fast(ref[nr][r] - next);
             ref[nr][r] = next;
             sum[nr][r] *= keep[nr][r];
           }
-        vfield = field;
 #pragma unroll
         for (int k = 0; k < DP / 16; ++k)
 #pragma unroll
           for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
             for (int e = 0; e < 4; ++e) o[k][nr][e] *= keep[nr][e & 1];
+        if (odd_keys && lane == 0) left_out[warp] = 1;
       }
       uint32_t pf[NR][2];  // P^T: keys 2 t, 2 t + 1 (and + 8) of row g
 #pragma unroll
@@ -509,10 +516,10 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
         for (int k = 0; k < 4; ++k) {
           const int key = 2 * t + (k & 1) + 8 * (k >> 1);
           load_words<P::kVPart / 4>(st + P::kSide + voff[kWide ? k & 1 : k][part] + (kWide ? 8 * (k >> 1) * P::kRowBytes : 0), w[k]);
-          if (nan_keys)
+          if (nan_keys | odd_keys)
 #pragma unroll
             for (int q = 0; q < P::kVPart / 4; ++q)
-              if ((nan_keys >> key) & 1u) w[k][q] = 0u;
+              if (((nan_keys | odd_keys) >> key) & 1u) w[k][q] = 0u;
         }
 #pragma unroll
         for (int q = 0; q < P::kVPart / 4; ++q) {
@@ -580,6 +587,32 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           mo[(g * (DP / 8) + 2 * k + (e >> 1)) * kRows + 8 * nr + 2 * t + (e & 1)] = o[k][nr][e];
+    __syncwarp();
+    if (left_out[warp]) {
+      // The values of odd keys in fp32, to the rows that see them; a row's score of the key is worked out again.
+      for (int i = 0; i < steps; ++i) {
+        const int mine = key0 + i * kKeys + lane, pg = lane < kStep && mine < key1 ? table[mine >> c.page_shift] : -1;
+        const int64_t own = pg >= 0 && pg < c.pages ? (((int64_t)pg * c.heads + it.head) << c.page_shift) + (mine & (c.page_size - 1)) : -1;
+        for (uint32_t odd = __ballot_sync(0xFFFFFFFFu, own >= 0 && odd_values<S>(c, own)); odd; odd &= odd - 1) {
+          const int from = __ffs(odd) - 1, at = key0 + i * kKeys + from;
+          const int64_t row = __shfl_sync(0xFFFFFFFFu, own, from);
+          for (int in = 0; in < kRows && it.tile * kRows + in < rows; ++in) {
+            const int r = it.tile * kRows + in;
+            int row_lo, row_hi;
+            visible(a, s, r / a.group, row_lo, row_hi);
+            if (at < row_lo || at >= row_hi) continue;
+            const T *qp = static_cast<const T *>(a.q) + (s.q0 + r / a.group) * a.q_tok + (it.head * a.group + r % a.group) * a.q_head;
+            float dot = 0.0f;
+            for (int d = lane; d < dim; d += 32)
+              dot = __fmaf_rn(Io<T>::get(qp[d]), cached<T>(c, c.k + row * row_bytes, c.ks + row * scale_bytes, d), dot);
+            for (int k = 16; k; k >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, k);
+            const float w = exp2_fast(dot * a.scale - merge_top[warp][in]);
+            for (int d = lane; d < dim; d += 32)
+              mo[d * kRows + in] = __fmaf_rn(w, cached<T>(c, c.v + row * row_bytes, c.vs + row * scale_bytes, d), mo[d * kRows + in]);
+          }
+        }
+      }
+    }
     __syncthreads();
     const bool done = it.at == 0 && it.n == it.units;
     float *part = parts + (size_t)(2 * blockIdx.x + (it.at > 0 ? 0 : 1)) * partial_floats(kRows, DP);

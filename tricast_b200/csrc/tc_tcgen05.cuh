@@ -102,6 +102,12 @@ __device__ __forceinline__ void tmem_ld_frag32(uint32_t taddr, uint32_t (&r)[16]
       : "r"(taddr));
 }
 
+// 8 columns: the four registers of j = 0 (tmem_wait_ld waits for them).
+__device__ __forceinline__ void tmem_ld_frag8(uint32_t taddr, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(taddr));
+}
+
 // Wait for the loads of these registers, which pass through the statements behind the wait so that no use of
 // them moves above it.
 template <int N>
