@@ -126,14 +126,14 @@ def test_a_seen_key_of_large_values_and_little_weight(scheme, factor, new, total
 
 @pytest.mark.parametrize("kind", ["inf", "nan"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
-@pytest.mark.parametrize("scheme", ["fp8_row", "int8_row", "mxfp4"])
+@pytest.mark.parametrize("scheme", [None, "fp8_row", "int8_row", "mxfp4"])
 @pytest.mark.parametrize("new,total,heads,kv_heads,window", SHAPES)
 def test_seen_values_that_are_not_finite_reach_their_elements(scheme, dtype, kind, new, total, heads, kv_heads, window):
-    """The first key of the chunk, in units that some rows see and others do not; sums and other elements stay."""
-    b = Batch([new], [total], heads, kv_heads, 128, 16, scheme, dtype, seed=new)
-    odd = sorted({total - new, max(total - 40, total - new), total - 1})
-    _put(b, odd, v=_odd_values(b, odd, kind))
-    _check(b, window)
+    """In units that some rows see and others do not, and in one that all see; sums and other elements stay."""
+    for odd in (sorted({total - new, max(total - 40, total - new), total - 1}), [130] if not window else [total - 30]):
+        b = Batch([new], [total], heads, kv_heads, 128, 16, scheme, dtype, seed=new)
+        _put(b, odd, v=_odd_values(b, odd, kind))
+        _check(b, window)
 
 
 @pytest.mark.parametrize("scheme", [None, "fp8_row", "mxfp4"])

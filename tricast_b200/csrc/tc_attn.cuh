@@ -250,10 +250,23 @@ __device__ __forceinline__ float cached(const KvCache &c, const unsigned char *c
   return __fmul_rn(c.scheme == KV_FP8_ROW ? decode_e4m3(codes[d]) : (float)(signed char)codes[d], s);
 }
 
-// Whether the products leave a row's values out. S: the scheme where it is known, KV_NONE for rows without scales.
-template <int S>
+// Either half of a word is an element whose exponent is all ones.
+template <typename T>
+__device__ __forceinline__ bool not_finite2(uint32_t w) {
+  const uint32_t m = Same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
+  return (w & m) == m || ((w >> 16) & m) == m;
+}
+
+// Whether the products leave a row's values out: those under an odd scale, and values without scales that are not
+// finite, where rows differ in what they see. S: the scheme where it is known.
+template <typename T, int S>
 __device__ __forceinline__ bool odd_values(const KvCache &c, int64_t row) {
-  if (S == KV_NONE) return false;
+  if (S == KV_NONE) {
+    const uint32_t *v = reinterpret_cast<const uint32_t *>(c.v + row * c.row_bytes);
+    bool odd = false;
+    for (int d = 0; d < c.row_bytes / 4; ++d) odd |= not_finite2<T>(v[d]);
+    return odd;
+  }
   if (c.scheme != KV_MXFP4) return odd_scale(*reinterpret_cast<const uint32_t *>(c.vs + row * 4));
   uint32_t big = 0u;
   for (int q = 0; q < c.scale_bytes; ++q) big = max(big, (uint32_t)c.vs[row * c.scale_bytes + q]);

@@ -58,10 +58,10 @@ constexpr int kOdd = 0x7FFFFFFF;
 struct __align__(16) KeySlot {
   float k[kKeys], v[kKeys];
   uint32_t valid[4];  // keys that are there
-  uint32_t dead[4];   // keys whose rows of scores or values are not numbers: their scales here are 1, their V
-                      // is 0, and the rows that see them become NaN
-  // Largest and least exponent field of the value scales, by quarter (0 and 255: none). A key whose values' scale is
-  // odd (tc_attn.cuh) has the scale 0 here, and makes its quarter's largest kOdd, which no reference is low enough for.
+  uint32_t dead[4];   // keys whose scale is not a number: it is 1 here, and the rows that see them become NaN
+  // Largest and least exponent field of the value scales, by quarter (0 and 255: none). A key whose values the products
+  // leave out (tc_attn.cuh) has the scale 0 here, and makes its quarter's largest kOdd, which no reference is low enough
+  // for.
   int top[4], low[4];
 };
 
@@ -227,10 +227,10 @@ __device__ __forceinline__ void granule(const uint32_t (&w)[4], int g, uint32_t 
     }
   }
 }
-// A quarter's entries of its unit's slot, a lane a key: its scales' words, whether it is there, and whether its
-// rows of an unquantized cache are not numbers.
+// A quarter's entries of its unit's slot, a lane a key: its scales' words, whether it is there, and whether the products
+// leave out its values of an unquantized cache.
 template <int S, int DP>
-__device__ __forceinline__ void put_keys(KeySlot &sl, int quarter, bool there, uint32_t kw, uint32_t vw, bool dead) {
+__device__ __forceinline__ void put_keys(KeySlot &sl, int quarter, bool there, uint32_t kw, uint32_t vw, bool odd) {
   const int lane = threadIdx.x & 31;
   float k = 1.0f, v = 1.0f;
   if (S == KV_MXFP4) {
@@ -240,8 +240,8 @@ __device__ __forceinline__ void put_keys(KeySlot &sl, int quarter, bool there, u
     k = u2f(kw);
     v = u2f(vw);
   }
-  dead |= k != k;
-  const bool odd = there && odd_scale(f2u(v));
+  const bool dead = k != k;
+  odd = there && (odd || odd_scale(f2u(v)));
   if (!there || dead) k = 1.0f;
   if (!there) v = 1.0f;
   if (odd) v = 0.0f;
@@ -335,16 +335,8 @@ __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsign
     return r.page >= 0 ? scale_word<S, DP>(c, scales, row_at(r, r.page, lane)) : 0u;
   };
   // Where rows of a job differ in what they see, a V row of an unquantized cache that is not finite must not
-  // reach the others: the whole row counts as 0 and the weights of the rows that see it become NaN.
-  auto not_finite = [&](const Job &r) {
-    bool bad = false;
-    if (r.mixed && r.page >= 0) {
-      const uint32_t m = Same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
-      const uint32_t *v = reinterpret_cast<const uint32_t *>(c.v + row_at(r, r.page, lane) * c.row_bytes);
-      for (int d = 0; d < c.row_bytes / 4; ++d) bad |= (v[d] & m) == m || ((v[d] >> 16) & m) == m;
-    }
-    return bad;
-  };
+  // reach the others: the products take it as 0.
+  auto not_finite = [&](const Job &r) { return r.mixed && r.page >= 0 && odd_values<T, S>(c, row_at(r, r.page, lane)); };
   // The keys' entries of the unit's slot.
   auto put_slot = [&](uint32_t job, const Job &r, uint32_t kw, uint32_t vw) {
     put_keys<S, DP>(slots[(job >> 3) % kSlots], job & 3, r.page >= 0, kw, vw, S == KV_NONE && not_finite(r));
@@ -743,7 +735,9 @@ __device__ __noinline__ void add_odd(const Args &a, const Stash &mine, const uns
 #pragma unroll 1
   for (int at0 = mine.p.key0; at0 < mine.p.key1; at0 += 32) {
     const int64_t own = at0 + lane < mine.p.key1 ? row_of(at0 + lane) : -1;
-    uint32_t odd = __ballot_sync(0xFFFFFFFFu, own >= 0 && odd_values<S>(c, own));
+    const int unit = at0 - (at0 - mine.p.key0) % kKeys;
+    if (S == KV_NONE && unit >= mine.p.all_lo && unit + kKeys <= mine.p.all_hi) continue;  // every row sees the unit
+    uint32_t odd = __ballot_sync(0xFFFFFFFFu, own >= 0 && odd_values<T, S>(c, own));
 #pragma unroll 1
     for (; odd; odd &= odd - 1) {
       const int at = at0 + __ffs(odd) - 1;
@@ -900,6 +894,7 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
             Rows x;
             rows_of(raw[half], x);
             if (!whole) {
+              if (S == KV_NONE && max(max(sl.top[0], sl.top[1]), max(sl.top[2], sl.top[3])) == kOdd) mine.odd = true;
               int lo[4], hi[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {

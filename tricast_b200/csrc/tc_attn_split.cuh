@@ -66,13 +66,6 @@ struct Shape {
 // 16-byte granule i of a stage side, swizzled so that reads along a key and across keys spread over the banks.
 __device__ __forceinline__ int granule(int i) { return i ^ ((i >> 3) & 7); }
 
-// A 16-bit element whose exponent is all ones.
-template <typename T>
-__device__ __forceinline__ bool not_finite2(uint32_t w) {
-  const uint32_t m = Same<T, __nv_bfloat16>::value ? 0x7F80u : 0x7C00u;
-  return (w & m) == m || ((w >> 16) & m) == m;
-}
-
 // PAD: head_dim is below DP (the general, slower addressing).
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t r;
@@ -406,22 +399,18 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
         for (int h = 0; h < 2; ++h)
           if (!((valid >> (g + 8 * h)) & 1u)) vscale[h] = 0.0f;
       }
-      uint32_t nan_keys = 0u;  // keys whose values are not numbers
-      uint32_t odd_keys = 0u;  // keys whose values' scales are odd (tc_attn.cuh)
+      uint32_t odd_keys = 0u;  // keys whose values the products leave out (tc_attn.cuh)
       if (S == KV_NONE && !whole) {
         // Rows of the step differ in what they see: a value that is not finite must not reach the others.
-        // Its whole row counts as 0 and the weights of the rows that see it become NaN.
         for (int r = 0; r < kStep; ++r) {
           bool bad = false;
           for (int w = lane; w < P::kRowBytes / 4; w += 32) {
             const int at = r * P::kRowBytes + 4 * w;
             bad |= not_finite2<T>(*reinterpret_cast<const uint32_t *>(st + P::kSide + 16 * granule(at / 16) + at % 16));
           }
-          if (__any_sync(0xFFFFFFFFu, bad)) nan_keys |= 1u << r;
+          if (__any_sync(0xFFFFFFFFu, bad)) odd_keys |= 1u << r;
         }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          if ((nan_keys >> (g + 8 * h)) & 1u) vscale[h] = u2f(kQNaN);
+        if (odd_keys && lane == 0) left_out[warp] = 1;
       }
 
       // May a row's reference have to move?
@@ -490,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
           for (int r = 0; r < 2; ++r) {
             p[r] = exp2_fast(x[nr][2 * h + r] - ref[nr][r]);
             sum[nr][r] += p[r];
-            if (S != KV_NONE || nan_keys) p[r] = nan_keys && p[r] == 0.0f ? 0.0f : p[r] * vscale[h];
+            if (S != KV_NONE) p[r] *= vscale[h];
           }
           pf[nr][h] = transpose8x8(kBf16 ? pack_bf16(p[0], p[1]) : pack_half(p[0], p[1]));
         }
@@ -516,10 +505,10 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
         for (int k = 0; k < 4; ++k) {
           const int key = 2 * t + (k & 1) + 8 * (k >> 1);
           load_words<P::kVPart / 4>(st + P::kSide + voff[kWide ? k & 1 : k][part] + (kWide ? 8 * (k >> 1) * P::kRowBytes : 0), w[k]);
-          if (nan_keys | odd_keys)
+          if (odd_keys)
 #pragma unroll
             for (int q = 0; q < P::kVPart / 4; ++q)
-              if (((nan_keys | odd_keys) >> key) & 1u) w[k][q] = 0u;
+              if ((odd_keys >> key) & 1u) w[k][q] = 0u;
         }
 #pragma unroll
         for (int q = 0; q < P::kVPart / 4; ++q) {
@@ -593,7 +582,14 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
       for (int i = 0; i < steps; ++i) {
         const int mine = key0 + i * kKeys + lane, pg = lane < kStep && mine < key1 ? table[mine >> c.page_shift] : -1;
         const int64_t own = pg >= 0 && pg < c.pages ? (((int64_t)pg * c.heads + it.head) << c.page_shift) + (mine & (c.page_size - 1)) : -1;
-        for (uint32_t odd = __ballot_sync(0xFFFFFFFFu, own >= 0 && odd_values<S>(c, own)); odd; odd &= odd - 1) {
+        if (S == KV_NONE) {  // only where rows differ in what they see
+          int lo_r, hi_r, unused;
+          visible(a, s, it.tile * kRows / a.group, unused, hi_r);
+          visible(a, s, (min((it.tile + 1) * kRows, rows) - 1) / a.group, lo_r, unused);
+          const int p0 = key0 + i * kKeys;
+          if (__ballot_sync(0xFFFFFFFFu, own >= 0) == 0xFFFFu && p0 >= lo_r && p0 + kStep <= hi_r) continue;
+        }
+        for (uint32_t odd = __ballot_sync(0xFFFFFFFFu, own >= 0 && odd_values<T, S>(c, own)); odd; odd &= odd - 1) {
           const int from = __ffs(odd) - 1, at = key0 + i * kKeys + from;
           const int64_t row = __shfl_sync(0xFFFFFFFFu, own, from);
           for (int in = 0; in < kRows && it.tile * kRows + in < rows; ++in) {
