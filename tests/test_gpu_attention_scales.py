@@ -124,6 +124,21 @@ def test_a_seen_key_of_large_values_and_little_weight(scheme, factor, new, total
     _check(b, 0)
 
 
+@pytest.mark.parametrize("scheme", ["fp8_row", "int8_row", "mxfp4"])
+@pytest.mark.parametrize("new,total,heads,kv_heads,window", SHAPES)
+@pytest.mark.parametrize("size", [1e-2, 1e-5, 1e-9])
+def test_rows_of_zeros_among_small_values(scheme, size, new, total, heads, kv_heads, window):
+    """A row of zeros has a scale of its own (1): it is no measure of the others."""
+    b = Batch([new], [total], heads, kv_heads, 128, 16, scheme, torch.bfloat16, seed=new)
+    everything = list(range(total))
+    v = b.v[0] * size
+    v[::7] = 0
+    v[0] = -v[0]  # zeros of either sign
+    v[-3:] = 0
+    _put(b, everything, v=v)
+    _check(b, window)
+
+
 @pytest.mark.parametrize("kind", ["inf", "nan"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16], ids=str)
 @pytest.mark.parametrize("scheme", [None, "fp8_row", "int8_row", "mxfp4"])

@@ -232,6 +232,13 @@ constexpr int kLeastLift = -60, kMostLift = 40;
 // Lifts this close under the largest may count as the largest: the reference moves less often, and 16 of the 20 binades
 // remain.
 constexpr int kNarrow = 4;
+// A row of zeros has the scale 1, which says nothing of other rows: no reference follows it.
+constexpr uint32_t kOneScale = 0x3F800000u;
+// The bits of four codes that make them other than zeros (of either sign).
+template <int S>
+__device__ __forceinline__ uint32_t nonzero_codes(uint32_t w) {
+  return S == KV_FP8_ROW ? w & 0x7F7F7F7Fu : w;
+}
 // For the exponent field of a scale.
 __device__ __forceinline__ float lift_of(int field) { return (float)max(field - 127, kLeastLift); }
 // A value scale (its bits) that the fp16 products do not take: beyond 2**kMostLift, infinite, NaN or negative.

@@ -61,7 +61,7 @@ struct __align__(16) KeySlot {
   uint32_t dead[4];   // keys whose scale is not a number: it is 1 here, and the rows that see them become NaN
   // Largest and least exponent field of the value scales, by quarter (0 and 255: none). A key whose values the products
   // leave out (tc_attn.cuh) has the scale 0 here, and makes its quarter's largest kOdd, which no reference is low enough
-  // for.
+  // for; one whose values are zeros has the scale 0 too, and counts in neither.
   int top[4], low[4];
 };
 
@@ -227,11 +227,12 @@ __device__ __forceinline__ void granule(const uint32_t (&w)[4], int g, uint32_t 
     }
   }
 }
-// A quarter's entries of its unit's slot, a lane a key: its scales' words, whether it is there, and whether the products
-// leave out its values of an unquantized cache.
+// A quarter's entries of its unit's slot, a lane a key: its row in the cache (-1: it is not there), its scales' words, and
+// whether the products leave out its values of an unquantized cache.
 template <int S, int DP>
-__device__ __forceinline__ void put_keys(KeySlot &sl, int quarter, bool there, uint32_t kw, uint32_t vw, bool odd) {
+__device__ __forceinline__ void put_keys(const KvCache &c, KeySlot &sl, int quarter, int64_t row, uint32_t kw, uint32_t vw, bool odd) {
   const int lane = threadIdx.x & 31;
+  const bool there = row >= 0;
   float k = 1.0f, v = 1.0f;
   if (S == KV_MXFP4) {
     k = pow2_value((uint32_t)biggest<DP>(kw)) * (1.0f / (1 << kGroupShift));
@@ -244,12 +245,22 @@ __device__ __forceinline__ void put_keys(KeySlot &sl, int quarter, bool there, u
   odd = there && (odd || odd_scale(f2u(v)));
   if (!there || dead) k = 1.0f;
   if (!there) v = 1.0f;
-  if (odd) v = 0.0f;
+  bool zeros = false;
+  if ((S == KV_FP8_ROW || S == KV_INT8_ROW) && there && vw == kOneScale) {
+    uint32_t bits = 0u;
+    for (int d = 0; d < c.row_bytes; d += 16) {
+      uint32_t w[4];
+      load_words<4>(c.v + row * c.row_bytes + d, w);
+      bits |= nonzero_codes<S>(w[0] | w[1] | w[2] | w[3]);
+    }
+    zeros = bits == 0u;
+  }
+  if (odd || zeros) v = 0.0f;
   sl.k[32 * quarter + lane] = k;
   sl.v[32 * quarter + lane] = v;
   const uint32_t valid = __ballot_sync(0xFFFFFFFFu, there), dead_keys = __ballot_sync(0xFFFFFFFFu, there && dead);
   const int top = (int)__reduce_max_sync(0xFFFFFFFFu, odd ? (unsigned)kOdd : there ? f2u(v) >> 23 : 0u);
-  const int low = (int)__reduce_min_sync(0xFFFFFFFFu, there && !odd ? f2u(v) >> 23 : 255u);
+  const int low = (int)__reduce_min_sync(0xFFFFFFFFu, there && !odd && !zeros ? f2u(v) >> 23 : 255u);
   if (lane == 0) {
     sl.valid[quarter] = valid;
     sl.dead[quarter] = dead_keys;
@@ -339,7 +350,8 @@ __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsign
   auto not_finite = [&](const Job &r) { return r.mixed && r.page >= 0 && odd_values<T, S>(c, row_at(r, r.page, lane)); };
   // The keys' entries of the unit's slot.
   auto put_slot = [&](uint32_t job, const Job &r, uint32_t kw, uint32_t vw) {
-    put_keys<S, DP>(slots[(job >> 3) % kSlots], job & 3, r.page >= 0, kw, vw, S == KV_NONE && not_finite(r));
+    put_keys<S, DP>(c, slots[(job >> 3) % kSlots], job & 3, r.page >= 0 ? row_at(r, r.page, lane) : -1, kw, vw,
+                    S == KV_NONE && not_finite(r));
   };
   auto wait_empty = [&](uint32_t job) {
     const uint32_t unit = job >> 3, st = unit & 1, parity = ((unit >> 1) & 1) ^ 1;
@@ -1138,7 +1150,8 @@ __global__ void __launch_bounds__(256) pack_kernel(Args a, unsigned char *packed
   uint32_t word = vw;
   if (side == 0) {
     word = page >= 0 ? scale_word<S, DP>(c, c.ks, row_at(page, lane)) : 0u;
-    put_keys<S, DP>(*reinterpret_cast<KeySlot *>(to + Packed<DP>::kSlot), quarter, page >= 0, word, vw, false);
+    put_keys<S, DP>(c, *reinterpret_cast<KeySlot *>(to + Packed<DP>::kSlot), quarter, page >= 0 ? row_at(page, lane) : -1, word,
+                    vw, false);
   }
   // A key with a NaN value scale has NaN codes, which would be 0 * NaN for every row: they count as 0.
   const uint32_t dead = S == KV_FP8_ROW && side ? __ballot_sync(0xFFFFFFFFu, (vw & 0x7FFFFFFFu) > kInf) : 0u;

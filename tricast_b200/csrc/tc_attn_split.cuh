@@ -427,7 +427,21 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
       if (__any_sync(0xFFFFFFFFu, any)) {
         float lift[2] = {0.0f, 0.0f};
         if (S != KV_NONE) {
-          uint32_t f = 0u;
+          uint32_t f = 0u, zeros = 0u;  // zeros: of this lane's two keys
+          if ((S == KV_FP8_ROW || S == KV_INT8_ROW) &&
+              __any_sync(0xFFFFFFFFu, f2u(vscale[0]) == kOneScale || f2u(vscale[1]) == kOneScale)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              uint32_t bits = 0u;
+              for (int k = t; k < P::kRowBytes / 4; k += 4) {
+                const int at = (g + 8 * h) * P::kRowBytes + 4 * k;
+                bits |= nonzero_codes<S>(*reinterpret_cast<const uint32_t *>(st + P::kSide + 16 * granule(at / 16) + at % 16));
+              }
+              bits |= __shfl_xor_sync(0xFFFFFFFFu, bits, 1);
+              bits |= __shfl_xor_sync(0xFFFFFFFFu, bits, 2);
+              if (bits == 0u && f2u(vscale[h]) == kOneScale) zeros |= 1u << h;
+            }
+          }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t v = f2u(vscale[h]);
@@ -435,6 +449,9 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
             // scale is NaN so are the codes).
             if (odd_scale(v)) {
               odd_keys |= 1u << (g + 8 * h);
+              vscale[h] = 0.0f;
+              lift[h] = (float)kLeastLift;
+            } else if ((zeros >> h) & 1u) {
               vscale[h] = 0.0f;
               lift[h] = (float)kLeastLift;
             } else {
