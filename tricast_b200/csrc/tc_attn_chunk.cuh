@@ -855,7 +855,7 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
           for (int k = 0; k < DP / 2; ++k)
             big = fmaxf(big, fmaxf(fabsf(half_bits_to_float<T>(w[k] & 0xFFFFu)), fabsf(half_bits_to_float<T>(w[k] >> 16))));
           const Pow2 f = fp16_shift(big);
-          qmul *= f.inverse;
+          qmul = fmaxf(qmul * f.inverse, 1.1754943508222875e-38f);  // not 0, whatever the row's size
 #pragma unroll
           for (int k = 0; k < DP / 2; ++k)
             w[k] = pack_half(half_bits_to_float<T>(w[k] & 0xFFFFu) * f.factor, half_bits_to_float<T>(w[k] >> 16) * f.factor);
