@@ -244,6 +244,7 @@ __device__ __forceinline__ void put_keys(const KvCache &c, KeySlot &sl, int quar
   const bool dead = k != k;
   odd = there && (odd || odd_scale(f2u(v)));
   if (!there || dead) k = 1.0f;
+  k = k == 0.0f ? 1.1754943508222875e-38f : k;  // a slot that was never written: scores of 0, hidden ones still -Inf
   if (!there) v = 1.0f;
   bool zeros = false;
   if ((S == KV_FP8_ROW || S == KV_INT8_ROW) && there && vw == kOneScale) {
