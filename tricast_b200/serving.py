@@ -31,10 +31,10 @@ class AttentionLayer:
         self.spec = get_preset(preset).with_(out_format="fp32")
         self.w_qkv, self.w_out = quantize(w_qkv, scheme), quantize(w_out, scheme)
 
-    def __call__(self, x, residual, cache: PagedKVCache, slots, block_table, seq_lens, cu_q=None, *, max_q_len: int = 1):
+    def __call__(self, x, residual, cache: PagedKVCache, slots, block_table, seq_lens, cu_q=None, *, max_q_len: int | None = None):
         """``(out, h)`` for the new tokens ``x`` ``[tokens, hidden]``: their keys and values go to ``slots`` of the
-        cache, and they attend to the ``seq_lens`` tokens of their sequences (:func:`paged_attention`). ``h`` is the
-        residual stream, ``x + residual`` (``x`` itself without one)."""
+        cache, and they attend to the ``seq_lens`` tokens of their sequences (:func:`paged_attention`, which also says
+        what ``cu_q`` and ``max_q_len`` are and default to). ``h`` is the residual stream, ``x + residual`` (``x`` itself without one)."""
         normed, h = rms_norm_quantize(x, self.gain, self.scheme, residual=residual, eps=self.eps)
         qkv = gemm(normed, self.w_qkv, self.spec).to(self.dtype).view(-1, self.heads + 2 * self.kv_heads, self.head_dim)
         q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)  # views: strides are the operators' to follow
