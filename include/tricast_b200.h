@@ -312,13 +312,14 @@ size_t tc_paged_attention_workspace(const tc_kv_cache *cache, int32_t q_heads, i
 /* out = softmax(scale * q k^T) v over each sequence's cached keys and values, for the last tokens of the
  * sequence: q and out [total_q][q_heads][head_dim] of the cache's dtype (q with token and head strides in
  * elements, out contiguous), query head h reading key / value head h / (q_heads / kv_heads). cu_q
- * [batch + 1]: sequence b's new tokens are cu_q[b] .. cu_q[b + 1] - 1, at most max_q_len of them; NULL:
- * one each. seq_lens [batch]: its context, the new tokens (already written) included; token i of n sits
+ * [batch + 1]: sequence b's new tokens are cu_q[b] .. cu_q[b + 1] - 1, of which the first max_q_len are
+ * computed; NULL: one each. seq_lens [batch]: its context, the new tokens (already written) included; token i of n sits
  * at position seq_lens[b] - n + i. block_table [batch][max_pages] (row stride table_stride): the page of
  * each page_size positions; keys on a page outside the cache count as absent. causal: a token sees itself
  * and earlier positions, the last `window` of them where window > 0; otherwise the whole context. Scores,
  * softmax and sums are fp32. A row that sees no key gives zeros, and -Inf in lse (NULL, or the fp32
- * [total_q][q_heads] natural logarithms of the softmax sums). */
+ * [total_q][q_heads] natural logarithms of the softmax sums), as does a token of no sequence (before
+ * cu_q[0], from cu_q[batch] on) or beyond max_q_len. */
 int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64_t q_token_stride, int64_t q_head_stride,
                        int64_t total_q, int32_t q_heads, const int32_t *block_table, int64_t table_stride,
                        int32_t max_pages, const int32_t *seq_lens, const int32_t *cu_q, int32_t batch, int32_t max_q_len,

@@ -20,15 +20,16 @@ def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens:
 
     ``q`` ``[total_q, heads, head_dim]`` of the cache's dtype (any strides with contiguous elements), query head
     ``h`` reading key / value head ``h // (heads // kv_heads)``. ``cu_q`` (int32 ``[batch + 1]``): sequence ``b``'s
-    new tokens are ``q[cu_q[b]:cu_q[b + 1]]``, at most ``max_q_len`` of them (default: ``total_q``); without it
-    every sequence has one. ``seq_lens`` (int32 ``[batch]``): the sequence's context, the new tokens, written
+    new tokens are ``q[cu_q[b]:cu_q[b + 1]]``, of which the first ``max_q_len`` are computed (default: ``total_q``);
+    without it every sequence has one. ``seq_lens`` (int32 ``[batch]``): the sequence's context, the new tokens, written
     before this call, included. ``block_table`` (int32 ``[batch, max_pages]``): the page of each ``page_size``
     positions; entries past the context are not read, and keys on a page outside the cache (``-1``) count as
     absent. ``causal``: a token sees itself and what precedes it, the last ``window`` positions of that where
     ``window > 0``. ``scale`` defaults to ``1 / sqrt(head_dim)``.
 
     Returns ``[total_q, heads, head_dim]`` in the cache's dtype, and with ``return_lse`` the fp32 natural
-    logarithms of the softmax sums ``[total_q, heads]``. A token that sees no key gives zeros and ``-inf``.
+    logarithms of the softmax sums ``[total_q, heads]``. A token that sees no key gives zeros and ``-inf``, as does one
+    of no sequence (before ``cu_q[0]``, from ``cu_q[batch]`` on) or beyond ``max_q_len``.
     Chunks of many tokens over a quantized cache take up to 512 MiB of scratch memory while they run."""
     device = cache.device
     if q.ndim != 3 or q.shape[2] != cache.head_dim or q.dtype != cache.dtype or q.device != device:

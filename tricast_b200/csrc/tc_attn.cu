@@ -121,8 +121,8 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
   const int st = kv_cache_check(cache, a.c);
   if (st != TC_OK) return st;
   auto bad = [](const char *m) { return set_error(std::string("tc_paged_attention: ") + m), (int)TC_INVALID_ARGUMENT; };
-  if (total_q == 0 || batch == 0) return TC_OK;
-  if (!q || !block_table || !seq_lens || !out) return bad("null pointer");
+  if (total_q == 0) return TC_OK;
+  if (!q || !out || (batch > 0 && (!block_table || !seq_lens))) return bad("null pointer");
   if ((uintptr_t)out % 16 || (uintptr_t)workspace % 16) return bad("out and workspace must be 16-byte aligned");
   if (total_q < 0 || total_q > 0x7FFFFFFFll || batch < 0 || max_pages < 0 || max_q_len < 1) return bad("sizes out of range");
   if (!cu_q && total_q != batch) return bad("without cu_q every sequence has one new token");
@@ -150,9 +150,12 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
   a.out = out;
   a.lse = lse;
   cudaStream_t s = (cudaStream_t)stream;
-  if (a.c.dtype == TC_F32) {
+  if (a.c.dtype == TC_F32 || batch == 0) {
     const int64_t want = (total_q * q_heads + 7) / 8, most = (int64_t)sm_count() * 8;
-    attn::plain_kernel<float><<<(unsigned)(want < most ? want : most), attn::kThreads, 0, s>>>(a);
+    const unsigned grid = (unsigned)(want < most ? want : most);
+    if (a.c.dtype == TC_F32) attn::plain_kernel<float><<<grid, attn::kThreads, 0, s>>>(a);
+    else if (a.c.dtype == TC_BF16) attn::plain_kernel<__nv_bfloat16><<<grid, attn::kThreads, 0, s>>>(a);
+    else attn::plain_kernel<__half><<<grid, attn::kThreads, 0, s>>>(a);
     count_launch();
   } else {
     if (!workspace || workspace_bytes < tc_paged_attention_workspace(cache, q_heads, total_q, batch, a.max_q, max_pages))

@@ -24,7 +24,8 @@ struct Args {
   float *lse;                     // [total_q][heads] or nullptr
 };
 
-// New tokens [q0, q0 + n) and context length of a sequence, clamped to what the tensors hold.
+// New tokens [q0, q0 + n) and context length of a sequence, clamped to what the tensors hold. Of more than max_q new
+// tokens the first ones count, at their own positions: to them the context ends where theirs do.
 struct Seq {
   int64_t q0;
   int n, len;
@@ -38,6 +39,7 @@ __device__ __forceinline__ Seq sequence(const Args &a, int b) {
   s.n = (int)min(hi - lo, (int64_t)a.max_q);
   const int64_t held = (int64_t)a.max_pages << a.c.page_shift;
   s.len = (int)min((int64_t)max(a.lens[b], 0), held);
+  if (a.causal) s.len -= (int)(hi - lo) - s.n;
   return s;
 }
 
@@ -292,7 +294,9 @@ __device__ __noinline__ void plain_rows(const Args &a, int64_t warp, int64_t war
     // The last sequence whose first token is not after this one (idle sequences share their start with
     // the next one).
     int b = 0;
-    if (a.cu) {
+    if (a.batch == 0) {
+      b = -1;
+    } else if (a.cu) {
       int hi = a.batch;
       while (b + 1 < hi) {
         const int mid = (b + hi) >> 1;
@@ -302,8 +306,12 @@ __device__ __noinline__ void plain_rows(const Args &a, int64_t warp, int64_t war
     } else {
       b = (int)token;
     }
-    const Seq s = sequence(a, b);
-    if (token < s.q0 || token >= s.q0 + s.n) continue;
+    const Seq s = b < 0 ? Seq{0, 0, 0} : sequence(a, b);
+    if (token < s.q0 || token >= s.q0 + s.n) {
+      for (int d = lane; d < a.c.dim; d += 32) static_cast<T *>(a.out)[r * a.c.dim + d] = Io<T>::put(0.0f);
+      if (a.lse && lane == 0) a.lse[r] = -INFINITY;
+      continue;
+    }
     int lo, hi;
     visible(a, s, (int)(token - s.q0), lo, hi);
     const T *qp = static_cast<const T *>(a.q) + token * a.q_tok + head * a.q_head;
@@ -364,6 +372,35 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 // block of the kernel before gave up a wait (which takes a fault elsewhere, or a test), everything is computed again
 // by the plain rows.
 constexpr int kJoinThreads = 256;
+
+// Zeros (and -Inf) for the tokens that no sequence covers, by one warp a block: the ones before the first sequence and
+// after the last by all of them, those beyond max_q of a sequence by one. Nobody else writes there, so this needs no wait.
+template <typename T>
+__device__ __forceinline__ void fill_tokens(const Args &a, int64_t lo, int64_t hi, int64_t part, int64_t parts) {
+  const int64_t rows = (hi - lo) * a.heads, words = rows * a.c.dim * (int64_t)sizeof(T) / 16;  // head_dim is a multiple of 16
+  uint4 *out = reinterpret_cast<uint4 *>(static_cast<T *>(a.out) + lo * a.heads * a.c.dim);
+  for (int64_t k = part * 32 + (threadIdx.x & 31); k < words; k += parts * 32) out[k] = make_uint4(0, 0, 0, 0);
+  if (a.lse)
+    for (int64_t k = part * 32 + (threadIdx.x & 31); k < rows; k += parts * 32) a.lse[lo * a.heads + k] = -INFINITY;
+}
+template <typename T>
+__device__ __forceinline__ void fill_uncovered(const Args &a) {
+  const int64_t block = blockIdx.x, blocks = gridDim.x;
+  const int64_t first = a.cu[0], last = a.cu[a.batch];
+  for (int64_t b0 = block * 32; b0 < a.batch; b0 += blocks * 32) {
+    const int64_t b = b0 + (threadIdx.x & 31);
+    int64_t lo = 0, hi = 0;
+    if (b < a.batch) {
+      lo = min(max((int64_t)a.cu[b], (int64_t)0) + a.max_q, a.total_q);
+      hi = min((int64_t)a.cu[b + 1], a.total_q);
+    }
+    for (uint32_t some = __ballot_sync(0xFFFFFFFFu, lo < hi); some; some &= some - 1)
+      fill_tokens<T>(a, __shfl_sync(0xFFFFFFFFu, lo, __ffs(some) - 1), __shfl_sync(0xFFFFFFFFu, hi, __ffs(some) - 1), 0, 1);
+  }
+  if (first > 0) fill_tokens<T>(a, 0, min(first, a.total_q), block, blocks);
+  if (last < a.total_q) fill_tokens<T>(a, max(last, (int64_t)0), a.total_q, block, blocks);
+}
+
 template <typename T, int kRows, int kJoinRows>
 __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float *parts, const Stretch *stretches, int dim_pad, int most, const int *status) {
   constexpr int kJoinParts = 2048 / kJoinRows;
@@ -372,6 +409,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float 
   __shared__ float part_top[kJoinParts][kJoinRows], part_sum[kJoinParts][kJoinRows];
   __shared__ float top[kJoinRows], sum[kJoinRows], keep[kJoinRows];
   const int c = blockIdx.x + 1, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (blockIdx.y == 0 && warp == 1 && a.cu) fill_uncovered<T>(a);  // beside what the first warp looks up
   wait_for_previous();
   if (status) {
     int bad = 0;
