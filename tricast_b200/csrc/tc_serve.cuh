@@ -73,12 +73,13 @@ __device__ __forceinline__ float decode_e4m3(uint32_t c) {
 
 // RN(x / s) for finite x without a division: with r = RN(1 / s) a quotient within an ulp or two is corrected
 // twice by its exact remainder (Markstein's theorem: the second step rounds correctly). s in
-// [2**-100, 2**100]; quotients below 2**-60, which every format here rounds to 0, may lose bits.
+// [2**-100, 2**100]; quotients below 2**-60, which every format here rounds to 0, may lose bits. The remainder is taken
+// negated: of q = x = -0 it is +0, and -0 * r + q keeps the sign.
 __device__ __forceinline__ bool divides_fast(float s) { return s >= 7.888609052210118e-31f && s <= 1.2676506002282294e30f; }
 __device__ __forceinline__ float divide_fast(float x, float s, float r) {
   float q = __fmul_rn(x, r);
-  q = __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
-  return __fmaf_rn(__fmaf_rn(-q, s, x), r, q);
+  q = __fmaf_rn(-__fmaf_rn(q, s, -x), r, q);
+  return __fmaf_rn(-__fmaf_rn(q, s, -x), r, q);
 }
 
 // Codes of two values of magnitude at most a hair above the format's largest (finite): low byte first.
