@@ -297,7 +297,8 @@ typedef struct tc_kv_cache {
 
 /* Quantize the keys and values of `tokens` tokens ([tokens][kv_heads][head_dim] with token and head
  * strides in elements, head_dim contiguous) into their slots. Slots outside the cache (-1) are skipped;
- * of two tokens with one slot, either may stay. */
+ * the others must differ: tokens are written in no order and in pieces, so a slot that two of them name
+ * may end with codes of one and scales of the other (no other slot is touched). */
 int tc_kv_write(const tc_kv_cache *cache, const void *k, int64_t k_token_stride, int64_t k_head_stride, const void *v,
                 int64_t v_token_stride, int64_t v_head_stride, const int64_t *slots, int64_t tokens, tc_stream stream);
 

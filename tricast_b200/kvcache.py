@@ -82,8 +82,8 @@ class PagedKVCache:
 
     def write(self, k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor) -> None:
         """Quantize ``k`` and ``v`` ``[tokens, kv_heads, head_dim]`` into ``slots`` (int64 ``[tokens]``) on the
-        current stream. Tokens whose slot is outside the cache (``-1``) are skipped; of several tokens with
-        one slot, any one may stay."""
+        current stream. Tokens whose slot is outside the cache (``-1``) are skipped. The other slots must differ: one
+        that several tokens name may end with codes of one and scales of another (no other slot is touched)."""
         slots = self._slots(slots)
         tokens = slots.shape[0]
         k, v = self._rows(k, tokens, "k"), self._rows(v, tokens, "v")
