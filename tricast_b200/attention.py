@@ -55,6 +55,8 @@ def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens:
         raise ValueError("max_q_len must be positive")
     if cu_q is None:
         max_q_len = 1
+    # Both go on as 32-bit numbers: beyond these they bound nothing (contexts hold at most 2**30 tokens).
+    max_q_len, window = min(max_q_len, max(total, 1)), min(window, 1 << 30)
     if q.stride(2) != 1:
         q = q.contiguous()
     table_stride, one = block_table.stride()

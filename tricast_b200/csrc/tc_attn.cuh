@@ -49,7 +49,8 @@ __device__ __forceinline__ Seq sequence(const Args &a, int b) {
 __device__ __forceinline__ void visible(const Args &a, const Seq &s, int i, int &lo, int &hi) {
   const int at = s.len - s.n + i;
   hi = a.causal ? max(at + 1, 0) : s.len;
-  lo = a.window > 0 ? max(at + 1 - a.window, 0) : 0;
+  // (Far before the first key the difference may wrap round, to an empty range as well.)
+  lo = a.window > 0 ? max((int)((uint32_t)at + 1u - (uint32_t)a.window), 0) : 0;
 }
 
 // ---------------------------------------------------------------- work split
