@@ -518,11 +518,10 @@ __device__ __forceinline__ bool fetch(const Args &a, Item it, const unsigned cha
     if (it.left == 0) break;
     W::next(a, it);
   }
-  // The block's shared memory stays until the copies are in.
-  for (uint32_t k = nk > 2 ? nk - 2 : 0; k < nk; ++k) {
-    mbar_wait_sleep(&bar.kfull[k & 1], (k >> 1) & 1);
-    mbar_wait_sleep(&bar.slot[k % kSlots], (k / kSlots) & 1);
-  }
+  // The block's shared memory stays until the copies are in. A K copy is in before the unit after the next is asked for;
+  // nothing says so of a slot, which is waited for while its barrier is its own.
+  for (uint32_t k = nk > 2 ? nk - 2 : 0; k < nk; ++k) mbar_wait_sleep(&bar.kfull[k & 1], (k >> 1) & 1);
+  for (uint32_t k = nk > kSlots ? nk - kSlots : 0; k < nk; ++k) mbar_wait_sleep(&bar.slot[k % kSlots], (k / kSlots) & 1);
   for (uint32_t k = nv > 2 ? nv - 2 : 0; k < nv; ++k) mbar_wait_sleep(&bar.vfull[k & 1], (k >> 1) & 1);
   return ok;
 }
