@@ -127,7 +127,8 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
   if (total_q < 0 || total_q > 0x7FFFFFFFll || batch < 0 || max_pages < 0 || max_q_len < 1) return bad("sizes out of range");
   if (!cu_q && total_q != batch) return bad("without cu_q every sequence has one new token");
   if (q_heads < 1 || q_heads % cache->kv_heads) return bad("query heads must be a multiple of the cache's");
-  if (!std::isfinite(scale)) return bad("scale must be finite");
+  // The kernels take it times log2(e).
+  if (!std::isfinite((float)((double)scale * 1.4426950408889634))) return bad("scale must be finite, with room for a factor log2(e)");
   if (window < 0 || (window && !causal)) return bad("a window must be positive and needs causal");
   if (((int64_t)max_pages << a.c.page_shift) > (1ll << 30)) return bad("contexts are limited to 2**30 tokens");
   if (total_q * q_heads > 0x7FFFFFFFll) return bad("queries are limited to 2**31 - 1 rows");
