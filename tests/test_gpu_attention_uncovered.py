@@ -60,6 +60,20 @@ def test_no_sequences(dtype):
     assert (out == 0).all() and (lse == float("-inf")).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=str)
+@pytest.mark.parametrize("new", [[1, 1], [200, 3]])
+def test_a_table_without_pages(dtype, new):
+    """No sequence has a page: none of its tokens sees a key."""
+    cache = PagedKVCache(2, 16, 2, 64, dtype=dtype)
+    q = torch.randn(sum(new), 8, 64, device="cuda").to(dtype)
+    cu = torch.tensor([0, new[0], sum(new)], dtype=torch.int32, device="cuda")
+    _leave_nan_behind()
+    for lens in ([0, 0], [5, 900]):
+        out, lse = paged_attention(q, cache, torch.empty((2, 0), dtype=torch.int32, device="cuda"),
+                                   torch.tensor(lens, dtype=torch.int32, device="cuda"), cu, max_q_len=max(new), return_lse=True)
+        assert (out == 0).all() and (lse == float("-inf")).all()
+
+
 def test_a_padded_batch_in_a_graph():
     """The same graph with other counts of tokens: what is padding is read on the device."""
     b = Batch([6, 1, 4], [90, 300, 64], 8, 2, 128, 16, "fp8_row", torch.bfloat16)

@@ -122,7 +122,7 @@ extern "C" int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64
   if (st != TC_OK) return st;
   auto bad = [](const char *m) { return set_error(std::string("tc_paged_attention: ") + m), (int)TC_INVALID_ARGUMENT; };
   if (total_q == 0) return TC_OK;
-  if (!q || !out || (batch > 0 && (!block_table || !seq_lens))) return bad("null pointer");
+  if (!q || !out || (batch > 0 && ((!block_table && max_pages) || !seq_lens))) return bad("null pointer");
   if ((uintptr_t)out % 16 || (uintptr_t)workspace % 16) return bad("out and workspace must be 16-byte aligned");
   if (total_q < 0 || total_q > 0x7FFFFFFFll || batch < 0 || max_pages < 0 || max_q_len < 1) return bad("sizes out of range");
   if (!cu_q && total_q != batch) return bad("without cu_q every sequence has one new token");
