@@ -30,7 +30,8 @@ def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens:
     Returns ``[total_q, heads, head_dim]`` in the cache's dtype, and with ``return_lse`` the fp32 natural
     logarithms of the softmax sums ``[total_q, heads]``. A token that sees no key gives zeros and ``-inf``, as does one
     of no sequence (before ``cu_q[0]``, from ``cu_q[batch]`` on) or beyond ``max_q_len``.
-    Chunks of many tokens over a quantized cache take up to 512 MiB of scratch memory while they run."""
+    Chunks of many tokens over a quantized cache take up to 512 MiB of scratch memory while they run. No gradients
+    pass: the outputs are detached."""
     device = cache.device
     if q.ndim != 3 or q.shape[2] != cache.head_dim or q.dtype != cache.dtype or q.device != device:
         raise ValueError(f"q must be [tokens, heads, {cache.head_dim}] of {cache.dtype} on the cache's device")

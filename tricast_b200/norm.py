@@ -7,11 +7,12 @@ from __future__ import annotations
 import torch
 
 from . import _native as N
-from .operand import QTensor
+from .formats import container_dtype
+from .operand import QTensor, qtensor_class
 from .quantize import _qspec
 
 _CODE_DTYPES = {("float", 4): torch.float8_e4m3fn, ("float", 5): torch.float8_e5m2}
-_PREPARED: dict = {}  # spec object -> (it, its C descriptor, code dtype, group size, scale dtype)
+_PREPARED: dict = {}  # spec object -> (it, its C descriptor, code dtype, group size, scale dtype, class of the result)
 
 
 def _prepared(spec):
@@ -25,7 +26,8 @@ def _prepared(spec):
         if len(_PREPARED) >= 64:
             _PREPARED.clear()
         hit = _PREPARED[id(spec)] = (
-            spec, _qspec(spec), code, group, torch.float8_e8m0fnu if spec.scale.format.kind == "pow2" else torch.float32)
+            spec, _qspec(spec), code, group, torch.float8_e8m0fnu if spec.scale.format.kind == "pow2" else torch.float32,
+            qtensor_class(spec))
     return hit
 
 
@@ -48,13 +50,14 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None, spec, *, res
     ``spec``: a scheme name or spec with 8-bit elements (``fp8_e4m3``, ``fp8_e5m2``, ``int8``), row or group
     granularity and fp32 absmax or E8M0 scales (``fp8_row``, ``int8_row``, ``fp8_group128``, ``mxfp8_*``).
     The QTensor's values are held in the 8-bit torch dtype of the format and E8M0 scales in
-    ``torch.float8_e8m0fnu``; it is an operand of :func:`gemm` like any other. The norm is computed in fp32
-    from the unrounded ``h``, and codes and scales are those :func:`quantize` gives for the fp32 result."""
+    ``torch.float8_e8m0fnu``; it is an operand of :func:`gemm` like any other (with a spec of TriCast's own it is
+    TriCast's class, as :func:`quantize` returns it). The norm is computed in fp32 from the unrounded ``h``, and codes
+    and scales are those :func:`quantize` gives for the fp32 result. No gradients pass: both outputs are detached."""
     if isinstance(spec, str):
         from .spec import get_scheme
 
         spec = get_scheme(spec)
-    _, qs, code_dtype, group, scale_dtype = _prepared(spec)
+    _, qs, code_dtype, group, scale_dtype, cls = _prepared(spec)
     if not x.is_cuda:
         raise ValueError("the B200 backend requires a CUDA tensor")
     shape = x.shape
@@ -88,7 +91,9 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None, spec, *, res
             None if h is None else h.data_ptr(), N.raw_stream(index))
     if status:
         N.check(status, "tc_rms_norm_quantize")
-    return QTensor(values, scale, None, None, spec, tuple(shape)), h
+    if cls is not QTensor:  # TriCast's holds values in the format's container and scales in fp32
+        values, scale = values.to(container_dtype(spec.format)), scale.to(torch.float32)
+    return cls(values, scale, None, None, spec, tuple(shape)), h
 
 
 __all__ = ["rms_norm_quantize"]
