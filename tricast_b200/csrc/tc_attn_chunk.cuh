@@ -722,20 +722,21 @@ __device__ __forceinline__ void highest(const Args &a, const Stash &mine, const 
 }
 
 // Adds what the products left out: the values of odd keys, in fp32, to the outputs of the rows that see them. A thread
-// works out the scores of one row of its warp's 32 again, from Q as it lies in shared memory.
+// works out the scores of one row of its warp's 32 again, from Q as it lies in shared memory. Rare, and a call of its own:
+// inlined it took the softmax loop 8% of its time. 2 us a warp and key.
 template <typename T, int S, int DP>
-__device__ __noinline__ void add_odd(const Args &a, const Stash &mine, const unsigned char *q0, int tile, uint32_t to,
-                                        float4 qm4, float4 ref4) {
-  const float qm[4] = {qm4.x, qm4.y, qm4.z, qm4.w}, ref[4] = {ref4.x, ref4.y, ref4.z, ref4.w};
+__device__ __noinline__ void add_odd(const Args &a, const Stash &mine, const unsigned char *q0, int tile, uint32_t to, float4 qm4, float4 ref4) {
   constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
-  const KvCache &c = a.c;
+  const float qm[4] = {qm4.x, qm4.y, qm4.z, qm4.w}, ref[4] = {ref4.x, ref4.y, ref4.z, ref4.w};
+  const KvCache c = a.c;
   const int lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3, row0 = 32 * ((threadIdx.x >> 5) & 3);
+  const int head = mine.it.head, key0 = mine.p.key0, key1 = mine.p.key1, all_lo = mine.p.all_lo, all_hi = mine.p.all_hi;
   const int *table = a.table + (int64_t)mine.it.b * a.table_stride;
   auto row_of = [&](int at) -> int64_t {
     const int page = table[at >> c.page_shift];
-    return page < 0 || page >= c.pages ? -1 : (((int64_t)page * c.heads + mine.it.head) << c.page_shift) + (at & (c.page_size - 1));
+    return page < 0 || page >= c.pages ? -1 : (((int64_t)page * c.heads + head) << c.page_shift) + (at & (c.page_size - 1));
   };
-  // Of this thread's row.
+  // Of this thread's row; `below` is NaN for one that nothing changes any more.
   float qmul = 0.0f, below = 0.0f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -745,47 +746,67 @@ __device__ __noinline__ void add_odd(const Args &a, const Stash &mine, const uns
   int lo, hi;
   visible(a, mine.p.s, min(mine.it.tile * kRows + tile * kTile + row0 + lane, mine.p.rows - 1) / a.group, lo, hi);
 #pragma unroll 1
-  for (int at0 = mine.p.key0; at0 < mine.p.key1; at0 += 32) {
-    const int64_t own = at0 + lane < mine.p.key1 ? row_of(at0 + lane) : -1;
-    const int unit = at0 - (at0 - mine.p.key0) % kKeys;
-    if (S == KV_NONE && unit >= mine.p.all_lo && unit + kKeys <= mine.p.all_hi) continue;  // every row sees the unit
+  for (int at0 = key0; at0 < key1; at0 += 32) {
+    if (!__any_sync(0xFFFFFFFFu, below == below && lo < at0 + 32 && hi > at0)) continue;
+    const int64_t own = at0 + lane < key1 ? row_of(at0 + lane) : -1;
+    const int unit = at0 - (at0 - key0) % kKeys;
+    if (S == KV_NONE && unit >= all_lo && unit + kKeys <= all_hi) continue;  // every row sees the unit
     uint32_t odd = __ballot_sync(0xFFFFFFFFu, own >= 0 && odd_values<T, S>(c, own));
 #pragma unroll 1
     for (; odd; odd &= odd - 1) {
       const int at = at0 + __ffs(odd) - 1;
       const int64_t row = __shfl_sync(0xFFFFFFFFu, own, at - at0);
-      float dot = 0.0f;
-#pragma unroll 1
-      for (int d = 0; d < c.dim; ++d) {
-        const unsigned char *q = q0 + tile_at(row0 + lane, d >> 3) + 2 * (d & 7);
-        const uint32_t bits = *reinterpret_cast<const unsigned short *>(q);
-        dot = __fmaf_rn(kBf16 ? half_bits_to_float<__nv_bfloat16>(bits) : half_bits_to_float<__half>(bits),
-                        cached<T>(c, c.k + row * c.row_bytes, c.ks + row * c.scale_bytes, d), dot);
-      }
-      const bool sees = at >= lo && at < hi;
-      const float weight = exp2_fast(dot * qmul - below);
+      const bool sees = at >= lo && at < hi && below == below;
       const uint32_t who = __ballot_sync(0xFFFFFFFFu, sees);
+      if (who == 0u) continue;
+      float k[DP / 32], v[DP / 32];  // elements lane + 32 i of the key's rows
+      bool nan = true;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) {
+        const int d = lane + 32 * i;
+        k[i] = v[i] = 0.0f;
+        if (d < c.dim) {
+          k[i] = cached<T>(c, c.k + row * c.row_bytes, c.ks + row * c.scale_bytes, d);
+          v[i] = cached<T>(c, c.v + row * c.row_bytes, c.vs + row * c.scale_bytes, d);
+          nan = nan && v[i] != v[i];
+        }
+      }
+      float dot = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i)
+#pragma unroll 8
+        for (int d = 0; d < 32; d += 2) {
+          const int at2 = 32 * i + d;  // zeros past head_dim, in Q too
+          const uint32_t q = *reinterpret_cast<const uint32_t *>(q0 + tile_at(row0 + lane, at2 >> 3) + 2 * (at2 & 7));
+          dot = __fmaf_rn(kBf16 ? half_bits_to_float<__nv_bfloat16>(q & 0xFFFFu) : half_bits_to_float<__half>(q & 0xFFFFu), __shfl_sync(0xFFFFFFFFu, k[i], d), dot);
+          dot = __fmaf_rn(kBf16 ? half_bits_to_float<__nv_bfloat16>(q >> 16) : half_bits_to_float<__half>(q >> 16), __shfl_sync(0xFFFFFFFFu, k[i], d + 1), dot);
+        }
+      const float weight = exp2_fast(dot * qmul - below);
       float w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = __shfl_sync(0xFFFFFFFFu, weight, 8 * i + g4);
-#pragma unroll 1
-      for (int i = 0; i < 2 * (DP / 32); ++i) {
-        const int h = i & 1;
-        const uint32_t out = to + (h ? 16u << 16 : 0u) + 32 * (i >> 1);
-        uint32_t o[16];
-        tc5::tmem_ld_frag32(out, o);
-        tc5::tmem_wait_ld_frag(o);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          const int d = 32 * (i >> 1) + 8 * (e >> 2) + 2 * t4 + (e & 1), r = 16 * h + (e & 2 ? 8 : 0) + g4;
-          const float mult = h ? (e & 2 ? w[3] : w[2]) : (e & 2 ? w[1] : w[0]);
-          if (d < c.dim && ((who >> r) & 1u))
-            o[e] = f2u(__fmaf_rn(mult, cached<T>(c, c.v + row * c.row_bytes, c.vs + row * c.scale_bytes, d), u2f(o[e])));
+      for (int i = 0; i < DP / 32; ++i) {
+        float part[8];  // columns 8 k + 2 t + e of the 32
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[e] = __shfl_sync(0xFFFFFFFFu, v[i], 8 * (e >> 1) + 2 * t4 + (e & 1));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t out = to + (h ? 16u << 16 : 0u) + 32 * i;
+          uint32_t o[16];
+          tc5::tmem_ld_frag32(out, o);
+          tc5::tmem_wait_ld_frag(o);
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int r = 2 * h + ((e >> 1) & 1);
+            const float sum = __fmaf_rn(w[r], part[2 * (e >> 2) + (e & 1)], u2f(o[e]));
+            o[e] = (who >> (8 * r + g4)) & 1u ? f2u(sum) : o[e];
+          }
+          tc5::tmem_st_frag32(out, o);
         }
-        __syncwarp();
-        tc5::tmem_st_frag32(out, o);
       }
       tc5::tmem_wait_st();
+      if (__all_sync(0xFFFFFFFFu, nan) && sees) below = u2f(kQNaN);  // nothing but NaN is left of the row
     }
   }
 }
@@ -967,7 +988,19 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
       if (!warp_wait_sleep(&bar.ofull[t], items++ & 1, polls)) return false;
       tc5::fence_after_sync();
       __syncwarp();
-      if (mine.odd) add_odd<T, S, DP>(a, mine, q0, t, to, make_float4(qm[0], qm[1], qm[2], qm[3]), make_float4(ref[0], ref[1], ref[2], ref[3]));
+      if (mine.odd) {
+        float live[4];  // the reference; NaN for a row whose sum is NaN, which it stays
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float s0, s1;
+          unpack2(sum2[i], s0, s1);
+          s0 += s1;
+          s0 += __shfl_xor_sync(0xFFFFFFFFu, s0, 1);
+          s0 += __shfl_xor_sync(0xFFFFFFFFu, s0, 2);
+          live[i] = s0 != s0 ? s0 : ref[i];
+        }
+        add_odd<T, S, DP>(a, mine, q0, t, to, make_float4(qm[0], qm[1], qm[2], qm[3]), make_float4(live[0], live[1], live[2], live[3]));
+      }
       const Part p = mine.p;
       const Item it = mine.it;
       const int first = it.tile * kRows + t * kTile + row0;

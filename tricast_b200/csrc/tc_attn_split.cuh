@@ -596,6 +596,9 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
     __syncwarp();
     if (left_out[warp]) {
       // The values of odd keys in fp32, to the rows that see them; a row's score of the key is worked out again.
+      uint32_t gone = 0u;  // rows that nothing changes any more: all NaN
+      for (int in = 0; in < kRows; ++in)
+        if (merge_sum[warp][in] != merge_sum[warp][in]) gone |= 1u << in;
       for (int i = 0; i < steps; ++i) {
         const int mine = key0 + i * kKeys + lane, pg = lane < kStep && mine < key1 ? table[mine >> c.page_shift] : -1;
         const int64_t own = pg >= 0 && pg < c.pages ? (((int64_t)pg * c.heads + it.head) << c.page_shift) + (mine & (c.page_size - 1)) : -1;
@@ -613,15 +616,20 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
             const int r = it.tile * kRows + in;
             int row_lo, row_hi;
             visible(a, s, r / a.group, row_lo, row_hi);
-            if (at < row_lo || at >= row_hi) continue;
+            if (at < row_lo || at >= row_hi || ((gone >> in) & 1u)) continue;
             const T *qp = static_cast<const T *>(a.q) + (s.q0 + r / a.group) * a.q_tok + (it.head * a.group + r % a.group) * a.q_head;
             float dot = 0.0f;
             for (int d = lane; d < dim; d += 32)
               dot = __fmaf_rn(Io<T>::get(qp[d]), cached<T>(c, c.k + row * row_bytes, c.ks + row * scale_bytes, d), dot);
             for (int k = 16; k; k >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, k);
             const float w = exp2_fast(dot * a.scale - merge_top[warp][in]);
-            for (int d = lane; d < dim; d += 32)
-              mo[d * kRows + in] = __fmaf_rn(w, cached<T>(c, c.v + row * row_bytes, c.vs + row * scale_bytes, d), mo[d * kRows + in]);
+            bool nan = true;
+            for (int d = lane; d < dim; d += 32) {
+              const float sum = __fmaf_rn(w, cached<T>(c, c.v + row * row_bytes, c.vs + row * scale_bytes, d), mo[d * kRows + in]);
+              mo[d * kRows + in] = sum;
+              nan = nan && sum != sum;
+            }
+            if (__all_sync(0xFFFFFFFFu, nan)) gone |= 1u << in;
           }
         }
       }
