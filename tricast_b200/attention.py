@@ -50,14 +50,15 @@ def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens:
         raise ValueError("without cu_q every sequence has one new token: q needs as many tokens as block_table rows")
     if window < 0 or (window and not causal):
         raise ValueError("window must be positive and needs causal=True")
-    if max_q_len is None:
-        max_q_len = max(total, 1)
-    elif max_q_len < 1:
+    if max_q_len is not None and max_q_len < 1:
         raise ValueError("max_q_len must be positive")
+    # Both bounds go on as 32-bit numbers: beyond these they bound nothing (contexts hold at most 2**30 tokens).
     if cu_q is None:
         max_q_len = 1
-    # Both go on as 32-bit numbers: beyond these they bound nothing (contexts hold at most 2**30 tokens).
-    max_q_len, window = min(max_q_len, max(total, 1)), min(window, 1 << 30)
+    elif max_q_len is None or max_q_len > total:
+        max_q_len = total or 1
+    if window > 1 << 30:
+        window = 1 << 30
     if q.stride(2) != 1:
         q = q.contiguous()
     table_stride, one = block_table.stride()

@@ -25,29 +25,27 @@ struct Args {
 };
 
 // New tokens [q0, q0 + n) and context length of a sequence, clamped to what the tensors hold. Of more than max_q new
-// tokens the first ones count, at their own positions: to them the context ends where theirs do.
+// tokens (`all`) the first ones count, at their own positions.
 struct Seq {
   int64_t q0;
-  int n, len;
+  int n, len, all;
 };
 __device__ __forceinline__ Seq sequence(const Args &a, int b) {
   Seq s;
-  int64_t lo = a.cu ? a.cu[b] : b, hi = a.cu ? a.cu[b + 1] : b + 1;
-  lo = min(max(lo, (int64_t)0), a.total_q);
-  hi = min(max(hi, lo), a.total_q);
+  const int total = (int)a.total_q;  // below 2**31
+  const int lo = min(max(a.cu ? a.cu[b] : b, 0), total), hi = min(max(a.cu ? a.cu[b + 1] : b + 1, lo), total);
   s.q0 = lo;
-  s.n = (int)min(hi - lo, (int64_t)a.max_q);
-  const int64_t held = (int64_t)a.max_pages << a.c.page_shift;
-  s.len = (int)min((int64_t)max(a.lens[b], 0), held);
-  if (a.causal) s.len -= (int)(hi - lo) - s.n;
+  s.all = hi - lo;
+  s.n = min(s.all, a.max_q);
+  s.len = min(max(a.lens[b], 0), a.max_pages << a.c.page_shift);  // at most 2**30
   return s;
 }
 
-// Keys [lo, hi) that new token i of the sequence sees: it sits at position len - n + i, after the
+// Keys [lo, hi) that new token i of the sequence sees: it sits at position len - all + i, after the
 // sequence's earlier context, and sees itself and what comes before it, at most `window` keys. A
 // position below 0 (more new tokens than context) sees none.
 __device__ __forceinline__ void visible(const Args &a, const Seq &s, int i, int &lo, int &hi) {
-  const int at = s.len - s.n + i;
+  const int at = s.len - s.all + i;
   hi = a.causal ? max(at + 1, 0) : s.len;
   // (Far before the first key the difference may wrap round, to an empty range as well.)
   lo = a.window > 0 ? max((int)((uint32_t)at + 1u - (uint32_t)a.window), 0) : 0;
@@ -107,7 +105,7 @@ struct Work {
   static __device__ __forceinline__ void scan(const Args &a, F visit) {
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
-      Seq s{0, 0, 0};
+      Seq s{0, 0, 0, 0};
       int one = 0;
       if (b0 + lane < a.batch) {
         s = sequence(a, b0 + lane);
@@ -121,6 +119,7 @@ struct Work {
           t.q0 = __shfl_sync(0xFFFFFFFFu, s.q0, i);
           t.n = __shfl_sync(0xFFFFFFFFu, s.n, i);
           t.len = __shfl_sync(0xFFFFFFFFu, s.len, i);
+          t.all = __shfl_sync(0xFFFFFFFFu, s.all, i);
           u = head_units(a, t);
         }
         if (!visit(b0 + i, u)) return;
@@ -132,7 +131,7 @@ struct Work {
     int64_t sum = 0;
     const int lane = threadIdx.x & 31;
     for (int b0 = 0; b0 < a.batch; b0 += 32) {
-      Seq s{0, 0, 0};
+      Seq s{0, 0, 0, 0};
       int n = 0;
       if (b0 + lane < a.batch) {
         s = sequence(a, b0 + lane);
@@ -147,6 +146,7 @@ struct Work {
         t.q0 = 0;
         t.n = __shfl_sync(0xFFFFFFFFu, s.n, i);
         t.len = __shfl_sync(0xFFFFFFFFu, s.len, i);
+        t.all = __shfl_sync(0xFFFFFFFFu, s.all, i);
         const int nt = tiles(a, t);
         for (int k = lane; k < nt; k += 32) sum += units(a, t, k);
       }
@@ -307,7 +307,7 @@ __device__ __noinline__ void plain_rows(const Args &a, int64_t warp, int64_t war
     } else {
       b = (int)token;
     }
-    const Seq s = b < 0 ? Seq{0, 0, 0} : sequence(a, b);
+    const Seq s = b < 0 ? Seq{0, 0, 0, 0} : sequence(a, b);
     if (token < s.q0 || token >= s.q0 + s.n) {
       for (int d = lane; d < a.c.dim; d += 32) static_cast<T *>(a.out)[r * a.c.dim + d] = Io<T>::put(0.0f);
       if (a.lse && lane == 0) a.lse[r] = -INFINITY;
@@ -369,9 +369,10 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 // sums are read side by side into shared memory (as many parts at a time as it holds). 64 rows a block keep the
 // chunk kernel's join to one wave of blocks; where few items are cut into many parts, 16 rows a block have more
 // loads in flight (427 rows of one head over 13476 keys: 150 us a call with 64, 82 with 16). The split kernel's
-// items have 8 or 16. Where `status` is given and a
-// block of the kernel before gave up a wait (which takes a fault elsewhere, or a test), everything is computed again
-// by the plain rows.
+// items have 8 or 16. Where `status` is given and a block of the kernel before gave up a wait (which takes a fault
+// elsewhere, or a test), everything is computed again by the plain rows. Four blocks an SM, so that one wave takes the
+// split kernel's, and arguments that the call of the plain rows reads where they are: copied for it by every block they
+// cost 2 us and more (64 sequences of 8192 keys 144 us a call, 138 so; 20 of 1612 27.0 and 25.1).
 constexpr int kJoinThreads = 256;
 
 // Zeros (and -Inf) for the tokens that no sequence covers, by one warp a block: the ones before the first sequence and
@@ -403,7 +404,7 @@ __device__ __forceinline__ void fill_uncovered(const Args &a) {
 }
 
 template <typename T, int kRows, int kJoinRows>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(Args a, const float *parts, const Stretch *stretches, int dim_pad, int most, const int *status) {
+__global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const __grid_constant__ Args a, const float *parts, const Stretch *stretches, int dim_pad, int most, const int *status) {
   constexpr int kJoinParts = 2048 / kJoinRows;
   __shared__ Item item;
   __shared__ int from, upto;
