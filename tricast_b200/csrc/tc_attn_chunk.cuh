@@ -181,7 +181,7 @@ __device__ __forceinline__ Part part_of(const Args &a, const Item &it) {
 struct Stash {
   Item it;
   Part p;
-  bool odd;  // the products left values out (of an item of the softmax)
+  bool odd;  // the products left values out (of an item of the softmax, over a quantized cache)
 };
 // The stash is written by one lane and read by all; the barriers keep the compiler from holding copies.
 __device__ __forceinline__ void put(Stash &st, const Item &it, const Part &p) {
@@ -227,10 +227,9 @@ __device__ __forceinline__ void granule(const uint32_t (&w)[4], int g, uint32_t 
     }
   }
 }
-// A quarter's entries of its unit's slot, a lane a key: its row in the cache (-1: it is not there), its scales' words, and
-// whether the products leave out its values of an unquantized cache.
+// A quarter's entries of its unit's slot, a lane a key: its row in the cache (-1: it is not there) and its scales' words.
 template <int S, int DP>
-__device__ __forceinline__ void put_keys(const KvCache &c, KeySlot &sl, int quarter, int64_t row, uint32_t kw, uint32_t vw, bool odd) {
+__device__ __forceinline__ void put_keys(const KvCache &c, KeySlot &sl, int quarter, int64_t row, uint32_t kw, uint32_t vw) {
   const int lane = threadIdx.x & 31;
   const bool there = row >= 0;
   float k = 1.0f, v = 1.0f;
@@ -242,7 +241,7 @@ __device__ __forceinline__ void put_keys(const KvCache &c, KeySlot &sl, int quar
     v = u2f(vw);
   }
   const bool dead = k != k;
-  odd = there && (odd || odd_scale(f2u(v)));
+  const bool odd = there && odd_scale(f2u(v));
   if (!there || dead) k = 1.0f;
   k = k == 0.0f ? 1.1754943508222875e-38f : k;  // a slot that was never written: scores of 0, hidden ones still -Inf
   if (!there) v = 1.0f;
@@ -295,7 +294,7 @@ struct Job {
 
 template <typename T, int S, int DP>
 __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsigned char *vs, KeySlot *slots, Stash &mine,
-                                        Barriers &bar, int polls) {
+                                        Barriers &bar, int polls, volatile int &left_out) {
   constexpr int kRowBytes = S == KV_NONE ? 2 * DP : S == KV_MXFP4 ? DP / 2 : DP;
   constexpr int kCpr = kRowBytes / 16;                            // 16-byte chunks of a row
   constexpr int kOwn = kCpr;                                      // chunks a lane and job
@@ -351,8 +350,8 @@ __device__ __forceinline__ bool produce(const Args &a, unsigned char *ks, unsign
   auto not_finite = [&](const Job &r) { return r.mixed && r.page >= 0 && odd_values<T, S>(c, row_at(r, r.page, lane)); };
   // The keys' entries of the unit's slot.
   auto put_slot = [&](uint32_t job, const Job &r, uint32_t kw, uint32_t vw) {
-    put_keys<S, DP>(c, slots[(job >> 3) % kSlots], job & 3, r.page >= 0 ? row_at(r, r.page, lane) : -1, kw, vw,
-                    S == KV_NONE && not_finite(r));
+    put_keys<S, DP>(c, slots[(job >> 3) % kSlots], job & 3, r.page >= 0 ? row_at(r, r.page, lane) : -1, kw, vw);
+    if (S == KV_NONE && not_finite(r)) left_out = 1;
   };
   auto wait_empty = [&](uint32_t job) {
     const uint32_t unit = job >> 3, st = unit & 1, parity = ((unit >> 1) & 1) ^ 1;
@@ -830,7 +829,7 @@ __device__ __forceinline__ void rescale(const float (&keep)[4], uint32_t to) {
 
 template <typename T, int S, int DP>
 __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const KeySlot *slots, Stash &mine, uint32_t tmem,
-                                        Barriers &bar, int polls, float *parts) {
+                                        Barriers &bar, int polls, float *parts, volatile int &left_out) {
   constexpr bool kBf16 = S == KV_NONE && Same<T, __nv_bfloat16>::value;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g4 = lane >> 2, t4 = lane & 3;
   const int t = warp >> 2, row0 = 32 * (warp & 3);  // a warp reaches the 32 TMEM lanes of its index
@@ -927,7 +926,6 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
             Rows x;
             rows_of(raw[half], x);
             if (!whole) {
-              if (S == KV_NONE && max(max(sl.top[0], sl.top[1]), max(sl.top[2], sl.top[3])) == kOdd) mine.odd = true;
               int lo[4], hi[4];
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
@@ -988,7 +986,7 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
       if (!warp_wait_sleep(&bar.ofull[t], items++ & 1, polls)) return false;
       tc5::fence_after_sync();
       __syncwarp();
-      if (mine.odd) {
+      if (S == KV_NONE ? __any_sync(0xFFFFFFFFu, left_out) : (int)mine.odd) {
         float live[4];  // the reference; NaN for a row whose sum is NaN, which it stays
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -1076,7 +1074,7 @@ __global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 
   __shared__ __align__(8) Barriers bar;
   __shared__ Item first;
   __shared__ uint32_t tmem_base;
-  __shared__ int failed;
+  __shared__ int failed, left_out;  // left_out: a producer of unquantized units has met values that the products leave out
   unsigned char *smem = raw + (1024 - (smem_addr(raw) & 1023)) % 1024;  // the swizzle is of address bits
   unsigned char *qs = smem, *ks = qs + 2 * Shape<DP>::kOperand, *vs = ks + 2 * Shape<DP>::kOperand;
   const int warp = (int)uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -1086,6 +1084,7 @@ __global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 
       first = mine.first;
       stretches[blockIdx.x] = mine;
       failed = 0;
+      left_out = 0;
     }
   }
   if (threadIdx.x == 0) {
@@ -1118,7 +1117,7 @@ __global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 
     if (warp < kSoftmaxWarps) {
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(softmax_regs(kPacked)));
       put(stash[warp], it, part_of(a, it));
-      ok = softmax<T, S, DP>(a, qs, slots, stash[warp], tmem, bar, polls, parts);
+      ok = softmax<T, S, DP>(a, qs, slots, stash[warp], tmem, bar, polls, parts, left_out);
     } else {
       asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(other_regs(kPacked)));
       if (warp < kSoftmaxWarps + kFeeders) {
@@ -1126,7 +1125,7 @@ __global__ void __launch_bounds__((S == KV_PACKED ? kPackedThreads : kThreads), 
           if (lane == 0) ok = fetch<DP>(a, it, packed, max_units, ks, vs, slots, bar, polls);
         } else {
           put(stash[warp], it, part_of(a, it));
-          ok = produce<T, S, DP>(a, ks, vs, slots, stash[warp], bar, polls);
+          ok = produce<T, S, DP>(a, ks, vs, slots, stash[warp], bar, polls, left_out);
           cp_async_wait_all();
         }
       } else if (warp == kSoftmaxWarps + kFeeders) {
@@ -1184,7 +1183,7 @@ __global__ void __launch_bounds__(256) pack_kernel(Args a, unsigned char *packed
   if (side == 0) {
     word = page >= 0 ? scale_word<S, DP>(c, c.ks, row_at(page, lane)) : 0u;
     put_keys<S, DP>(c, *reinterpret_cast<KeySlot *>(to + Packed<DP>::kSlot), quarter, page >= 0 ? row_at(page, lane) : -1, word,
-                    vw, false);
+                    vw);
   }
   // A key with a NaN value scale has NaN codes, which would be 0 * NaN for every row: they count as 0.
   const uint32_t dead = S == KV_FP8_ROW && side ? __ballot_sync(0xFFFFFFFFu, (vw & 0x7FFFFFFFu) > kInf) : 0u;
