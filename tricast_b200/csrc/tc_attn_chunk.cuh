@@ -1225,7 +1225,14 @@ int launch(const Args &a, float *parts, Stretch *stretches, int *status, int mos
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
   if (dev >= 128 || !((ready[dev >> 6].load(std::memory_order_relaxed) >> (dev & 63)) & 1)) {
-    e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kSmem);
+    // The warps share out the registers that the block is launched with: with fewer their first request would not end.
+    constexpr int kBlockThreads = S == KV_PACKED ? kPackedThreads : kThreads;
+    constexpr int kShares = 32 * kSoftmaxWarps * softmax_regs(S == KV_PACKED) + (kBlockThreads - 32 * kSoftmaxWarps) * other_regs(S == KV_PACKED);
+    cudaFuncAttributes built;
+    e = cudaFuncGetAttributes(&built, kern);
+    if (e == cudaSuccess && built.numRegs * kBlockThreads < kShares)
+      return set_error("tc_paged_attention: the chunk kernel was built with too few registers a thread"), TC_CUDA_ERROR;
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<DP>::kSmem);
     if (e != cudaSuccess) return set_error(std::string("tc_paged_attention: ") + cudaGetErrorString(e)), TC_CUDA_ERROR;
     if (dev < 128) ready[dev >> 6].fetch_or(1ull << (dev & 63), std::memory_order_relaxed);
   }
