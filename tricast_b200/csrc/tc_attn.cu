@@ -37,9 +37,10 @@ static int launch_split(const Args &a, float *parts, cudaStream_t s) {
 }
 
 // From kChunkRows query rows of a key / value head the chunk kernel's tiles of 128 rows pay, unless the call is
-// small: its start and its join are some 25 us more. Split against chunk kernel, us, 8 heads of 128 over fp8: 16
-// sequences of 2048 keys 62 and 80 (32 rows), 97 and 82 (64 rows); 16 of 8192 145 and 195, 259 and 198; one of 16384
-// 79 and 84 (128 rows), 131 and 98 (256); one of 2048 37 and 58 (256), 83 and 61 (1024).
+// small. Split against chunk kernel, us, 8 heads of 128 over fp8: 16 sequences of 2048 keys 60 and 82 (32 rows), 93 and
+// 85 (64 rows), 126 and 86 (96); 16 of 8192 141 and 202, 253 and 206, 364 and 207; one of 16384 52 and 59 (64 rows), 78
+// and 61 (128), 128 and 76 (256); one of 2048 32 and 33 (128), 38 and 39 (256), 69 and 57 (768). The rule is at its worst
+// for one long sequence of 65 to 255 rows, where the split kernel's 78 us stand against 61.
 constexpr int64_t kChunkRows = 65, kChunkTotalRows = 256;
 static bool use_chunk(const KvCache &c, int group, int batch, int64_t max_q) {
   const int64_t rows = max_q * group;
@@ -61,8 +62,8 @@ static size_t chunk_bytes(const KvCache &c) {
 // Whether the chunk kernel's operands are laid out once, before it, and not by every row tile again: for quantized
 // caches (the others need no conversion), from kPackRows query rows of a key / value head on, while the tables'
 // width bounds the room it takes by kPackBytes. Laid out by every tile against once (fp8, 8 heads of 128): 512 rows
-// over one sequence of 16384 keys 112 and 117 us, over sixteen of 2048 193 and 201; 1024 rows 150 and 139, 330 and
-// 287; 2048 rows 239 and 193, 529 and 439.
+// over one sequence of 16384 keys 98 and 105 us, over sixteen of 2048 181 and 185; 768 rows 123 and 119, 248 and 229;
+// 1024 rows 149 and 143, 315 and 271; 2048 rows 241 and 201, 518 and 421.
 constexpr int64_t kPackRows = 768;
 constexpr size_t kPackBytes = (size_t)1 << 29;
 static int pack_units(const KvCache &c, int max_pages) {

@@ -368,7 +368,7 @@ __device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontr
 // stretches and up to 64 rows of the item; it acts if the border is the first inside its item. A row's maxima and
 // sums are read side by side into shared memory (as many parts at a time as it holds). 64 rows a block keep the
 // chunk kernel's join to one wave of blocks; where few items are cut into many parts, 16 rows a block have more
-// loads in flight (427 rows of one head over 13476 keys: 150 us a call with 64, 82 with 16). The split kernel's
+// loads in flight (427 rows of one head over 13476 keys: 133 us a call with 64, 70 with 16). The split kernel's
 // items have 8 or 16. Where `status` is given and a block of the kernel before gave up a wait (which takes a fault
 // elsewhere, or a test), everything is computed again by the plain rows. Four blocks an SM, so that one wave takes the
 // split kernel's, and arguments that the call of the plain rows reads where they are: copied for it by every block they
@@ -593,7 +593,7 @@ inline int launch_join(const Args &a, const float *parts, const Stretch *stretch
   return TC_OK;
 }
 
-// Blocks per multiprocessor of the split kernel, and its width of a head.
+// The width of a head in the kernels' tiles and partial results.
 inline int split_width(int dim) { return dim <= 64 ? 64 : dim <= 128 ? 128 : 256; }
 
 }  // namespace attn

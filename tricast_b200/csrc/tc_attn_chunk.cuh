@@ -13,8 +13,9 @@
 //    of S it has read, half a unit at a time. One tile's softmax runs under the other's MMAs.
 // TMEM: S of the two tiles (128 columns each, P of a half over the half's first 32), O of the two (DP columns each).
 //
-// 4096 new tokens at the end of 16384, 32 query and 8 key heads of 128, E4M3, causal: 956 us, 1006 TFLOP/s, 62% of
-// the measured bf16 peak. The MMAs with everything but the weights' arithmetic take 730 us; a unit's 256 x 128
+// 4096 new tokens at the end of 16384, 32 query and 8 key heads of 128, E4M3, causal: 952 to 983 us, 979 to 1010 TFLOP/s,
+// 61 to 63% of the measured bf16 peak (1056 us a call among others with inputs of their own, 56%). The MMAs with
+// everything but the weights' arithmetic take 730 us; a unit's 256 x 128
 // exponentials are 2048 cycles of the 4500 a unit takes, and the two do not overlap fully: a tile's next scores
 // wait for its weights. Scores in halves of 64 keys, so that they need not, took more MMAs of the same price each
 // and gained nothing; two issuing warps lost 6%.

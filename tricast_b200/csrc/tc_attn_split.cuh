@@ -20,8 +20,9 @@
 // an output over a cache of its own type (fp16 ones over any) is off by 1.4 to 1.6 times what rounding it alone would
 // give. Weights in two parts would undo that for twice the MMAs of the values.
 //
-// 64 sequences of 8192 keys, 8 heads of 128 over E4M3, 4 query heads each: 138 us, 4.8 TB/s of codes. 16 sequences
-// of 4000 keys and 4 new tokens over bf16: 46 us, 2.9 TB/s. One of 1025 keys: 15 us, start, one unit and join.
+// 64 sequences of up to 8192 keys, 8 heads of 128 over E4M3, 4 query heads each: 133 us, 4.9 TB/s of codes (57% of issue
+// slots, 62% of DRAM's cycles busy). 16 sequences of up to 4000 keys and 4 new tokens over bf16: 44 us, 3.1 TB/s. One of
+// 1025 keys: 13.5 us, start, one unit and join.
 #pragma once
 
 #include <atomic>
@@ -66,13 +67,14 @@ struct Shape {
 // 16-byte granule i of a stage side, swizzled so that reads along a key and across keys spread over the banks.
 __device__ __forceinline__ int granule(int i) { return i ^ ((i >> 3) & 7); }
 
-// PAD: head_dim is below DP (the general, slower addressing).
+// An 8 x 8 matrix of 16-bit elements as the MMAs hold it, transposed.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
   return r;
 }
 
+// PAD: head_dim is below DP (the general, slower addressing).
 template <typename T, int S, int DP, int NR, bool PAD>
 __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_kernel(Args a, float *parts, Stretch *stretches, int most) {
   using P = Shape<S, DP, NR>;

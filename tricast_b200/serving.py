@@ -1,7 +1,8 @@
-"""One attention layer as a server runs it, with every product under an emulated accumulation rule: norm to an
-8-bit operand, QKV GEMM, cache write, attention over the cache, output GEMM. It shows the serving operators
-together and measures what a cache scheme costs end to end; ``python -m tricast_b200.serving`` prints that for
-every scheme. No TriCast counterpart (its cache emulation, ``src/tricast/kv/``, has no attention of its own)."""
+"""One attention layer as a server runs it: norm to an 8-bit operand, QKV GEMM, cache write, attention over the cache,
+output GEMM, the GEMMs under an emulated accumulation rule (attention's two products run on the tensor cores as they
+are). It shows the serving operators together and measures what a cache scheme costs end to end; ``python -m
+tricast_b200.serving`` prints that for every scheme. No TriCast counterpart (its cache emulation, ``src/tricast/kv/``,
+has no attention of its own)."""
 
 from __future__ import annotations
 
@@ -34,7 +35,8 @@ class AttentionLayer:
     def __call__(self, x, residual, cache: PagedKVCache, slots, block_table, seq_lens, cu_q=None, *, max_q_len: int | None = None):
         """``(out, h)`` for the new tokens ``x`` ``[tokens, hidden]``: their keys and values go to ``slots`` of the
         cache, and they attend to the ``seq_lens`` tokens of their sequences (:func:`paged_attention`, which also says
-        what ``cu_q`` and ``max_q_len`` are and default to). ``h`` is the residual stream, ``x + residual`` (``x`` itself without one)."""
+        what ``cu_q`` and ``max_q_len`` are and default to). ``h`` is the residual stream, ``x + residual`` (``x`` itself
+        without one)."""
         normed, h = rms_norm_quantize(x, self.gain, self.scheme, residual=residual, eps=self.eps)
         qkv = gemm(normed, self.w_qkv, self.spec).to(self.dtype).view(-1, self.heads + 2 * self.kv_heads, self.head_dim)
         q, k, v = qkv.split((self.heads, self.kv_heads, self.kv_heads), dim=1)  # views: strides are the operators' to follow
