@@ -20,8 +20,8 @@ def paged_attention(q: torch.Tensor, cache, block_table: torch.Tensor, seq_lens:
 
     ``q`` ``[total_q, heads, head_dim]`` of the cache's dtype (any strides with contiguous elements), query head
     ``h`` reading key / value head ``h // (heads // kv_heads)``. ``cu_q`` (int32 ``[batch + 1]``): sequence ``b``'s
-    new tokens are ``q[cu_q[b]:cu_q[b + 1]]``, of which the first ``max_q_len`` are computed (default: ``total_q``);
-    without it every sequence has one. ``seq_lens`` (int32 ``[batch]``): the sequence's context, the new tokens, written
+    new tokens are ``q[cu_q[b]:cu_q[b + 1]]``, of which the first ``max_q_len`` are computed (default: ``total_q``; the
+    bound also chooses the kernel, so a decode step should give it); without it every sequence has one. ``seq_lens`` (int32 ``[batch]``): the sequence's context, the new tokens, written
     before this call, included. ``block_table`` (int32 ``[batch, max_pages]``): the page of each ``page_size``
     positions; entries past the context are not read, and keys on a page outside the cache (``-1``) count as
     absent. ``causal``: a token sees itself and what precedes it, the last ``window`` positions of that where
