@@ -168,3 +168,28 @@ def test_keys_that_are_not_numbers(scheme, new, total, heads, kv_heads):
     assert torch.isnan(out[rows:]).all() and torch.isnan(lse[rows:]).all()
     assert ((out.double() - want).abs()[:rows] <= _bound(torch.bfloat16, scheme) * size[:rows]).all()
     assert ((lse.double() - want_lse)[:rows].abs() <= 1e-4).all()
+
+
+@pytest.mark.parametrize("scheme", ["fp8_row", "int8_row", "mxfp4"])
+@pytest.mark.parametrize("size", [1e-18, 1e-25, 1e-29])
+@pytest.mark.parametrize("new,total,heads,kv_heads,window", SHAPES)
+def test_tiny_values(scheme, size, new, total, heads, kv_heads, window):
+    """What bf16 holds of them an output holds too."""
+    b = Batch([new], [total], heads, kv_heads, 128, 16, scheme, torch.bfloat16, seed=new)
+    _put(b, list(range(total)), v=b.v[0] * size)
+    _check(b, window)
+
+
+@pytest.mark.parametrize("scheme", ["fp8_row", "int8_row", "mxfp4"])
+@pytest.mark.parametrize("low,high", [(2.0 ** -60, 2.0 ** 20), (2.0 ** -85, 2.0 ** 35), (2.0 ** -85, 2.0 ** 60)])
+@pytest.mark.parametrize("new,total", [(1, 3000), (4, 3000), (100, 3000), (1100, 3000)])
+def test_parts_of_different_sizes_weigh_the_same(scheme, low, high, new, total):
+    """One stretch of the context has tiny values, the other large ones, in either order: the tiny ones' weights count in
+    the sum although their values count for nothing."""
+    for order in (1, -1):
+        b = Batch([new], [total], 1, 1, 64, 16, scheme, torch.bfloat16, seed=new, q_scale=0.5)
+        v = b.v[0]
+        half = torch.arange(total, device="cuda")[:, None, None] < 1700
+        v = torch.where(half if order > 0 else ~half, v * low, v * high)
+        _put(b, list(range(total)), v=v)
+        _check(b, 0)

@@ -227,11 +227,13 @@ struct Work {
 // what the products take in fp16. With lift = floor(log2(value scale)), the reference follows the largest x + lift of
 // the keys that the row sees, kBelow under it, and moves when one comes kHeadroom above it: products stay below
 // 2**15, and those within 2**20 of a row's largest keep fp16's 11 bits whatever the scales of other keys are. lift is
-// held at kLeastLift, so that P stays below 2**(kHeadroom - kLeastLift); a value scale above 2**kMostLift, or one that
-// is not a number, stays out of the fp16 products. What a part loses against another whose reference is 2**126
-// higher then had less than 2**(kMostLift - kLeastLift - 126) = 2**-26 of its weight.
+// held at kLeastLift, so that P stays below 2**(kHeadroom - kLeastLift), with room for the sum of 2**19 such keys. A
+// value scale above 2**kMostLift, or one that is not a number, stays out of the fp16 products, its values being added in
+// fp32; it counts as kOddLift, where neither P times its values nor the products of ordinary scales leave their range.
+// Parts whose references differ meet with weights down to 2**-149 (exp2_wide): what one loses had less than
+// 2**(kMostLift - kLeastLift - 149) = 2**-19 of the other's weight.
 constexpr float kBelow = 6.0f, kHeadroom = 14.0f;
-constexpr int kLeastLift = -60, kMostLift = 40;
+constexpr int kLeastLift = -94, kMostLift = 36, kOddLift = -20;
 // Lifts this close under the largest may count as the largest: the reference moves less often, and 16 of the 20 binades
 // remain.
 constexpr int kNarrow = 4;
@@ -481,14 +483,14 @@ __global__ void __launch_bounds__(kJoinThreads, 4) join_kernel(const __grid_cons
       for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
       float l = 0.0f;
       for (int k = lane; k < n; k += 32) {
-        const float w = part_top[k][r] == -INFINITY ? 0.0f : exp2_fast(part_top[k][r] - m);
+        const float w = part_top[k][r] == -INFINITY ? 0.0f : exp2_wide(part_top[k][r] - m);
         // A part that saw no key has no weight; one whose scores were all NaN has a NaN sum that stays.
         l += part_sum[k][r] == 0.0f ? 0.0f : w == 0.0f && part_sum[k][r] == part_sum[k][r] ? 0.0f : part_sum[k][r] * (part_sum[k][r] == part_sum[k][r] ? w : 1.0f);
         part_top[k][r] = w;
       }
       for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x);
       if (lane == 0) {
-        const float f = old == -INFINITY ? 0.0f : exp2_fast(old - m);
+        const float f = old == -INFINITY ? 0.0f : exp2_wide(old - m);
         keep[r] = f;
         sum[r] = sum[r] * f + l;
         top[r] = m;

@@ -61,8 +61,8 @@ struct __align__(16) KeySlot {
   uint32_t valid[4];  // keys that are there
   uint32_t dead[4];   // keys whose scale is not a number: it is 1 here, and the rows that see them become NaN
   // Largest and least exponent field of the value scales, by quarter (0 and 255: none). A key whose values the products
-  // leave out (tc_attn.cuh) has the scale 0 here, and makes its quarter's largest kOdd, which no reference is low enough
-  // for; one whose values are zeros has the scale 0 too, and counts in neither.
+  // leave out (tc_attn.cuh) has the scale -0 here, and makes its quarter's largest kOdd, which no reference is low enough
+  // for; one whose values are zeros has the scale 0, and counts in neither.
   int top[4], low[4];
 };
 
@@ -256,7 +256,8 @@ __device__ __forceinline__ void put_keys(const KvCache &c, KeySlot &sl, int quar
     }
     zeros = bits == 0u;
   }
-  if (odd || zeros) v = 0.0f;
+  if (zeros) v = 0.0f;
+  if (odd) v = -0.0f;
   sl.k[32 * quarter + lane] = k;
   sl.v[32 * quarter + lane] = v;
   const uint32_t valid = __ballot_sync(0xFFFFFFFFu, there), dead_keys = __ballot_sync(0xFFFFFFFFu, there && dead);
@@ -713,7 +714,7 @@ __device__ __forceinline__ void highest(const Args &a, const Stash &mine, const 
     for (int e = 0; e < 2; ++e) {
       const int key = kHalf * half + 8 * j + 2 * t4 + e;
       const bool there = ((sl.valid[key >> 5] & ~sl.dead[key >> 5]) >> (key & 31)) & 1u;
-      const float k = sl.k[key], lift = lift_of((int)(f2u(sl.v[key]) >> 23));
+      const float k = sl.k[key], lift = f2u(sl.v[key]) == 0x80000000u ? (float)kOddLift : lift_of((int)(f2u(sl.v[key]) >> 23));
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         if (there && key >= lo[i] && key < hi[i]) m[i] = fmaxf(m[i], u2f(s[i >> 1][2 * (i & 1) + e]) * k * qm[i] + lift);
@@ -781,7 +782,7 @@ __device__ __noinline__ void add_odd(const Args &a, const Stash &mine, const uns
           dot = __fmaf_rn(kBf16 ? half_bits_to_float<__nv_bfloat16>(q & 0xFFFFu) : half_bits_to_float<__half>(q & 0xFFFFu), __shfl_sync(0xFFFFFFFFu, k[i], d), dot);
           dot = __fmaf_rn(kBf16 ? half_bits_to_float<__nv_bfloat16>(q >> 16) : half_bits_to_float<__half>(q >> 16), __shfl_sync(0xFFFFFFFFu, k[i], d + 1), dot);
         }
-      const float weight = exp2_fast(dot * qmul - below);
+      const float weight = exp2_wide(dot * qmul - below);
       float w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) w[i] = __shfl_sync(0xFFFFFFFFu, weight, 8 * i + g4);
@@ -957,7 +958,7 @@ __device__ __forceinline__ bool softmax(const Args &a, unsigned char *qs, const 
               m[i] = fmaxf(m[i], __shfl_xor_sync(0xFFFFFFFFu, m[i], 2));
               const float next = m[i] > ref[i] + kHeadroom ? ceilf(m[i]) - kBelow : ref[i];
               any |= next != ref[i];
-              keep[i] = exp2_fast(ref[i] - next);
+              keep[i] = S == KV_NONE ? exp2_fast(ref[i] - next) : exp2_wide(ref[i] - next);
               ref[i] = next;
               sum2[i] = mul2(sum2[i], pack2(keep[i], keep[i]));
             }

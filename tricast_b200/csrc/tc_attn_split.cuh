@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
             if (odd_scale(v)) {
               odd_keys |= 1u << (g + 8 * h);
               vscale[h] = 0.0f;
-              lift[h] = (float)kLeastLift;
+              lift[h] = (float)kOddLift;
             } else if ((zeros >> h) & 1u) {
               vscale[h] = 0.0f;
               lift[h] = (float)kLeastLift;
@@ -465,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
           vfield = max(vfield, (int)warp_max(f));
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            if (lift[h] >= lift_of(vfield) - kNarrow) lift[h] = lift_of(vfield);
+            if (lift[h] >= lift_of(vfield) - kNarrow) lift[h] = fmaxf(lift[h], lift_of(vfield));
         }
         float keep[NR][2];
 #pragma unroll
@@ -476,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
 #pragma unroll
             for (int k = 4; k < 32; k <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
             const float next = top > ref[nr][r] + kHeadroom ? ceilf(top) - kBelow : ref[nr][r];
-            keep[nr][r] = exp2_fast(ref[nr][r] - next);
+            keep[nr][r] = exp2_wide(ref[nr][r] - next);
             ref[nr][r] = next;
             sum[nr][r] *= keep[nr][r];
           }
@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
             for (int d = lane; d < dim; d += 32)
               dot = __fmaf_rn(Io<T>::get(qp[d]), cached<T>(c, c.k + row * row_bytes, c.ks + row * scale_bytes, d), dot);
             for (int k = 16; k; k >>= 1) dot += __shfl_xor_sync(0xFFFFFFFFu, dot, k);
-            const float w = exp2_fast(dot * a.scale - merge_top[warp][in]);
+            const float w = exp2_wide(dot * a.scale - merge_top[warp][in]);
             bool nan = true;
             for (int d = lane; d < dim; d += 32) {
               const float sum = __fmaf_rn(w, cached<T>(c, c.v + row * row_bytes, c.vs + row * scale_bytes, d), mo[d * kRows + in]);
@@ -646,7 +646,7 @@ __global__ void __launch_bounds__(kThreads, Shape<S, DP, NR>::kBlocks) split_ker
     float weight[kWarps], total = 0.0f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      weight[w] = merge_top[w][row] == -INFINITY ? 0.0f : exp2_fast(merge_top[w][row] - m);
+      weight[w] = merge_top[w][row] == -INFINITY ? 0.0f : exp2_wide(merge_top[w][row] - m);
       total += merge_sum[w][row] * weight[w];
     }
     const int r = it.tile * kRows + row;

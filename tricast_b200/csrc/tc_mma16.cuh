@@ -54,6 +54,13 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// The same down to 2**-149.
+__device__ __forceinline__ float exp2_wide(float x) {
+  float y;
+  asm("ex2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   uint32_t r;
   asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
