@@ -270,7 +270,8 @@ def _run_plan(st):
     start = (new.cumsum(0) - new).clamp(max=tokens)
     new = torch.minimum(new, tokens - start)
     used = (lens + page - 1) // page
-    need = (((lens + new + page - 1) // page).clamp(max=width) - used).clamp(min=0)
+    wanted = (lens + new + page - 1) // page - used
+    need = torch.minimum(wanted, (width - used).clamp(min=0))
     first = taken + need.cumsum(0) - need
     col = torch.arange(width, device=table.device)
     at = first[:, None] + col - used[:, None]
@@ -287,8 +288,9 @@ def _run_plan(st):
     slots = torch.where(real & (held >= 0), held * page + pos % page, -1)
     total = taken + need.sum()
     after = total.clamp(max=free.numel())
+    missing = total - after + (wanted - need).sum()
     return [table, (lens + new).to(torch.int32), cu.to(torch.int32), slots, torch.where(real, seq, -1).to(torch.int32),
-            torch.where(real, pos, -1).to(torch.int32), after.to(torch.int32), (total - after).to(torch.int32)]
+            torch.where(real, pos, -1).to(torch.int32), after.to(torch.int32), missing.to(torch.int32)]
 
 
 def _run_adapt(st):
