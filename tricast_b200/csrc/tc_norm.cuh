@@ -3,28 +3,17 @@
 // per row or per group of the row. h and y stay in fp32; h is rounded once where it is stored.
 #pragma once
 
-#include <cmath>
-#include <string>
-
-#include "tc_mma16.cuh"
-#include "tc_quant.cuh"
-#include "tc_serve.cuh"
+#include "tc_cast8.cuh"
 
 namespace tc {
 namespace norm {
 
-struct Args {
+struct Args : Cast8 {
   const void *x, *res, *w;
   void *h;
-  unsigned char *codes;
-  void *scale;          // fp32, or E8M0 bytes
-  int64_t rows, K, x_stride, res_stride;
-  int group;            // elements that share a scale (K for row scales)
-  int group_shift;      // its logarithm where it is a power of two
-  int64_t groups;       // per row
+  int64_t rows, x_stride, res_stride;
   int w_dtype;
-  int e8m0, emax;
-  float max_elem, eps;
+  float eps;
 };
 
 constexpr int kThreads = 256;
@@ -99,72 +88,6 @@ __global__ void __launch_bounds__(kThreads) row_kernel(Args a) {
     }
     __syncthreads();
   }
-}
-
-// Eight elements as fp32, from 16-bit or fp32 memory at a 16-byte boundary.
-template <typename T>
-__device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-  } else {
-    const uint4 w = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if constexpr (Same<T, __nv_bfloat16>::value) {
-        v[2 * k] = u2f(u[k] << 16);
-        v[2 * k + 1] = u2f(u[k] & 0xFFFF0000u);
-      } else {
-        v[2 * k] = __half2float(__ushort_as_half((unsigned short)(u[k] & 0xFFFFu)));
-        v[2 * k + 1] = __half2float(__ushort_as_half((unsigned short)(u[k] >> 16)));
-      }
-    }
-  }
-}
-template <typename T>
-__device__ __forceinline__ void store8(T *p, const float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    *reinterpret_cast<uint4 *>(p) = make_uint4(pack16<T>(v[0], v[1]), pack16<T>(v[2], v[3]), pack16<T>(v[4], v[5]), pack16<T>(v[6], v[7]));
-  }
-}
-
-// max(m, |v|), NaN if either is.
-__device__ __forceinline__ float max_abs(float m, float v) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(v)));
-  return r;
-}
-
-// A scale from its domain's largest magnitude: what values are multiplied by (POW2) or divided by.
-struct Scale {
-  float s, r;   // the scale (absmax) and a reciprocal
-  bool fast;    // finite, and divide_fast holds
-  uint32_t code;
-};
-template <bool POW2>
-__device__ __forceinline__ Scale make_scale(uint32_t top, const Args &a) {
-  Scale c;
-  if (POW2) {
-    c.code = pow2_code(top, a.emax);
-    c.r = pow2_inverse(c.code);
-    c.s = 0.0f;
-    c.fast = c.code != 0xFFu;
-  } else {
-    c.s = absmax_scale(top, a.max_elem);
-    c.fast = divides_fast(c.s);
-    c.r = __frcp_rn(c.s);
-    c.code = 0u;
-  }
-  return c;
-}
-template <bool POW2>
-__device__ __forceinline__ void store_scale(const Args &a, int64_t at, const Scale &c) {
-  if (POW2) static_cast<unsigned char *>(a.scale)[at] = (unsigned char)c.code;
-  else static_cast<float *>(a.scale)[at] = c.s;
 }
 
 // One block a row that its registers hold, read once and written once. A thread has NV vectors

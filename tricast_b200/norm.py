@@ -15,11 +15,11 @@ _CODE_DTYPES = {("float", 4): torch.float8_e4m3fn, ("float", 5): torch.float8_e5
 _PREPARED: dict = {}  # spec object -> (it, its C descriptor, code dtype, group size, scale dtype, class of the result)
 
 
-def _prepared(spec):
+def _prepared(spec, what: str):
     hit = _PREPARED.get(id(spec))
     if hit is None or hit[0] is not spec:
         if getattr(spec, "scale", None) is None:
-            raise NotImplementedError("rms_norm_quantize needs a spec with scales")
+            raise NotImplementedError(f"{what} needs a spec with scales")
         f = spec.format
         code = torch.int8 if f.kind == "int" else _CODE_DTYPES.get((f.kind, getattr(f, "ebits", 0)), torch.uint8)
         group = spec.group_size if spec.granularity == "group" else 0
@@ -57,7 +57,7 @@ def rms_norm_quantize(x: torch.Tensor, weight: torch.Tensor | None, spec, *, res
         from .spec import get_scheme
 
         spec = get_scheme(spec)
-    _, qs, code_dtype, group, scale_dtype, cls = _prepared(spec)
+    _, qs, code_dtype, group, scale_dtype, cls = _prepared(spec, "rms_norm_quantize")
     if not x.is_cuda:
         raise ValueError("the B200 backend requires a CUDA tensor")
     shape = x.shape
