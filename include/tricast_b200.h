@@ -327,6 +327,63 @@ int tc_paged_attention(const tc_kv_cache *cache, const void *q, int64_t q_token_
                        float scale, int32_t causal, int32_t window, void *out, float *lse, void *workspace,
                        size_t workspace_bytes, tc_stream stream);
 
+/* Bytes of scratch tc_plan_pages / tc_release_pages need for this many sequences. */
+size_t tc_plan_pages_workspace(int32_t batch);
+size_t tc_release_pages_workspace(int32_t batch);
+
+/* Pages and slots of a batch's new tokens. Sequence i has seq_lens[i] tokens in a paged cache and gets new_lens[i] more, the
+ * batch's new tokens one after the other; those from `tokens` on are left out (the sequences they belong to get fewer). Pages of
+ * page_size (a power of two) tokens that a sequence lacks are taken from the stack free_pages [num_free], whose entries
+ * from *taken on are free, in the order of sequences and positions, and written into its row of block_table
+ * [batch][max_pages] (row stride table_stride); no other entry is touched. Where the stack is empty the entry becomes -1,
+ * and pages beyond max_pages are not taken. Written: out_lens [batch], the lengths with the new tokens; cu_q [batch + 1], where
+ * the sequences' new tokens begin; per new token ([tokens], -1 behind the last) its slot (-1 without a page), sequence and
+ * position; *out_taken, the stack's new top; *missing, pages that were lacking. Nothing else is kept: a program copies out_lens
+ * and out_taken where its next call reads them. No output may alias an input. Lengths below 0 count as 0. */
+int tc_plan_pages(const int32_t *seq_lens, const int32_t *new_lens, int32_t batch, int32_t *block_table, int64_t table_stride,
+                  int32_t max_pages, const int32_t *free_pages, int64_t num_free, const int32_t *taken, int32_t page_size,
+                  int64_t tokens, int32_t *out_lens, int32_t *cu_q, int64_t *slots, int32_t *sequence, int32_t *positions,
+                  int32_t *out_taken, int32_t *missing, void *workspace, size_t workspace_bytes, tc_stream stream);
+
+/* The pages (entries >= 0) of the sequences with ended[i] != 0 go back below the stack's top, in the order of sequences and
+ * columns, and their rows of block_table become -1; *out_taken is the new top. A page must stand in one row only. */
+int tc_release_pages(int32_t *block_table, int64_t table_stride, int32_t max_pages, const uint8_t *ended, int32_t batch,
+                     int32_t *free_pages, int64_t num_free, const int32_t *taken, int32_t *out_taken, void *workspace,
+                     size_t workspace_bytes, tc_stream stream);
+
+/* What the x of tc_low_rank_add holds besides a tc_dtype: 8-bit codes with one fp32 scale a row. */
+typedef enum tc_x_codes { TC_X_E4M3 = 3, TC_X_E5M2 = 4, TC_X_INT8 = 5 } tc_x_codes;
+
+/* Low-rank adapters beside a projection: out[t] = y[t] + gain[i] * b[i] (a[i] x[t]) with i = index[t], and out[t] = y[t] where i
+ * is not in [0, adapters). y [tokens][n] and x [tokens][k] have row strides in elements, out [tokens][n] has none; a
+ * [adapters][rank][k] and b [adapters][n][rank] of w_dtype; gain fp32 [adapters] or NULL (1). x_kind: a tc_dtype, or a
+ * tc_x_codes; x_scale: NULL, or fp32 [tokens], a factor of each row (codes need it). Products and sums are fp32, out is rounded once. rank at most 1024. No output may
+ * alias an input. */
+int tc_low_rank_add(const void *y, int32_t y_dtype, int64_t y_stride, const void *x, int32_t x_kind, int64_t x_stride,
+                    const float *x_scale, int64_t tokens, int64_t k, int64_t n, const void *a, const void *b, int32_t w_dtype,
+                    int32_t adapters, int32_t rank, const float *gain, const int32_t *index, void *out, int32_t out_dtype,
+                    tc_stream stream);
+
+/* The activation of tc_gated_quantize. */
+typedef enum tc_activation { TC_SILU = 0, TC_GELU = 1, TC_GELU_TANH = 2, TC_RELU = 3 } tc_activation;
+
+/* y = activation(gate) * up in fp32, codes and scales as tc_quantize gives them for y. gate and up: [rows][K] of dtype with
+ * row strides in elements (two halves of one projection's rows, say); codes, scale and spec as tc_rms_norm_quantize's. */
+int tc_gated_quantize(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, int32_t dtype, int64_t rows,
+                      int64_t K, int32_t activation, const tc_quant_spec *spec, void *codes, void *scale, tc_stream stream);
+
+/* Tokens drawn from logits [rows][vocab] of dtype (row stride in elements) by given random numbers uniform [rows] in [0, 1):
+ * w_i = exp((l_i - max l) / temperature), weights below 2**-126 counting as 0; of those the top_k largest (ties to the lower
+ * index; <= 0: all); of those, in descending order, the fewest whose weights reach top_p of their sum (>= 1: all); of those
+ * the ones with w_i >= min_p (<= 0: all; the largest always stays). tokens[r] is the first index at which the sum of the kept weights, in
+ * index order, exceeds uniform[r] times their total; logprobs (or NULL) log(w / total). temperature <= 0: the first largest
+ * logit, log-probability 0. A row without a logit above -Inf gives -1 and -Inf, one with a NaN -1 and NaN. Settings: one
+ * a row where the array is given, else the value beside it; NaN settings bound nothing, a NaN temperature is 0. */
+int tc_sample_tokens(const void *logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t stride, const float *uniform,
+                     const float *temperature, float all_temperature, const int32_t *top_k, int32_t all_top_k,
+                     const float *top_p, float all_top_p, const float *min_p, float all_min_p, int64_t *tokens, float *logprobs,
+                     tc_stream stream);
+
 /* Library version string. */
 const char *tc_version(void);
 

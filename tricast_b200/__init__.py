@@ -18,13 +18,17 @@ package does not load it until the first call.
 """
 
 from . import formats, rounding, spec  # noqa: F401
+from .adapters import low_rank_add  # noqa: F401
 from .attention import paged_attention  # noqa: F401
 from .formats import get_format  # noqa: F401
+from .gated import gated_quantize  # noqa: F401
 from .kvcache import PagedKVCache  # noqa: F401
 from .mma import gemm, gemm_triton  # noqa: F401
 from .norm import rms_norm_quantize  # noqa: F401
 from .operand import Operand, QTensor, as_operand  # noqa: F401
+from .paging import PagePlan, plan_pages, release_pages  # noqa: F401
 from .quantize import QuantizePlan, quantize, quantize_into, quantize_triton, round_to_format_triton  # noqa: F401
+from .sampling import sample_tokens  # noqa: F401
 from .spec import PRESETS, SCHEMES, MMASpec, QuantSpec, ScaleSpec, get_preset, get_scheme  # noqa: F401
 
 __version__ = "0.1.0"

@@ -1,0 +1,255 @@
+// Page plans of a batch: which pages its new tokens take, the slot, sequence and position of every one, and the
+// pages of ended sequences back on the stack of free ones.
+//   used_i = ceil(len_i / P), n_i = the new tokens that fit, need_i = min(ceil((len_i + n_i) / P), max_pages) - used_i
+//   page (i, used_i + j) = free[taken + need_0 + .. + need_(i-1) + j],   slot = page * P + position % P
+#include <string>
+
+#include "tc_common.cuh"
+
+namespace tc {
+namespace plan {
+
+constexpr int kThreads = 1024;
+
+struct Args {
+  const int32_t *lens, *fresh;  // tokens that a sequence has, and new ones
+  int32_t *table;
+  int64_t table_stride;
+  const int32_t *free_pages;
+  int64_t num_free;
+  const int32_t *taken;
+  int64_t tokens;
+  int32_t batch, width, shift;  // rows and columns of the table, logarithm of the page size
+  int32_t *out_lens, *cu, *sequence, *positions, *out_taken, *missing;
+  int64_t *slots;
+  int64_t *first;  // workspace: of each sequence, where its first new page stands in free_pages
+};
+
+// Exclusive prefix sum of a value a thread over the block; total in every thread.
+__device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t *part, int64_t &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int64_t s = v;
+#pragma unroll
+  for (int m = 1; m < 32; m <<= 1) {
+    const int64_t o = __shfl_up_sync(0xFFFFFFFFu, s, m);
+    if (lane >= m) s += o;
+  }
+  if (lane == 31) part[warp] = s;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w < warp) before += part[w];
+    total += part[w];
+  }
+  __syncthreads();
+  return before + s - v;
+}
+
+__device__ __forceinline__ int64_t taken_at_start(const Args &a) {
+  const int64_t t = *a.taken;
+  return t < 0 ? 0 : t < a.num_free ? t : a.num_free;
+}
+
+// A sequence's pages before its new tokens, and the new ones: its table's room bounds both.
+__device__ __forceinline__ int64_t used_pages(const Args &a, int64_t len) { return (len + (1ll << a.shift) - 1) >> a.shift; }
+__device__ __forceinline__ int64_t new_pages(const Args &a, int64_t len, int64_t n) {
+  const int64_t used = used_pages(a, len);
+  return min(used_pages(a, len + n) - used, max(a.width - used, (int64_t)0));
+}
+
+__global__ void __launch_bounds__(kThreads) scan_kernel(Args a) {
+  __shared__ int64_t part[kThreads / 32];
+  int64_t tokens = 0, pages = taken_at_start(a), beyond = 0;
+  for (int64_t at = 0; at < a.batch; at += kThreads) {
+    const int64_t i = at + threadIdx.x;
+    const bool real = i < a.batch;
+    const int64_t len = real ? max(a.lens[i], 0) : 0, want = real ? max(a.fresh[i], 0) : 0;
+    int64_t total;
+    const int64_t start = min(tokens + block_prefix(want, part, total), a.tokens);
+    tokens += total;
+    const int64_t n = min(want, a.tokens - start);
+    const int64_t need = real ? new_pages(a, len, n) : 0;
+    const int64_t first = pages + block_prefix(need, part, total);
+    pages += total;
+    if (real) {
+      beyond += used_pages(a, len + n) - used_pages(a, len) - need;
+      a.cu[i] = (int32_t)start;
+      a.out_lens[i] = (int32_t)(len + n);
+      a.first[i] = first;
+      if (i == a.batch - 1) a.cu[a.batch] = (int32_t)(start + n);
+    }
+  }
+  int64_t none;
+  block_prefix(beyond, part, none);
+  if (threadIdx.x == 0) {
+    const int64_t out = min(pages, a.num_free);
+    *a.out_taken = (int32_t)out;
+    *a.missing = (int32_t)min(pages - out + none, (int64_t)INT32_MAX);
+    if (a.batch == 0) a.cu[0] = 0;
+  }
+}
+
+// Tokens by threads, new table entries by warps.
+__global__ void __launch_bounds__(256) fill_kernel(Args a) {
+  const int64_t thread = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, threads = (int64_t)gridDim.x * blockDim.x;
+  const int64_t real = a.batch ? a.cu[a.batch] : 0;
+  for (int64_t t = thread; t < a.tokens; t += threads) {
+    int64_t slot = -1;
+    int32_t seq = -1, pos = -1;
+    if (t < real) {
+      int lo = 0, hi = a.batch - 1;  // the last sequence that starts at t or before and is not empty: the first whose end is behind t
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid + 1] > t) hi = mid;
+        else lo = mid + 1;
+      }
+      const int64_t len = max(a.lens[lo], 0), p = len + t - a.cu[lo], column = p >> a.shift, used = used_pages(a, len);
+      const int64_t at = a.first[lo] + column - used;
+      int32_t page = -1;
+      if (column < used && column < a.width) page = a.table[lo * a.table_stride + column];
+      else if (column < a.width && at < a.num_free) page = a.free_pages[at];
+      if (page >= 0) slot = ((int64_t)page << a.shift) + (p & ((1ll << a.shift) - 1));
+      seq = lo;
+      pos = (int32_t)p;
+    }
+    a.slots[t] = slot;
+    a.sequence[t] = seq;
+    a.positions[t] = pos;
+  }
+  for (int64_t i = thread >> 5; i < a.batch; i += threads >> 5) {
+    const int64_t len = max(a.lens[i], 0), n = a.cu[i + 1] - a.cu[i], used = used_pages(a, len), need = new_pages(a, len, n);
+    for (int64_t j = threadIdx.x & 31; j < need; j += 32) {
+      const int64_t at = a.first[i] + j;
+      a.table[i * a.table_stride + used + j] = at < a.num_free ? a.free_pages[at] : -1;
+    }
+  }
+}
+
+struct Release {
+  int32_t *table;
+  int64_t table_stride;
+  const unsigned char *ended;
+  int32_t batch, width;
+  int32_t *free_pages;
+  int64_t num_free;
+  const int32_t *taken;
+  int32_t *out_taken;
+  int32_t *counts;  // workspace: pages of each ended sequence
+};
+
+__device__ __forceinline__ int warp_sum(int v) { return __reduce_add_sync(0xFFFFFFFFu, v); }
+
+__global__ void __launch_bounds__(256) count_kernel(Release a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warps = (int64_t)gridDim.x * 8;
+  for (int64_t i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); i < a.batch; i += warps) {
+    int n = 0;
+    if (a.ended[i])
+      for (int64_t c = lane; c < a.width; c += 32) n += a.table[i * a.table_stride + c] >= 0;
+    n = warp_sum(n);
+    if (lane == 0) a.counts[i] = n;
+  }
+}
+
+// A warp a sequence; every block adds the counts before its eight sequences, and all of them.
+__global__ void __launch_bounds__(256) push_kernel(Release a) {
+  __shared__ int64_t part[2][8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row0 = (int64_t)blockIdx.x * 8;
+  int64_t before = 0, all = 0;
+  for (int64_t i = threadIdx.x; i < a.batch; i += 256) {
+    const int64_t n = a.counts[i];
+    all += n;
+    if (i < row0) before += n;
+  }
+#pragma unroll
+  for (int m = 16; m; m >>= 1) before += __shfl_xor_sync(0xFFFFFFFFu, before, m), all += __shfl_xor_sync(0xFFFFFFFFu, all, m);
+  if (lane == 0) part[0][warp] = before, part[1][warp] = all;
+  __syncthreads();
+  before = all = 0;
+  for (int w = 0; w < 8; ++w) before += part[0][w], all += part[1][w];
+  int64_t base = *a.taken;
+  base = (base < a.num_free ? base : a.num_free) - all;  // below 0 where pages come back that were not taken: those are dropped
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.out_taken = (int32_t)(base < 0 ? 0 : base);
+  const int64_t i = row0 + warp;
+  if (i >= a.batch || !a.ended[i]) return;
+  for (int64_t r = row0; r < i; ++r) before += a.counts[r];
+  int64_t at = base + before;
+  for (int64_t c0 = 0; c0 < a.width; c0 += 32) {
+    const int64_t c = c0 + lane;
+    const int32_t page = c < a.width ? a.table[i * a.table_stride + c] : -1;
+    const unsigned held = __ballot_sync(0xFFFFFFFFu, page >= 0);
+    const int64_t to = at + __popc(held & ((1u << lane) - 1u));
+    if (page >= 0 && to >= 0) a.free_pages[to] = page;
+    if (c < a.width) a.table[i * a.table_stride + c] = -1;
+    at += __popc(held);
+  }
+}
+
+}  // namespace plan
+}  // namespace tc
+
+using namespace tc;
+
+static int plan_status(const char *what) {
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_error(std::string(what) + ": " + cudaGetErrorString(e)), TC_CUDA_ERROR;
+  count_launch();
+  return TC_OK;
+}
+
+extern "C" size_t tc_plan_pages_workspace(int32_t batch) { return batch > 0 ? (size_t)batch * sizeof(int64_t) : 0; }
+
+extern "C" int tc_plan_pages(const int32_t *seq_lens, const int32_t *new_lens, int32_t batch, int32_t *block_table,
+                             int64_t table_stride, int32_t max_pages, const int32_t *free_pages, int64_t num_free,
+                             const int32_t *taken, int32_t page_size, int64_t tokens, int32_t *out_lens, int32_t *cu_q,
+                             int64_t *slots, int32_t *sequence, int32_t *positions, int32_t *out_taken, int32_t *missing,
+                             void *workspace, size_t workspace_bytes, tc_stream stream) {
+  auto bad = [](const char *m) { return set_error(std::string("tc_plan_pages: ") + m), (int)TC_INVALID_ARGUMENT; };
+  if (batch < 0 || max_pages < 0 || tokens < 0 || num_free < 0) return bad("negative size");
+  if (tokens > 0x7FFFFFFFll || num_free > 0x7FFFFFFFll) return bad("more than 2**31 - 1 tokens or pages");
+  if (page_size < 1 || page_size > (1 << 20) || (page_size & (page_size - 1))) return bad("page_size must be a power of two");
+  if (max_pages > (1 << 30) / page_size) return bad("contexts hold at most 2**30 tokens");
+  if (batch > 1 && table_stride < max_pages) return bad("table_stride must be at least max_pages");
+  if ((batch && (!seq_lens || !new_lens || !out_lens)) || (batch && max_pages && !block_table) || (num_free && !free_pages) ||
+      !taken || !cu_q || !out_taken || !missing || (tokens && (!slots || !sequence || !positions)))
+    return bad("null pointer");
+  if (batch && (!workspace || workspace_bytes < tc_plan_pages_workspace(batch)))
+    return set_error("tc_plan_pages: workspace too small"), TC_WORKSPACE_TOO_SMALL;
+  plan::Args a{seq_lens, new_lens, block_table, table_stride, free_pages, num_free, taken, tokens, batch, max_pages, 0,
+               out_lens, cu_q, sequence, positions, out_taken, missing, slots, static_cast<int64_t *>(workspace)};
+  while ((1 << a.shift) < page_size) ++a.shift;
+  cudaStream_t s = (cudaStream_t)stream;
+  plan::scan_kernel<<<1, plan::kThreads, 0, s>>>(a);
+  if (const int st = plan_status("tc_plan_pages")) return st;
+  const int64_t work = tokens > (int64_t)batch * 32 ? tokens : (int64_t)batch * 32;
+  if (work == 0) return TC_OK;
+  const int64_t blocks = (work + 255) / 256, most = (int64_t)sm_count() * 8;
+  plan::fill_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(a);
+  return plan_status("tc_plan_pages");
+}
+
+extern "C" size_t tc_release_pages_workspace(int32_t batch) { return batch > 0 ? (size_t)batch * sizeof(int32_t) : 0; }
+
+extern "C" int tc_release_pages(int32_t *block_table, int64_t table_stride, int32_t max_pages, const uint8_t *ended, int32_t batch,
+                                int32_t *free_pages, int64_t num_free, const int32_t *taken, int32_t *out_taken, void *workspace,
+                                size_t workspace_bytes, tc_stream stream) {
+  auto bad = [](const char *m) { return set_error(std::string("tc_release_pages: ") + m), (int)TC_INVALID_ARGUMENT; };
+  if (batch < 0 || max_pages < 0 || num_free < 0 || num_free > 0x7FFFFFFFll) return bad("sizes out of range");
+  if (batch > 1 && table_stride < max_pages) return bad("table_stride must be at least max_pages");
+  if ((batch && !ended) || (batch && max_pages && !block_table) || (num_free && !free_pages) || !taken || !out_taken)
+    return bad("null pointer");
+  if (batch && (!workspace || workspace_bytes < tc_release_pages_workspace(batch)))
+    return set_error("tc_release_pages: workspace too small"), TC_WORKSPACE_TOO_SMALL;
+  plan::Release a{block_table, table_stride, ended, batch, max_pages, free_pages, num_free, taken, out_taken,
+                  static_cast<int32_t *>(workspace)};
+  cudaStream_t s = (cudaStream_t)stream;
+  const int64_t blocks = ((int64_t)batch + 7) / 8, most = (int64_t)sm_count() * 8;
+  if (blocks) {
+    plan::count_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(a);
+    if (const int st = plan_status("tc_release_pages")) return st;
+  }
+  plan::push_kernel<<<(unsigned)(blocks ? blocks : 1), 256, 0, s>>>(a);
+  return plan_status("tc_release_pages");
+}
