@@ -19,14 +19,146 @@ struct Args : Cast8 {
 
 constexpr int kThreads = 256;
 
-__device__ __forceinline__ float activate(float g, int act) {
-  if (act == ACT_SILU) return __fdiv_rn(g, __fadd_rn(1.0f, expf(-g)));
-  if (act == ACT_GELU) return __fmul_rn(__fmul_rn(0.5f, g), erfcf(__fmul_rn(g, -0.70710678f)));
-  if (act == ACT_GELU_TANH) {
-    const float z = __fmul_rn(0.79788456f, __fmaf_rn(__fmul_rn(__fmul_rn(0.044715f, g), g), g, g));
-    return __fdiv_rn(g, __fadd_rn(1.0f, expf(__fmul_rn(-2.0f, z))));
+// g / (1 + 2**t), t = -log2(e) times the logistic function's argument. The hardware's exponential and reciprocal are good to 2
+// and 1 steps of fp32; t's rounding is |t| half steps of the exponential, at most half a step of g in the result, since
+// |t| / (1 + 2**t) stays below 1 where 2**t is large.
+__device__ __forceinline__ float logistic(float g, float t) {
+  float r;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, exp2_wide(t))));
+  return __fmul_rn(g, r);
+}
+
+// act(g) * u of eight elements.
+__device__ __forceinline__ void gate8(float (&g)[8], const float (&u)[8], int act) {
+  constexpr float kLog2E = 1.44269504f;
+  if (act == ACT_SILU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = logistic(g[e], __fmul_rn(g[e], -kLog2E));
+  } else if (act == ACT_GELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = __fmul_rn(__fmul_rn(0.5f, g[e]), erfcf(__fmul_rn(g[e], -0.70710678f)));
+  } else if (act == ACT_GELU_TANH) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float z = __fmul_rn(0.79788456f, __fmaf_rn(__fmul_rn(__fmul_rn(0.044715f, g[e]), g[e]), g[e], g[e]));
+      g[e] = logistic(g[e], __fmul_rn(z, -2.0f * kLog2E));
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = g[e] > 0.0f ? g[e] : g[e] != g[e] ? g[e] : 0.0f;
   }
-  return g > 0.0f ? g : g != g ? g : 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) g[e] = __fmul_rn(g[e], u[e]);
+}
+
+// Eight codes; values beyond the format's largest need encode8's clamp: only a power-of-two scale leaves them.
+template <int E, bool POW2>
+__device__ __forceinline__ uint2 encode_all(const float (&y)[8], const Scale &sc) {
+  uint32_t q[4];
+  if (sc.fast && !(POW2 && E == E8_INT8)) {
+    auto quotient = [&](float v) { return POW2 ? __fmul_rn(v, sc.r) : divide_fast(v, sc.s, sc.r); };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[k] = encode8x2<E>(quotient(y[2 * k]), quotient(y[2 * k + 1]));
+  } else {
+    auto slow = [&](float v) { return encode8<E>(POW2 ? __fmul_rn(v, sc.r) : __fdiv_rn(v, sc.s)); };
+#pragma unroll
+    for (int k = 0; k < 4; ++k) q[k] = slow(y[2 * k]) | (slow(y[2 * k + 1]) << 8);
+  }
+  return make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
+}
+
+__device__ __forceinline__ float largest8(const float (&y)[8]) {
+  float m = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max_abs(m, y[e]);
+  return m;
+}
+
+// Eight neighbouring elements from c on, zeros behind the row.
+template <typename T, bool VEC>
+__device__ __forceinline__ void fetch8(const T *p, int64_t c, int64_t K, float (&v)[8]) {
+  if (VEC) {
+    if (c < K) load8(p + c, v);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < K) v[e] = Io<T>::get(p[c + e]);
+  }
+}
+template <bool VEC>
+__device__ __forceinline__ void put8(unsigned char *p, int64_t c, int64_t K, uint2 q) {
+  if (VEC) {
+    if (c < K) *reinterpret_cast<uint2 *>(p + c) = q;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < K) p[c + e] = (unsigned char)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+  }
+}
+
+// Groups of 16 to 256 elements, a power of two: 2 to 32 lanes of 8 elements each, and nothing is shared beyond them. Threads walk over
+// the matrix with every row filled up to whole groups (`width` vectors), so a group's lanes are neighbours in a warp.
+template <typename T, int E, bool VEC, bool POW2>
+__global__ void __launch_bounds__(kThreads) group_kernel(Args a, int64_t width) {
+  const int64_t step = (int64_t)gridDim.x * kThreads, start = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  const int64_t rows_a_step = step / width, rest = step - rows_a_step * width;
+  int64_t r = start / width, v = start - r * width;
+  // A warp's lanes go on together: some may be behind the last row.
+  for (int64_t base = start - (threadIdx.x & 31); base < a.rows * width; base += step) {
+    const bool real = r < a.rows;
+    const int64_t c = v * 8;
+    float y[8], u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) y[e] = u[e] = 0.0f;
+    if (real) {
+      fetch8<T, VEC>(static_cast<const T *>(a.gate) + r * a.gate_stride, c, a.K, y);
+      fetch8<T, VEC>(static_cast<const T *>(a.up) + r * a.up_stride, c, a.K, u);
+    }
+    gate8(y, u, a.act);
+    uint32_t top = abs_bits(largest8(y));
+    for (int k = a.group >> 4; k; k >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
+    const Scale sc = make_scale<POW2>(top, a);
+    if (real && c < a.K) {
+      if ((c & (a.group - 1)) == 0) store_scale<POW2>(a, r * a.groups + (c >> a.group_shift), sc);
+      put8<VEC>(a.codes + r * a.K, c, a.K, encode_all<E, POW2>(y, sc));
+    }
+    r += rows_a_step;
+    v += rest;
+    if (v >= width) v -= width, ++r;
+  }
+}
+
+// One scale a row, which a block's registers hold: NV vectors of 8 neighbouring elements a thread.
+template <typename T, int E, int NV, bool VEC, bool POW2>
+__global__ void __launch_bounds__(1024) held_kernel(Args a) {
+  __shared__ uint32_t tops[2][32];
+  const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5, threads = blockDim.x;
+  int flip = 0;  // the two halves of the exchange buffer alternate, so one barrier a row suffices
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, flip ^= 1) {
+    const T *gate = static_cast<const T *>(a.gate) + r * a.gate_stride, *up = static_cast<const T *>(a.up) + r * a.up_stride;
+    float y[NV][8], u[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) y[i][e] = u[i][e] = 0.0f;
+      const int64_t c = (int64_t)(tid + i * threads) * 8;
+      fetch8<T, VEC>(gate, c, a.K, y[i]);
+      fetch8<T, VEC>(up, c, a.K, u[i]);
+    }
+    float m = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      gate8(y[i], u[i], a.act);
+      m = max_abs(m, largest8(y[i]));
+    }
+    const uint32_t top = warp_max(abs_bits(m));
+    if (lane == 0) tops[flip][tid >> 5] = top;
+    __syncthreads();
+    const Scale sc = make_scale<POW2>(warp_max(lane < warps ? tops[flip][lane] : 0u), a);
+    if (tid == 0) store_scale<POW2>(a, r, sc);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) put8<VEC>(a.codes + r * a.K, (int64_t)(tid + i * threads) * 8, a.K, encode_all<E, POW2>(y[i], sc));
+  }
 }
 
 // One block a row, any length, alignment and group: the row is read once per group for its maximum and again for its
@@ -37,42 +169,76 @@ __global__ void __launch_bounds__(kThreads) row_kernel(Args a) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const T *gate = static_cast<const T *>(a.gate) + r * a.gate_stride, *up = static_cast<const T *>(a.up) + r * a.up_stride;
-    auto y_at = [&](int64_t c) { return __fmul_rn(activate(Io<T>::get(gate[c]), a.act), Io<T>::get(up[c])); };
     const bool shared_group = a.groups == 1;
     if (threadIdx.x == 0) top = 0u;
     __syncthreads();
-    const int64_t step = shared_group ? kThreads : 32;
+    const int64_t step = shared_group ? 8 * kThreads : 256;
     for (int64_t g = shared_group ? 0 : warp; g < a.groups; g += shared_group ? 1 : kThreads / 32) {
       const int64_t lo = g * a.group, hi = min(lo + (int64_t)a.group, a.K);
-      const int64_t first = lo + (shared_group ? threadIdx.x : lane);
+      const int64_t first = lo + 8 * (shared_group ? threadIdx.x : lane);
+      auto y_at = [&](int64_t c, float (&y)[8]) {
+        float u[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = u[e] = 0.0f;
+        fetch8<T, false>(gate, c, hi, y);
+        fetch8<T, false>(up, c, hi, u);
+        gate8(y, u, a.act);
+      };
+      float y[8];
       uint32_t m = 0u;
-      for (int64_t c = first; c < hi; c += step) m = max(m, abs_bits(y_at(c)));
+      for (int64_t c = first; c < hi; c += step) {
+        y_at(c, y);
+        m = max(m, abs_bits(largest8(y)));
+      }
       m = warp_max(m);
       if (shared_group) {
         if (lane == 0) atomicMax(&top, m);
         __syncthreads();
         m = top;
       }
-      const uint32_t sc = a.e8m0 ? pow2_code(m, a.emax) : 0u;
-      const float s = a.e8m0 ? pow2_inverse(sc) : absmax_scale(m, a.max_elem);
-      if (first == lo) {
-        if (a.e8m0) static_cast<unsigned char *>(a.scale)[r * a.groups + g] = (unsigned char)sc;
-        else static_cast<float *>(a.scale)[r * a.groups + g] = s;
-      }
+      const Scale p = make_scale<true>(m, a), s = make_scale<false>(m, a);
+      if (first == lo) a.e8m0 ? store_scale<true>(a, r * a.groups + g, p) : store_scale<false>(a, r * a.groups + g, s);
       for (int64_t c = first; c < hi; c += step) {
-        const float y = y_at(c);
-        a.codes[r * a.K + c] = (unsigned char)encode8<E>(a.e8m0 ? __fmul_rn(y, s) : __fdiv_rn(y, s));
+        y_at(c, y);
+        put8<false>(a.codes + r * a.K, c, hi, a.e8m0 ? encode_all<E, true>(y, p) : encode_all<E, false>(y, s));
       }
     }
     __syncthreads();
   }
 }
 
+template <typename T, int E, bool VEC, bool POW2>
+static void launch_scale(const Args &a, bool lanes, cudaStream_t s) {
+  if (lanes) {
+    const int64_t width = a.groups * (a.group / 8), blocks = (a.rows * width + kThreads - 1) / kThreads, most = (int64_t)sm_count() * 8;
+    group_kernel<T, E, VEC, POW2><<<(unsigned)(blocks < most ? blocks : most), kThreads, 0, s>>>(a, width);
+  } else {
+    const int64_t vectors = (a.K + 7) / 8;
+    int threads = 64;
+    while (threads < 512 && threads < vectors) threads *= 2;
+    while (threads < 1024 && threads * 2 < vectors) threads *= 2;
+    const int64_t most = (int64_t)sm_count() * (2048 / threads);
+    const unsigned grid = (unsigned)(a.rows < most ? a.rows : most);
+    if (vectors <= threads) held_kernel<T, E, 1, VEC, POW2><<<grid, threads, 0, s>>>(a);
+    else held_kernel<T, E, 2, VEC, POW2><<<grid, threads, 0, s>>>(a);
+  }
+  count_launch();
+}
+
 template <typename T, int E>
 static void launch_elem(const Args &a, cudaStream_t s) {
-  const int64_t most = (int64_t)sm_count() * 8;
-  row_kernel<T, E><<<(unsigned)(a.rows < most ? a.rows : most), kThreads, 0, s>>>(a);
-  count_launch();
+  auto aligned = [](const void *p, size_t n) { return (uintptr_t)p % n == 0; };
+  const bool vec = a.K % 8 == 0 && a.gate_stride % 8 == 0 && a.up_stride % 8 == 0 && aligned(a.gate, 16) && aligned(a.up, 16) &&
+                   aligned(a.codes, 8);
+  const bool lanes = a.groups > 1 && a.group >= 16 && a.group <= 256 && (a.group & (a.group - 1)) == 0;
+  if (lanes || (a.groups == 1 && a.K <= 16384)) {
+    if (vec) a.e8m0 ? launch_scale<T, E, true, true>(a, lanes, s) : launch_scale<T, E, true, false>(a, lanes, s);
+    else a.e8m0 ? launch_scale<T, E, false, true>(a, lanes, s) : launch_scale<T, E, false, false>(a, lanes, s);
+  } else {
+    const int64_t most = (int64_t)sm_count() * 8;
+    row_kernel<T, E><<<(unsigned)(a.rows < most ? a.rows : most), kThreads, 0, s>>>(a);
+    count_launch();
+  }
 }
 
 template <typename T>

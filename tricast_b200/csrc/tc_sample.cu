@@ -6,20 +6,37 @@
 namespace tc {
 namespace sample {
 
-template <typename T>
-static cudaError_t launch(const Args &a, cudaStream_t s) {
-  const int blocks = a.vocab >= 16384 ? 8 : 1;
+constexpr int64_t kMaxVocab = 1 << 23;  // histograms add 12-bit parts of 2**20 weights a block in 32 bits
+constexpr int64_t kMaxHeld = 54272;     // weights that a block's shared memory holds beside the rest
+
+template <typename T, bool HELD>
+static cudaError_t launch_as(const Args &a, cudaStream_t s) {
+  const size_t bytes = HELD ? (size_t)a.part * sizeof(float) : 0;
+  cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(a.rows * blocks));
+  cfg.gridDim = dim3((unsigned)(a.rows * a.blocks));
   cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = bytes;
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = blocks;
+  attr[0].val.clusterDim.x = a.blocks;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, sample_kernel<T>, a);
+  return cudaLaunchKernelEx(&cfg, sample_kernel<T, HELD>, a);
+}
+
+template <typename T>
+static cudaError_t launch(Args a, cudaStream_t s) {
+  // Stretches short enough for two blocks an SM, and more of them while the card is not full and they stay long enough to be worth it.
+  a.blocks = 1;
+  while (a.blocks < 8 && (a.vocab > 24576 * (int64_t)a.blocks ||
+                          (a.rows * a.blocks < 2 * sm_count() && a.vocab > 4096 * (int64_t)a.blocks)))
+    a.blocks *= 2;
+  a.part = ((a.vocab + 8 + a.blocks - 1) / a.blocks + 7) / 8 * 8;  // positions begin up to 7 elements before the row
+  return a.part <= kMaxHeld ? launch_as<T, true>(a, s) : launch_as<T, false>(a, s);
 }
 
 }  // namespace sample
@@ -32,12 +49,13 @@ extern "C" int tc_sample_tokens(const void *logits, int32_t dtype, int64_t rows,
   using namespace tc;
   if (rows == 0) return TC_OK;
   auto bad = [](const char *m) { return set_error(std::string("tc_sample_tokens: ") + m), (int)TC_INVALID_ARGUMENT; };
-  if (rows < 0 || rows > (1 << 27) || vocab < 1 || vocab > 0x7FFFFFFFll) return bad("rows and vocab out of range");
+  if (rows < 0 || rows > (1 << 27) || vocab < 1 || vocab > sample::kMaxVocab)
+    return bad("rows and vocab out of range (at most 2**27 and 2**23)");
   if (dtype < 0 || dtype > 2) return bad("unsupported dtype");
   if (!logits || !uniform || !tokens) return bad("null pointer");
   if (rows > 1 && stride < vocab) return bad("the row stride must be at least vocab");
   sample::Args a{logits, rows, vocab, stride, uniform, temperature, top_p, min_p, top_k, all_temperature, all_top_p, all_min_p,
-                 all_top_k, tokens, logprobs};
+                 all_top_k, tokens, logprobs, 1, vocab};
   cudaStream_t s = (cudaStream_t)stream;
   const cudaError_t e = dtype == TC_F32    ? sample::launch<float>(a, s)
                         : dtype == TC_BF16 ? sample::launch<__nv_bfloat16>(a, s)

@@ -25,7 +25,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     if not logits.is_cuda:
         raise ValueError("the B200 backend requires a CUDA tensor")
     if logits.ndim != 2 or logits.shape[1] == 0:
-        raise ValueError("logits must be [rows, vocab] with a vocabulary that is not empty")
+        raise ValueError("logits must be [rows, vocab] with a vocabulary that is not empty (at most 2**23)")
     rows, vocab = logits.shape
     device = logits.device
     dtype = N.dtype_code(logits.dtype)
