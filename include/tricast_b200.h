@@ -354,6 +354,9 @@ int tc_release_pages(int32_t *block_table, int64_t table_stride, int32_t max_pag
 /* What the x of tc_low_rank_add holds besides a tc_dtype: 8-bit codes with one fp32 scale a row. */
 typedef enum tc_x_codes { TC_X_E4M3 = 3, TC_X_E5M2 = 4, TC_X_INT8 = 5 } tc_x_codes;
 
+/* Bytes of scratch tc_low_rank_add needs for these sizes (0 when none). */
+size_t tc_low_rank_add_workspace(int64_t tokens, int32_t x_kind, int32_t w_dtype, int32_t rank, int32_t y_dtype, int32_t out_dtype);
+
 /* Low-rank adapters beside a projection: out[t] = y[t] + gain[i] * b[i] (a[i] x[t]) with i = index[t], and out[t] = y[t] where i
  * is not in [0, adapters). y [tokens][n] and x [tokens][k] have row strides in elements, out [tokens][n] has none; a
  * [adapters][rank][k] and b [adapters][n][rank] of w_dtype; gain fp32 [adapters] or NULL (1). x_kind: a tc_dtype, or a
@@ -362,7 +365,7 @@ typedef enum tc_x_codes { TC_X_E4M3 = 3, TC_X_E5M2 = 4, TC_X_INT8 = 5 } tc_x_cod
 int tc_low_rank_add(const void *y, int32_t y_dtype, int64_t y_stride, const void *x, int32_t x_kind, int64_t x_stride,
                     const float *x_scale, int64_t tokens, int64_t k, int64_t n, const void *a, const void *b, int32_t w_dtype,
                     int32_t adapters, int32_t rank, const float *gain, const int32_t *index, void *out, int32_t out_dtype,
-                    tc_stream stream);
+                    void *workspace, size_t workspace_bytes, tc_stream stream);
 
 /* The activation of tc_gated_quantize. */
 typedef enum tc_activation { TC_SILU = 0, TC_GELU = 1, TC_GELU_TANH = 2, TC_RELU = 3 } tc_activation;

@@ -78,6 +78,17 @@ def test_orders_of_tokens(order, tokens):
         assert torch.equal(low_rank_add(y, x, a, b, index), y)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rank", [8, 16, 24, 40, 64, 96, 128])
+def test_ranks_of_many_tokens(rank, dtype):
+    """Stretches without an adapter, with one, and with several, beside one another."""
+    y, x, a, b, index, gain = inputs(700, 264, 200, rank, 5, dtype, torch.float32, seed=rank)
+    t = torch.arange(700, device="cuda")
+    index = torch.where(t < 150, -1, torch.where(t < 350, 2, torch.where(t < 500, t % 7 - 1, index))).to(torch.int32)
+    for out in (torch.float32, dtype):
+        close(low_rank_add(y, x, a, b, index, gain=gain, dtype=out), y, x, a, b, index, gain)
+
+
 @pytest.mark.parametrize("scheme", ["fp8_row", "int8_row", "fp8_e5m2"])
 @pytest.mark.parametrize("tokens, k, n, rank", [(1, 512, 264, 16), (20, 1024, 512, 8), (300, 328, 640, 32), (13, 45, 19, 5)])
 def test_operands_of_the_projection(scheme, tokens, k, n, rank):

@@ -53,7 +53,7 @@ def test_adapter_arguments_are_checked():
 
     def call(y=P, yd=0, ys=64, x=P, xk=1, xs=32, scale=None, tokens=2, k=32, n=64, a=P, b=P, wd=1, adapters=3, rank=8, gain=None,
              index=P, out=P, od=1):
-        return lib.tc_low_rank_add(y, yd, ys, x, xk, xs, scale, tokens, k, n, a, b, wd, adapters, rank, gain, index, out, od, None)
+        return lib.tc_low_rank_add(y, yd, ys, x, xk, xs, scale, tokens, k, n, a, b, wd, adapters, rank, gain, index, out, od, None, 0, None)
 
     for kw in (dict(y=None), dict(x=None), dict(a=None), dict(b=None), dict(index=None), dict(out=None), dict(yd=3), dict(xk=6),
                dict(xk=-1), dict(wd=3), dict(od=-1), dict(ys=63), dict(xs=31), dict(xk=3), dict(tokens=-1), dict(k=-1),

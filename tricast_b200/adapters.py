@@ -61,11 +61,15 @@ def low_rank_add(y: torch.Tensor, x, a: torch.Tensor, b: torch.Tensor, index: to
         gain = gain.contiguous()
     out = torch.empty((tokens, n), dtype=dtype, device=device)
     at = device.index
+    lib, rank = N.lib(), a.shape[1]
     with N.on_device(at):
-        status = N.lib().tc_low_rank_add(
+        nbytes = lib.tc_low_rank_add_workspace(tokens, kind, w_code, rank, y_code, out_code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+        status = lib.tc_low_rank_add(
             y.data_ptr(), y_code, max(y.stride(0), n), x.data_ptr(), kind, max(x.stride(0), k),
-            None if scale is None else scale.data_ptr(), tokens, k, n, a.data_ptr(), b.data_ptr(), w_code, a.shape[0], a.shape[1],
-            None if gain is None else gain.data_ptr(), index.data_ptr(), out.data_ptr(), out_code, N.raw_stream(at))
+            None if scale is None else scale.data_ptr(), tokens, k, n, a.data_ptr(), b.data_ptr(), w_code, a.shape[0], rank,
+            None if gain is None else gain.data_ptr(), index.data_ptr(), out.data_ptr(), out_code,
+            None if ws is None else ws.data_ptr(), nbytes, N.raw_stream(at))
     if status:
         N.check(status, "tc_low_rank_add")
     return out

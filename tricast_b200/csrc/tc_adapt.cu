@@ -37,60 +37,30 @@ __global__ void __launch_bounds__(256) plain_kernel(Args a) {
   }
 }
 
-template <typename T, int NG, int RW, bool VEC>
-static cudaError_t launch_tiles(Args a, cudaStream_t s) {
-  const int rows = (a.rank + RW - 1) / RW * RW, row_blocks = rows / RW;
-  const size_t bytes = (size_t)kWarps / row_blocks * 8 * NG * rows * sizeof(float) + (size_t)3 * 8 * NG * (rows + 8) * sizeof(uint16_t) +
-                       (Same<T, __half>::value ? (size_t)8 * NG * rows * sizeof(float) : 0);
-  cudaError_t e = cudaFuncSetAttribute(tile_kernel<T, NG, RW, VEC>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((a.tokens + a.tile - 1) / a.tile * a.blocks));
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = a.blocks;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, tile_kernel<T, NG, RW, VEC>, a);
-}
+cudaError_t launch_bf16(const Args &a, cudaStream_t s);
+cudaError_t launch_f16(const Args &a, cudaStream_t s);
 
-template <typename T>
-static cudaError_t launch_as(Args a, cudaStream_t s) {
-  auto aligned = [](const void *p, size_t n) { return (uintptr_t)p % n == 0; };
-  const int y16 = a.y_dtype == TC_F32 ? 4 : 8;
-  const bool vec = a.k % 8 == 0 && a.n % 8 == 0 && a.rank % (a.rank <= 16 ? 4 : 8) == 0 && a.x_stride % 8 == 0 &&
-                   a.y_stride % y16 == 0 && aligned(a.x, a.x_kind <= X_F16 ? 16 : 8) && aligned(a.y, 16) && aligned(a.a, 16) &&
-                   aligned(a.b, 16) && aligned(a.out, 16);
-  // Few tokens: tiles of at most 8, as small as the card has clusters of 8 blocks for. Many: tiles of 32.
-  const int sms = sm_count();
-  const bool few = a.tokens <= 8 * (int64_t)sms / 4;
-  if (few) {
-    a.tile = 1;
-    while (a.tile < 8 && (a.tokens + a.tile - 1) / a.tile * 8 > sms) a.tile *= 2;
-  } else {
-    a.tile = 32;
-  }
-  a.blocks = 1;
-  while (a.blocks < 8 && (a.tokens + a.tile - 1) / a.tile * a.blocks * 2 <= (few ? 1 : 4) * sms) a.blocks *= 2;
-  if (few) {
-    if (a.rank <= 16) return vec ? launch_tiles<T, 1, 16, true>(a, s) : launch_tiles<T, 1, 16, false>(a, s);
-    return vec ? launch_tiles<T, 1, 32, true>(a, s) : launch_tiles<T, 1, 32, false>(a, s);
-  }
-  if (a.rank <= 16) return vec ? launch_tiles<T, 4, 16, true>(a, s) : launch_tiles<T, 4, 16, false>(a, s);
-  return vec ? launch_tiles<T, 4, 32, true>(a, s) : launch_tiles<T, 4, 32, false>(a, s);
+// y and out of 32 bits or of the weights' type.
+static bool on_tensor_cores(int x_kind, int w_dtype, int rank, int y_dtype, int out_dtype) {
+  auto fits = [&](int d) { return d == TC_F32 || d == w_dtype; };
+  return w_dtype != TC_F32 && (x_kind == w_dtype || x_kind > X_F16) && fits(y_dtype) && fits(out_dtype) && rank <= kMaxRank;
 }
 
 }  // namespace adapt
 }  // namespace tc
 
+// h in up to three parts of 16 bits, and a factor a token.
+extern "C" size_t tc_low_rank_add_workspace(int64_t tokens, int32_t x_kind, int32_t w_dtype, int32_t rank, int32_t y_dtype,
+                                            int32_t out_dtype) {
+  using namespace tc;
+  if (rank < 1 || tokens <= adapt::few_tokens() || !adapt::on_tensor_cores(x_kind, w_dtype, rank, y_dtype, out_dtype)) return 0;
+  return (size_t)tokens * ((size_t)adapt::rank_rows(rank) * 3 * sizeof(uint16_t) + sizeof(float));
+}
+
 extern "C" int tc_low_rank_add(const void *y, int32_t y_dtype, int64_t y_stride, const void *x, int32_t x_kind, int64_t x_stride,
                                const float *x_scale, int64_t tokens, int64_t k, int64_t n, const void *a, const void *b,
                                int32_t w_dtype, int32_t adapters, int32_t rank, const float *gain, const int32_t *index, void *out,
-                               int32_t out_dtype, tc_stream stream) {
+                               int32_t out_dtype, void *workspace, size_t workspace_bytes, tc_stream stream) {
   using namespace tc;
   if (tokens == 0 || n == 0) return TC_OK;
   auto bad = [](const char *m) { return set_error(std::string("tc_low_rank_add: ") + m), (int)TC_INVALID_ARGUMENT; };
@@ -103,13 +73,20 @@ extern "C" int tc_low_rank_add(const void *y, int32_t y_dtype, int64_t y_stride,
   if (!y || !index || !out || (k && !x) || (adapters && k && (!a || !b))) return bad("null pointer");
   if (x_kind > adapt::X_F16 && !x_scale) return bad("codes need scales");
   if (y_stride < n || x_stride < k) return bad("row strides must be at least the row's length");
-  adapt::Args g{y, x, a, b, x_scale, gain, index, out, tokens, k, n, y_stride, x_stride, rank, adapters, y_dtype, x_kind, w_dtype, out_dtype, 0, 0};
+  adapt::Args g{y, x, a, b, x_scale, gain, index, out, tokens, k, n, y_stride, x_stride, rank, adapters, y_dtype, x_kind, w_dtype, out_dtype, 0, 0,
+                nullptr, nullptr};
   if (k == 0) g.adapters = 0;  // nothing to add
+  if (const size_t need = tc_low_rank_add_workspace(tokens, x_kind, w_dtype, rank, y_dtype, out_dtype)) {
+    if (!workspace || workspace_bytes < need) return set_error("tc_low_rank_add: workspace too small"), TC_WORKSPACE_TOO_SMALL;
+    if ((uintptr_t)workspace % 16) return bad("workspace must be 16-byte aligned");
+    g.parts = static_cast<uint16_t *>(workspace);
+    g.factors = reinterpret_cast<float *>(g.parts + (size_t)tokens * adapt::rank_rows(rank) * 3);
+  }
   cudaStream_t s = (cudaStream_t)stream;
   cudaError_t e;
   // MMAs take operands of one 16-bit type, which holds 8-bit codes exactly; the rest goes element by element.
-  if (w_dtype != TC_F32 && (x_kind == w_dtype || x_kind > adapt::X_F16) && rank <= adapt::kMaxRank) {
-    e = w_dtype == TC_BF16 ? adapt::launch_as<__nv_bfloat16>(g, s) : adapt::launch_as<__half>(g, s);
+  if (adapt::on_tensor_cores(x_kind, w_dtype, rank, y_dtype, out_dtype)) {
+    e = w_dtype == TC_BF16 ? adapt::launch_bf16(g, s) : adapt::launch_f16(g, s);
   } else {
     const int64_t most = (int64_t)sm_count() * 8;
     adapt::plain_kernel<<<(unsigned)(tokens < most ? tokens : most), 256, 0, s>>>(g);

@@ -25,9 +25,14 @@ struct Args {
   void *out;  // [tokens][n]
   int64_t tokens, k, n, y_stride, x_stride;
   int rank, adapters, y_dtype, x_kind, w_dtype, out_dtype;
-  int tile;    // tokens of a cluster
+  int tile;    // tokens of a cluster, or of a block of the first kernel of two
   int blocks;  // of a cluster
+  // Workspace of the two kernels: h in parts of 16 bits [tokens][terms][rows], and fp16's factors [tokens].
+  uint16_t *parts;
+  float *factors;
 };
+
+__host__ __device__ __forceinline__ int rank_rows(int rank) { return rank <= 16 ? 16 : (rank + 31) / 32 * 32; }
 
 __device__ __forceinline__ float x_at(const Args &a, int64_t i) {
   if (a.x_kind <= X_F16) return load_as_float(a.x, a.x_kind, i);
@@ -94,51 +99,61 @@ __device__ __forceinline__ void load16(const uint16_t *p, int64_t at, int64_t en
   }
 }
 
-// Eight elements of x[row] from k on.
-template <typename T, bool VEC>
+// Eight elements of x[row] from k on, as they are: pairs of T, or codes in the first two words.
+template <bool CODES, bool VEC>
 __device__ __forceinline__ void load_x(const Args &a, int64_t row, int64_t k, uint32_t (&w)[4]) {
-  if (a.x_kind <= X_F16) {
+  if constexpr (!CODES) {
     load16<8, VEC>(static_cast<const uint16_t *>(a.x) + row * a.x_stride, k, a.k, w);
   } else {
-    uint2 c = make_uint2(0u, 0u);
+    w[0] = w[1] = 0u;
     const unsigned char *p = static_cast<const unsigned char *>(a.x) + row * a.x_stride + k;
     if (VEC) {
-      if (k < a.k) c = __ldg(reinterpret_cast<const uint2 *>(p));
+      if (k < a.k) {
+        const uint2 c = __ldg(reinterpret_cast<const uint2 *>(p));
+        w[0] = c.x, w[1] = c.y;
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e)
-        if (k + e < a.k) (e < 4 ? c.x : c.y) |= (uint32_t)p[e] << (8 * (e & 3));
+        if (k + e < a.k) w[e >> 2] |= (uint32_t)p[e] << (8 * (e & 3));
     }
-    const uint4 v = widen<T>(c, a.x_kind);
-    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
   }
 }
 
-// Eight numbers of y or out, as they are in memory (fp32 in all of `u`, 16 bits in its first half).
+// Eight numbers of y[row] from n0 on: as they are in memory (y_floats widens them), or one by one.
 template <bool VEC>
-__device__ __forceinline__ void load_y(const void *y, int dtype, int64_t at, int valid, uint32_t (&u)[8]) {
+__device__ __forceinline__ void load_y(const Args &a, int64_t row, int64_t n0, int valid, uint4 (&u)[2], float (&v)[8]) {
+  const int64_t at = row * a.y_stride + n0;
   if (VEC) {
     if (valid <= 0) return;
-    if (dtype == TC_F32) {
-      const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(y) + at);
-      const uint4 a = __ldg(p), b = __ldg(p + 1);
-      u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w, u[4] = b.x, u[5] = b.y, u[6] = b.z, u[7] = b.w;
+    if (a.y_dtype == TC_F32) {
+      const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(a.y) + at);
+      u[0] = __ldg(p), u[1] = __ldg(p + 1);
     } else {
-      const uint4 a = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(y) + at));
-      u[0] = a.x, u[1] = a.y, u[2] = a.z, u[3] = a.w;
+      u[0] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.y) + at));
     }
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < valid) u[e] = f2u(load_as_float(y, dtype, at + e));
+      if (e < valid) v[e] = load_as_float(a.y, a.y_dtype, at + e);
   }
 }
 template <bool VEC>
-__device__ __forceinline__ void y_floats(int dtype, const uint32_t (&u)[8], float (&v)[8]) {
+__device__ __forceinline__ void y_floats(int dtype, const uint4 (&x)[2], float (&v)[8]) {
+  if (!VEC) return;
+  const uint32_t u[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+  if (dtype == TC_F32) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const uint32_t half = (u[e >> 1] >> (16 * (e & 1))) & 0xFFFFu;
-    v[e] = !VEC || dtype == TC_F32 ? u2f(u[e]) : dtype == TC_BF16 ? u2f(half << 16) : __half2float(__ushort_as_half((unsigned short)half));
+    for (int e = 0; e < 8; ++e) v[e] = u2f(u[e]);
+  } else if (dtype == TC_BF16) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[2 * e] = u2f(u[e] << 16), v[2 * e + 1] = u2f(u[e] & 0xFFFF0000u);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&u[e]));
+      v[2 * e] = f.x, v[2 * e + 1] = f.y;
+    }
   }
 }
 template <bool VEC>
@@ -148,11 +163,12 @@ __device__ __forceinline__ void store_out(void *out, int dtype, int64_t at, int 
     if (dtype == TC_F32) {
       float4 *p = reinterpret_cast<float4 *>(static_cast<float *>(out) + at);
       p[0] = make_float4(v[0], v[1], v[2], v[3]), p[1] = make_float4(v[4], v[5], v[6], v[7]);
+    } else if (dtype == TC_BF16) {
+      *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + at) =
+          make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
     } else {
-      uint32_t u[4];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) u[e] = dtype == TC_BF16 ? pack_bf16(v[2 * e], v[2 * e + 1]) : pack_half(v[2 * e], v[2 * e + 1]);
-      *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + at) = make_uint4(u[0], u[1], u[2], u[3]);
+      *reinterpret_cast<uint4 *>(static_cast<uint16_t *>(out) + at) =
+          make_uint4(pack_half(v[0], v[1]), pack_half(v[2], v[3]), pack_half(v[4], v[5]), pack_half(v[6], v[7]));
     }
   } else {
 #pragma unroll
@@ -161,48 +177,35 @@ __device__ __forceinline__ void store_out(void *out, int dtype, int64_t at, int 
   }
 }
 
-// A cluster takes a tile of up to 8 NG tokens; its blocks share the sums over k, add them up through distributed shared memory, and
-// share the columns of out. Both products run on m16n8k16 MMAs with weights in rows and tokens in columns, so a single token
-// wastes none of the weights' traffic; operands go from memory to registers as vectors of 16 bytes (8 where a row of B has
-// 16 ranks or fewer: RW), which the order of k inside a product allows: any, as long as both operands have the same.
-// The tile's distinct adapters are taken in turn, each for the tokens that name it; a column's result is
-// selected, not added, so what is not finite in an adapter stays with its tokens. h = A x is fp32 and enters the second
-// product in parts of 16 bits, each the rounded rest of the one before: two where out has 16 bits (2**-16 of h is left out), three
-// where it has 32. fp16 parts are taken of h times a power of two, a token's own, that brings its largest to 2**13.
-template <typename T, int NG, int RW, bool VEC>
-__global__ void __launch_bounds__(kThreads, 2) tile_kernel(Args a) {
-  constexpr int kTokens = 8 * NG, kRowTiles = RW / 16;
-  constexpr bool kBf16 = Same<T, __nv_bfloat16>::value;
-  extern __shared__ __align__(16) unsigned char dynamic[];
-  __shared__ int index[kTokens], adapters[kTokens];
-  __shared__ uint32_t members[kTokens];  // of each distinct adapter, the groups of 8 tokens that it has
-  __shared__ int distinct;
-  __shared__ uint32_t peak[kTokens];     // fp16: of each token, the largest |h|
-  cg::cluster_group cluster = cg::this_cluster();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const int blocks = a.blocks, rank = (int)cluster.block_rank();
-  const int64_t t0 = (int64_t)(blockIdx.x / blocks) * a.tile;
-  const int tokens = (int)min((int64_t)a.tile, a.tokens - t0);
-  const uint16_t *A = static_cast<const uint16_t *>(a.a), *B = static_cast<const uint16_t *>(a.b);
+// The tokens of a tile and their adapters.
+template <int NG>
+struct Tile {
+  int index[8 * NG], adapters[8 * NG];
+  uint32_t members[8 * NG];  // of each distinct adapter, the groups of 8 tokens that it has
+  int distinct;
+  uint32_t peak[8 * NG];     // fp16: of each token, the largest |h|
 
-  if (warp == 0) {
-    int mine[(kTokens + 31) / 32];
+  // One warp.
+  __device__ __forceinline__ void fill(const Args &a, int64_t t0, int tokens) {
+    constexpr int kEach = (8 * NG + 31) / 32;
+    const int lane = threadIdx.x & 31;
+    int mine[kEach];
 #pragma unroll
-    for (int i = 0; i < (kTokens + 31) / 32; ++i) {
+    for (int i = 0; i < kEach; ++i) {
       const int t = lane + 32 * i;
       mine[i] = t < tokens ? a.index[t0 + t] : -1;
       if (mine[i] >= a.adapters) mine[i] = -1;
-      if (t < kTokens) index[t] = max(mine[i], -1), peak[t] = 0u;
+      if (t < 8 * NG) index[t] = max(mine[i], -1), peak[t] = 0u;
     }
     int n = 0;
 #pragma unroll
-    for (int i = 0; i < (kTokens + 31) / 32; ++i) {
+    for (int i = 0; i < kEach; ++i) {
       unsigned open;
       while ((open = __ballot_sync(0xFFFFFFFFu, mine[i] >= 0))) {
         const int v = __shfl_sync(0xFFFFFFFFu, mine[i], __ffs(open) - 1);
         uint32_t groups = 0u;
 #pragma unroll
-        for (int o = i; o < (kTokens + 31) / 32; ++o) {
+        for (int o = i; o < kEach; ++o) {
           const unsigned same = __ballot_sync(0xFFFFFFFFu, mine[o] == v);
 #pragma unroll
           for (int b = 0; b < 4; ++b) groups |= ((same >> (8 * b)) & 255u ? 1u : 0u) << (4 * o + b);
@@ -214,89 +217,171 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(Args a) {
     }
     if (lane == 0) distinct = n;
   }
-  __syncthreads();
-  const int count = distinct;
+};
 
-  const int rows = (a.rank + RW - 1) / RW * RW;        // of h, filled up with zeros
-  const int row_blocks = rows / RW;
-  int splits = kWarps;                                 // warps that share a sum over k
+// How many warps share a sum over k: as many as there are for every adapter (one at least) and block of RW rows of A.
+__device__ __forceinline__ int splits_of(int count, int row_blocks) {
+  int splits = kWarps;
   while (splits > 1 && splits * count * row_blocks > kWarps) splits >>= 1;
-  float *part = reinterpret_cast<float *>(dynamic);    // [splits][kTokens][rows]
-  const int row_stride = rows + 8;                     // of h's parts: rows of 16 bytes more, against bank conflicts
-  uint16_t *parts = reinterpret_cast<uint16_t *>(dynamic + (size_t)kWarps / row_blocks * kTokens * rows * sizeof(float));
-  const int terms = a.out_dtype == TC_F32 ? 3 : 2;
-  float *full = reinterpret_cast<float *>(parts + 3 * kTokens * row_stride);  // fp16: h
-  auto split = [&](float v, int t, int r) {
-    for (int p = 0; p < terms; ++p) {
-      const uint32_t h = pack16<T>(v, 0.0f) & 0xFFFFu;
-      parts[(p * kTokens + t) * row_stride + r] = (uint16_t)h;
-      const float back = half_bits_to_float<T>(h);
-      v = fabsf(back) < INFINITY ? __fsub_rn(v, back) : 0.0f;  // what is not finite stands in the first part
-    }
-  };
+  return splits;
+}
 
-  if (count) {
-    const int64_t chunks = (a.k + 31) / 32, each = (chunks + blocks - 1) / blocks;
-    const int64_t c0 = min(each * rank, chunks), c1 = min(c0 + each, chunks);
-    for (int item = warp; item < count * row_blocks * splits; item += kWarps) {
-      const int s = item % splits, rb = item / splits % row_blocks, j = item / splits / row_blocks;
-      const int who = adapters[j];
-      const uint32_t groups = members[j];
-      float acc[NG][kRowTiles][4];
+// Sums over the elements [32 c0, 32 c1) of x of a tile's tokens, each with its own adapter's rows: part [token][rows].
+// m16n8k16 MMAs with A's rows in rows and tokens in columns, so a single token wastes none of A's traffic; operands go from memory to
+// registers as vectors of 16 bytes, which the order of k inside a product allows: any, as long as both operands have the
+// same. The distinct adapters are taken one by one, and a token's result is stored by its own only, so what is not
+// finite in an adapter stays with its tokens.
+template <typename T, int NG, int RW, bool CODES, bool VEC>
+__device__ __forceinline__ void sum_rows(const Args &a, const Tile<NG> &tile, int64_t t0, int tokens, int64_t c0, int64_t c1, float *part) {
+  constexpr int kTokens = 8 * NG, kRowTiles = RW / 16;
+  constexpr bool kBf16 = Same<T, __nv_bfloat16>::value;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const uint16_t *A = static_cast<const uint16_t *>(a.a);
+  const int rows = RW == 16 ? 16 : rank_rows(a.rank), row_blocks = RW == 16 ? 1 : rows / RW, count = tile.distinct, splits = splits_of(count, row_blocks);
+  for (int item = warp; item < count * row_blocks * splits; item += kWarps) {
+    const int s = item % splits, rb = item / splits % row_blocks, j = item / splits / row_blocks;
+    const int who = tile.adapters[j];
+    const uint32_t has = tile.members[j];
+    float acc[NG][kRowTiles][4];
 #pragma unroll
-      for (int i = 0; i < NG; ++i)
+    for (int i = 0; i < NG; ++i)
 #pragma unroll
-        for (int r = 0; r < kRowTiles; ++r) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.0f;
+      for (int r = 0; r < kRowTiles; ++r) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.0f;
 #pragma unroll 2
-      for (int64_t c = c0 + s; c < c1; c += splits) {
-        const int64_t k = c * 32 + q * 8;
-        uint32_t w[kRowTiles][2][4], x[NG][4];
+    for (int64_t c = c0 + s; c < c1; c += splits) {
+      const int64_t k = c * 32 + q * 8;
+      uint32_t w[kRowTiles][2][4], x[NG][4];
 #pragma unroll
-        for (int r = 0; r < kRowTiles; ++r)
+      for (int r = 0; r < kRowTiles; ++r)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int row = rb * RW + r * 16 + h * 8 + g;
-            load16<8, VEC>(A + ((int64_t)who * a.rank + row) * a.k, k, row < a.rank ? a.k : 0, w[r][h]);
-          }
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0u;
-          if ((groups >> i & 1u) && i * 8 + g < tokens) load_x<T, VEC>(a, t0 + i * 8 + g, k, x[i]);
+        for (int h = 0; h < 2; ++h) {
+          const int row = rb * RW + r * 16 + h * 8 + g;
+          load16<8, VEC>(A + ((int64_t)who * a.rank + row) * a.k, k, row < a.rank ? a.k : 0, w[r][h]);
         }
 #pragma unroll
-        for (int i = 0; i < NG; ++i)
-          if (groups >> i & 1u)
+      for (int i = 0; i < NG; ++i) {
+        x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0u;
+        if ((has >> i & 1u) && i * 8 + g < tokens) load_x<CODES, VEC>(a, t0 + i * 8 + g, k, x[i]);
+      }
+      if (CODES) {  // after every load is on its way
 #pragma unroll
-            for (int r = 0; r < kRowTiles; ++r)
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t f[4] = {w[r][0][2 * h], w[r][1][2 * h], w[r][0][2 * h + 1], w[r][1][2 * h + 1]};
-                mma16<kBf16>(acc[i][r], f, x[i][2 * h], x[i][2 * h + 1]);
-              }
+        for (int i = 0; i < NG; ++i) {
+          const uint4 v = widen<T>(make_uint2(x[i][0], x[i][1]), a.x_kind);
+          x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+        }
       }
 #pragma unroll
       for (int i = 0; i < NG; ++i)
-        if (groups >> i & 1u)
+        if (has >> i & 1u)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int t = i * 8 + q * 2 + e;
-            if (index[t] == who)
+          for (int r = 0; r < kRowTiles; ++r)
 #pragma unroll
-              for (int r = 0; r < kRowTiles; ++r) {
-                float *to = part + ((int64_t)s * kTokens + t) * rows + rb * RW + r * 16 + g;
-                to[0] = acc[i][r][e], to[8] = acc[i][r][2 + e];
-              }
-          }
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t f[4] = {w[r][0][2 * h], w[r][1][2 * h], w[r][0][2 * h + 1], w[r][1][2 * h + 1]};
+              mma16<kBf16>(acc[i][r], f, x[i][2 * h], x[i][2 * h + 1]);
+            }
     }
-    __syncthreads();
-    for (int e = tid; e < kTokens * rows; e += kThreads) {
-      float v = 0.0f;
-      for (int s = 0; s < splits; ++s) v = __fadd_rn(v, part[s * kTokens * rows + e]);
-      part[e] = v;
+#pragma unroll
+    for (int i = 0; i < NG; ++i)
+      if (has >> i & 1u)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int t = i * 8 + q * 2 + e;
+          if (tile.index[t] == who)
+#pragma unroll
+            for (int r = 0; r < kRowTiles; ++r) {
+              float *to = part + ((int64_t)s * kTokens + t) * rows + rb * RW + r * 16 + g;
+              to[0] = acc[i][r][e], to[8] = acc[i][r][2 + e];
+            }
+        }
+  }
+  __syncthreads();
+  for (int e = tid; e < kTokens * rows; e += kThreads) {
+    float v = 0.0f;
+    for (int s = 0; s < splits; ++s) v = __fadd_rn(v, part[s * kTokens * rows + e]);
+    part[e] = v;
+  }
+}
+// Floats of `part`, its splits included.
+__host__ __device__ __forceinline__ size_t part_floats(int ng, int rw, int rows) { return (size_t)(kWarps / (rows / rw)) * 8 * ng * rows; }
+
+// h in parts of 16 bits, each the rounded rest of the one before, `apart` elements from one another.
+template <typename T>
+__device__ __forceinline__ void split_parts(float v, int terms, uint16_t *to, int apart) {
+  for (int p = 0; p < terms; ++p) {
+    const uint32_t h = pack16<T>(v, 0.0f) & 0xFFFFu;
+    to[p * apart] = (uint16_t)h;
+    const float back = half_bits_to_float<T>(h);
+    v = fabsf(back) < INFINITY ? __fsub_rn(v, back) : 0.0f;  // what is not finite stands in the first part
+  }
+}
+
+// d = the products of one adapter's 64 columns (w: of its B the rows n0 + 2 k + h, n0 a lane's own) with eight tokens' h, a part
+// after the other.
+template <typename T, int RW>
+__device__ __forceinline__ void multiply(const uint32_t (&w)[4][2][RW / 8], const uint32_t (&h)[RW / 8], float (&d)[4][4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int st = 0; st < RW / 16; ++st) {
+      const uint32_t f[4] = {w[k][0][2 * st], w[k][1][2 * st], w[k][0][2 * st + 1], w[k][1][2 * st + 1]};
+      mma16<Same<T, __nv_bfloat16>::value>(d[k], f, h[2 * st], h[2 * st + 1]);
     }
+}
+template <int RW>
+__device__ __forceinline__ void load_h(const uint16_t *from, uint32_t (&h)[RW / 8]) {
+  if constexpr (RW == 32) {
+    const uint4 v = *reinterpret_cast<const uint4 *>(from);
+    h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
+  } else {
+    const uint2 v = *reinterpret_cast<const uint2 *>(from);
+    h[0] = v.x, h[1] = v.y;
+  }
+}
+template <int RW, bool VEC>
+__device__ __forceinline__ void load_rows(const Args &a, int who, int64_t n0, int valid, int kc, int q, uint32_t (&w)[4][2][RW / 8]) {
+  const uint16_t *from = static_cast<const uint16_t *>(a.b) + ((int64_t)who * a.n + n0) * a.rank;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      load16<RW / 4, VEC>(from + (2 * k + h) * a.rank, kc * 32 + q * (RW / 4), 2 * k + h < valid ? a.rank : 0, w[k][h]);
+}
+// The sums of one of a lane's two tokens, on top of its y.
+__device__ __forceinline__ void take(const float (&d)[4][4], int e, float factor, float (&v)[8]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[2 * k] = __fmaf_rn(d[k][e], factor, v[2 * k]), v[2 * k + 1] = __fmaf_rn(d[k][2 + e], factor, v[2 * k + 1]);
+}
+
+// Few tokens: both products in one kernel. A cluster takes a tile of up to 8 NG tokens; its blocks share the sums over k, add them up through
+// distributed shared memory, and share the columns of out. h = A x is fp32 and enters the second product in parts
+// of 16 bits: two where out has 16 bits (2**-16 of h is left out), three where it has 32; fp16 parts are taken of h times a power of two, a
+// token's own, that brings its largest to 2**13.
+template <typename T, int NG, int RW, bool CODES, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) tile_kernel(Args a) {
+  constexpr int kTokens = 8 * NG;
+  constexpr bool kBf16 = Same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  __shared__ Tile<NG> tile;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int blocks = a.blocks, rank = (int)cluster.block_rank();
+  const int64_t t0 = (int64_t)(blockIdx.x / blocks) * a.tile;
+  const int tokens = (int)min((int64_t)a.tile, a.tokens - t0);
+  if (warp == 0) tile.fill(a, t0, tokens);
+  __syncthreads();
+  const int count = tile.distinct, rows = RW == 16 ? 16 : rank_rows(a.rank), row_blocks = RW == 16 ? 1 : rows / RW;
+  const int row_stride = rows + 8;                     // of h's parts: rows of 16 bytes more, against bank conflicts
+  float *part = reinterpret_cast<float *>(dynamic);    // [splits][kTokens][rows]
+  uint16_t *parts = reinterpret_cast<uint16_t *>(part + part_floats(NG, RW, rows));
+  float *full = reinterpret_cast<float *>(parts + 3 * kTokens * row_stride);  // fp16: h
+  const int terms = a.out_dtype == TC_F32 ? 3 : 2;
+  if (count) {
+    const int64_t chunks = (a.k + 31) / 32, each = (chunks + blocks - 1) / blocks, c0 = min(each * rank, chunks);
+    sum_rows<T, NG, RW, CODES, VEC>(a, tile, t0, tokens, c0, min(c0 + each, chunks), part);
     cluster.sync();
     for (int e = tid; e < kTokens * rows; e += kThreads) {
-      const int t = e / rows, r = e - t * rows, who = index[t];
+      const int t = e / rows, r = e - t * rows, who = tile.index[t];
       float v = 0.0f;
       if (who >= 0) {
         for (int b = 0; b < blocks; ++b) v = __fadd_rn(v, *cluster.map_shared_rank(part + e, b));
@@ -304,14 +389,15 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(Args a) {
         if (a.gain) f = __fmul_rn(f, a.gain[who]);
         v = __fmul_rn(v, f);
       }
-      if (kBf16) split(v, t, r);
-      else full[e] = v, atomicMax(&peak[t], abs_bits(v));
+      if (kBf16) split_parts<T>(v, terms, parts + t * row_stride + r, kTokens * row_stride);
+      else full[e] = v, atomicMax(&tile.peak[t], abs_bits(v));
     }
     __syncthreads();
     if (!kBf16) {
       for (int e = tid; e < kTokens * rows; e += kThreads) {
         const int t = e / rows;
-        split(__fmul_rn(full[e], fp16_shift(u2f(peak[t])).factor), t, e - t * rows);
+        split_parts<T>(__fmul_rn(full[e], fp16_shift(u2f(tile.peak[t])).factor), terms, parts + t * row_stride + e - t * rows,
+                       kTokens * row_stride);
       }
       __syncthreads();
     }
@@ -323,84 +409,344 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(Args a) {
   for (int64_t c = each * rank + warp; c < c1; c += kWarps) {
     const int64_t n0 = c * 64 + g * 8;
     const int valid = (int)min(max(a.n - n0, (int64_t)0), (int64_t)8);
-    uint32_t w[4][2][RW / 8];  // the rows n0 + 2 i + h of one adapter
+    uint32_t w[4][2][RW / 8];
     int loaded = -1;
-    auto load_rows = [&](int who, int kc) {
+    for (int i = 0; i * 8 < tokens; ++i) {
+      uint4 u[2][2];
+      float v[2][8];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int64_t row = n0 + 2 * i + h;
-          load16<RW / 4, VEC>(B + ((int64_t)who * a.n + row) * a.rank, kc * 32 + q * (RW / 4), row < a.n ? a.rank : 0, w[i][h]);
-        }
-    };
-    for (int i = 0; i < NG; ++i) {
-      if (i * 8 >= tokens) break;
-      uint32_t u[2][8];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int t = i * 8 + q * 2 + e;
-        load_y<VEC>(a.y, a.y_dtype, (t0 + t) * a.y_stride + n0, t < tokens ? valid : 0, u[e]);
-      }
-      float sum[2][8];
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int k = 0; k < 8; ++k) sum[e][k] = 0.0f;
-      const int who0 = index[i * 8 + q * 2], who1 = index[i * 8 + q * 2 + 1];
+      for (int e = 0; e < 2; ++e) load_y<VEC>(a, t0 + i * 8 + q * 2 + e, n0, i * 8 + q * 2 + e < tokens ? valid : 0, u[e], v[e]);
+      const int who0 = tile.index[i * 8 + q * 2], who1 = tile.index[i * 8 + q * 2 + 1];
+      bool widened = false;
       for (int j = 0; j < count; ++j) {
-        if (!(members[j] >> i & 1u)) continue;
-        const int who = adapters[j];
+        if (!(tile.members[j] >> i & 1u)) continue;
+        const int who = tile.adapters[j];
         float d[4][4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) d[k][0] = d[k][1] = d[k][2] = d[k][3] = 0.0f;
         for (int kc = 0; kc < row_blocks; ++kc) {
-          if (row_blocks > 1 || loaded != who) load_rows(who, kc);
+          if (row_blocks > 1 || loaded != who) load_rows<RW, VEC>(a, who, n0, valid, kc, q, w);
           for (int p = 0; p < terms; ++p) {
             uint32_t h[RW / 8];
-            const uint16_t *from = parts + (p * kTokens + i * 8 + g) * row_stride + kc * 32 + q * (RW / 4);
-            if constexpr (RW == 32) {
-              const uint4 v = *reinterpret_cast<const uint4 *>(from);
-              h[0] = v.x, h[1] = v.y, h[2] = v.z, h[3] = v.w;
-            } else {
-              const uint2 v = *reinterpret_cast<const uint2 *>(from);
-              h[0] = v.x, h[1] = v.y;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-              for (int st = 0; st < RW / 16; ++st) {
-                const uint32_t f[4] = {w[k][0][2 * st], w[k][1][2 * st], w[k][0][2 * st + 1], w[k][1][2 * st + 1]};
-                mma16<kBf16>(d[k], f, h[2 * st], h[2 * st + 1]);
-              }
+            load_h<RW>(parts + (p * kTokens + i * 8 + g) * row_stride + kc * 32 + q * (RW / 4), h);
+            multiply<T, RW>(w, h, d);
           }
         }
         loaded = who;
-        if (!kBf16) {
-          const float f0 = fp16_shift(u2f(peak[i * 8 + q * 2])).inverse, f1 = fp16_shift(u2f(peak[i * 8 + q * 2 + 1])).inverse;
-#pragma unroll
-          for (int k = 0; k < 4; ++k)
-            d[k][0] = __fmul_rn(d[k][0], f0), d[k][2] = __fmul_rn(d[k][2], f0), d[k][1] = __fmul_rn(d[k][1], f1), d[k][3] = __fmul_rn(d[k][3], f1);
+        if (!widened) {
+          y_floats<VEC>(a.y_dtype, u[0], v[0]), y_floats<VEC>(a.y_dtype, u[1], v[1]);
+          widened = true;
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (who0 == who) sum[0][2 * k] = d[k][0], sum[0][2 * k + 1] = d[k][2];
-          if (who1 == who) sum[1][2 * k] = d[k][1], sum[1][2 * k + 1] = d[k][3];
-        }
+        if (who0 == who) take(d, 0, kBf16 ? 1.0f : fp16_shift(u2f(tile.peak[i * 8 + q * 2])).inverse, v[0]);
+        if (who1 == who) take(d, 1, kBf16 ? 1.0f : fp16_shift(u2f(tile.peak[i * 8 + q * 2 + 1])).inverse, v[1]);
       }
+      if (!widened) y_floats<VEC>(a.y_dtype, u[0], v[0]), y_floats<VEC>(a.y_dtype, u[1], v[1]);
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         const int t = i * 8 + q * 2 + e;
-        float v[8];
-        y_floats<VEC>(a.y_dtype, u[e], v);
-        if ((e ? who1 : who0) >= 0)
-#pragma unroll
-          for (int k = 0; k < 8; ++k) v[k] = __fadd_rn(v[k], sum[e][k]);
-        store_out<VEC>(a.out, a.out_dtype, (t0 + t) * a.n + n0, t < tokens ? valid : 0, v);
+        store_out<VEC>(a.out, a.out_dtype, (t0 + t) * a.n + n0, t < tokens ? valid : 0, v[e]);
       }
     }
   }
   if (count) cluster.sync();  // the other blocks may still read this one's sums
+}
+
+// Many tokens, in two kernels. h first: a cluster a tile of tokens, whose blocks share the sums over k, and then the tokens.
+template <typename T, int NG, int RW, bool CODES, bool VEC>
+__global__ void __launch_bounds__(kThreads, RW == 16 ? 4 : 3) down_kernel(Args a) {
+  constexpr int kTokens = 8 * NG;
+  constexpr bool kBf16 = Same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  __shared__ Tile<NG> tile;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, blocks = a.blocks, rank = (int)cluster.block_rank();
+  const int64_t t0 = (int64_t)(blockIdx.x / blocks) * kTokens;
+  const int tokens = (int)min((int64_t)kTokens, a.tokens - t0);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (tid < 32) tile.fill(a, t0, tokens);
+  __syncthreads();
+  if (tile.distinct == 0) return;  // nobody reads the tile's h
+  const int rows = RW == 16 ? 16 : rank_rows(a.rank), terms = a.out_dtype == TC_F32 ? 3 : 2;
+  float *part = reinterpret_cast<float *>(dynamic);
+  const int64_t chunks = (a.k + 31) / 32, each = (chunks + blocks - 1) / blocks, c0 = min(each * rank, chunks);
+  sum_rows<T, NG, RW, CODES, VEC>(a, tile, t0, tokens, c0, min(c0 + each, chunks), part);
+  cluster.sync();
+  auto sum = [&](int e, int t, int who) {
+    float v = 0.0f;
+    for (int b = 0; b < blocks; ++b) v = __fadd_rn(v, *cluster.map_shared_rank(part + e, b));
+    float f = a.x_scale ? a.x_scale[t0 + t] : 1.0f;
+    if (a.gain) f = __fmul_rn(f, a.gain[who]);
+    return __fmul_rn(v, f);
+  };
+  const int warp = tid >> 5, lane = tid & 31;
+  for (int t = rank * kWarps + warp; t < tokens; t += blocks * kWarps) {  // a warp a token
+    const int who = tile.index[t];
+    if (who < 0) continue;
+    float v[kMaxRank / 32];
+    float top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kMaxRank / 32; ++i) {
+      const int r = lane + 32 * i;
+      v[i] = r < rows ? sum(t * rows + r, t, who) : 0.0f;
+      if (!kBf16) top = fmaxf(top, u2f(abs_bits(v[i])));
+    }
+    float factor = 1.0f;
+    if (!kBf16) {
+      const Pow2 p = fp16_shift(u2f(warp_max(f2u(top))));
+      factor = p.factor;
+      if (lane == 0) a.factors[t0 + t] = p.inverse;
+    }
+#pragma unroll
+    for (int i = 0; i < kMaxRank / 32; ++i)
+      if (lane + 32 * i < rows) split_parts<T>(__fmul_rn(v[i], factor), terms, a.parts + (t0 + t) * terms * rows + lane + 32 * i, rows);
+  }
+  cluster.sync();  // the other blocks may still read this one's sums
+}
+
+// Then out: a warp takes 64 columns and a run of tokens, a lane 8 neighbouring columns of two tokens of each eight. The rows of B stay in
+// registers as long as the adapter does; y, h and the adapters of the next eight tokens are on their way while these are
+// computed. Y, O: y and out have 32 bits (else 16). With 16 bits out, y is what the products are added to in the MMAs.
+template <typename T, int RW, bool Y, bool O, bool VEC>
+__global__ void __launch_bounds__(kThreads, 2) up_kernel(Args a) {
+  constexpr bool kBf16 = Same<T, __nv_bfloat16>::value;
+  constexpr int kTerms = O ? 3 : 2;
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int64_t columns = (a.n + 63) / 64, item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int64_t run = item / columns, n0 = (item - run * columns) * 64 + g * 8, t0 = run * a.tile;
+  if (t0 >= a.tokens) return;
+  int left = (int)min((int64_t)a.tile, a.tokens - t0);
+  int64_t token = t0 + q * 2;
+  const int valid = (int)min(max(a.n - n0, (int64_t)0), (int64_t)8);
+  const int rows = RW == 16 ? 16 : rank_rows(a.rank), row_blocks = RW == 16 ? 1 : rows / RW;
+  // Where this lane's two tokens and, for h, its one of the eight stand.
+  const int32_t *index = a.index + t0 + q * 2;
+  int64_t y_at = (t0 + q * 2) * a.y_stride + n0, out_at = (t0 + q * 2) * a.n + n0;
+  const uint16_t *parts = a.parts + (t0 + g) * kTerms * rows + q * (RW / 4);
+  // Beyond 32 ranks the rows of B stand in shared memory, a lane's own pieces of 16 bytes side by side with the other lanes'.
+  extern __shared__ __align__(16) unsigned char dynamic[];
+  uint4 *kept = reinterpret_cast<uint4 *>(dynamic) + (size_t)(threadIdx.x >> 5) * row_blocks * 8 * 32 + lane;
+  uint32_t w[4][2][RW / 8], h[kTerms][RW / 8];
+  int loaded = -1, who[2];
+  uint4 u[2][Y ? 2 : 1];
+  float v[2][VEC ? 1 : 8];
+  auto ask = [&](int64_t y_from, const int32_t *from, int tokens) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bool real = q * 2 + e < tokens;
+      who[e] = real ? __ldg(from + e) : -1;
+      if constexpr (!VEC) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[e][k] = real && k < valid ? load_as_float(a.y, a.y_dtype, y_from + e * a.y_stride + k) : 0.0f;
+      }
+      if (VEC && real && valid > 0) {
+        if constexpr (Y) {
+          const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(a.y) + y_from + e * a.y_stride);
+          u[e][0] = __ldg(p), u[e][1] = __ldg(p + 1);
+        } else {
+          u[e][0] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.y) + y_from + e * a.y_stride));
+        }
+      }
+    }
+  };
+  auto ask_h = [&](const uint16_t *from, bool real) {
+    if (real && row_blocks == 1)
+#pragma unroll
+      for (int p = 0; p < kTerms; ++p) load_h<RW>(from + p * rows, h[p]);
+  };
+  ask(y_at, index, left);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // the first kernel's h
+  ask_h(parts, g < left);
+  for (; left > 0; left -= 8) {
+    float y[2][8];
+    int mine[2];
+    uint32_t own[kTerms][RW / 8];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      mine[e] = (unsigned)who[e] < (unsigned)a.adapters ? who[e] : -1;
+      if constexpr (!VEC) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[e][k] = v[e][k];
+      } else if constexpr (Y) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          y[e][4 * k] = u2f(u[e][k].x), y[e][4 * k + 1] = u2f(u[e][k].y), y[e][4 * k + 2] = u2f(u[e][k].z), y[e][4 * k + 3] = u2f(u[e][k].w);
+      } else {
+        const uint32_t v[4] = {u[e][0].x, u[e][0].y, u[e][0].z, u[e][0].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) y[e][2 * k] = half_bits_to_float<T>(v[k] & 0xFFFFu), y[e][2 * k + 1] = half_bits_to_float<T>(v[k] >> 16);
+      }
+    }
+#pragma unroll
+    for (int p = 0; p < kTerms; ++p)
+#pragma unroll
+      for (int k = 0; k < RW / 8; ++k) own[p][k] = h[p][k];
+    const uint16_t *now = parts;
+    y_at += 8 * a.y_stride, index += 8, parts += 8 * kTerms * rows;
+    ask(y_at, index, left - 8);
+    ask_h(parts, g < left - 8);
+
+    float d[4][4];
+    // The products of one adapter with the eight tokens, on top of d.
+    auto products = [&](int i) {
+      if (row_blocks == 1) {
+        if (loaded != i) load_rows<RW, VEC>(a, i, n0, valid, 0, q, w);
+#pragma unroll
+        for (int p = 0; p < kTerms; ++p) multiply<T, RW>(w, own[p], d);
+      } else if constexpr (RW == 32) {
+        for (int kc = 0; kc < row_blocks; ++kc) {
+          uint4 *piece = kept + kc * 8 * 32;
+          if (loaded != i) {
+            load_rows<RW, VEC>(a, i, n0, valid, kc, q, w);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) piece[k * 32] = make_uint4(w[k >> 1][k & 1][0], w[k >> 1][k & 1][1], w[k >> 1][k & 1][2], w[k >> 1][k & 1][3]);
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const uint4 x = piece[k * 32];
+              w[k >> 1][k & 1][0] = x.x, w[k >> 1][k & 1][1] = x.y, w[k >> 1][k & 1][2] = x.z, w[k >> 1][k & 1][3] = x.w;
+            }
+          }
+#pragma unroll
+          for (int p = 0; p < kTerms; ++p) {
+            uint32_t x[RW / 8];
+#pragma unroll
+            for (int k = 0; k < RW / 8; ++k) x[k] = 0u;
+            if (g < left) load_h<RW>(now + p * rows + kc * 32, x);
+            multiply<T, RW>(w, x, d);
+          }
+        }
+      }
+      loaded = i;
+    };
+    const int one = __shfl_sync(0xFFFFFFFFu, mine[0], 0);
+    if (!O && kBf16 && one >= 0 && __all_sync(0xFFFFFFFFu, mine[0] == one && mine[1] == one)) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) d[k][0] = y[0][2 * k], d[k][1] = y[1][2 * k], d[k][2] = y[0][2 * k + 1], d[k][3] = y[1][2 * k + 1];
+      products(one);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) y[0][2 * k] = d[k][0], y[1][2 * k] = d[k][1], y[0][2 * k + 1] = d[k][2], y[1][2 * k + 1] = d[k][3];
+    } else {
+      unsigned open[2] = {__ballot_sync(0xFFFFFFFFu, mine[0] >= 0), __ballot_sync(0xFFFFFFFFu, mine[1] >= 0)};
+      while (open[0] | open[1]) {
+        const int i = open[0] ? __shfl_sync(0xFFFFFFFFu, mine[0], __ffs(open[0]) - 1) : __shfl_sync(0xFFFFFFFFu, mine[1], __ffs(open[1]) - 1);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) d[k][0] = d[k][1] = d[k][2] = d[k][3] = 0.0f;
+        products(i);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          if (mine[e] == i) take(d, e, kBf16 ? 1.0f : a.factors[token + e], y[e]);
+          open[e] &= ~__ballot_sync(0xFFFFFFFFu, mine[e] == i);
+        }
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) store_out<VEC>(a.out, O ? TC_F32 : kBf16 ? TC_BF16 : TC_F16, out_at + e * a.n, q * 2 + e < left ? valid : 0, y[e]);
+    out_at += 8 * a.n, token += 8;
+  }
+}
+
+static cudaLaunchConfig_t config(int64_t blocks, size_t bytes, cudaStream_t s, cudaLaunchAttribute *attr) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = attr ? 1 : 0;
+  return cfg;
+}
+
+template <typename K>
+static cudaError_t room(K kernel, size_t bytes) {
+  return bytes > 48 << 10 ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes) : cudaSuccess;
+}
+
+template <typename T, int RW, bool CODES, bool VEC>
+static cudaError_t launch_tiles(const Args &a, cudaStream_t s) {
+  const int rows = rank_rows(a.rank);
+  const size_t bytes = part_floats(1, RW, rows) * sizeof(float) + (size_t)3 * 8 * (rows + 8) * sizeof(uint16_t) +
+                       (Same<T, __half>::value ? (size_t)8 * rows * sizeof(float) : 0);
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = a.blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  const cudaLaunchConfig_t cfg = config((a.tokens + a.tile - 1) / a.tile * a.blocks, bytes, s, &attr);
+  const cudaError_t e = room(tile_kernel<T, 1, RW, CODES, VEC>, bytes);
+  return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, tile_kernel<T, 1, RW, CODES, VEC>, a);
+}
+
+constexpr int kDownGroups = 2;  // of 8 tokens, a block of the first kernel
+
+template <typename T, int RW, bool CODES, bool VEC>
+static cudaError_t launch_two(Args a, cudaStream_t s) {
+  const size_t bytes = part_floats(kDownGroups, RW, rank_rows(a.rank)) * sizeof(float);
+  cudaError_t e = room(down_kernel<T, kDownGroups, RW, CODES, VEC>, bytes);
+  if (e != cudaSuccess) return e;
+  const int64_t tiles = (a.tokens + 8 * kDownGroups - 1) / (8 * kDownGroups);
+  a.blocks = 1;
+  while (a.blocks < 8 && tiles * a.blocks < 4 * (int64_t)sm_count()) a.blocks *= 2;  // a wave: four an SM
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = a.blocks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = config(tiles * a.blocks, bytes, s, &attr);
+  e = cudaLaunchKernelEx(&cfg, down_kernel<T, kDownGroups, RW, CODES, VEC>, a);
+  if (e != cudaSuccess) return e;
+  count_launch();
+  const int64_t columns = (a.n + 63) / 64;
+  a.tile = 128;
+  while (a.tile > 16 && (a.tokens + a.tile - 1) / a.tile * columns < 48 * (int64_t)sm_count()) a.tile /= 2;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  const int row_blocks = rank_rows(a.rank) / RW;
+  const size_t kept = row_blocks > 1 ? (size_t)kWarps * row_blocks * 8 * 512 : 0;
+  cfg = config(((a.tokens + a.tile - 1) / a.tile * columns + kWarps - 1) / kWarps, kept, s, &attr);
+  auto up = [&](auto kernel) {
+    const cudaError_t r = room(kernel, kept);
+    return r != cudaSuccess ? r : cudaLaunchKernelEx(&cfg, kernel, a);
+  };
+  if (!VEC) {  // any type of y
+    return a.out_dtype == TC_F32 ? up(up_kernel<T, RW, false, true, false>)
+                                 : up(up_kernel<T, RW, false, false, false>);
+  }
+  if (a.y_dtype == TC_F32)
+    return a.out_dtype == TC_F32 ? up(up_kernel<T, RW, true, true, true>)
+                                 : up(up_kernel<T, RW, true, false, true>);
+  return a.out_dtype == TC_F32 ? up(up_kernel<T, RW, false, true, true>)
+                               : up(up_kernel<T, RW, false, false, true>);
+}
+
+// Up to this many tokens one kernel does both products. One and two kernels, us, 4096 -> 4096, rank 16, fp32 to bf16, runs of 6
+// adapters: 32 tokens 7.7 and 12.5, 128 10.1 and 11.1, 256 12.5 and 11.1, 512 20 and 11, 1024 37 and 17.
+inline int64_t few_tokens() { return sm_count(); }
+
+template <typename T, bool CODES>
+static cudaError_t launch_two_as(const Args &a, bool vec, cudaStream_t s) {
+  if (a.rank <= 16) return vec ? launch_two<T, 16, CODES, true>(a, s) : launch_two<T, 16, CODES, false>(a, s);
+  return vec ? launch_two<T, 32, CODES, true>(a, s) : launch_two<T, 32, CODES, false>(a, s);
+}
+template <typename T, bool CODES>
+static cudaError_t launch_tiles_as(const Args &a, bool vec, cudaStream_t s) {
+  if (a.rank <= 16) return vec ? launch_tiles<T, 16, CODES, true>(a, s) : launch_tiles<T, 16, CODES, false>(a, s);
+  return vec ? launch_tiles<T, 32, CODES, true>(a, s) : launch_tiles<T, 32, CODES, false>(a, s);
+}
+
+template <typename T>
+static cudaError_t launch_as(Args a, cudaStream_t s) {
+  auto aligned = [](const void *p, size_t n) { return (uintptr_t)p % n == 0; };
+  const int y16 = a.y_dtype == TC_F32 ? 4 : 8;
+  const bool vec = a.k % 8 == 0 && a.n % 8 == 0 && a.rank % (a.rank <= 16 ? 4 : 8) == 0 && a.x_stride % 8 == 0 &&
+                   a.y_stride % y16 == 0 && aligned(a.x, a.x_kind <= X_F16 ? 16 : 8) && aligned(a.y, 16) && aligned(a.a, 16) &&
+                   aligned(a.b, 16) && aligned(a.out, 16);
+  const bool codes = a.x_kind > X_F16;
+  if (a.tokens > few_tokens()) return codes ? launch_two_as<T, true>(a, vec, s) : launch_two_as<T, false>(a, vec, s);
+  // Tiles of at most 8 tokens, as small as the card has clusters of 8 blocks for.
+  const int sms = sm_count();
+  a.tile = 1;
+  while (a.tile < 8 && (a.tokens + a.tile - 1) / a.tile * 8 > sms) a.tile *= 2;
+  a.blocks = 1;
+  while (a.blocks < 8 && (a.tokens + a.tile - 1) / a.tile * a.blocks * 2 <= sms) a.blocks *= 2;
+  return codes ? launch_tiles_as<T, true>(a, vec, s) : launch_tiles_as<T, false>(a, vec, s);
 }
 
 }  // namespace adapt
