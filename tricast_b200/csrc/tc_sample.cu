@@ -35,7 +35,7 @@ static cudaError_t launch(Args a, cudaStream_t s) {
   while (a.blocks < 8 && (a.vocab > 24576 * (int64_t)a.blocks ||
                           (a.rows * a.blocks < 2 * sm_count() && a.vocab > 4096 * (int64_t)a.blocks)))
     a.blocks *= 2;
-  a.part = ((a.vocab + 8 + a.blocks - 1) / a.blocks + 7) / 8 * 8;  // positions begin up to 7 elements before the row
+  a.part = (int)(((a.vocab + 8 + a.blocks - 1) / a.blocks + 127) / 128 * 128);  // positions begin up to 7 elements before the row
   return a.part <= kMaxHeld ? launch_as<T, true>(a, s) : launch_as<T, false>(a, s);
 }
 
@@ -55,7 +55,7 @@ extern "C" int tc_sample_tokens(const void *logits, int32_t dtype, int64_t rows,
   if (!logits || !uniform || !tokens) return bad("null pointer");
   if (rows > 1 && stride < vocab) return bad("the row stride must be at least vocab");
   sample::Args a{logits, rows, vocab, stride, uniform, temperature, top_p, min_p, top_k, all_temperature, all_top_p, all_min_p,
-                 all_top_k, tokens, logprobs, 1, vocab};
+                 all_top_k, tokens, logprobs, 1, 0};
   cudaStream_t s = (cudaStream_t)stream;
   const cudaError_t e = dtype == TC_F32    ? sample::launch<float>(a, s)
                         : dtype == TC_BF16 ? sample::launch<__nv_bfloat16>(a, s)

@@ -23,7 +23,8 @@ namespace sample {
 
 namespace cg = cooperative_groups;
 
-constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 512, kChunks = 256, kMaxBlocks = 16;
+constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 512, kMaxBlocks = 8;
+constexpr int kWarpChunks = 8, kChunks = kWarps * kWarpChunks;  // a stretch is cut into runs of a warp, these into chunks
 static_assert(kBins == kThreads, "a thread a bin");
 
 struct Args {
@@ -37,18 +38,23 @@ struct Args {
   int64_t *tokens;
   float *logprobs;
   int blocks;     // of a cluster
-  int64_t part;   // positions of a block's stretch, a multiple of 8
+  int part;       // positions of a block's stretch, a multiple of 128, at most 2**20
 };
 
 struct Shared {
   uint32_t hist[2][2][kBins];         // by turns (others may still read the last one): lower and upper parts, or counts
   double slots[2][kMaxBlocks];        // by turns: what each block of the cluster has sent
   double part[kWarps];
+  uint32_t tops[kWarps];
+  uint32_t peak[kChunks];             // of each chunk, the largest weight's bits
   double mass[kChunks];
   int ties[kChunks];
   double found[3];                    // of a histogram's scan
   int bin;
 };
+
+// The warp's number, said in a way that lets the compiler know that its lanes agree on it.
+__device__ __forceinline__ int warp_number() { return __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0); }
 
 __device__ __forceinline__ uint32_t key_of(float v) {
   const uint32_t u = f2u(__fadd_rn(v, 0.0f));  // both zeros are equal
@@ -95,142 +101,135 @@ struct Weight {
   __device__ __forceinline__ double log(float l) const { return ((double)l - top) * c * 0.6931471805599453; }
 };
 
-// A block's stretch of a row. Positions count from a 16-byte boundary at or before the row's begin (`skip` elements before it), so that
-// vectors are aligned for every row; positions outside the row read as -Inf.
+// A block's stretch of a row. Positions count from a 16-byte boundary at or before the row's begin, so that vectors are aligned for
+// every row; positions outside the row read as -Inf.
 template <typename T>
 struct Stretch {
-  const T *base;  // position 0
-  int64_t lo, hi;        // this block's positions
-  int64_t first, end;    // the row's
-  static constexpr int kVec = 16 / sizeof(T);
-  // kVec logits from position lo + i.
-  __device__ __forceinline__ void load(int64_t i, float (&v)[kVec]) const {
-    const int64_t p = lo + i;
-    if (p >= first && p + kVec <= end) {
-      const uint4 w = *reinterpret_cast<const uint4 *>(base + p);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+  const T *p;      // this block's position 0
+  int first, end;  // its positions inside the row
+  // Four logits from position i on, i a multiple of 4.
+  __device__ __forceinline__ float4 load(int i) const {
+    float v[4];
+    if (i >= first && i + 4 <= end) {
+      if constexpr (sizeof(T) == 4) return *reinterpret_cast<const float4 *>(p + i);
+      const uint2 w = *reinterpret_cast<const uint2 *>(p + i);
+      const uint32_t u[2] = {w.x, w.y};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if constexpr (sizeof(T) == 4) {
-          v[k] = u2f(u[k]);
-        } else if constexpr (Same<T, __nv_bfloat16>::value) {
-          v[2 * k] = u2f(u[k] << 16), v[2 * k + 1] = u2f(u[k] & 0xFFFF0000u);
-        } else {
-          v[2 * k] = __half2float(__ushort_as_half((unsigned short)(u[k] & 0xFFFFu)));
-          v[2 * k + 1] = __half2float(__ushort_as_half((unsigned short)(u[k] >> 16)));
-        }
-      }
+      for (int k = 0; k < 2; ++k) v[2 * k] = half_bits_to_float<Half>(u[k] & 0xFFFFu), v[2 * k + 1] = half_bits_to_float<Half>(u[k] >> 16);
     } else {
 #pragma unroll
-      for (int k = 0; k < kVec; ++k) v[k] = p + k >= first && p + k < end ? Io<T>::get(base[p + k]) : -INFINITY;
+      for (int k = 0; k < 4; ++k) v[k] = i + k >= first && i + k < end ? Io<T>::get(p[i + k]) : -INFINITY;
     }
+    return make_float4(v[0], v[1], v[2], v[3]);
   }
-  __device__ __forceinline__ float at(int64_t i) const { return Io<T>::get(base[lo + i]); }
+  __device__ __forceinline__ float at(int i) const { return Io<T>::get(p[i]); }
+
+ private:
+  template <typename U, bool B>
+  struct Or { using type = U; };
+  template <typename U>
+  struct Or<U, true> { using type = __half; };
+  using Half = typename Or<T, sizeof(T) == 4>::type;  // fp32 never gets there
 };
 
-// HELD: weights stand in shared memory; otherwise (rows beyond what a cluster holds) they are computed again by every pass.
+// HELD: weights stand in shared memory; otherwise (rows beyond what a cluster holds) they are computed again by every pass. A warp takes
+// a run of positions in chunks of `span`, each lane 4 neighbouring ones of every 128, in all passes alike: no barrier between them.
 template <typename T, bool HELD>
 struct Row {
   Stretch<T> z;
   Weight w;
   Shared &sh;
   float *held;
-  int64_t n;      // positions, a multiple of 8
+  int n, run, span;  // positions of the stretch, of a warp and of a chunk, multiples of 128
   int blocks, rank, turn, hist_turn;
   bool infinite;  // the row's largest logit is: its equals share everything, as logits of 0 beside -Inf
   cg::cluster_group cluster;
 
-  __device__ __forceinline__ Row(Shared &s, float *h) : sh(s), held(h), turn(0), hist_turn(0), infinite(false), cluster(cg::this_cluster()) {}
+  __device__ __forceinline__ Row(Shared &s, float *h)
+      : sh(s), held(h), turn(0), hist_turn(0), infinite(false), cluster(cg::this_cluster()) {}
 
-  // f(position, four weights) for the block's positions.
+  static __device__ __forceinline__ float finite(float l) { return l == INFINITY ? 0.0f : -INFINITY; }
+  __device__ __forceinline__ float4 weigh(float4 l) const {
+    if (infinite) l = make_float4(finite(l.x), finite(l.y), finite(l.z), finite(l.w));
+    return make_float4(w(l.x), w(l.y), w(l.z), w(l.w));
+  }
+  __device__ __forceinline__ float4 four(int i) const {
+    return HELD ? *reinterpret_cast<const float4 *>(held + i) : weigh(z.load(i));
+  }
+  // f(position, the bits of four weights) for the chunks of this warp whose largest weight is `from` at least.
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    if (HELD) {
-      for (int i = threadIdx.x * 4; i < (int)n; i += kThreads * 4) f((int64_t)i, *reinterpret_cast<const float4 *>(held + i));
-    } else {
-      for (int64_t i = (int64_t)threadIdx.x * 8; i < n; i += kThreads * 8) {
-        float4 a, b;
-        weights8(i, a, b);
-        f(i, a);
-        f(i + 4, b);
-      }
+  __device__ __forceinline__ void each(uint32_t from, F f) const {
+    chunks([&](int c, int at, int end) {
+      if (sh.peak[c] >= from)
+        steps(at, end, [&](int i) {
+          const float4 q = four(i);
+          f(i, make_uint4(f2u(q.x), f2u(q.y), f2u(q.z), f2u(q.w)));
+        });
+    });
+  }
+  // f(chunk, its first position, its end) for this warp's chunks, empty ones among them.
+  template <typename F>
+  __device__ __forceinline__ void chunks(F f) const {
+    const int warp = warp_number(), end = min((warp + 1) * run, n);
+#pragma unroll 1
+    for (int c = 0; c < kWarpChunks; ++c) {
+      const int at = warp * run + c * span;
+      f(warp * kWarpChunks + c, at, min(at + span, end));
     }
   }
-  __device__ __forceinline__ void logits8(int64_t i, float (&v)[8]) const {
-    constexpr int kVec = Stretch<T>::kVec;
+  // f(this lane's position) for 128 positions after the other; four times 128, what a chunk has where it is whole, without a loop.
+  template <typename F>
+  __device__ __forceinline__ void steps(int at, int end, F f) const {
+    const int mine = (threadIdx.x & 31) * 4;
+    for (; at + 512 <= end; at += 512)
 #pragma unroll
-    for (int k = 0; k < 8; k += kVec) {
-      float x[kVec];
-      z.load(i + k, x);
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) v[k + e] = x[e];
-    }
+      for (int k = 0; k < 4; ++k) f(at + k * 128 + mine);
+#pragma unroll 1
+    for (; at < end; at += 128) f(at + mine);
   }
-  static __device__ __forceinline__ void finite8(float (&v)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = v[k] == INFINITY ? 0.0f : -INFINITY;
-  }
-  __device__ __forceinline__ void weights8(int64_t i, float4 &a, float4 &b) const {
-    float v[8];
-    logits8(i, v);
-    if (infinite) finite8(v);
-    a = make_float4(w(v[0]), w(v[1]), w(v[2]), w(v[3]));
-    b = make_float4(w(v[4]), w(v[5]), w(v[6]), w(v[7]));
-  }
-  __device__ __forceinline__ float4 four(int64_t i) const {
-    if (HELD) return *reinterpret_cast<const float4 *>(held + i);
-    float4 a, b;
-    weights8(i & ~(int64_t)7, a, b);
-    return (i & 4) ? b : a;
-  }
+  __device__ __forceinline__ int begin_of(int c) const { return c / kWarpChunks * run + c % kWarpChunks * span; }
+  __device__ __forceinline__ int end_of(int c) const { return min(begin_of(c) + span, min((c / kWarpChunks + 1) * run, n)); }
 
-  // A number from each block, to all of them: slots() after it. Two meetings apart the slots are used again, and between
-  // them lies a barrier that a block reaches only after reading.
+  // A number from each block to all of them, to be read after the cluster's next barrier. Two turns apart the slots are used again,
+  // and between them lies a barrier that a block reaches only after reading.
   __device__ __forceinline__ const double *tell(double v) {
     double *to = sh.slots[turn];
     if ((int)threadIdx.x < blocks) cluster.map_shared_rank(to, threadIdx.x)[rank] = v;
-    cluster.sync();
     turn ^= 1;
     return to;
   }
-  // Sum over the block's threads, in every one of them.
+  // Sums in every thread of the block, in a fixed order: over a warp's lanes, then the warps' sums over 16 lanes of each warp.
   __device__ __forceinline__ double block_sum(double v) {
 #pragma unroll
     for (int m = 16; m; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = 0.0;
+    v = sh.part[threadIdx.x & (kWarps - 1)];
 #pragma unroll
-    for (int i = 0; i < kWarps; ++i) v += sh.part[i];
+    for (int m = kWarps / 2; m; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
     return v;
   }
-  __device__ __forceinline__ double cluster_sum(double v) {
-    const double *all = tell(block_sum(v));
-    v = 0.0;
-    for (int i = 0; i < blocks; ++i) v += all[i];
+  __device__ __forceinline__ double all_of(const double *slots) const {
+    const int lane = threadIdx.x & (kMaxBlocks - 1);
+    double v = lane < blocks ? slots[lane] : 0.0;
+#pragma unroll
+    for (int m = kMaxBlocks / 2; m; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
     return v;
   }
-  __device__ __forceinline__ double cluster_max(double v) {
-#pragma unroll
-    for (int m = 16; m; m >>= 1) v = fmax(v, __shfl_xor_sync(0xFFFFFFFFu, v, m));
+  // The largest of a key a thread, over the cluster.
+  __device__ __forceinline__ uint32_t cluster_max(uint32_t v) {
+    v = warp_max(v);
     __syncthreads();
-    if ((threadIdx.x & 31) == 0) sh.part[threadIdx.x >> 5] = v;
+    if ((threadIdx.x & 31) == 0) sh.tops[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = sh.part[0];
-#pragma unroll
-    for (int i = 1; i < kWarps; ++i) v = fmax(v, sh.part[i]);
-    const double *all = tell(v);
-    v = all[0];
-    for (int i = 1; i < blocks; ++i) v = fmax(v, all[i]);
-    return v;
+    v = warp_max(sh.tops[threadIdx.x & (kWarps - 1)]);
+    const double *all = tell((double)v);
+    cluster.sync();
+    const int lane = threadIdx.x & (kMaxBlocks - 1);
+    return warp_max(lane < blocks ? (uint32_t)all[lane] : 0u);
   }
 
-  __device__ __forceinline__ void clear() {
-    sh.hist[hist_turn][0][threadIdx.x] = 0u;
-    sh.hist[hist_turn][1][threadIdx.x] = 0u;
-    __syncthreads();
-  }
   // Adds a weight's bits to its bin: its count, or its 24-bit significand in parts of 12 bits (a stretch has at most 2**20
   // positions, so neither sum passes 32 bits).
   template <bool MASS>
@@ -243,13 +242,15 @@ struct Row {
       atomicAdd(&h[0][bin], 1u);
     }
   }
-  // The first bin at which counts or masses of the cluster, on top of `over`, reach `want`, kBins where none does (then, with
-  // `last`, the last one that is not empty). over: what is before it. c: its own count; exponent(bin): of the bin's weights.
-  template <bool MASS, typename X>
-  __device__ __forceinline__ int reach(double want, double &over, double &own, bool last, X exponent) {
+  // The first bin at which counts or masses of the cluster, on top of `over`, reach want(), kBins where none does (then, with
+  // `last`, the last one that is not empty). over: what is before it; own: what is in it; exponent(bin): of the bin's weights. The
+  // next histogram, which every block has read, is cleared.
+  template <bool MASS, typename Q, typename X>
+  __device__ __forceinline__ int reach(Q want, double &over, double &own, bool last, X exponent) {
     cluster.sync();
-    const int bin = threadIdx.x, lane = bin & 31, warp = bin >> 5;
-    double v = 0.0;
+    const int bin = threadIdx.x, lane = bin & 31, warp = warp_number();
+    const double need = want();
+    double v;
     {
       uint64_t lo = 0, hi = 0;
       for (int b = 0; b < blocks; ++b) {
@@ -257,9 +258,10 @@ struct Row {
         if (MASS) hi += *cluster.map_shared_rank(&sh.hist[hist_turn][1][bin], b);
       }
       v = (double)(lo + (hi << 12));
-      if (MASS) v = scalbn(v, exponent(bin) - 23);
+      if (MASS) v *= __longlong_as_double((long long)(1023 + exponent(bin) - 23) << 52);
     }
     hist_turn ^= 1;
+    sh.hist[hist_turn][0][bin] = 0u, sh.hist[hist_turn][1][bin] = 0u;
     double s = v;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -269,11 +271,16 @@ struct Row {
     if (lane == 31) sh.part[warp] = s;
     if (bin == 0) sh.bin = kBins;
     __syncthreads();
-    double base = over;
-    for (int i = 0; i < warp; ++i) base += sh.part[i];
-    double all = base;
-    for (int i = warp; i < kWarps; ++i) all += sh.part[i];
-    if (v > 0.0 && base + s >= want) atomicMin(&sh.bin, bin);
+    double base = sh.part[lane & (kWarps - 1)];  // the warps' totals, added up over 16 lanes
+#pragma unroll
+    for (int m = 1; m < kWarps; m <<= 1) {
+      const double o = __shfl_up_sync(0xFFFFFFFFu, base, m);
+      if ((lane & (kWarps - 1)) >= m) base += o;
+    }
+    const double all = over + __shfl_sync(0xFFFFFFFFu, base, kWarps - 1);
+    base = __shfl_sync(0xFFFFFFFFu, base, max(warp - 1, 0));
+    base = warp ? over + base : over;
+    if (v > 0.0 && base + s >= need) atomicMin(&sh.bin, bin);
     __syncthreads();
     if (last && sh.bin == kBins) {  // the sums' last bits
       __syncthreads();
@@ -284,9 +291,8 @@ struct Row {
     }
     const int b = sh.bin;
     if (bin == b) sh.found[0] = base + (s - v), sh.found[1] = v;
-    if (bin == 0) sh.found[2] = all;
     __syncthreads();
-    over = b < kBins ? sh.found[0] : sh.found[2];
+    over = b < kBins ? sh.found[0] : all;
     own = b < kBins ? sh.found[1] : 0.0;
     return b;
   }
@@ -296,30 +302,26 @@ struct Row {
   static constexpr int kWindows = (int)(kTop + kBins - 1 - (0x00800000u >> 18)) / kBins + 1;
   static __device__ __forceinline__ int bin_of(uint32_t u, int window) { return (int)(kTop - (u >> 18)) - window * kBins; }
 
-  template <bool MASS>
-  __device__ __forceinline__ void fill(int window, uint32_t from) {
-    clear();
-    each([&](int64_t, float4 q) {
-      const float v[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const uint32_t u = f2u(v[k]);
-        const int b = bin_of(u, window);
-        if (b >= 0 && b < kBins && u >= from) add<MASS>(b, u);
-      }
-    });
-  }
-
-  // The weight (its bits) at which counts or masses in descending order reach `want`; over: those above it, equals: how many
+  // The weight (its bits) at which counts or masses in descending order reach want(); over: those above it, equals: how many
   // have it. Weights below `from` do not count. false where all of them stay below. The first window's histogram is
   // there already where `filled`.
-  template <bool MASS>
-  __device__ bool cut(double want, uint32_t from, bool filled, uint32_t &weight, double &over, double &equals) {
+  template <bool MASS, typename Q>
+  __device__ bool cut(Q want, uint32_t from, bool filled, uint32_t &weight, double &over, double &equals) {
     over = 0.0;
     double own;
     int window = 0, b = kBins;
     for (; window < kWindows; ++window) {
-      if (window || !filled) fill<MASS>(window, from);
+      if (window || !filled) {
+        const uint32_t below = (uint32_t)max((int)kTop + 1 - (window + 1) * kBins, 0) << 18;  // the window's least
+        each(max(from, below), [&](int, uint4 q) {
+          const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int bin = bin_of(u[k], window);
+            if ((unsigned)bin < (unsigned)kBins && u[k] >= from) add<MASS>(bin, u[k]);
+          }
+        });
+      }
       b = reach<MASS>(want, over, own, false, [&](int bin) { return (int)((kTop - bin - window * kBins) >> 5) - 127; });
       if (b < kBins) break;
     }
@@ -328,14 +330,15 @@ struct Row {
     const int exponent = (int)(high >> 5) - 127;
 #pragma unroll 1
     for (int shift = 9; shift >= 0; shift -= 9) {
-      clear();
-      each([&](int64_t, float4 q) {
-        const float v[4] = {q.x, q.y, q.z, q.w};
+      each(high << (shift + 9), [&](int, uint4 q) {
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+        bool hit = false;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint32_t u = f2u(v[k]);
-          if (u >> (shift + 9) == high && u >= from) add<MASS>(kBins - 1 - (int)((u >> shift) & (kBins - 1)), u);
-        }
+        for (int k = 0; k < 4; ++k) hit |= u[k] - (high << (shift + 9)) < 1u << (shift + 9);
+        if (hit)
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (u[k] >> (shift + 9) == high && u[k] >= from) add<MASS>(kBins - 1 - (int)((u[k] >> shift) & (kBins - 1)), u[k]);
       });
       b = reach<MASS>(want, over, own, true, [&](int) { return exponent; });
       high = (high << 9) | (uint32_t)(kBins - 1 - b);
@@ -345,40 +348,74 @@ struct Row {
     return true;
   }
 
-  // Of the `equals` tokens of a weight the first `want` are kept, larger logits first: the logit at which they end, and
-  // how many of that logit's tokens stay.
+  // Of the tokens of a weight the first `want` are kept, larger logits first: the logit at which they end, and how many of
+  // that logit's tokens stay.
   __device__ void cut_logits(uint32_t weight, int64_t want, float &logit, int64_t &quota) {
     double over = 0.0, own = 0.0;
     uint32_t high = 0;
 #pragma unroll 1
     for (int shift = 27; shift >= 0; shift -= 9) {  // 5, 9, 9 and 9 bits
-      clear();
-      each([&](int64_t i, float4 q) {
-        const float v[4] = {q.x, q.y, q.z, q.w};
+      each(weight, [&](int i, uint4 q) {
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (f2u(v[k]) == weight) {
+          if (u[k] == weight) {
             const uint32_t key = key_of(z.at(i + k));
             if (shift == 27 || key >> (shift + 9) == high) add<false>(kBins - 1 - (int)((key >> shift) & (kBins - 1)), 0u);
           }
       });
-      const int b = reach<false>((double)want, over, own, true, [](int) { return 0; });
+      const int b = reach<false>([&] { return (double)want; }, over, own, true, [](int) { return 0; });
       high = (high << 9) | (uint32_t)(kBins - 1 - b);
     }
     logit = u2f((high >> 31) ? high & 0x7FFFFFFFu : ~high);
     quota = want - (int64_t)over;
   }
 
+  // This thread's part of the weights above one.
   __device__ __forceinline__ double mass_above(uint32_t weight) {
     double s = 0.0;
-    each([&](int64_t, float4 q) {
-      const float v[4] = {q.x, q.y, q.z, q.w};
+    each(weight + 1, [&](int, uint4 q) {
+      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
       float t = 0.0f;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) t = __fadd_rn(t, f2u(v[k]) > weight ? v[k] : 0.0f);
+      for (int k = 0; k < 4; ++k) t = __fadd_rn(t, u[k] > weight ? u2f(u[k]) : 0.0f);
       s += (double)t;
     });
-    return cluster_sum(s);
+    return s;
+  }
+
+  // Weights in the logits' place, the chunks' largest, this thread's part of their sum, and the histogram that the first
+  // filter begins with (FIRST: 0 none, 1 counts, 2 masses).
+  template <int FIRST>
+  __device__ __forceinline__ double prepare() {
+    const int lane = threadIdx.x & 31;
+    double sum = 0.0;
+    chunks([&](int c, int at, int end) {
+      uint32_t top = 0u;
+      steps(at, end, [&](int i) {
+        float4 q;
+        if (HELD) {
+          q = *reinterpret_cast<const float4 *>(held + i);
+          q = make_float4(w(q.x), w(q.y), w(q.z), w(q.w));
+          *reinterpret_cast<float4 *>(held + i) = q;
+        } else {
+          q = four(i);
+        }
+        sum += (double)__fadd_rn(__fadd_rn(q.x, q.y), __fadd_rn(q.z, q.w));
+        const uint32_t u[4] = {f2u(q.x), f2u(q.y), f2u(q.z), f2u(q.w)};
+        top = max(max(max(u[0], u[1]), max(u[2], u[3])), top);
+        if (FIRST)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int b = bin_of(u[k], 0);
+            if (b < kBins) add<FIRST == 2>(b, u[k]);
+          }
+      });
+      top = warp_max(top);
+      if (lane == 0) sh.peak[c] = top;
+    });
+    __syncwarp();
+    return sum;
   }
 };
 
@@ -387,39 +424,52 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
   extern __shared__ __align__(16) unsigned char dynamic[];
   __shared__ Shared shared;
   Row<T, HELD> row(shared, reinterpret_cast<float *>(dynamic));
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = warp_number();
   const int blocks = row.blocks = a.blocks, rank = row.rank = (int)row.cluster.block_rank();
   const int64_t r = blockIdx.x / blocks;
+  int64_t origin;  // of position i the token is origin + i
   {
     const T *p = static_cast<const T *>(a.logits) + r * a.stride;
-    const int64_t skip = (int64_t)((uintptr_t)p % 16 / sizeof(T));
-    row.z.base = p - skip;
-    row.z.first = skip, row.z.end = skip + a.vocab;
-    row.z.lo = min(a.part * rank, (row.z.end + 7) / 8 * 8);
-    row.z.hi = min(row.z.lo + a.part, (row.z.end + 7) / 8 * 8);
-    row.n = row.z.hi - row.z.lo;
+    const int64_t skip = (int64_t)((uintptr_t)p % 16 / sizeof(T)), lo = (int64_t)a.part * rank, end = skip + a.vocab - lo;
+    row.z.p = p - skip + lo;
+    row.z.first = rank ? 0 : (int)skip;
+    row.z.end = (int)max(min((int64_t)a.part, end), (int64_t)0);
+    row.n = (row.z.end + 127) / 128 * 128;
+    // Chunks of 512 positions (their sums' reduction over the warp then costs little), longer ones where those are too many.
+    const int each = (row.n / 128 + kWarps - 1) / kWarps;
+    row.run = each * 128;
+    row.span = max(4, (each + kWarpChunks - 1) / kWarpChunks) * 128;
+    origin = lo - skip;
   }
   const Stretch<T> &z = row.z;
-  const int64_t n = row.n;
+  const int n = row.n;
   float *held = row.held;
-  const int64_t origin = z.lo - z.first;  // of position i the token is origin + i
+  shared.hist[0][0][threadIdx.x] = 0u, shared.hist[0][1][threadIdx.x] = 0u;  // added to after cluster_max's barriers
+  auto started = row.cluster.barrier_arrive();
 
-  // The logits, once, and the largest.
+  // The logits, once, and the largest. fp32 goes to shared memory without a detour, all of a thread's at once.
   float top = -INFINITY;
-  for (int64_t i = (int64_t)threadIdx.x * 8; i < n; i += kThreads * 8) {
-    float v[8];
-    row.logits8(i, v);
-    if (HELD) {
-      *reinterpret_cast<float4 *>(held + i) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4 *>(held + i + 4) = make_float4(v[4], v[5], v[6], v[7]);
-    }
-#pragma unroll
-    for (int k = 0; k < 8; ++k) top = max_nan(top, v[k]);
+  auto largest = [&](float4 v) { top = max_nan(top, max_nan(max_nan(v.x, v.y), max_nan(v.z, v.w))); };
+  const int run_begin = warp * row.run, run_end = min(run_begin + row.run, n);
+  if constexpr (HELD && sizeof(T) == 4) {
+    row.steps(run_begin, run_end, [&](int i) {
+      if (i >= z.first && i + 4 <= z.end) cp_async16(held + i, z.p + i);
+      else *reinterpret_cast<float4 *>(held + i) = z.load(i);
+    });
+    cp_async_wait_all();
+    row.steps(run_begin, run_end, [&](int i) { largest(*reinterpret_cast<const float4 *>(held + i)); });
+  } else {
+    row.steps(run_begin, run_end, [&](int i) {
+      const float4 v = z.load(i);
+      if (HELD) *reinterpret_cast<float4 *>(held + i) = v;
+      largest(v);
+    });
   }
+  row.cluster.barrier_wait(static_cast<decltype(started) &&>(started));  // blocks that have not begun have no shared memory to write to
   {
     // NaN above Inf above every number.
-    const double t = row.cluster_max(top != top ? DBL_MAX : top == INFINITY ? (double)FLT_MAX * 2.0 : top == -INFINITY ? -DBL_MAX : (double)top);
-    top = t == DBL_MAX ? u2f(kQNaN) : t > (double)FLT_MAX ? INFINITY : t == -DBL_MAX ? -INFINITY : (float)t;
+    const uint32_t t = row.cluster_max(top != top ? 0xFFFFFFFFu : key_of(top));
+    top = t == 0xFFFFFFFFu ? u2f(kQNaN) : u2f((t >> 31) ? t & 0x7FFFFFFFu : ~t);
   }
   const float heat = a.temperature ? a.temperature[r] : a.all_temperature;
   auto answer = [&](int64_t token, float logprob) {
@@ -429,65 +479,42 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
   if (!(top > -INFINITY)) {
     if (rank == 0 && threadIdx.x == 0) answer(-1, top);
   } else if (!(heat > 0.0f)) {
-    double at = -DBL_MAX;  // the negated first index
-    for (int64_t i = (int64_t)threadIdx.x * 8; i < n && at == -DBL_MAX; i += kThreads * 8) {
-      float v[8];
-      if (HELD) {
-        const float4 x = *reinterpret_cast<const float4 *>(held + i), y = *reinterpret_cast<const float4 *>(held + i + 4);
-        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-      } else {
-        row.logits8(i, v);
-      }
-#pragma unroll
-      for (int k = 7; k >= 0; --k)
-        if (v[k] == top) at = -(double)(origin + i + k);
-    }
+    uint32_t at = 0u;  // the first index, from the end
+    row.steps(run_begin, run_end, [&](int i) {
+      const float4 v = HELD ? *reinterpret_cast<const float4 *>(held + i) : z.load(i);
+      const int k = v.x == top ? 0 : v.y == top ? 1 : v.z == top ? 2 : v.w == top ? 3 : -1;
+      if (k >= 0 && !at) at = 0xFFFFFFFFu - (uint32_t)(origin + i + k);
+    });
     at = row.cluster_max(at);
-    if (rank == 0 && threadIdx.x == 0) answer((int64_t)-at, 0.0f);
+    if (rank == 0 && threadIdx.x == 0) answer((int64_t)(0xFFFFFFFFu - at), 0.0f);
   } else {
     row.infinite = top == INFINITY;
     row.w.set(row.infinite ? 0.0f : top, heat);
-    const Weight w = row.w;
     if (HELD && row.infinite)
-      for (int64_t i = threadIdx.x * 4; i < n; i += kThreads * 4)
-        for (int64_t e = i; e < i + 4; ++e) held[e] = held[e] == INFINITY ? 0.0f : -INFINITY;
+      row.steps(run_begin, run_end, [&](int i) {
+        for (int e = i; e < i + 4; ++e) held[e] = Row<T, HELD>::finite(held[e]);
+      });
     const int64_t k = a.top_k ? a.top_k[r] : a.all_top_k;
     const float p = a.top_p ? a.top_p[r] : a.all_top_p, low = a.min_p ? a.min_p[r] : a.all_min_p;
     const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.0f;
-    // Weights in the logits' place, their sum, and the histogram that the first filter begins with.
-    row.clear();
-    double sum = 0.0;
-    for (int64_t i = (int64_t)threadIdx.x * 4; i < n; i += kThreads * 4) {
-      float4 q;
-      if (HELD) {
-        q = *reinterpret_cast<const float4 *>(held + i);
-        q = make_float4(w(q.x), w(q.y), w(q.z), w(q.w));
-        *reinterpret_cast<float4 *>(held + i) = q;
-      } else {
-        q = row.four(i);
-      }
-      sum += (double)__fadd_rn(__fadd_rn(q.x, q.y), __fadd_rn(q.z, q.w));
-      if (by_count || by_mass) {
-        const float v[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t u = f2u(v[e]);
-          const int b = Row<T, HELD>::bin_of(u, 0);
-          if (b < kBins) by_count ? row.template add<false>(b, u) : row.template add<true>(b, u);
-        }
-      }
-    }
+    double sum = by_count ? row.template prepare<1>() : by_mass ? row.template prepare<2>() : row.template prepare<0>();
     // Kept: weights above `cut`, and of the tokens at it the first m.
     uint32_t cut = 0;
     double m = 0.0, equals = 0.0, over;
-    if (by_count && row.template cut<false>((double)k, 1u, true, cut, over, equals)) m = (double)k - over;
+    if (by_count && row.template cut<false>([&] { return (double)k; }, 1u, true, cut, over, equals)) m = (double)k - over;
     if (by_mass) {
-      if (!by_count) sum = row.cluster_sum(sum);
-      else sum = row.mass_above(cut) + m * (double)u2f(cut);
+      if (by_count) sum = row.mass_above(cut);
+      const double *all = row.tell(row.block_sum(sum));
+      double aim = 0.0;
+      bool summed = false;
+      auto want = [&] {  // after the next barrier
+        if (!summed) aim = (double)p * (row.all_of(all) + m * (double)u2f(cut)), summed = true;
+        return aim;
+      };
       uint32_t c;
       double e;
-      if (row.template cut<true>((double)p * sum, max(cut, 1u), !by_count, c, over, e)) {
-        const double need = fmin(fmax(ceil(((double)p * sum - over) / (double)u2f(c)), 1.0), e);
+      if (row.template cut<true>(want, max(cut, 1u), !by_count, c, over, e)) {
+        const double need = fmin(fmax(ceil((aim - over) / (double)u2f(c)), 1.0), e);
         m = c == cut ? fmin(need, m) : need;
         cut = c, equals = e;
       }
@@ -503,66 +530,82 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
     float tie = 0.0f;
     int64_t quota = 0;
     if (some) row.cut_logits(cut, (int64_t)m, tie, quota);
-    auto equal = [&](int64_t i, float v, bool &above) {  // the tie's own, or one whose logit is above it
-      if (f2u(v) != cut) return false;
+    auto equal = [&](int i, uint32_t u, bool &above) {  // the tie's own, or one whose logit is above it
+      if (u != cut) return false;
       const float l = z.at(i);
       above = l > tie;
       return l == tie;
     };
 
-    // Masses and ties by chunks of consecutive positions, a warp a chunk.
-    const int64_t span = ((n + kChunks - 1) / kChunks + 127) / 128 * 128;
+    // Masses and ties by chunks.
     double ties = 0.0;
-    for (int c = warp; c < kChunks; c += kWarps) {
+    row.chunks([&](int c, int at, int end) {
       double s = 0.0;
       int e = 0;
-      for (int64_t i = c * span + lane * 4; i < min((c + 1) * span, n); i += 128) {
-        const float4 q = row.four(i);
-        const float v[4] = {q.x, q.y, q.z, q.w};
-        float t = 0.0f;
+      const uint32_t peak = shared.peak[c];
+      if (!some && peak > cut) {
+        row.steps(at, end, [&](int i) {
+          const float4 q = row.four(i);
+          auto kept = [&](float v) { return f2u(v) > cut ? v : 0.0f; };
+          s += (double)__fadd_rn(__fadd_rn(kept(q.x), kept(q.y)), __fadd_rn(kept(q.z), kept(q.w)));
+        });
+      } else if (some && peak >= cut) {
+        for (; at < end; at += 128) {
+          const int i = at + lane * 4;
+          const float4 q = row.four(i);
+          const float v[4] = {q.x, q.y, q.z, q.w};
+          float t[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          bool keep = f2u(v[x]) > cut;
-          if (some && !keep) e += equal(i + x, v[x], keep);
-          t = __fadd_rn(t, keep ? v[x] : 0.0f);
+          for (int x = 0; x < 4; ++x) {
+            bool keep = f2u(v[x]) > cut;
+            if (!keep) e += equal(i + x, f2u(v[x]), keep);
+            t[x] = keep ? v[x] : 0.0f;
+          }
+          s += (double)__fadd_rn(__fadd_rn(t[0], t[1]), __fadd_rn(t[2], t[3]));
         }
-        s += (double)t;
+        e = (int)__reduce_add_sync(0xFFFFFFFFu, e);
       }
+      if (peak > cut || (some && peak == cut)) {
 #pragma unroll
-      for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
-      if (some) e = (int)__reduce_add_sync(0xFFFFFFFFu, e);
+        for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
+      }
       if (lane == 0) shared.mass[c] = s, shared.ties[c] = e, ties += e;
-    }
+    });
     int64_t left = 0;  // ties that this block may keep
     if (some) {
       const double *all = row.tell(row.block_sum(ties));
+      row.cluster.sync();
       left = quota;
       for (int i = 0; i < rank; ++i) left -= (int64_t)all[i];
       left = max(left, (int64_t)0);
     }
     __syncthreads();
-    // Chunks in order, eight a lane of the first warp: ties that are left, and the mass before each.
+    // Chunks in order, four a lane of the first warp: ties that are left, and the mass before each.
     constexpr int kLane = kChunks / 32;
-    double own = 0.0, before = 0.0;
+    double before = 0.0;
     if (warp == 0) {
-      int64_t mine = 0;
+      double own = 0.0;
+      if (some) {
+        int64_t mine = 0;
 #pragma unroll
-      for (int c = 0; c < kLane; ++c) mine += shared.ties[lane * kLane + c];
-      int64_t upto = mine;
+        for (int c = 0; c < kLane; ++c) mine += shared.ties[lane * kLane + c];
+        int64_t upto = mine;
 #pragma unroll
-      for (int x = 1; x < 32; x <<= 1) {
-        const int64_t o = __shfl_up_sync(0xFFFFFFFFu, upto, x);
-        if (lane >= x) upto += o;
+        for (int x = 1; x < 32; x <<= 1) {
+          const int64_t o = __shfl_up_sync(0xFFFFFFFFu, upto, x);
+          if (lane >= x) upto += o;
+        }
+        int64_t room = max(left - (upto - mine), (int64_t)0);
+#pragma unroll
+        for (int c = 0; c < kLane; ++c) {
+          const int64_t take = min((int64_t)shared.ties[lane * kLane + c], room);
+          shared.ties[lane * kLane + c] = (int)take;
+          room -= take;
+          shared.mass[lane * kLane + c] += (double)take * (double)u2f(cut);
+        }
       }
-      int64_t room = max(left - (upto - mine), (int64_t)0);
 #pragma unroll
-      for (int c = 0; c < kLane; ++c) {
-        const int64_t take = min((int64_t)shared.ties[lane * kLane + c], room);
-        shared.ties[lane * kLane + c] = (int)take;
-        room -= take;
-        shared.mass[lane * kLane + c] += (double)take * (double)u2f(cut);
-        own += shared.mass[lane * kLane + c];
-      }
+      for (int c = 0; c < kLane; ++c) own += shared.mass[lane * kLane + c];
       before = own;
 #pragma unroll
       for (int x = 1; x < 32; x <<= 1) {
@@ -575,11 +618,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
     }
     __syncthreads();
     const double *all = row.tell(shared.found[0]);
+    row.cluster.sync();
+    if (warp) return;
     // The block whose stretch the aim falls in; behind all of them (u = 1, or the last bits of the sums) the last one that
     // keeps anything.
-    double total = 0.0;
-    for (int i = 0; i < blocks; ++i) total += all[i];
-    const double aim = fmax((double)a.uniform[r] * total, 0.0);
+    const double total = row.all_of(all), aim = fmax((double)a.uniform[r] * total, 0.0);
     int owner = -1;
     double start = 0.0, at = 0.0;
     for (int i = 0; i < blocks; ++i) {
@@ -587,7 +630,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
       at += all[i];
       if (all[i] > 0.0 && at > aim) break;
     }
-    if (rank == owner && warp == 0) {
+    if (rank == owner) {
       // Its chunk, likewise.
       const double rest = aim - start;
       int chunk = -1;
@@ -603,19 +646,17 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
       const int source = hit ? __ffs(hit) - 1 : 31 - __clz(any);
       chunk = __shfl_sync(0xFFFFFFFFu, chunk, source);
       double need = rest - __shfl_sync(0xFFFFFFFFu, chunk_start, source);
-      int64_t room = shared.ties[chunk], found = -1, kept = -1;
+      int room = shared.ties[chunk], found = -1, kept = -1;
       // Its tokens, 32 at a time.
-      for (int64_t i0 = chunk * span; found < 0 && i0 < min((chunk + 1) * span, n); i0 += 32) {
-        const int64_t i = i0 + lane;
-        const bool real = i < n;
-        float4 q = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (real) q = row.four(i & ~(int64_t)3);
-        const float v = real ? ((i & 2) ? ((i & 1) ? q.w : q.z) : (i & 1) ? q.y : q.x) : 0.0f;
+      for (int i0 = row.begin_of(chunk); found < 0 && i0 < row.end_of(chunk); i0 += 32) {
+        const int i = i0 + lane;
+        const float4 q = row.four(i & ~3);
+        const float v = (i & 2) ? ((i & 1) ? q.w : q.z) : (i & 1) ? q.y : q.x;
         bool keep = f2u(v) > cut, mine = false;
-        if (some && !keep) mine = equal(i, v, keep);
+        if (some && !keep) mine = equal(i, f2u(v), keep);
         const unsigned same = __ballot_sync(0xFFFFFFFFu, mine);
         if (mine) keep = __popc(same & ((1u << lane) - 1u)) < room;
-        room = max(room - __popc(same), (int64_t)0);
+        room = max(room - __popc(same), 0);
         const unsigned mask = __ballot_sync(0xFFFFFFFFu, keep);
         double x = keep ? (double)v : 0.0;
 #pragma unroll
@@ -629,10 +670,11 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
         need -= __shfl_sync(0xFFFFFFFFu, x, 31);
       }
       if (found < 0) found = kept;
-      if (lane == 0) answer(origin + found, (float)((row.infinite ? 0.0 : w.log(z.at(found))) - log(total)));
+      if (lane == 0) answer(origin + found, (float)((row.infinite ? 0.0 : row.w.log(z.at(found))) - log(total)));
     }
   }
-  row.cluster.sync();  // the other blocks may still read this one's shared memory
+  // The last barrier before this line comes after every block's last look at another one's shared memory, except where blocks tell
+  // each other numbers: those are written before it.
 }
 
 }  // namespace sample
