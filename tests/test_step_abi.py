@@ -19,7 +19,7 @@ BAD = N.TC_INVALID_ARGUMENT
 
 def test_plan_arguments_are_checked():
     lib = N.lib()
-    assert lib.tc_plan_pages_workspace(-1) == 0 and lib.tc_plan_pages_workspace(3) >= 24
+    assert lib.tc_plan_pages_workspace(-1) == 0 and lib.tc_plan_pages_workspace(3000) >= 24000
 
     def call(lens=P, new=P, batch=3, table=P, stride=4, width=4, free=P, nfree=8, taken=P, page=16, tokens=5, out=P, cu=P,
              slots=P, seq=P, pos=P, top=P, missing=P, ws=P, nbytes=1 << 12):
@@ -32,7 +32,7 @@ def test_plan_arguments_are_checked():
                dict(tokens=1 << 31), dict(nfree=1 << 31), dict(width=1 << 27, stride=1 << 27)):
         assert call(**kw) == BAD, kw
         assert b"tc_plan_pages" in lib.tc_last_error()
-    assert call(ws=None) == N.TC_WORKSPACE_TOO_SMALL and call(nbytes=8) == N.TC_WORKSPACE_TOO_SMALL
+    assert call(batch=3000, ws=None) == N.TC_WORKSPACE_TOO_SMALL and call(batch=3000, nbytes=8) == N.TC_WORKSPACE_TOO_SMALL
 
 
 def test_release_arguments_are_checked():

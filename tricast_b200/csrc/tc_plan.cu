@@ -86,44 +86,94 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(Args a) {
     const int64_t out = min(pages, a.num_free);
     *a.out_taken = (int32_t)out;
     *a.missing = (int32_t)min(pages - out + none, (int64_t)INT32_MAX);
-    if (a.batch == 0) a.cu[0] = 0;
   }
 }
 
-// Tokens by threads, new table entries by warps.
+// What a new token of sequence i gets: its slot, where its page is one of the row's or a new one.
+__device__ __forceinline__ int64_t slot_of(const Args &a, int i, int64_t len, int64_t first, int64_t p) {
+  const int64_t column = p >> a.shift, used = used_pages(a, len), at = first + column - used;
+  int32_t page = -1;
+  if (column < used && column < a.width) page = a.table[i * a.table_stride + column];
+  else if (column < a.width && at < a.num_free) page = a.free_pages[at];
+  return page < 0 ? -1 : ((int64_t)page << a.shift) + (p & ((1ll << a.shift) - 1));
+}
+__device__ __forceinline__ void fill_row(const Args &a, int64_t i, int64_t len, int64_t n, int64_t first) {
+  const int64_t used = used_pages(a, len), need = new_pages(a, len, n);
+  for (int64_t j = threadIdx.x & 31; j < need; j += 32) {
+    const int64_t at = first + j;
+    a.table[i * a.table_stride + used + j] = at < a.num_free ? a.free_pages[at] : -1;
+  }
+}
+__device__ __forceinline__ void no_token(const Args &a, int64_t t) { a.slots[t] = -1, a.sequence[t] = -1, a.positions[t] = -1; }
+
+// Many sequences, after scan_kernel: tokens by threads, which look their sequence up, new table entries by warps.
 __global__ void __launch_bounds__(256) fill_kernel(Args a) {
   const int64_t thread = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, threads = (int64_t)gridDim.x * blockDim.x;
-  const int64_t real = a.batch ? a.cu[a.batch] : 0;
+  const int64_t real = a.cu[a.batch];
   for (int64_t t = thread; t < a.tokens; t += threads) {
-    int64_t slot = -1;
-    int32_t seq = -1, pos = -1;
-    if (t < real) {
-      int lo = 0, hi = a.batch - 1;  // the last sequence that starts at t or before and is not empty: the first whose end is behind t
-      while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu[mid + 1] > t) hi = mid;
-        else lo = mid + 1;
-      }
-      const int64_t len = max(a.lens[lo], 0), p = len + t - a.cu[lo], column = p >> a.shift, used = used_pages(a, len);
-      const int64_t at = a.first[lo] + column - used;
-      int32_t page = -1;
-      if (column < used && column < a.width) page = a.table[lo * a.table_stride + column];
-      else if (column < a.width && at < a.num_free) page = a.free_pages[at];
-      if (page >= 0) slot = ((int64_t)page << a.shift) + (p & ((1ll << a.shift) - 1));
-      seq = lo;
-      pos = (int32_t)p;
+    if (t >= real) {
+      no_token(a, t);
+      continue;
     }
-    a.slots[t] = slot;
-    a.sequence[t] = seq;
-    a.positions[t] = pos;
+    int lo = 0, hi = a.batch - 1;  // the first sequence whose end is behind t
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (a.cu[mid + 1] > t) hi = mid;
+      else lo = mid + 1;
+    }
+    const int64_t len = max(a.lens[lo], 0), p = len + t - a.cu[lo];
+    a.slots[t] = slot_of(a, lo, len, a.first[lo], p);
+    a.sequence[t] = lo;
+    a.positions[t] = (int32_t)p;
   }
-  for (int64_t i = thread >> 5; i < a.batch; i += threads >> 5) {
-    const int64_t len = max(a.lens[i], 0), n = a.cu[i + 1] - a.cu[i], used = used_pages(a, len), need = new_pages(a, len, n);
-    for (int64_t j = threadIdx.x & 31; j < need; j += 32) {
-      const int64_t at = a.first[i] + j;
-      a.table[i * a.table_stride + used + j] = at < a.num_free ? a.free_pages[at] : -1;
+  for (int64_t i = thread >> 5; i < a.batch; i += threads >> 5)
+    fill_row(a, i, max(a.lens[i], 0), a.cu[i + 1] - a.cu[i], a.first[i]);
+}
+
+// Up to kThreads sequences in one kernel: every block adds the lengths up itself (a thread a sequence, some 2 us, which a kernel of its own
+// and the launch after it would cost too), keeps the sums in shared memory and fills its share of the tokens and rows.
+__global__ void __launch_bounds__(kThreads) plan_kernel(Args a) {
+  __shared__ int64_t part[kThreads / 32];
+  __shared__ int32_t start[kThreads + 1], length[kThreads];
+  __shared__ int64_t first[kThreads];
+  const int i = threadIdx.x;
+  const bool real = i < a.batch;
+  const int64_t len = real ? max(a.lens[i], 0) : 0, want = real ? max(a.fresh[i], 0) : 0;
+  int64_t total, pages, beyond;
+  const int64_t at = min(block_prefix(want, part, total), a.tokens), n = min(want, a.tokens - at);
+  const int64_t need = real ? new_pages(a, len, n) : 0, taken = taken_at_start(a);
+  first[i] = taken + block_prefix(need, part, pages);
+  start[i] = (int32_t)at, length[i] = (int32_t)len;
+  if (i == kThreads - 1) start[kThreads] = (int32_t)(at + n);
+  if (blockIdx.x == 0) {
+    block_prefix(used_pages(a, len + n) - used_pages(a, len) - need, part, beyond);
+    if (real) a.cu[i] = (int32_t)at, a.out_lens[i] = (int32_t)(len + n);
+    if (i == 0) {
+      const int64_t out = min(taken + pages, a.num_free);
+      *a.out_taken = (int32_t)out;
+      *a.missing = (int32_t)min(taken + pages - out + beyond, (int64_t)INT32_MAX);
     }
   }
+  __syncthreads();
+  const int32_t end = start[kThreads];  // behind the batch's sequences every start is the end
+  if (blockIdx.x == 0 && i == 0) a.cu[a.batch] = end;
+  const int64_t threads = (int64_t)gridDim.x * kThreads, thread = (int64_t)blockIdx.x * kThreads + i;
+  for (int64_t t = thread; t < a.tokens; t += threads) {
+    if (t >= end) {
+      no_token(a, t);
+      continue;
+    }
+    int lo = 0;  // the last sequence that begins at t or before: an empty one begins where the next one does
+#pragma unroll
+    for (int step = kThreads / 2; step; step >>= 1)
+      if (start[lo + step] <= t) lo += step;
+    const int64_t l = length[lo], p = l + t - start[lo];
+    a.slots[t] = slot_of(a, lo, l, first[lo], p);
+    a.sequence[t] = lo;
+    a.positions[t] = (int32_t)p;
+  }
+  for (int64_t row = thread >> 5; row < a.batch; row += threads >> 5)
+    fill_row(a, row, length[row], start[row + 1] - start[row], first[row]);
 }
 
 struct Release {
@@ -199,7 +249,7 @@ static int plan_status(const char *what) {
   return TC_OK;
 }
 
-extern "C" size_t tc_plan_pages_workspace(int32_t batch) { return batch > 0 ? (size_t)batch * sizeof(int64_t) : 0; }
+extern "C" size_t tc_plan_pages_workspace(int32_t batch) { return batch > plan::kThreads ? (size_t)batch * sizeof(int64_t) : 0; }
 
 extern "C" int tc_plan_pages(const int32_t *seq_lens, const int32_t *new_lens, int32_t batch, int32_t *block_table,
                              int64_t table_stride, int32_t max_pages, const int32_t *free_pages, int64_t num_free,
@@ -215,16 +265,21 @@ extern "C" int tc_plan_pages(const int32_t *seq_lens, const int32_t *new_lens, i
   if ((batch && (!seq_lens || !new_lens || !out_lens)) || (batch && max_pages && !block_table) || (num_free && !free_pages) ||
       !taken || !cu_q || !out_taken || !missing || (tokens && (!slots || !sequence || !positions)))
     return bad("null pointer");
-  if (batch && (!workspace || workspace_bytes < tc_plan_pages_workspace(batch)))
+  if (batch > plan::kThreads && (!workspace || workspace_bytes < tc_plan_pages_workspace(batch)))
     return set_error("tc_plan_pages: workspace too small"), TC_WORKSPACE_TOO_SMALL;
   plan::Args a{seq_lens, new_lens, block_table, table_stride, free_pages, num_free, taken, tokens, batch, max_pages, 0,
                out_lens, cu_q, sequence, positions, out_taken, missing, slots, static_cast<int64_t *>(workspace)};
   while ((1 << a.shift) < page_size) ++a.shift;
   cudaStream_t s = (cudaStream_t)stream;
+  if (batch <= plan::kThreads) {
+    const int64_t work = tokens > (int64_t)batch * 32 ? tokens : (int64_t)batch * 32, blocks = (work + plan::kThreads - 1) / plan::kThreads;
+    const int64_t most = sm_count();
+    plan::plan_kernel<<<(unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most), plan::kThreads, 0, s>>>(a);
+    return plan_status("tc_plan_pages");
+  }
   plan::scan_kernel<<<1, plan::kThreads, 0, s>>>(a);
   if (const int st = plan_status("tc_plan_pages")) return st;
   const int64_t work = tokens > (int64_t)batch * 32 ? tokens : (int64_t)batch * 32;
-  if (work == 0) return TC_OK;
   const int64_t blocks = (work + 255) / 256, most = (int64_t)sm_count() * 8;
   plan::fill_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, s>>>(a);
   return plan_status("tc_plan_pages");

@@ -7,7 +7,7 @@ namespace tc {
 namespace sample {
 
 constexpr int64_t kMaxVocab = 1 << 23;  // histograms add 12-bit parts of 2**20 weights a block in 32 bits
-constexpr int64_t kMaxHeld = 54272;     // weights that a block's shared memory holds beside the rest
+constexpr int64_t kMaxHeld = 53248;     // weights that a block's shared memory holds beside the rest
 
 template <typename T, bool HELD>
 static cudaError_t launch_as(const Args &a, cudaStream_t s) {
@@ -32,7 +32,7 @@ template <typename T>
 static cudaError_t launch(Args a, cudaStream_t s) {
   // Stretches short enough for two blocks an SM, and more of them while the card is not full and they stay long enough to be worth it.
   a.blocks = 1;
-  while (a.blocks < 8 && (a.vocab > 24576 * (int64_t)a.blocks ||
+  while (a.blocks < 8 && (a.vocab > 23552 * (int64_t)a.blocks ||
                           (a.rows * a.blocks < 2 * sm_count() && a.vocab > 4096 * (int64_t)a.blocks)))
     a.blocks *= 2;
   a.part = (int)(((a.vocab + 8 + a.blocks - 1) / a.blocks + 127) / 128 * 128);  // positions begin up to 7 elements before the row

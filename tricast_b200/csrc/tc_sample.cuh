@@ -24,6 +24,7 @@ namespace sample {
 namespace cg = cooperative_groups;
 
 constexpr int kThreads = 512, kWarps = kThreads / 32, kBins = 512, kMaxBlocks = 8;
+constexpr int kList = 512;  // tokens that one block finishes alone
 constexpr int kWarpChunks = 8, kChunks = kWarps * kWarpChunks;  // a stretch is cut into runs of a warp, these into chunks
 static_assert(kBins == kThreads, "a thread a bin");
 
@@ -42,14 +43,17 @@ struct Args {
 };
 
 struct Shared {
-  uint32_t hist[2][2][kBins];         // by turns (others may still read the last one): lower and upper parts, or counts
-  double slots[2][kMaxBlocks];        // by turns: what each block of the cluster has sent
+  uint2 hist[2][kBins];               // by turns (others may still read the last one): lower and upper parts, or counts
+  double slots[2][kMaxBlocks][3];     // by turns: what each block of the cluster has sent
   double part[kWarps];
   uint32_t tops[kWarps];
   uint32_t peak[kChunks];             // of each chunk, the largest weight's bits
   double mass[kChunks];
   int ties[kChunks];
-  double found[3];                    // of a histogram's scan
+  double found[2];                    // of a histogram's scan
+  uint64_t shares[kMaxBlocks];        // what each block has in the bin that was found
+  uint64_t list[kList];               // the first block's: logits of the cluster and where they stand, largest first
+  int listed, mine, base;
   int bin;
 };
 
@@ -142,11 +146,12 @@ struct Row {
   float *held;
   int n, run, span;  // positions of the stretch, of a warp and of a chunk, multiples of 128
   int blocks, rank, turn, hist_turn;
+  bool exact;     // whether cut() added masses last
   bool infinite;  // the row's largest logit is: its equals share everything, as logits of 0 beside -Inf
   cg::cluster_group cluster;
 
   __device__ __forceinline__ Row(Shared &s, float *h)
-      : sh(s), held(h), turn(0), hist_turn(0), infinite(false), cluster(cg::this_cluster()) {}
+      : sh(s), held(h), turn(0), hist_turn(0), exact(false), infinite(false), cluster(cg::this_cluster()) {}
 
   static __device__ __forceinline__ float finite(float l) { return l == INFINITY ? 0.0f : -INFINITY; }
   __device__ __forceinline__ float4 weigh(float4 l) const {
@@ -190,11 +195,32 @@ struct Row {
   __device__ __forceinline__ int begin_of(int c) const { return c / kWarpChunks * run + c % kWarpChunks * span; }
   __device__ __forceinline__ int end_of(int c) const { return min(begin_of(c) + span, min((c / kWarpChunks + 1) * run, n)); }
 
-  // A number from each block to all of them, to be read after the cluster's next barrier. Two turns apart the slots are used again,
-  // and between them lies a barrier that a block reaches only after reading.
-  __device__ __forceinline__ const double *tell(double v) {
-    double *to = sh.slots[turn];
-    if ((int)threadIdx.x < blocks) cluster.map_shared_rank(to, threadIdx.x)[rank] = v;
+  // The cluster's barrier: what its threads wrote before is seen by those that read after.
+  static __device__ __forceinline__ void meet() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
+  // Another block's word (both of them where MASS) at an address of this one's shared memory.
+  template <bool MASS>
+  static __device__ __forceinline__ uint2 look(uint32_t here, int block) {
+    uint2 v = make_uint2(0u, 0u);
+    if (MASS)
+      asm volatile("{\n.reg .u32 a;\nmapa.shared::cluster.u32 a, %2, %3;\nld.shared::cluster.v2.u32 {%0, %1}, [a];\n}"
+                   : "=r"(v.x), "=r"(v.y)
+                   : "r"(here), "r"(block)
+                   : "memory");
+    else
+      asm volatile("{\n.reg .u32 a;\nmapa.shared::cluster.u32 a, %1, %2;\nld.shared::cluster.u32 %0, [a];\n}" : "=r"(v.x) : "r"(here), "r"(block) : "memory");
+    return v;
+  }
+  // Up to three numbers from each block to all of them, to be read after the cluster's next barrier. Two turns apart the slots are
+  // used again, and between them lies a barrier that a block reaches only after reading.
+  using Slot = const double (*)[3];
+  __device__ __forceinline__ Slot tell(double v, double x = 0.0, double y = 0.0) {
+    double (*to)[3] = sh.slots[turn];
+    if ((int)threadIdx.x < blocks) {
+      double *there = cluster.map_shared_rank(&to[rank][0], threadIdx.x);
+      there[0] = v, there[1] = x, there[2] = y;
+    }
     turn ^= 1;
     return to;
   }
@@ -210,36 +236,42 @@ struct Row {
     for (int m = kWarps / 2; m; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
     return v;
   }
-  __device__ __forceinline__ double all_of(const double *slots) const {
+  __device__ __forceinline__ double all_of(Slot slots) const {
     const int lane = threadIdx.x & (kMaxBlocks - 1);
-    double v = lane < blocks ? slots[lane] : 0.0;
+    double v = lane < blocks ? slots[lane][0] : 0.0;
 #pragma unroll
     for (int m = kMaxBlocks / 2; m; m >>= 1) v += __shfl_xor_sync(0xFFFFFFFFu, v, m);
     return v;
   }
-  // The largest of a key a thread, over the cluster.
-  __device__ __forceinline__ uint32_t cluster_max(uint32_t v) {
+  // The largest of a key a thread: in every thread of the block, or of the cluster.
+  __device__ __forceinline__ uint32_t block_max(uint32_t v) {
     v = warp_max(v);
     __syncthreads();
     if ((threadIdx.x & 31) == 0) sh.tops[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = warp_max(sh.tops[threadIdx.x & (kWarps - 1)]);
-    const double *all = tell((double)v);
-    cluster.sync();
+    return warp_max(sh.tops[threadIdx.x & (kWarps - 1)]);
+  }
+  __device__ __forceinline__ uint32_t largest_told(Slot all, int which) const {
     const int lane = threadIdx.x & (kMaxBlocks - 1);
-    return warp_max(lane < blocks ? (uint32_t)all[lane] : 0u);
+    return warp_max(lane < blocks ? (uint32_t)all[lane][which] : 0u);
+  }
+  __device__ __forceinline__ uint32_t cluster_max(uint32_t v) {
+    Slot all = tell((double)block_max(v));
+    meet();
+    return largest_told(all, 0);
   }
 
   // Adds a weight's bits to its bin: its count, or its 24-bit significand in parts of 12 bits (a stretch has at most 2**20
   // positions, so neither sum passes 32 bits).
   template <bool MASS>
-  __device__ __forceinline__ void add(int bin, uint32_t u) {
-    uint32_t (*h)[kBins] = sh.hist[hist_turn];
+  __device__ __forceinline__ void add(int bin, uint32_t u, bool yes) const {
+    if (!yes) return;
+    uint2 *to = &sh.hist[hist_turn][bin];
     if (MASS) {
-      atomicAdd(&h[0][bin], u & 0xFFFu);
-      atomicAdd(&h[1][bin], ((u >> 12) & 0x7FFu) | 0x800u);
+      atomicAdd(&to->x, u & 0xFFFu);
+      atomicAdd(&to->y, ((u >> 12) & 0x7FFu) | 0x800u);
     } else {
-      atomicAdd(&h[0][bin], 1u);
+      atomicAdd(&to->x, 1u);
     }
   }
   // The first bin at which counts or masses of the cluster, on top of `over`, reach want(), kBins where none does (then, with
@@ -247,21 +279,23 @@ struct Row {
   // next histogram, which every block has read, is cleared.
   template <bool MASS, typename Q, typename X>
   __device__ __forceinline__ int reach(Q want, double &over, double &own, bool last, X exponent) {
-    cluster.sync();
+    meet();
     const int bin = threadIdx.x, lane = bin & 31, warp = warp_number();
     const double need = want();
     double v;
-    {
-      uint64_t lo = 0, hi = 0;
-      for (int b = 0; b < blocks; ++b) {
-        lo += *cluster.map_shared_rank(&sh.hist[hist_turn][0][bin], b);
-        if (MASS) hi += *cluster.map_shared_rank(&sh.hist[hist_turn][1][bin], b);
-      }
-      v = (double)(lo + (hi << 12));
-      if (MASS) v *= __longlong_as_double((long long)(1023 + exponent(bin) - 23) << 52);
-    }
+    // All of them asked for before the first is used, and without a branch between them: a look at another block's shared memory
+    // takes some 700 cycles.
+    uint2 part[kMaxBlocks];
+    const uint32_t here = smem_addr(&sh.hist[hist_turn][bin]);
+#pragma unroll
+    for (int b = 0; b < kMaxBlocks; ++b) part[b] = look<MASS>(here, min(b, blocks - 1));
+    uint64_t sum = 0;
+#pragma unroll
+    for (int b = 0; b < kMaxBlocks; ++b) sum += b < blocks ? part[b].x + (MASS ? (uint64_t)part[b].y << 12 : 0) : 0;
+    v = (double)sum;
+    if (MASS) v *= __longlong_as_double((long long)(1023 + exponent(bin) - 23) << 52);
     hist_turn ^= 1;
-    sh.hist[hist_turn][0][bin] = 0u, sh.hist[hist_turn][1][bin] = 0u;
+    sh.hist[hist_turn][bin] = make_uint2(0u, 0u);
     double s = v;
 #pragma unroll
     for (int m = 1; m < 32; m <<= 1) {
@@ -290,7 +324,11 @@ struct Row {
       __syncthreads();
     }
     const int b = sh.bin;
-    if (bin == b) sh.found[0] = base + (s - v), sh.found[1] = v;
+    if (bin == b) {
+      sh.found[0] = base + (s - v), sh.found[1] = v;
+#pragma unroll
+      for (int i = 0; i < kMaxBlocks; ++i) sh.shares[i] = part[i].x + (MASS ? (uint64_t)part[i].y << 12 : 0);
+    }
     __syncthreads();
     over = b < kBins ? sh.found[0] : all;
     own = b < kBins ? sh.found[1] : 0.0;
@@ -318,7 +356,7 @@ struct Row {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int bin = bin_of(u[k], window);
-            if ((unsigned)bin < (unsigned)kBins && u[k] >= from) add<MASS>(bin, u[k]);
+            add<MASS>(bin, u[k], (unsigned)bin < (unsigned)kBins && u[k] >= from);
           }
         });
       }
@@ -335,17 +373,156 @@ struct Row {
         bool hit = false;
 #pragma unroll
         for (int k = 0; k < 4; ++k) hit |= u[k] - (high << (shift + 9)) < 1u << (shift + 9);
-        if (hit)
+        if (__any_sync(0xFFFFFFFFu, hit))
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (u[k] >> (shift + 9) == high && u[k] >= from) add<MASS>(kBins - 1 - (int)((u[k] >> shift) & (kBins - 1)), u[k]);
+            add<MASS>(kBins - 1 - (int)((u[k] >> shift) & (kBins - 1)), u[k], u[k] >> (shift + 9) == high && u[k] >= from);
       });
       b = reach<MASS>(want, over, own, true, [&](int) { return exponent; });
       high = (high << 9) | (uint32_t)(kBins - 1 - b);
     }
     weight = high;
     equals = MASS ? rint(own / (double)u2f(high)) : own;
+    exact = MASS;
     return true;
+  }
+
+  // How many tokens at the weight that cut() found the blocks before this one have.
+  __device__ __forceinline__ double equals_before(uint32_t weight) const {
+    const double one = exact ? (double)((weight & 0x7FFFFFu) | 0x800000u) : 1.0;
+    double n = 0.0;
+    for (int i = 0; i < rank; ++i) n += rint((double)sh.shares[i] / one);
+    return n;
+  }
+
+  // Whether one value of T alone has this weight: a logit computed from it, or a neighbour of that, has it, and the next ones on
+  // both sides do not (weights are monotone).
+  __device__ bool one_logit(uint32_t weight) const {
+    if (infinite) return true;
+    const float guess = (float)(w.top + log2((double)u2f(weight)) / w.c);
+    int at;  // T's values in their order, as whole numbers
+    if constexpr (sizeof(T) == 4) {
+      at = (int)(key_of(guess) ^ 0x80000000u);
+    } else {
+      const T t = Io<T>::put(guess);
+      const int bits = *reinterpret_cast<const unsigned short *>(&t);
+      at = bits & 0x8000 ? 0x7FFF - bits : bits;
+    }
+    auto weight_at = [&](int k) {
+      float l;
+      if constexpr (sizeof(T) == 4) {
+        const uint32_t key = (uint32_t)k ^ 0x80000000u;
+        l = u2f((key >> 31) ? key & 0x7FFFFFFFu : ~key);
+      } else {
+        const unsigned short bits = (unsigned short)(k < 0 ? 0x7FFF - k : k);
+        l = Io<T>::get(*reinterpret_cast<const T *>(&bits));
+      }
+      return f2u(w(l));
+    };
+    int have = 0, edges = 0;
+#pragma unroll 1
+    for (int k = -3; k <= 3; ++k) {
+      const bool same = weight_at(at + k) == weight;
+      have += same;
+      edges += same && (k == -3 || k == 3);
+    }
+    return have == 1 && edges == 0;
+  }
+
+  // Where the `want` largest weights, with the rest of the last one's bin, are kList at most: they stand in the first block's list
+  // then, logits and places as one number, in no order. Otherwise `over` is unchanged and the histogram's bin is found again.
+  __device__ bool gather(double want, int64_t origin) {
+    double over = 0.0, own;
+    const int b = reach<false>([&] { return want; }, over, own, false, [](int) { return 0; });
+    if (over + own > (double)kList || b == kBins) return false;
+    uint64_t *local = reinterpret_cast<uint64_t *>(sh.hist[hist_turn]);  // clear, and as long as the list
+    static_assert(sizeof(sh.hist[0]) == kList * sizeof(uint64_t), "a list's room");
+    const uint32_t from = (kTop - (uint32_t)b) << 18;
+    each(from, [&](int i, uint4 q) {
+      const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (u[k] >= from) local[atomicAdd(&sh.mine, 1)] = (uint64_t)key_of(z.at(i + k)) << 32 | (0xFFFFFFFFu - (uint32_t)(origin + i + k));
+    });
+    __syncthreads();
+    const int mine = sh.mine;
+    if (threadIdx.x == 0) sh.base = atomicAdd(cluster.map_shared_rank(&sh.listed, 0), mine);
+    __syncthreads();
+    if ((int)threadIdx.x < mine) cluster.map_shared_rank(sh.list, 0)[sh.base + threadIdx.x] = local[threadIdx.x];
+    meet();
+    return true;
+  }
+
+  // The first block: the rest of the definition for the tokens of its list. Descending order by a bitonic sort, a thread a token.
+  template <typename A>
+  __device__ void finish(int64_t k, float p, float bound, double uniform, A answer) {
+    const int n = sh.listed, t = threadIdx.x;
+    int size = 32;
+    while (size < n) size *= 2;
+    uint64_t mine = t < n ? sh.list[t] : 0ull;
+    for (int width = 2; width <= size; width *= 2)
+      for (int step = width / 2; step; step /= 2) {
+        uint64_t other;
+        if (step >= 32) {
+          __syncthreads();
+          sh.list[t] = mine;
+          __syncthreads();
+          other = sh.list[t ^ step];
+        } else {
+          other = __shfl_xor_sync(0xFFFFFFFFu, mine, step);
+        }
+        const bool larger = ((t & step) == 0) == ((t & width) == 0 || width == size);
+        mine = (other > mine) == larger ? other : mine;
+      }
+    const uint32_t key = (uint32_t)(mine >> 32), place = (uint32_t)mine;  // places count from the end
+    float logit = u2f((key >> 31) ? key & 0x7FFFFFFFu : ~key);
+    if (infinite) logit = finite(logit);
+    const float weight = t < n && t < k ? w(logit) : 0.0f;
+    // Sums of the weights up to each, over the block.
+    auto scan = [&](double v, double &all) {
+      const int lane = t & 31, warp = warp_number();
+      double x = v;
+#pragma unroll
+      for (int m = 1; m < 32; m <<= 1) {
+        const double o = __shfl_up_sync(0xFFFFFFFFu, x, m);
+        if (lane >= m) x += o;
+      }
+      __syncthreads();
+      if (lane == 31) sh.part[warp] = x;
+      __syncthreads();
+      double before = 0.0;
+      all = 0.0;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        const double o = sh.part[i];
+        before = i < warp ? before + o : before;
+        all += o;
+      }
+      return before + x;
+    };
+    double all, total;
+    const double upto = scan((double)weight, all);
+    const bool keep = weight > 0.0f && !(weight < bound) && (t == 0 || !(p < 1.0f) || upto - (double)weight < (double)p * all);
+    scan(keep ? (double)weight : 0.0, total);
+    // In index order: of each kept token, the sum up to it.
+    const int kept = __syncthreads_count(keep);
+    sh.list[t] = (uint64_t)f2u(weight) << 32 | place;
+    __syncthreads();
+    const double aim = fmax(uniform * total, 0.0);
+    uint32_t hit = 0u, last = 0u;  // the first token that passes the aim, and the last one of all, as a place
+    if (keep) {
+      double s = 0.0;
+      for (int i = 0; i < kept; ++i) {
+        const uint64_t o = sh.list[i];
+        if ((uint32_t)o >= place) s += (double)u2f((uint32_t)(o >> 32));
+      }
+      if (s > aim) hit = place;
+      last = 0xFFFFFFFFu - place;
+    }
+    hit = block_max(hit);
+    last = block_max(last);
+    const uint32_t found = hit ? hit : 0xFFFFFFFFu - last;
+    if (keep && place == found) answer((int64_t)(0xFFFFFFFFu - place), (float)((infinite ? 0.0 : w.log(logit)) - log(total)));
   }
 
   // Of the tokens of a weight the first `want` are kept, larger logits first: the logit at which they end, and how many of
@@ -361,7 +538,7 @@ struct Row {
         for (int k = 0; k < 4; ++k)
           if (u[k] == weight) {
             const uint32_t key = key_of(z.at(i + k));
-            if (shift == 27 || key >> (shift + 9) == high) add<false>(kBins - 1 - (int)((key >> shift) & (kBins - 1)), 0u);
+            add<false>(kBins - 1 - (int)((key >> shift) & (kBins - 1)), 0u, shift == 27 || key >> (shift + 9) == high);
           }
       });
       const int b = reach<false>([&] { return (double)want; }, over, own, true, [](int) { return 0; });
@@ -408,7 +585,7 @@ struct Row {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int b = bin_of(u[k], 0);
-            if (b < kBins) add<FIRST == 2>(b, u[k]);
+            add<FIRST == 2>(b, u[k], b < kBins);
           }
       });
       top = warp_max(top);
@@ -444,7 +621,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
   const Stretch<T> &z = row.z;
   const int n = row.n;
   float *held = row.held;
-  shared.hist[0][0][threadIdx.x] = 0u, shared.hist[0][1][threadIdx.x] = 0u;  // added to after cluster_max's barriers
+  shared.hist[0][threadIdx.x] = make_uint2(0u, 0u);  // added to after cluster_max's barriers
+  if (threadIdx.x == 0) shared.listed = shared.mine = 0;
   auto started = row.cluster.barrier_arrive();
 
   // The logits, once, and the largest. fp32 goes to shared memory without a detour, all of a thread's at once.
@@ -498,13 +676,22 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
     const float p = a.top_p ? a.top_p[r] : a.all_top_p, low = a.min_p ? a.min_p[r] : a.all_min_p;
     const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.0f;
     double sum = by_count ? row.template prepare<1>() : by_mass ? row.template prepare<2>() : row.template prepare<0>();
+    const float bound = low > 1.0f ? 1.0f : low;  // NaN bounds nothing
+    bool counted = by_count;  // whether the histogram of counts still stands
+    if (by_count && k <= kList) {
+      if (row.gather((double)k, origin)) {
+        if (rank == 0) row.finish(k, p, bound, (double)a.uniform[r], answer);
+        return;
+      }
+      counted = false;
+    }
     // Kept: weights above `cut`, and of the tokens at it the first m.
     uint32_t cut = 0;
     double m = 0.0, equals = 0.0, over;
-    if (by_count && row.template cut<false>([&] { return (double)k; }, 1u, true, cut, over, equals)) m = (double)k - over;
+    if (by_count && row.template cut<false>([&] { return (double)k; }, 1u, counted, cut, over, equals)) m = (double)k - over;
     if (by_mass) {
       if (by_count) sum = row.mass_above(cut);
-      const double *all = row.tell(row.block_sum(sum));
+      const auto all = row.tell(row.block_sum(sum));
       double aim = 0.0;
       bool summed = false;
       auto want = [&] {  // after the next barrier
@@ -519,26 +706,45 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
         cut = c, equals = e;
       }
     }
-    const float bound = low > 1.0f ? 1.0f : low;  // NaN bounds nothing
     if (m > 0.0 && (u2f(cut) < bound || m == equals)) {  // none or all of the equals
       if (!(u2f(cut) < bound)) cut -= 1;
       m = 0.0;
     }
     if (bound > u2f(cut)) cut = max(cut, f2u(bound) - 1);
-    // Some of the equals: the logit at which they end.
+    // Some of the equals, in the order of their logits: those above `tie`, and of those that have it the first `quota`. Equal
+    // weights mostly come of equal logits.
     const bool some = m > 0.0;
+    bool alike = true;
     float tie = 0.0f;
-    int64_t quota = 0;
-    if (some) row.cut_logits(cut, (int64_t)m, tie, quota);
-    auto equal = [&](int i, uint32_t u, bool &above) {  // the tie's own, or one whose logit is above it
-      if (u != cut) return false;
+    int64_t left = 0;  // ties that this block may keep
+    if (some) {
+      int64_t quota = (int64_t)m;
+      double others = row.equals_before(cut);
+      alike = row.one_logit(cut);
+      if (!alike) {
+        row.cut_logits(cut, (int64_t)m, tie, quota);
+        double mine = 0.0;
+        row.each(cut, [&](int i, uint4 q) {
+          const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (u[e] == cut && z.at(i + e) == tie) mine += 1.0;
+        });
+        const auto all = row.tell(row.block_sum(mine));
+        row.meet();
+        others = 0.0;
+        for (int i = 0; i < rank; ++i) others += all[i][0];
+      }
+      left = max(quota - (int64_t)others, (int64_t)0);
+    }
+    auto equal = [&](int i, uint32_t u, bool &above) {  // a tie, or one whose logit is above it
+      if (u != cut || alike) return u == cut;
       const float l = z.at(i);
       above = l > tie;
       return l == tie;
     };
 
     // Masses and ties by chunks.
-    double ties = 0.0;
     row.chunks([&](int c, int at, int end) {
       double s = 0.0;
       int e = 0;
@@ -549,6 +755,13 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
           auto kept = [&](float v) { return f2u(v) > cut ? v : 0.0f; };
           s += (double)__fadd_rn(__fadd_rn(kept(q.x), kept(q.y)), __fadd_rn(kept(q.z), kept(q.w)));
         });
+      } else if (some && alike && peak >= cut) {
+        row.steps(at, end, [&](int i) {
+          const float4 q = row.four(i);
+          auto kept = [&](float v) { return e += f2u(v) == cut, f2u(v) > cut ? v : 0.0f; };
+          s += (double)__fadd_rn(__fadd_rn(kept(q.x), kept(q.y)), __fadd_rn(kept(q.z), kept(q.w)));
+        });
+        e = (int)__reduce_add_sync(0xFFFFFFFFu, e);
       } else if (some && peak >= cut) {
         for (; at < end; at += 128) {
           const int i = at + lane * 4;
@@ -569,16 +782,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
 #pragma unroll
         for (int x = 16; x; x >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, x);
       }
-      if (lane == 0) shared.mass[c] = s, shared.ties[c] = e, ties += e;
+      if (lane == 0) shared.mass[c] = s, shared.ties[c] = e;
     });
-    int64_t left = 0;  // ties that this block may keep
-    if (some) {
-      const double *all = row.tell(row.block_sum(ties));
-      row.cluster.sync();
-      left = quota;
-      for (int i = 0; i < rank; ++i) left -= (int64_t)all[i];
-      left = max(left, (int64_t)0);
-    }
     __syncthreads();
     // Chunks in order, four a lane of the first warp: ties that are left, and the mass before each.
     constexpr int kLane = kChunks / 32;
@@ -617,8 +822,8 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
       if (lane == 0) shared.found[0] = all;
     }
     __syncthreads();
-    const double *all = row.tell(shared.found[0]);
-    row.cluster.sync();
+    const auto all = row.tell(shared.found[0]);
+    row.meet();
     if (warp) return;
     // The block whose stretch the aim falls in; behind all of them (u = 1, or the last bits of the sums) the last one that
     // keeps anything.
@@ -626,9 +831,9 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
     int owner = -1;
     double start = 0.0, at = 0.0;
     for (int i = 0; i < blocks; ++i) {
-      if (all[i] > 0.0) owner = i, start = at;
-      at += all[i];
-      if (all[i] > 0.0 && at > aim) break;
+      if (all[i][0] > 0.0) owner = i, start = at;
+      at += all[i][0];
+      if (all[i][0] > 0.0 && at > aim) break;
     }
     if (rank == owner) {
       // Its chunk, likewise.
