@@ -25,25 +25,30 @@ struct Args {
   int64_t *first;  // workspace: of each sequence, where its first new page stands in free_pages
 };
 
-// Exclusive prefix sum of a value a thread over the block; total in every thread.
-__device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t *part, int64_t &total) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int64_t s = v;
+__device__ __forceinline__ int64_t warp_prefix(int64_t v) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int m = 1; m < 32; m <<= 1) {
-    const int64_t o = __shfl_up_sync(0xFFFFFFFFu, s, m);
-    if (lane >= m) s += o;
+    const int64_t o = __shfl_up_sync(0xFFFFFFFFu, v, m);
+    if (lane >= m) v += o;
   }
+  return v;
+}
+
+// Exclusive prefix sums of two values a thread over the block, and their totals in every thread.
+struct Two {
+  int64_t a, b;
+};
+__device__ __forceinline__ Two block_prefix(Two v, Two (&part)[32], Two &total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const Two s{warp_prefix(v.a), warp_prefix(v.b)};
   if (lane == 31) part[warp] = s;
   __syncthreads();
-  int64_t before = 0;
-  total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += part[w];
-    total += part[w];
-  }
+  const Two w = lane < warps ? part[lane] : Two{0, 0}, t{warp_prefix(w.a), warp_prefix(w.b)};
+  total = Two{__shfl_sync(0xFFFFFFFFu, t.a, 31), __shfl_sync(0xFFFFFFFFu, t.b, 31)};
+  const Two before{__shfl_sync(0xFFFFFFFFu, t.a - w.a, warp), __shfl_sync(0xFFFFFFFFu, t.b - w.b, warp)};
   __syncthreads();
-  return before + s - v;
+  return Two{before.a + s.a - v.a, before.b + s.b - v.b};
 }
 
 __device__ __forceinline__ int64_t taken_at_start(const Args &a) {
@@ -59,33 +64,31 @@ __device__ __forceinline__ int64_t new_pages(const Args &a, int64_t len, int64_t
 }
 
 __global__ void __launch_bounds__(kThreads) scan_kernel(Args a) {
-  __shared__ int64_t part[kThreads / 32];
+  __shared__ Two part[32];
   int64_t tokens = 0, pages = taken_at_start(a), beyond = 0;
   for (int64_t at = 0; at < a.batch; at += kThreads) {
     const int64_t i = at + threadIdx.x;
     const bool real = i < a.batch;
     const int64_t len = real ? max(a.lens[i], 0) : 0, want = real ? max(a.fresh[i], 0) : 0;
-    int64_t total;
-    const int64_t start = min(tokens + block_prefix(want, part, total), a.tokens);
-    tokens += total;
+    Two total;
+    const int64_t start = min(tokens + block_prefix(Two{want, 0}, part, total).a, a.tokens);
+    tokens += total.a;
     const int64_t n = min(want, a.tokens - start);
-    const int64_t need = real ? new_pages(a, len, n) : 0;
-    const int64_t first = pages + block_prefix(need, part, total);
-    pages += total;
+    const int64_t need = real ? new_pages(a, len, n) : 0, lacking = used_pages(a, len + n) - used_pages(a, len) - need;
+    const int64_t first = pages + block_prefix(Two{need, lacking}, part, total).a;
+    pages += total.a;
+    beyond += total.b;
     if (real) {
-      beyond += used_pages(a, len + n) - used_pages(a, len) - need;
       a.cu[i] = (int32_t)start;
       a.out_lens[i] = (int32_t)(len + n);
       a.first[i] = first;
       if (i == a.batch - 1) a.cu[a.batch] = (int32_t)(start + n);
     }
   }
-  int64_t none;
-  block_prefix(beyond, part, none);
   if (threadIdx.x == 0) {
     const int64_t out = min(pages, a.num_free);
     *a.out_taken = (int32_t)out;
-    *a.missing = (int32_t)min(pages - out + none, (int64_t)INT32_MAX);
+    *a.missing = (int32_t)min(pages - out + beyond, (int64_t)INT32_MAX);
   }
 }
 
@@ -130,42 +133,40 @@ __global__ void __launch_bounds__(256) fill_kernel(Args a) {
     fill_row(a, i, max(a.lens[i], 0), a.cu[i + 1] - a.cu[i], a.first[i]);
 }
 
-// Up to kThreads sequences in one kernel: every block adds the lengths up itself (a thread a sequence, some 2 us, which a kernel of its own
+// Up to kThreads sequences in one kernel: every block adds the lengths up itself (a thread a sequence: some 2 us, which a kernel of its own
 // and the launch after it would cost too), keeps the sums in shared memory and fills its share of the tokens and rows.
 __global__ void __launch_bounds__(kThreads) plan_kernel(Args a) {
-  __shared__ int64_t part[kThreads / 32];
+  __shared__ Two part[32];
   __shared__ int32_t start[kThreads + 1], length[kThreads];
   __shared__ int64_t first[kThreads];
-  const int i = threadIdx.x;
+  const int i = threadIdx.x, width = blockDim.x;
   const bool real = i < a.batch;
-  const int64_t len = real ? max(a.lens[i], 0) : 0, want = real ? max(a.fresh[i], 0) : 0;
-  int64_t total, pages, beyond;
-  const int64_t at = min(block_prefix(want, part, total), a.tokens), n = min(want, a.tokens - at);
-  const int64_t need = real ? new_pages(a, len, n) : 0, taken = taken_at_start(a);
-  first[i] = taken + block_prefix(need, part, pages);
+  const int64_t len = real ? max(a.lens[i], 0) : 0, want = real ? max(a.fresh[i], 0) : 0, taken = taken_at_start(a);
+  Two total;
+  const int64_t at = min(block_prefix(Two{want, 0}, part, total).a, a.tokens), n = min(want, a.tokens - at);
+  const int64_t need = real ? new_pages(a, len, n) : 0, lacking = used_pages(a, len + n) - used_pages(a, len) - need;
+  first[i] = taken + block_prefix(Two{need, lacking}, part, total).a;
   start[i] = (int32_t)at, length[i] = (int32_t)len;
-  if (i == kThreads - 1) start[kThreads] = (int32_t)(at + n);
+  if (i == width - 1) start[width] = (int32_t)(at + n);
   if (blockIdx.x == 0) {
-    block_prefix(used_pages(a, len + n) - used_pages(a, len) - need, part, beyond);
     if (real) a.cu[i] = (int32_t)at, a.out_lens[i] = (int32_t)(len + n);
     if (i == 0) {
-      const int64_t out = min(taken + pages, a.num_free);
+      const int64_t out = min(taken + total.a, a.num_free);
       *a.out_taken = (int32_t)out;
-      *a.missing = (int32_t)min(taken + pages - out + beyond, (int64_t)INT32_MAX);
+      *a.missing = (int32_t)min(taken + total.a - out + total.b, (int64_t)INT32_MAX);
     }
   }
   __syncthreads();
-  const int32_t end = start[kThreads];  // behind the batch's sequences every start is the end
+  const int32_t end = start[width];  // behind the batch's sequences every start is the end
   if (blockIdx.x == 0 && i == 0) a.cu[a.batch] = end;
-  const int64_t threads = (int64_t)gridDim.x * kThreads, thread = (int64_t)blockIdx.x * kThreads + i;
+  const int64_t threads = (int64_t)gridDim.x * width, thread = (int64_t)blockIdx.x * width + i;
   for (int64_t t = thread; t < a.tokens; t += threads) {
     if (t >= end) {
       no_token(a, t);
       continue;
     }
     int lo = 0;  // the last sequence that begins at t or before: an empty one begins where the next one does
-#pragma unroll
-    for (int step = kThreads / 2; step; step >>= 1)
+    for (int step = width / 2; step; step >>= 1)
       if (start[lo + step] <= t) lo += step;
     const int64_t l = length[lo], p = l + t - start[lo];
     a.slots[t] = slot_of(a, lo, l, first[lo], p);
@@ -272,9 +273,11 @@ extern "C" int tc_plan_pages(const int32_t *seq_lens, const int32_t *new_lens, i
   while ((1 << a.shift) < page_size) ++a.shift;
   cudaStream_t s = (cudaStream_t)stream;
   if (batch <= plan::kThreads) {
-    const int64_t work = tokens > (int64_t)batch * 32 ? tokens : (int64_t)batch * 32, blocks = (work + plan::kThreads - 1) / plan::kThreads;
-    const int64_t most = sm_count();
-    plan::plan_kernel<<<(unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most), plan::kThreads, 0, s>>>(a);
+    int threads = 256;  // a power of two, for the search
+    while (threads < batch) threads *= 2;
+    const int64_t work = tokens > (int64_t)batch * 32 ? tokens : (int64_t)batch * 32, blocks = (work + threads - 1) / threads;
+    const int64_t most = (int64_t)sm_count() * (1024 / threads);
+    plan::plan_kernel<<<(unsigned)(blocks < 1 ? 1 : blocks < most ? blocks : most), threads, 0, s>>>(a);
     return plan_status("tc_plan_pages");
   }
   plan::scan_kernel<<<1, plan::kThreads, 0, s>>>(a);
