@@ -21,10 +21,11 @@ constexpr int kThreads = 256;
 
 // g / (1 + 2**t), t = -log2(e) times the logistic function's argument. The hardware's exponential and reciprocal are good to 2
 // and 1 steps of fp32; t's rounding is |t| half steps of the exponential, at most half a step of g in the result, since
-// |t| / (1 + 2**t) stays below 1 where 2**t is large.
+// |t| / (1 + 2**t) stays below 1 where 2**t is large. Both flush what is below 2**-126 to 0: the exponential stands beside 1, and a result
+// that loses its factor this way is below 2**-119.
 __device__ __forceinline__ float logistic(float g, float t) {
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, exp2_wide(t))));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, exp2_fast(t))));
   return __fmul_rn(g, r);
 }
 
