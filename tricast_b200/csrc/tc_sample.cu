@@ -33,7 +33,7 @@ static cudaError_t launch(Args a, cudaStream_t s) {
   // Stretches short enough for two blocks an SM, and more of them while the card is not full and they stay long enough to be worth it.
   a.blocks = 1;
   while (a.blocks < 8 && (a.vocab > 23552 * (int64_t)a.blocks ||
-                          (a.rows * a.blocks < 2 * sm_count() && a.vocab > 4096 * (int64_t)a.blocks)))
+                          (a.rows * a.blocks <= sm_count() && a.vocab > 4096 * (int64_t)a.blocks)))
     a.blocks *= 2;
   a.part = (int)(((a.vocab + 8 + a.blocks - 1) / a.blocks + 127) / 128 * 128);  // positions begin up to 7 elements before the row
   return a.part <= kMaxHeld ? launch_as<T, true>(a, s) : launch_as<T, false>(a, s);

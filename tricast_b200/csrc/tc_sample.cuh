@@ -366,8 +366,18 @@ struct Row {
     if (b == kBins) return false;
     uint32_t high = kTop - (uint32_t)(b + window * kBins);
     const int exponent = (int)(high >> 5) - 127;
+    exact = MASS;
 #pragma unroll 1
     for (int shift = 9; shift >= 0; shift -= 9) {
+      if (MASS) {
+        // Two significands are 2**24 at least: a smaller sum is one token's, and says which weight it has.
+        const double units = own * __longlong_as_double((long long)(1023 - exponent + 23) << 52);
+        if (units < 16777216.0) {
+          weight = (uint32_t)(exponent + 127) << 23 | ((uint32_t)units & 0x7FFFFFu);
+          equals = 1.0;
+          return true;
+        }
+      }
       each(high << (shift + 9), [&](int, uint4 q) {
         const uint32_t u[4] = {q.x, q.y, q.z, q.w};
         bool hit = false;
@@ -383,7 +393,6 @@ struct Row {
     }
     weight = high;
     equals = MASS ? rint(own / (double)u2f(high)) : own;
-    exact = MASS;
     return true;
   }
 
