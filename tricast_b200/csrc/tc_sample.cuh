@@ -571,13 +571,14 @@ struct Row {
   }
 
   // Weights in the logits' place, the chunks' largest, this thread's part of their sum, and the histogram that the first
-  // filter begins with (FIRST: 0 none, 1 counts, 2 masses).
+  // filter begins with (FIRST: 1 counts, 2 masses); 0: no filter but a bound of the weights, so the chunks' sums of those above `cut`.
   template <int FIRST>
-  __device__ __forceinline__ double prepare() {
+  __device__ __forceinline__ double prepare(uint32_t cut) {
     const int lane = threadIdx.x & 31;
     double sum = 0.0;
     chunks([&](int c, int at, int end) {
       uint32_t top = 0u;
+      if (!FIRST) sum = 0.0;
       steps(at, end, [&](int i) {
         float4 q;
         if (HELD) {
@@ -587,7 +588,12 @@ struct Row {
         } else {
           q = four(i);
         }
+        if (!FIRST) {
+          auto kept = [&](float v) { return f2u(v) > cut ? v : 0.0f; };
+          q = make_float4(kept(q.x), kept(q.y), kept(q.z), kept(q.w));
+        }
         sum += (double)__fadd_rn(__fadd_rn(q.x, q.y), __fadd_rn(q.z, q.w));
+        if (!FIRST) return;
         const uint32_t u[4] = {f2u(q.x), f2u(q.y), f2u(q.z), f2u(q.w)};
         top = max(max(max(u[0], u[1]), max(u[2], u[3])), top);
         if (FIRST)
@@ -597,8 +603,14 @@ struct Row {
             add<FIRST == 2>(b, u[k], b < kBins);
           }
       });
-      top = warp_max(top);
-      if (lane == 0) sh.peak[c] = top;
+      if (FIRST) {
+        top = warp_max(top);
+        if (lane == 0) sh.peak[c] = top;
+      } else {
+#pragma unroll
+        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+        if (lane == 0) sh.mass[c] = sum, sh.ties[c] = 0;
+      }
     });
     __syncwarp();
     return sum;
@@ -684,8 +696,10 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
     const int64_t k = a.top_k ? a.top_k[r] : a.all_top_k;
     const float p = a.top_p ? a.top_p[r] : a.all_top_p, low = a.min_p ? a.min_p[r] : a.all_min_p;
     const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.0f;
-    double sum = by_count ? row.template prepare<1>() : by_mass ? row.template prepare<2>() : row.template prepare<0>();
     const float bound = low > 1.0f ? 1.0f : low;  // NaN bounds nothing
+    // Kept: weights above `cut`, and of the tokens at it the first m.
+    uint32_t cut = bound > 0.0f ? f2u(bound) - 1 : 0u;
+    double sum = by_count ? row.template prepare<1>(cut) : by_mass ? row.template prepare<2>(cut) : row.template prepare<0>(cut);
     bool counted = by_count;  // whether the histogram of counts still stands
     if (by_count && k <= kList) {
       if (row.gather((double)k, origin)) {
@@ -694,8 +708,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
       }
       counted = false;
     }
-    // Kept: weights above `cut`, and of the tokens at it the first m.
-    uint32_t cut = 0;
+    if (by_count || by_mass) cut = 0u;
     double m = 0.0, equals = 0.0, over;
     if (by_count && row.template cut<false>([&] { return (double)k; }, 1u, counted, cut, over, equals)) m = (double)k - over;
     if (by_mass) {
@@ -754,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
     };
 
     // Masses and ties by chunks.
-    row.chunks([&](int c, int at, int end) {
+    if (by_count || by_mass) row.chunks([&](int c, int at, int end) {
       double s = 0.0;
       int e = 0;
       const uint32_t peak = shared.peak[c];
