@@ -247,7 +247,8 @@ __device__ __forceinline__ void sum_rows(const Args &a, const Tile<NG> &tile, in
     for (int i = 0; i < NG; ++i)
 #pragma unroll
       for (int r = 0; r < kRowTiles; ++r) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.0f;
-#pragma unroll 2
+    constexpr int kAtOnce = NG == 1 ? 4 : 2;  // steps whose loads are on their way together
+#pragma unroll kAtOnce
     for (int64_t c = c0 + s; c < c1; c += splits) {
       const int64_t k = c * 32 + q * 8;
       uint32_t w[kRowTiles][2][4], x[NG][4];
@@ -353,16 +354,16 @@ __device__ __forceinline__ void take(const float (&d)[4][4], int e, float factor
   for (int k = 0; k < 4; ++k) v[2 * k] = __fmaf_rn(d[k][e], factor, v[2 * k]), v[2 * k + 1] = __fmaf_rn(d[k][2 + e], factor, v[2 * k + 1]);
 }
 
-// Few tokens: both products in one kernel. A cluster takes a tile of up to 8 NG tokens; its blocks share the sums over k, add them up through
+// Few tokens: both products in one kernel. A cluster takes a tile of up to 8 tokens; its blocks share the sums over k, add them up through
 // distributed shared memory, and share the columns of out. h = A x is fp32 and enters the second product in parts
 // of 16 bits: two where out has 16 bits (2**-16 of h is left out), three where it has 32; fp16 parts are taken of h times a power of two, a
-// token's own, that brings its largest to 2**13.
-template <typename T, int NG, int RW, bool CODES, bool VEC>
+// token's own, that brings its largest to 2**13. The rows of B that come first are asked for before h is there.
+template <typename T, int RW, bool CODES, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) tile_kernel(Args a) {
-  constexpr int kTokens = 8 * NG;
+  constexpr int kTokens = 8;
   constexpr bool kBf16 = Same<T, __nv_bfloat16>::value;
   extern __shared__ __align__(16) unsigned char dynamic[];
-  __shared__ Tile<NG> tile;
+  __shared__ Tile<1> tile;
   cg::cluster_group cluster = cg::this_cluster();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int blocks = a.blocks, rank = (int)cluster.block_rank();
@@ -373,24 +374,44 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(Args a) {
   const int count = tile.distinct, rows = RW == 16 ? 16 : rank_rows(a.rank), row_blocks = RW == 16 ? 1 : rows / RW;
   const int row_stride = rows + 8;                     // of h's parts: rows of 16 bytes more, against bank conflicts
   float *part = reinterpret_cast<float *>(dynamic);    // [splits][kTokens][rows]
-  uint16_t *parts = reinterpret_cast<uint16_t *>(part + part_floats(NG, RW, rows));
+  uint16_t *parts = reinterpret_cast<uint16_t *>(part + part_floats(1, RW, rows));
   float *full = reinterpret_cast<float *>(parts + 3 * kTokens * row_stride);  // fp16: h
   const int terms = a.out_dtype == TC_F32 ? 3 : 2;
+
+  // Columns: a warp takes 64 at a time, a lane 8 neighbouring ones of two tokens.
+  const int64_t columns = (a.n + 63) / 64, share = (columns + blocks - 1) / blocks, c1 = min(share * (rank + 1), columns);
+  int64_t c = share * rank + warp;
+  uint32_t w[4][2][RW / 8];
+  uint4 u[2][2];
+  float v[2][8];
+  auto valid_at = [&](int64_t column) { return (int)min(max(a.n - column * 64 - g * 8, (int64_t)0), (int64_t)8); };
+  auto ask_rows = [&](int64_t column, int j) {
+    if (row_blocks == 1 && column < c1 && j < count) load_rows<RW, VEC>(a, tile.adapters[j], column * 64 + g * 8, valid_at(column), 0, q, w);
+  };
+  auto ask_y = [&](int64_t column) {
+    if (column < c1)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        load_y<VEC>(a, t0 + q * 2 + e, column * 64 + g * 8, q * 2 + e < tokens ? valid_at(column) : 0, u[e], v[e]);
+  };
+  ask_y(c);
+  ask_rows(c, 0);
+
   if (count) {
-    const int64_t chunks = (a.k + 31) / 32, each = (chunks + blocks - 1) / blocks, c0 = min(each * rank, chunks);
-    sum_rows<T, NG, RW, CODES, VEC>(a, tile, t0, tokens, c0, min(c0 + each, chunks), part);
+    const int64_t chunks = (a.k + 31) / 32, each = (chunks + blocks - 1) / blocks, k0 = min(each * rank, chunks);
+    sum_rows<T, 1, RW, CODES, VEC>(a, tile, t0, tokens, k0, min(k0 + each, chunks), part);
     cluster.sync();
     for (int e = tid; e < kTokens * rows; e += kThreads) {
       const int t = e / rows, r = e - t * rows, who = tile.index[t];
-      float v = 0.0f;
+      float x = 0.0f;
       if (who >= 0) {
-        for (int b = 0; b < blocks; ++b) v = __fadd_rn(v, *cluster.map_shared_rank(part + e, b));
+        for (int b = 0; b < blocks; ++b) x = __fadd_rn(x, *cluster.map_shared_rank(part + e, b));
         float f = a.x_scale ? a.x_scale[t0 + t] : 1.0f;
         if (a.gain) f = __fmul_rn(f, a.gain[who]);
-        v = __fmul_rn(v, f);
+        x = __fmul_rn(x, f);
       }
-      if (kBf16) split_parts<T>(v, terms, parts + t * row_stride + r, kTokens * row_stride);
-      else full[e] = v, atomicMax(&tile.peak[t], abs_bits(v));
+      if (kBf16) split_parts<T>(x, terms, parts + t * row_stride + r, kTokens * row_stride);
+      else full[e] = x, atomicMax(&tile.peak[t], abs_bits(x));
     }
     __syncthreads();
     if (!kBf16) {
@@ -403,50 +424,35 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(Args a) {
     }
   }
 
-  // Columns: a warp takes 64 at a time, a lane 8 neighbouring ones of two tokens.
-  const int64_t chunks = (a.n + 63) / 64, each = (chunks + blocks - 1) / blocks;
-  const int64_t c1 = min(each * (rank + 1), chunks);
-  for (int64_t c = each * rank + warp; c < c1; c += kWarps) {
+  const int who0 = tile.index[q * 2], who1 = tile.index[q * 2 + 1];
+  for (; c < c1; c += kWarps) {
     const int64_t n0 = c * 64 + g * 8;
-    const int valid = (int)min(max(a.n - n0, (int64_t)0), (int64_t)8);
-    uint32_t w[4][2][RW / 8];
-    int loaded = -1;
-    for (int i = 0; i * 8 < tokens; ++i) {
-      uint4 u[2][2];
-      float v[2][8];
+    const int valid = valid_at(c);
+    float y[2][8];
+    y_floats<VEC>(a.y_dtype, u[0], v[0]), y_floats<VEC>(a.y_dtype, u[1], v[1]);
 #pragma unroll
-      for (int e = 0; e < 2; ++e) load_y<VEC>(a, t0 + i * 8 + q * 2 + e, n0, i * 8 + q * 2 + e < tokens ? valid : 0, u[e], v[e]);
-      const int who0 = tile.index[i * 8 + q * 2], who1 = tile.index[i * 8 + q * 2 + 1];
-      bool widened = false;
-      for (int j = 0; j < count; ++j) {
-        if (!(tile.members[j] >> i & 1u)) continue;
-        const int who = tile.adapters[j];
-        float d[4][4];
+    for (int k = 0; k < 8; ++k) y[0][k] = v[0][k], y[1][k] = v[1][k];
+    ask_y(c + kWarps);
+    for (int j = 0; j < count; ++j) {
+      const int who = tile.adapters[j];
+      float d[4][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) d[k][0] = d[k][1] = d[k][2] = d[k][3] = 0.0f;
-        for (int kc = 0; kc < row_blocks; ++kc) {
-          if (row_blocks > 1 || loaded != who) load_rows<RW, VEC>(a, who, n0, valid, kc, q, w);
-          for (int p = 0; p < terms; ++p) {
-            uint32_t h[RW / 8];
-            load_h<RW>(parts + (p * kTokens + i * 8 + g) * row_stride + kc * 32 + q * (RW / 4), h);
-            multiply<T, RW>(w, h, d);
-          }
+      for (int k = 0; k < 4; ++k) d[k][0] = d[k][1] = d[k][2] = d[k][3] = 0.0f;
+      for (int kc = 0; kc < row_blocks; ++kc) {
+        if (row_blocks > 1) load_rows<RW, VEC>(a, who, n0, valid, kc, q, w);
+        for (int p = 0; p < terms; ++p) {
+          uint32_t h[RW / 8];
+          load_h<RW>(parts + (p * kTokens + g) * row_stride + kc * 32 + q * (RW / 4), h);
+          multiply<T, RW>(w, h, d);
         }
-        loaded = who;
-        if (!widened) {
-          y_floats<VEC>(a.y_dtype, u[0], v[0]), y_floats<VEC>(a.y_dtype, u[1], v[1]);
-          widened = true;
-        }
-        if (who0 == who) take(d, 0, kBf16 ? 1.0f : fp16_shift(u2f(tile.peak[i * 8 + q * 2])).inverse, v[0]);
-        if (who1 == who) take(d, 1, kBf16 ? 1.0f : fp16_shift(u2f(tile.peak[i * 8 + q * 2 + 1])).inverse, v[1]);
       }
-      if (!widened) y_floats<VEC>(a.y_dtype, u[0], v[0]), y_floats<VEC>(a.y_dtype, u[1], v[1]);
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int t = i * 8 + q * 2 + e;
-        store_out<VEC>(a.out, a.out_dtype, (t0 + t) * a.n + n0, t < tokens ? valid : 0, v[e]);
-      }
+      if (j + 1 < count) ask_rows(c, j + 1);
+      else ask_rows(c + kWarps, 0);
+      if (who0 == who) take(d, 0, kBf16 ? 1.0f : fp16_shift(u2f(tile.peak[q * 2])).inverse, y[0]);
+      if (who1 == who) take(d, 1, kBf16 ? 1.0f : fp16_shift(u2f(tile.peak[q * 2 + 1])).inverse, y[1]);
     }
+#pragma unroll
+    for (int e = 0; e < 2; ++e) store_out<VEC>(a.out, a.out_dtype, (t0 + q * 2 + e) * a.n + n0, q * 2 + e < tokens ? valid : 0, y[e]);
   }
   if (count) cluster.sync();  // the other blocks may still read this one's sums
 }
@@ -671,8 +677,8 @@ static cudaError_t launch_tiles(const Args &a, cudaStream_t s) {
   attr.val.clusterDim.x = a.blocks;
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   const cudaLaunchConfig_t cfg = config((a.tokens + a.tile - 1) / a.tile * a.blocks, bytes, s, &attr);
-  const cudaError_t e = room(tile_kernel<T, 1, RW, CODES, VEC>, bytes);
-  return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, tile_kernel<T, 1, RW, CODES, VEC>, a);
+  const cudaError_t e = room(tile_kernel<T, RW, CODES, VEC>, bytes);
+  return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, tile_kernel<T, RW, CODES, VEC>, a);
 }
 
 constexpr int kDownGroups = 2;  // of 8 tokens, a block of the first kernel
@@ -716,9 +722,10 @@ static cudaError_t launch_two(Args a, cudaStream_t s) {
                                : up(up_kernel<T, RW, false, false, true>);
 }
 
-// Up to this many tokens one kernel does both products. One and two kernels, us, 4096 -> 4096, rank 16, fp32 to bf16, runs of 6
-// adapters: 32 tokens 7.7 and 12.5, 128 10.1 and 11.1, 256 12.5 and 11.1, 512 20 and 11, 1024 37 and 17.
-inline int64_t few_tokens() { return sm_count(); }
+// Up to this many tokens one kernel does both products: a little less than what clusters of 8 blocks with 8 tokens each hold when the
+// card is full. One and two kernels, us, 4096 -> 4096, rank 16, fp32 to bf16, runs of 6 adapters: 64 tokens 7.7 and 12.3, 160 9.0 and
+// 11.7, 256 8.7 and 11.3, 296 11.4 and 11.1.
+inline int64_t few_tokens() { return (int64_t)sm_count() * 7 / 4; }
 
 template <typename T, bool CODES>
 static cudaError_t launch_two_as(const Args &a, bool vec, cudaStream_t s) {
@@ -740,12 +747,14 @@ static cudaError_t launch_as(Args a, cudaStream_t s) {
                    aligned(a.b, 16) && aligned(a.out, 16);
   const bool codes = a.x_kind > X_F16;
   if (a.tokens > few_tokens()) return codes ? launch_two_as<T, true>(a, vec, s) : launch_two_as<T, false>(a, vec, s);
-  // Tiles of at most 8 tokens, as small as the card has clusters of 8 blocks for.
-  const int sms = sm_count();
+  // Tiles of at most 8 tokens, as small as the card holds clusters of 8 blocks for (two blocks an SM): tokens that share a tile
+  // wait for one another's adapters. 64 tokens with as many adapters, 4096 -> 4096, rank 32: tiles of 1, 2 and 4 in 18.5, 14.8 and
+  // 20.9 us; of one adapter 8.2 us with 2, 7.7 with 8.
+  const int room = 2 * sm_count();
   a.tile = 1;
-  while (a.tile < 8 && (a.tokens + a.tile - 1) / a.tile * 8 > sms) a.tile *= 2;
+  while (a.tile < 8 && (a.tokens + a.tile - 1) / a.tile * 8 > room) a.tile *= 2;
   a.blocks = 1;
-  while (a.blocks < 8 && (a.tokens + a.tile - 1) / a.tile * a.blocks * 2 <= sms) a.blocks *= 2;
+  while (a.blocks < 8 && (a.tokens + a.tile - 1) / a.tile * a.blocks * 2 <= room) a.blocks *= 2;
   return codes ? launch_tiles_as<T, true>(a, vec, s) : launch_tiles_as<T, false>(a, vec, s);
 }
 
