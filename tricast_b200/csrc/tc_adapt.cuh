@@ -509,63 +509,75 @@ __global__ void __launch_bounds__(kThreads, RW == 16 ? 4 : 3) down_kernel(Args a
   cluster.sync();  // the other blocks may still read this one's sums
 }
 
-// Then out: a warp takes 64 columns and a run of tokens, a lane 8 neighbouring columns of two tokens of each eight. The rows of B stay in
-// registers as long as the adapter does; y, h and the adapters of the next eight tokens are on their way while these are
-// computed. Y, O: y and out have 32 bits (else 16). With 16 bits out, y is what the products are added to in the MMAs.
+// Then out, with tokens in the MMAs' rows and columns of out in their columns: a warp takes 32 columns and a run of tokens, a lane 8
+// neighbouring columns of two tokens of each sixteen, so that four lanes read and write a token's columns side by side (with columns in the
+// rows, as above, every quarter of a warp touched four lines at a time, and L1 was the fullest resource). The rows of B stay in
+// registers as long as the adapter does; y and the adapters of the next sixteen tokens are on their way while these are computed. Y, O: y and out have 32 bits (else 16). With 16 bits out, y is what the products are added to in the MMAs.
 template <typename T, int RW, bool Y, bool O, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) up_kernel(Args a) {
   constexpr bool kBf16 = Same<T, __nv_bfloat16>::value;
-  constexpr int kTerms = O ? 3 : 2;
+  constexpr int kTerms = O ? 3 : 2, kWords = RW / 8;
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int64_t columns = (a.n + 63) / 64, item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  const int64_t run = item / columns, n0 = (item - run * columns) * 64 + g * 8, t0 = run * a.tile;
+  const int64_t columns = (a.n + 31) / 32, item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  const int64_t run = item / columns, base = (item - run * columns) * 32, n0 = base + q * 8, t0 = run * a.tile;
   if (t0 >= a.tokens) return;
   int left = (int)min((int64_t)a.tile, a.tokens - t0);
-  int64_t token = t0 + q * 2;
   const int valid = (int)min(max(a.n - n0, (int64_t)0), (int64_t)8);
   const int rows = RW == 16 ? 16 : rank_rows(a.rank), row_blocks = RW == 16 ? 1 : rows / RW;
-  // Where this lane's two tokens and, for h, its one of the eight stand.
-  const int32_t *index = a.index + t0 + q * 2;
-  int64_t y_at = (t0 + q * 2) * a.y_stride + n0, out_at = (t0 + q * 2) * a.n + n0;
-  const uint16_t *parts = a.parts + (t0 + g) * kTerms * rows + q * (RW / 4);
+  int64_t token = t0 + g;  // this lane's first; the other one stands 8 behind it
+  const int32_t *index = a.index + token;
+  int64_t y_at = token * a.y_stride + n0, out_at = token * a.n + n0;
+  const uint16_t *parts = a.parts + token * kTerms * rows + q * (RW / 4);
   // Beyond 32 ranks the rows of B stand in shared memory, a lane's own pieces of 16 bytes side by side with the other lanes'.
   extern __shared__ __align__(16) unsigned char dynamic[];
-  uint4 *kept = reinterpret_cast<uint4 *>(dynamic) + (size_t)(threadIdx.x >> 5) * row_blocks * 8 * 32 + lane;
-  uint32_t w[4][2][RW / 8], h[kTerms][RW / 8];
+  uint4 *kept = reinterpret_cast<uint4 *>(dynamic) + (size_t)(threadIdx.x >> 5) * row_blocks * 4 * 32 + lane;
+  uint32_t w[4][kWords], h[kTerms][2][kWords];
   int loaded = -1, who[2];
   uint4 u[2][Y ? 2 : 1];
   float v[2][VEC ? 1 : 8];
   auto ask = [&](int64_t y_from, const int32_t *from, int tokens) {
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const bool real = q * 2 + e < tokens;
-      who[e] = real ? __ldg(from + e) : -1;
+      const bool real = g + 8 * e < tokens;
+      who[e] = real ? __ldg(from + 8 * e) : -1;
+      const int64_t at = y_from + 8 * e * a.y_stride;
       if constexpr (!VEC) {
 #pragma unroll
-        for (int k = 0; k < 8; ++k) v[e][k] = real && k < valid ? load_as_float(a.y, a.y_dtype, y_from + e * a.y_stride + k) : 0.0f;
-      }
-      if (VEC && real && valid > 0) {
+        for (int k = 0; k < 8; ++k) v[e][k] = real && k < valid ? load_as_float(a.y, a.y_dtype, at + k) : 0.0f;
+      } else if (real && valid > 0) {
         if constexpr (Y) {
-          const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(a.y) + y_from + e * a.y_stride);
+          const uint4 *p = reinterpret_cast<const uint4 *>(static_cast<const float *>(a.y) + at);
           u[e][0] = __ldg(p), u[e][1] = __ldg(p + 1);
         } else {
-          u[e][0] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.y) + y_from + e * a.y_stride));
+          u[e][0] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint16_t *>(a.y) + at));
         }
       }
     }
   };
-  auto ask_h = [&](const uint16_t *from, bool real) {
-    if (real && row_blocks == 1)
+  auto load_parts = [&](const uint16_t *from, int tokens, uint32_t (&x)[kTerms][2][kWords]) {
 #pragma unroll
-      for (int p = 0; p < kTerms; ++p) load_h<RW>(from + p * rows, h[p]);
+    for (int p = 0; p < kTerms; ++p)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (g + 8 * e < tokens) load_h<RW>(from + (8 * e * kTerms + p) * rows, x[p][e]);
   };
+  // Of one adapter's B the rows of this lane's column of each MMA: column c of the j-th is the warp's 8 (c / 2) + 2 j + c % 2.
+  auto load_b = [&](int i, int kc) {
+    const int64_t column = base + (g >> 1) * 8 + (g & 1);
+    const uint16_t *from = static_cast<const uint16_t *>(a.b) + ((int64_t)i * a.n + column) * a.rank;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) load16<RW / 4, VEC>(from + 2 * j * a.rank, kc * 32 + q * (RW / 4), column + 2 * j < a.n ? a.rank : 0, w[j]);
+  };
+#pragma unroll
+  for (int p = 0; p < kTerms; ++p)
+#pragma unroll
+    for (int k = 0; k < kWords; ++k) h[p][0][k] = h[p][1][k] = 0u;
   ask(y_at, index, left);
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the first kernel's h
-  ask_h(parts, g < left);
-  for (; left > 0; left -= 8) {
+  if (row_blocks == 1) load_parts(parts, left, h);
+  for (; left > 0; left -= 16) {
     float y[2][8];
     int mine[2];
-    uint32_t own[kTerms][RW / 8];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       mine[e] = (unsigned)who[e] < (unsigned)a.adapters ? who[e] : -1;
@@ -577,49 +589,51 @@ __global__ void __launch_bounds__(kThreads, 2) up_kernel(Args a) {
         for (int k = 0; k < 2; ++k)
           y[e][4 * k] = u2f(u[e][k].x), y[e][4 * k + 1] = u2f(u[e][k].y), y[e][4 * k + 2] = u2f(u[e][k].z), y[e][4 * k + 3] = u2f(u[e][k].w);
       } else {
-        const uint32_t v[4] = {u[e][0].x, u[e][0].y, u[e][0].z, u[e][0].w};
+        const uint32_t x[4] = {u[e][0].x, u[e][0].y, u[e][0].z, u[e][0].w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) y[e][2 * k] = half_bits_to_float<T>(v[k] & 0xFFFFu), y[e][2 * k + 1] = half_bits_to_float<T>(v[k] >> 16);
+        for (int k = 0; k < 4; ++k) y[e][2 * k] = half_bits_to_float<T>(x[k] & 0xFFFFu), y[e][2 * k + 1] = half_bits_to_float<T>(x[k] >> 16);
       }
     }
-#pragma unroll
-    for (int p = 0; p < kTerms; ++p)
-#pragma unroll
-      for (int k = 0; k < RW / 8; ++k) own[p][k] = h[p][k];
-    const uint16_t *now = parts;
-    y_at += 8 * a.y_stride, index += 8, parts += 8 * kTerms * rows;
-    ask(y_at, index, left - 8);
-    ask_h(parts, g < left - 8);
+    y_at += 16 * a.y_stride, index += 16;
+    ask(y_at, index, left - 16);
 
     float d[4][4];
-    // The products of one adapter with the eight tokens, on top of d.
+    // The products of one adapter with the sixteen tokens, on top of d, a part of h after the other.
+    auto multiply_parts = [&](const uint32_t (&x)[kTerms][2][kWords]) {
+#pragma unroll
+      for (int p = 0; p < kTerms; ++p)
+#pragma unroll
+        for (int st = 0; st < RW / 16; ++st) {
+          const uint32_t f[4] = {x[p][0][2 * st], x[p][1][2 * st], x[p][0][2 * st + 1], x[p][1][2 * st + 1]};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma16<kBf16>(d[j], f, w[j][2 * st], w[j][2 * st + 1]);
+        }
+    };
     auto products = [&](int i) {
       if (row_blocks == 1) {
-        if (loaded != i) load_rows<RW, VEC>(a, i, n0, valid, 0, q, w);
-#pragma unroll
-        for (int p = 0; p < kTerms; ++p) multiply<T, RW>(w, own[p], d);
+        if (loaded != i) load_b(i, 0);
+        multiply_parts(h);
       } else if constexpr (RW == 32) {
         for (int kc = 0; kc < row_blocks; ++kc) {
-          uint4 *piece = kept + kc * 8 * 32;
+          uint4 *piece = kept + kc * 4 * 32;
           if (loaded != i) {
-            load_rows<RW, VEC>(a, i, n0, valid, kc, q, w);
+            load_b(i, kc);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) piece[k * 32] = make_uint4(w[k >> 1][k & 1][0], w[k >> 1][k & 1][1], w[k >> 1][k & 1][2], w[k >> 1][k & 1][3]);
+            for (int j = 0; j < 4; ++j) piece[j * 32] = make_uint4(w[j][0], w[j][1], w[j][2], w[j][3]);
           } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const uint4 x = piece[k * 32];
-              w[k >> 1][k & 1][0] = x.x, w[k >> 1][k & 1][1] = x.y, w[k >> 1][k & 1][2] = x.z, w[k >> 1][k & 1][3] = x.w;
+            for (int j = 0; j < 4; ++j) {
+              const uint4 x = piece[j * 32];
+              w[j][0] = x.x, w[j][1] = x.y, w[j][2] = x.z, w[j][3] = x.w;
             }
           }
+          uint32_t x[kTerms][2][kWords];
 #pragma unroll
-          for (int p = 0; p < kTerms; ++p) {
-            uint32_t x[RW / 8];
+          for (int p = 0; p < kTerms; ++p)
 #pragma unroll
-            for (int k = 0; k < RW / 8; ++k) x[k] = 0u;
-            if (g < left) load_h<RW>(now + p * rows + kc * 32, x);
-            multiply<T, RW>(w, x, d);
-          }
+            for (int k = 0; k < kWords; ++k) x[p][0][k] = x[p][1][k] = 0u;
+          load_parts(parts + kc * 32, left, x);
+          multiply_parts(x);
         }
       }
       loaded = i;
@@ -627,27 +641,35 @@ __global__ void __launch_bounds__(kThreads, 2) up_kernel(Args a) {
     const int one = __shfl_sync(0xFFFFFFFFu, mine[0], 0);
     if (!O && kBf16 && one >= 0 && __all_sync(0xFFFFFFFFu, mine[0] == one && mine[1] == one)) {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) d[k][0] = y[0][2 * k], d[k][1] = y[1][2 * k], d[k][2] = y[0][2 * k + 1], d[k][3] = y[1][2 * k + 1];
+      for (int j = 0; j < 4; ++j) d[j][0] = y[0][2 * j], d[j][1] = y[0][2 * j + 1], d[j][2] = y[1][2 * j], d[j][3] = y[1][2 * j + 1];
       products(one);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) y[0][2 * k] = d[k][0], y[1][2 * k] = d[k][1], y[0][2 * k + 1] = d[k][2], y[1][2 * k + 1] = d[k][3];
+      for (int j = 0; j < 4; ++j) y[0][2 * j] = d[j][0], y[0][2 * j + 1] = d[j][1], y[1][2 * j] = d[j][2], y[1][2 * j + 1] = d[j][3];
     } else {
       unsigned open[2] = {__ballot_sync(0xFFFFFFFFu, mine[0] >= 0), __ballot_sync(0xFFFFFFFFu, mine[1] >= 0)};
       while (open[0] | open[1]) {
         const int i = open[0] ? __shfl_sync(0xFFFFFFFFu, mine[0], __ffs(open[0]) - 1) : __shfl_sync(0xFFFFFFFFu, mine[1], __ffs(open[1]) - 1);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) d[k][0] = d[k][1] = d[k][2] = d[k][3] = 0.0f;
+        for (int j = 0; j < 4; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.0f;
         products(i);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (mine[e] == i) take(d, e, kBf16 ? 1.0f : a.factors[token + e], y[e]);
+          if (mine[e] == i) {
+            const float factor = kBf16 ? 1.0f : a.factors[token + 8 * e];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+              y[e][2 * j] = __fmaf_rn(d[j][2 * e], factor, y[e][2 * j]), y[e][2 * j + 1] = __fmaf_rn(d[j][2 * e + 1], factor, y[e][2 * j + 1]);
+          }
           open[e] &= ~__ballot_sync(0xFFFFFFFFu, mine[e] == i);
         }
       }
     }
+    parts += 16 * kTerms * rows;
+    if (row_blocks == 1) load_parts(parts, left - 16, h);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) store_out<VEC>(a.out, O ? TC_F32 : kBf16 ? TC_BF16 : TC_F16, out_at + e * a.n, q * 2 + e < left ? valid : 0, y[e]);
-    out_at += 8 * a.n, token += 8;
+    for (int e = 0; e < 2; ++e)
+      store_out<VEC>(a.out, O ? TC_F32 : kBf16 ? TC_BF16 : TC_F16, out_at + 8 * e * a.n, g + 8 * e < left ? valid : 0, y[e]);
+    out_at += 16 * a.n, token += 16;
   }
 }
 
@@ -699,13 +721,13 @@ static cudaError_t launch_two(Args a, cudaStream_t s) {
   e = cudaLaunchKernelEx(&cfg, down_kernel<T, kDownGroups, RW, CODES, VEC>, a);
   if (e != cudaSuccess) return e;
   count_launch();
-  const int64_t columns = (a.n + 63) / 64;
+  const int64_t columns = (a.n + 31) / 32;
   a.tile = 128;
   while (a.tile > 16 && (a.tokens + a.tile - 1) / a.tile * columns < 48 * (int64_t)sm_count()) a.tile /= 2;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   const int row_blocks = rank_rows(a.rank) / RW;
-  const size_t kept = row_blocks > 1 ? (size_t)kWarps * row_blocks * 8 * 512 : 0;
+  const size_t kept = row_blocks > 1 ? (size_t)kWarps * row_blocks * 4 * 512 : 0;
   cfg = config(((a.tokens + a.tile - 1) / a.tile * columns + kWarps - 1) / kWarps, kept, s, &attr);
   auto up = [&](auto kernel) {
     const cudaError_t r = room(kernel, kept);
