@@ -174,6 +174,58 @@ def test_streams_and_graphs():
     assert torch.equal(got, low_rank_add(y, x, a, b, index, gain=gain)) and not torch.equal(got, want)
 
 
+@pytest.mark.parametrize("tokens", [200, 600])
+def test_captured_calls_that_share_a_stream_replay(tokens):
+    """Both forms, one kernel and two, twice in one graph: each call has a workspace of its own."""
+    y, x, a, b, index, gain = inputs(tokens, 256, 512, 16, 6, torch.bfloat16, torch.float32, seed=tokens)
+    want = low_rank_add(y, x, a, b, index, gain=gain, dtype=torch.bfloat16)
+    other = low_rank_add(y, x.flip(0), a, b, index, dtype=torch.bfloat16)
+    flipped = x.flip(0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one = low_rank_add(y, x, a, b, index, gain=gain, dtype=torch.bfloat16)
+        two = low_rank_add(y, flipped, a, b, index, dtype=torch.bfloat16)
+    for _ in range(3):
+        one.zero_()
+        two.zero_()
+        graph.replay()
+        assert torch.equal(one, want) and torch.equal(two, other)
+
+
+def test_calls_on_two_streams_at_once():
+    sets = [inputs(700, 512, 768, 16, 6, torch.bfloat16, torch.float32, seed=s) for s in range(2)]
+    want = [low_rank_add(*v[:5], gain=v[5]) for v in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for v, stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(low_rank_add(*v[:5], gain=v[5]))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
+
+
+def test_types_that_do_not_meet_in_a_product():
+    """Operands of two 16-bit types, or a wide weight: element by element, the same definition."""
+    y, x, a, b, index, gain = inputs(40, 96, 130, 8, 3, torch.bfloat16, torch.float32)
+    close(low_rank_add(y, x.half(), a, b, index, gain=gain), y, x.half(), a, b, index, gain)
+    close(low_rank_add(y, x, a.float(), b.float(), index, gain=gain), y, x, a, b, index, gain)
+    close(low_rank_add(y.half(), x, a, b, index, gain=gain), y.half(), x, a, b, index, gain)
+    close(low_rank_add(y, x, a, b, index, gain=gain, dtype=torch.float16), y, x, a, b, index, gain)
+
+
+def test_large_and_small_products_in_fp16():
+    """h beyond fp16's range, and far below it, in one batch: a token's parts have a power of two of their own."""
+    for tokens in (9, 400):
+        y, x, a, b, index, gain = inputs(tokens, 128, 192, 16, 3, torch.float16, torch.float32)
+        x[0::3] *= 2000.0
+        a[0] *= 100.0
+        x[1::3] *= 2.0 ** -12
+        b = b * 2.0 ** -6
+        close(low_rank_add(y, x, a, b, index, gain=gain), y, x, a, b, index, gain)
+
+
 def test_refusals():
     y, x, a, b, index, gain = inputs(4, 64, 96, 8, 2, torch.bfloat16, torch.float32)
     for kw in (dict(x=x[:3]), dict(x=x[:, :32]), dict(x=x[0]), dict(a=a[0]), dict(b=b[:1]), dict(b=b[:, :95]), dict(b=b.float()),

@@ -183,10 +183,29 @@ def test_flat_rows_of_many_kept_tokens():
         check(z, u, **kw)
 
 
-def test_large_vocabularies():
-    z, u, _ = make(2, 600001)
-    for kw in (dict(), dict(top_k=50, top_p=0.9), dict(top_p=0.95), dict(temperature=0.0)):
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_vocabularies(dtype):
+    """Beyond what a cluster's shared memory holds: weights are computed anew by every pass."""
+    z, u, _ = make(2, 600001, dtype)
+    z[1, 3:7] = float("-inf")
+    for kw in (dict(), dict(top_k=50, top_p=0.9), dict(top_p=0.95), dict(temperature=0.0), dict(top_k=30000, top_p=0.8), dict(min_p=0.01),
+               dict(temperature=float("inf"), top_k=70001)):
         check(z, u, **kw)
+    z[0, 5] = z[0, 500000] = float("inf")
+    z[1, 400000] = float("nan")
+    check(z, u, top_p=0.9)
+
+
+@pytest.mark.parametrize("vocab", [513, 5000, 60000])
+def test_sets_as_long_as_one_block_finishes(vocab):
+    """Around 512 tokens, below and above which other code ends the work; runs of equals that pass it."""
+    for dtype in (torch.float32, torch.bfloat16):
+        z, u, _ = make(6, vocab, dtype, seed=11)
+        z[4] = (z[4] > 0).to(dtype)  # two values
+        z[5, 20:] = float("-inf")  # fewer tokens than top_k
+        for k in (2, 31, 33, 255, 500, 511, 512, 513, 600):
+            check(z, u, top_k=k)
+            check(z, u, top_k=k, top_p=0.7, min_p=0.01, temperature=1.3)
 
 
 def test_many_rows_and_strides():
@@ -231,6 +250,20 @@ def test_streams_and_graphs():
     u.copy_(u.flip(0))
     graph.replay()
     assert torch.equal(got, want.flip(0))
+
+
+def test_calls_on_two_streams_at_once():
+    sets = [make(40, 30000, seed=s)[:2] for s in range(2)]
+    want = [sample_tokens(z, u, top_p=0.9) for z, u in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = []
+        for (z, u), stream in zip(sets, streams):
+            with torch.cuda.stream(stream):
+                got.append(sample_tokens(z, u, top_p=0.9))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, w) for g, w in zip(got, want))
 
 
 def test_refusals():
