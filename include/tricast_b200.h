@@ -360,8 +360,9 @@ size_t tc_low_rank_add_workspace(int64_t tokens, int32_t x_kind, int32_t w_dtype
 /* Low-rank adapters beside a projection: out[t] = y[t] + gain[i] * b[i] (a[i] x[t]) with i = index[t], and out[t] = y[t] where i
  * is not in [0, adapters). y [tokens][n] and x [tokens][k] have row strides in elements, out [tokens][n] has none; a
  * [adapters][rank][k] and b [adapters][n][rank] of w_dtype; gain fp32 [adapters] or NULL (1). x_kind: a tc_dtype, or a
- * tc_x_codes; x_scale: NULL, or fp32 [tokens], a factor of each row (codes need it). Products and sums are fp32, out is rounded once. rank at most 1024. No output may
- * alias an input. */
+ * tc_x_codes; x_scale: NULL, or fp32 [tokens], a factor of each row (codes need it). Products and sums are fp32, out is rounded once. rank at most 1024. Weights of 16
+ * bits with x of their type or 8-bit codes, y and out of their type or fp32, and ranks up to 128 go through the tensor cores, everything else
+ * element by element. out may not alias an input. */
 int tc_low_rank_add(const void *y, int32_t y_dtype, int64_t y_stride, const void *x, int32_t x_kind, int64_t x_stride,
                     const float *x_scale, int64_t tokens, int64_t k, int64_t n, const void *a, const void *b, int32_t w_dtype,
                     int32_t adapters, int32_t rank, const float *gain, const int32_t *index, void *out, int32_t out_dtype,
@@ -381,7 +382,8 @@ int tc_gated_quantize(const void *gate, int64_t gate_stride, const void *up, int
  * the ones with w_i >= min_p (<= 0: all; the largest always stays). tokens[r] is the first index at which the sum of the kept weights, in
  * index order, exceeds uniform[r] times their total; logprobs (or NULL) log(w / total). temperature <= 0: the first largest
  * logit, log-probability 0. A row without a logit above -Inf gives -1 and -Inf, one with a NaN -1 and NaN. Settings: one
- * a row where the array is given, else the value beside it; NaN settings bound nothing, a NaN temperature is 0. */
+ * a row where the array is given, else the value beside it; NaN settings bound nothing, a NaN temperature is 0, one between 0 and
+ * 2**-100 is 2**-100. At most 2**27 rows and a vocabulary of 2**23. */
 int tc_sample_tokens(const void *logits, int32_t dtype, int64_t rows, int64_t vocab, int64_t stride, const float *uniform,
                      const float *temperature, float all_temperature, const int32_t *top_k, int32_t all_top_k,
                      const float *top_p, float all_top_p, const float *min_p, float all_min_p, int64_t *tokens, float *logprobs,

@@ -9,6 +9,9 @@ Public surface (TriCast's GPU backend API, ``src/tricast/kernels``):
 * ``rms_norm_quantize``, ``PagedKVCache``, ``paged_attention`` — serving operators without a TriCast
   counterpart: the norm that ends in an 8-bit operand, the quantized paged cache, and the attention of
   new tokens over it;
+* ``plan_pages``, ``release_pages``, ``low_rank_add``, ``gated_quantize``, ``sample_tokens`` — the rest of a serving
+  step: pages and slots from request lengths, low-rank adapters beside a projection, the gated activation
+  that ends in an 8-bit operand, and the next tokens from their logits;
 * ``install()`` — register this package as TriCast's GPU backend module (``tricast.kernels``), so
   ``tricast.quantize``/``tricast.gemm`` with ``backend="auto"`` or ``"triton"``, recipes,
   ``patch_model``, the CLI and the app run on it unchanged.

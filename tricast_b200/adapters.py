@@ -19,9 +19,11 @@ def low_rank_add(y: torch.Tensor, x, a: torch.Tensor, b: torch.Tensor, index: to
     and ``b`` ``[adapters, n, rank]`` (contiguous; ranks below the pool's are padded with zeros), ``index`` int32 ``[tokens]``: an
     index outside the pool (``-1``) adds nothing. ``gain`` fp32 ``[adapters]``: a factor of each adapter.
 
-    The products and the sum are fp32 (weights and ``x`` of 16 bits go through the tensor cores, which leaves them as they are), rounded
-    once to ``dtype`` (default ``y``'s). Tokens of one adapter that stand together share its weights' way through the chip;
-    any order is allowed. No gradients pass: the output is detached."""
+    The products and the sum are fp32, rounded once to ``dtype`` (default ``y``'s). Weights of 16 bits with ``x`` of their type or 8-bit
+    codes, ``y`` and ``dtype`` of their type or fp32, and ranks up to 128 go through the tensor cores, anything else element by
+    element. Any order of tokens is allowed; those of one adapter that stand together share its weights' way through the
+    chip. More than some 250 tokens take scratch memory (up to 6 bytes a token and rank) while they run. No gradients pass:
+    the output is detached."""
     if not y.is_cuda:
         raise ValueError("the B200 backend requires a CUDA tensor")
     device, scale = y.device, None

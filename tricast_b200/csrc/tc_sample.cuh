@@ -8,7 +8,14 @@
 // A row is cut into stretches, one a block of a cluster, which hold their weights in shared memory: the logits are read once.
 // The weight at the cut is found by its bits, nine at a time: histograms of counts (top_k) or masses (top_p) that the cluster adds
 // up through distributed shared memory. Equal high bits mean an equal exponent, so a bin's mass is a sum of 24-bit integers, exact
-// in two 32-bit words; totals are fp64 sums in a fixed order. Nothing depends on timing.
+// in two 32-bit words; totals are fp64 sums in a fixed order. Nothing depends on timing. Where top_k leaves few tokens (kList with the rest
+// of the last one's bin), one block sorts them and finishes alone.
+//
+// 256 rows of 150001 fp32 logits: 107 us without filters, 149 with top_k 50 and top_p, 220 with top_p alone (16000 tokens
+// kept of a row), where reading them takes 24; one row of 131072 in bf16 10.8, 15.3 and 27 us. A block's time there is 2 to 4 us for the
+// logits, 5 for weights and histogram, 2 a meeting of the cluster (1 of them the barrier), 1 to 2 a further pass over the weights. The large
+// case keeps 54% of issue slots busy with two blocks an SM, as many as 64 registers and the weights' room allow: instructions
+// bound it (28 a logit for weight and histogram), then the meetings, which the other block covers in part.
 #pragma once
 
 #include <cooperative_groups.h>
