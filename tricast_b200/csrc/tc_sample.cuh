@@ -202,8 +202,9 @@ struct Row {
   __device__ __forceinline__ int begin_of(int c) const { return c / kWarpChunks * run + c % kWarpChunks * span; }
   __device__ __forceinline__ int end_of(int c) const { return min(begin_of(c) + span, min((c / kWarpChunks + 1) * run, n)); }
 
-  // The cluster's barrier: what its threads wrote before is seen by those that read after.
+  // The cluster's barrier: what its threads wrote before is seen by those that read after. A warp's lanes come together for it.
   static __device__ __forceinline__ void meet() {
+    __syncwarp();
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   }
   // Another block's word (both of them where MASS) at an address of this one's shared memory.
@@ -446,7 +447,7 @@ struct Row {
   }
 
   // Where the `want` largest weights, with the rest of the last one's bin, are kList at most: they stand in the first block's list
-  // then, logits and places as one number, in no order. Otherwise `over` is unchanged and the histogram's bin is found again.
+  // then, logits and places as one number, in no order. Otherwise nothing is kept, and the counts are taken again.
   __device__ bool gather(double want, int64_t origin) {
     double over = 0.0, own;
     const int b = reach<false>([&] { return want; }, over, own, false, [](int) { return 0; });
