@@ -112,6 +112,23 @@ def test_activations(rows, K, activation, scheme, dtype):
     assert worst <= 1.0, worst
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("activation", ["silu", "gelu", "gelu_tanh"])
+@pytest.mark.parametrize("scheme, rows, K", [("int8_row", 3000, 4096), ("int8_row", 600, 16392), ("int8_row", 1000, 7781), ("group64", 3000, 4096)])
+def test_int8_codes_are_those_of_the_formula_step_by_step(scheme, rows, K, activation, dtype):
+    """Every operation of the formula rounded to fp32 by itself, the functions CUDA's: the same operations, so no code and no scale differs."""
+    spec = get_scheme("int8_row") if scheme == "int8_row" else get_scheme("int8_row").with_(granularity="group", group_size=64)
+    gate, up = halves(rows, K, dtype, seed=9)
+    g = gate.float()
+    if activation == "silu":
+        y = g / (1 + torch.exp(-g))
+    elif activation == "gelu":
+        y = 0.5 * g * (1 + torch.erf(g * math.sqrt(0.5)))
+    else:
+        y = 0.5 * g * (1 + torch.tanh(math.sqrt(2 / math.pi) * (g + 0.044715 * g * g * g)))
+    same(gated_quantize(gate, up, spec, activation=activation), quantize(y * up.float(), spec))
+
+
 @pytest.mark.parametrize("scheme", SCHEMES)
 @pytest.mark.parametrize("K", [64, 1000, 4096])
 def test_rows_that_are_not_finite(K, scheme):

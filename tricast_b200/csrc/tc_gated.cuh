@@ -2,10 +2,11 @@
 //   y = act(gate) * up,  codes = cast(y / s), s from amax |y| per row or per group of the row
 // in fp32. Activations: silu g / (1 + exp(-g)); gelu g * erfc(-g / sqrt 2) / 2, the same value as g (1 + erf) / 2 without
 // its cancellation; gelu_tanh g / (1 + exp(-2 z)), z = sqrt(2 / pi) (g + 0.044715 g**3), which is g (1 + tanh z) / 2; relu.
+// (INT8 codes: the forms with erf and tanh, see gate8.)
 //
 // 8192 rows of 12288 gates and as many ups in fp32, to MXFP8: 156 us, 5.8 TB/s (139 for the bytes; DRAM 76% busy); with a scale a row 161;
-// in bf16 134 and 154 (77 for the bytes: 65% of issue slots, the activation and cast bound it); gelu 245 (erfc). 333 rows of 1537 in
-// bf16 3.4 us.
+// in bf16 134 and 154 (77 for the bytes: 65% of issue slots, the activation and cast bound it); gelu 245 (erfc). INT8 with a scale a row
+// 194, in bf16 191 (gelu 217: its functions' instructions). 333 rows of 1537 in bf16 3.4 us.
 #pragma once
 
 #include "tc_cast8.cuh"
@@ -33,10 +34,43 @@ __device__ __forceinline__ float logistic(float g, float t) {
   return __fmul_rn(g, r);
 }
 
-// act(g) * u of eight elements.
+__device__ __forceinline__ float largest8(const float (&y)[8]) {
+  float m = 0.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) m = max_abs(m, y[e]);
+  return m;
+}
+
+// act(g) * u of eight elements. INT8 codes are whole numbers up to 127, of which the last bits of y move one in some hundred
+// thousands: for them (STEPS) y is what the formula gives with every step rounded by itself and CUDA's accurate functions.
+template <bool STEPS>
 __device__ __forceinline__ void gate8(float (&g)[8], const float (&u)[8], int act) {
   constexpr float kLog2E = 1.44269504f;
-  if (act == ACT_SILU) {
+  if (STEPS && act == ACT_SILU) {
+    if (largest8(g) <= 64.0f) {
+      // The quotient by divide_fast, whose reciprocal is one Newton step from the hardware's: 1 + exp(-g) is below 2**93.
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float d = __fadd_rn(1.0f, expf(-g[e]));
+        float r;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(d));
+        r = __fmaf_rn(__fmaf_rn(-d, r, 1.0f), r, r);
+        g[e] = divide_fast(g[e], d, r);
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) g[e] = __fdiv_rn(g[e], __fadd_rn(1.0f, expf(-g[e])));
+    }
+  } else if (STEPS && act == ACT_GELU) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) g[e] = __fmul_rn(__fmul_rn(0.5f, g[e]), __fadd_rn(1.0f, erff(__fmul_rn(g[e], 0.70710678f))));
+  } else if (STEPS && act == ACT_GELU_TANH) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float z = __fmul_rn(0.79788456f, __fadd_rn(g[e], __fmul_rn(__fmul_rn(__fmul_rn(0.044715f, g[e]), g[e]), g[e])));
+      g[e] = __fmul_rn(__fmul_rn(0.5f, g[e]), __fadd_rn(1.0f, tanhf(z)));
+    }
+  } else if (act == ACT_SILU) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) g[e] = logistic(g[e], __fmul_rn(g[e], -kLog2E));
   } else if (act == ACT_GELU) {
@@ -70,13 +104,6 @@ __device__ __forceinline__ uint2 encode_all(const float (&y)[8], const Scale &sc
     for (int k = 0; k < 4; ++k) q[k] = slow(y[2 * k]) | (slow(y[2 * k + 1]) << 8);
   }
   return make_uint2(q[0] | (q[1] << 16), q[2] | (q[3] << 16));
-}
-
-__device__ __forceinline__ float largest8(const float (&y)[8]) {
-  float m = 0.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) m = max_abs(m, y[e]);
-  return m;
 }
 
 // Eight neighbouring elements from c on, zeros behind the row.
@@ -119,7 +146,7 @@ __global__ void __launch_bounds__(kThreads) group_kernel(Args a, int64_t width) 
       fetch8<T, VEC>(static_cast<const T *>(a.gate) + r * a.gate_stride, c, a.K, y);
       fetch8<T, VEC>(static_cast<const T *>(a.up) + r * a.up_stride, c, a.K, u);
     }
-    gate8(y, u, a.act);
+    gate8<E == E8_INT8>(y, u, a.act);
     uint32_t top = abs_bits(largest8(y));
     for (int k = a.group >> 4; k; k >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
     const Scale sc = make_scale<POW2>(top, a);
@@ -153,7 +180,7 @@ __global__ void __launch_bounds__(1024) held_kernel(Args a) {
     float m = 0.0f;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      gate8(y[i], u[i], a.act);
+      gate8<E == E8_INT8>(y[i], u[i], a.act);
       m = max_abs(m, largest8(y[i]));
     }
     const uint32_t top = warp_max(abs_bits(m));
@@ -187,7 +214,7 @@ __global__ void __launch_bounds__(kThreads) row_kernel(Args a) {
         for (int e = 0; e < 8; ++e) y[e] = u[e] = 0.0f;
         fetch8<T, false>(gate, c, hi, y);
         fetch8<T, false>(up, c, hi, u);
-        gate8(y, u, a.act);
+        gate8<E == E8_INT8>(y, u, a.act);
       };
       float y[8];
       uint32_t m = 0u;
