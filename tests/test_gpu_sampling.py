@@ -196,6 +196,29 @@ def test_large_vocabularies(dtype):
     check(z, u, top_p=0.9)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("min_p", [None, 1e-3])
+def test_unfiltered_rows_of_large_vocabularies(dtype, min_p):
+    """Weights within 1.2e-10 move a share by 2.4e-10 at most, sums of n of them in 64 bits by n 2**-53: borders nearer than 4e-10 may
+    fall on either side, as may the bound. With 164724 tokens some row in ten thousand has such a border."""
+    rows, vocab = 256, 164724
+    z, u, g = make(rows, vocab, dtype)
+    w = torch.exp(z.double() - z.double().amax(1, keepdim=True))
+    if min_p is not None:
+        bound = float(np.float32(min_p))
+        assert not ((w / bound - 1).abs() < 1e-9).any()
+        w[w < bound] = 0.0
+    upto = w.cumsum(1)
+    share = upto / upto[:, -1:]
+    want = torch.searchsorted(share, u.double()[:, None], right=True)[:, 0].clamp(max=vocab - 1)
+    near = (share[:, :-1] - u.double()[:, None]).abs().amin(1) < 4e-10
+    assert near.sum() <= 1
+    tokens, logprobs = sample_tokens(z, u, min_p=min_p, return_logprobs=True)
+    assert torch.equal(tokens[~near], want[~near].to(tokens.dtype))
+    exact = (w.gather(1, tokens[:, None].long()) / upto[:, -1:]).log()[:, 0]
+    assert ((logprobs.double() - exact).abs() <= 2.0 ** -24 * exact.abs() + 1e-9).all()
+
+
 @pytest.mark.parametrize("vocab", [513, 5000, 60000])
 def test_sets_as_long_as_one_block_finishes(vocab):
     """Around 512 tokens, below and above which other code ends the work; runs of equals that pass it."""

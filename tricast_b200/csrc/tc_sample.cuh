@@ -11,8 +11,8 @@
 // in two 32-bit words; totals are fp64 sums in a fixed order. Nothing depends on timing. Where top_k leaves few tokens (kList with the rest
 // of the last one's bin), one block sorts them and finishes alone.
 //
-// 256 rows of 150001 fp32 logits: 107 us without filters, 149 with top_k 50 and top_p, 220 with top_p alone (16000 tokens
-// kept of a row), where reading them takes 24; one row of 131072 in bf16 10.8, 15.3 and 27 us. A block's time there is 2 to 4 us for the
+// 256 rows of 150001 fp32 logits: 114 us without filters, 149 with top_k 50 and top_p, 220 with top_p alone (16000 tokens
+// kept of a row), where reading them takes 24; one row of 131072 in bf16 12.3, 15.3 and 27 us. A block's time there is 2 to 4 us for the
 // logits, 5 for weights and histogram, 2 a meeting of the cluster (1 of them the barrier), 1 to 2 a further pass over the weights. The large
 // case keeps 54% of issue slots busy with two blocks an SM, as many as 64 registers and the weights' room allow: instructions
 // bound it (28 a logit for weight and histogram), then the meetings, which the other block covers in part.
@@ -107,6 +107,24 @@ struct Weight {
     q = __fmaf_rn(q, g, 9.8025817e-1f);
     q = __fmaf_rn(q, g, 1.4142135f);
     return l >= least ? u2f(f2u(q) + (y & 0xFF800000u)) : 0.0f;
+  }
+  // The same to 2e-10, in fp64, for rows without top-k and top-p: those keep up to all of their tokens, hundreds of thousands of borders, which a
+  // 16-bit type's few distinct logits (each with its own error) would shift together; no step needs such a weight's bits. 2**g, g the
+  // distance to the nearest whole number, is 1 + g p(g), p of degree 6 through (2**g - 1) / g at Chebyshev's nodes (error 1.1e-10): 1 at
+  // the largest logit, so that a bound of 1 keeps it.
+  __device__ __forceinline__ double precise(float l) const {
+    const double y = ((double)l - top) * c, t = y + 6755399441055744.0;  // 1.5 * 2**52: the whole number in the low word
+    const double g = y - (t - 6755399441055744.0);
+    double q = 1.529732318378528e-05;
+    q = fma(q, g, 0.00015461444698744708);
+    q = fma(q, g, 0.0013333502388099057);
+    q = fma(q, g, 0.009618056678519811);
+    q = fma(q, g, 0.05550410883908015);
+    q = fma(q, g, 0.24022650922288794);
+    q = fma(q, g, 0.6931471805599454);
+    q = fma(q, g, 1.0);
+    const double w = __hiloint2double(__double2hiint(q) + (__double2loint(t) << 20), __double2loint(q));
+    return l >= least ? w : 0.0;
   }
   // log(w), in fp64.
   __device__ __forceinline__ double log(float l) const { return ((double)l - top) * c * 0.6931471805599453; }
@@ -579,14 +597,13 @@ struct Row {
   }
 
   // Weights in the logits' place, the chunks' largest, this thread's part of their sum, and the histogram that the first
-  // filter begins with (FIRST: 1 counts, 2 masses); 0: no filter but a bound of the weights, so the chunks' sums of those above `cut`.
-  template <int FIRST>
-  __device__ __forceinline__ double prepare(uint32_t cut) {
+  // filter begins with: of counts, or of masses.
+  template <bool MASS>
+  __device__ __forceinline__ double prepare() {
     const int lane = threadIdx.x & 31;
     double sum = 0.0;
     chunks([&](int c, int at, int end) {
       uint32_t top = 0u;
-      if (!FIRST) sum = 0.0;
       steps(at, end, [&](int i) {
         float4 q;
         if (HELD) {
@@ -596,32 +613,42 @@ struct Row {
         } else {
           q = four(i);
         }
-        if (!FIRST) {
-          auto kept = [&](float v) { return f2u(v) > cut ? v : 0.0f; };
-          q = make_float4(kept(q.x), kept(q.y), kept(q.z), kept(q.w));
-        }
         sum += (double)__fadd_rn(__fadd_rn(q.x, q.y), __fadd_rn(q.z, q.w));
-        if (!FIRST) return;
         const uint32_t u[4] = {f2u(q.x), f2u(q.y), f2u(q.z), f2u(q.w)};
         top = max(max(max(u[0], u[1]), max(u[2], u[3])), top);
-        if (FIRST)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int b = bin_of(u[k], 0);
-            add<FIRST == 2>(b, u[k], b < kBins);
-          }
+        for (int k = 0; k < 4; ++k) {
+          const int b = bin_of(u[k], 0);
+          add<MASS>(b, u[k], b < kBins);
+        }
       });
-      if (FIRST) {
-        top = warp_max(top);
-        if (lane == 0) sh.peak[c] = top;
-      } else {
-#pragma unroll
-        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
-        if (lane == 0) sh.mass[c] = sum, sh.ties[c] = 0;
-      }
+      top = warp_max(top);
+      if (lane == 0) sh.peak[c] = top;
     });
     __syncwarp();
     return sum;
+  }
+
+  // No filter but a bound of the weights: logits stay, and the chunks' sums are of precise weights.
+  __device__ __forceinline__ float4 logits(int i) const {
+    float4 l = HELD ? *reinterpret_cast<const float4 *>(held + i) : z.load(i);
+    if (!HELD && infinite) l = make_float4(finite(l.x), finite(l.y), finite(l.z), finite(l.w));
+    return l;
+  }
+  static __device__ __forceinline__ double bounded(double w, float bound) { return w < (double)bound ? 0.0 : w; }
+  __device__ __forceinline__ void sum_all(float bound) {
+    const int lane = threadIdx.x & 31;
+    chunks([&](int c, int at, int end) {
+      double sum = 0.0;
+      steps(at, end, [&](int i) {
+        const float4 l = logits(i);
+        auto kept = [&](float v) { return bounded(w.precise(v), bound); };
+        sum += (kept(l.x) + kept(l.y)) + (kept(l.z) + kept(l.w));
+      });
+#pragma unroll
+      for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, x);
+      if (lane == 0) sh.mass[c] = sum, sh.ties[c] = 0;
+    });
   }
 };
 
@@ -706,8 +733,12 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
     const bool by_count = k > 0 && k < a.vocab, by_mass = p < 1.0f;
     const float bound = low > 1.0f ? 1.0f : low;  // NaN bounds nothing
     // Kept: weights above `cut`, and of the tokens at it the first m.
-    uint32_t cut = bound > 0.0f ? f2u(bound) - 1 : 0u;
-    double sum = by_count ? row.template prepare<1>(cut) : by_mass ? row.template prepare<2>(cut) : row.template prepare<0>(cut);
+    uint32_t cut = 0u;
+    double sum = 0.0;
+    const bool bare = !by_count && !by_mass;
+    if (by_count) sum = row.template prepare<false>();
+    else if (by_mass) sum = row.template prepare<true>();
+    else row.sum_all(bound);
     bool counted = by_count;  // whether the histogram of counts still stands
     if (by_count && k <= kList) {
       if (row.gather((double)k, origin)) {
@@ -716,7 +747,6 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
       }
       counted = false;
     }
-    if (by_count || by_mass) cut = 0u;
     double m = 0.0, equals = 0.0, over;
     if (by_count && row.template cut<false>([&] { return (double)k; }, 1u, counted, cut, over, equals)) m = (double)k - over;
     if (by_mass) {
@@ -775,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
     };
 
     // Masses and ties by chunks.
-    if (by_count || by_mass) row.chunks([&](int c, int at, int end) {
+    if (!bare) row.chunks([&](int c, int at, int end) {
       double s = 0.0;
       int e = 0;
       const uint32_t peak = shared.peak[c];
@@ -885,15 +915,16 @@ __global__ void __launch_bounds__(kThreads, 2) sample_kernel(Args a) {
       // Its tokens, 32 at a time.
       for (int i0 = row.begin_of(chunk); found < 0 && i0 < row.end_of(chunk); i0 += 32) {
         const int i = i0 + lane;
-        const float4 q = row.four(i & ~3);
+        const float4 q = bare ? row.logits(i & ~3) : row.four(i & ~3);
         const float v = (i & 2) ? ((i & 1) ? q.w : q.z) : (i & 1) ? q.y : q.x;
-        bool keep = f2u(v) > cut, mine = false;
+        double x = bare ? Row<T, HELD>::bounded(row.w.precise(v), bound) : (double)v;
+        bool keep = bare ? x > 0.0 : f2u(v) > cut, mine = false;
         if (some && !keep) mine = equal(i, f2u(v), keep);
         const unsigned same = __ballot_sync(0xFFFFFFFFu, mine);
         if (mine) keep = __popc(same & ((1u << lane) - 1u)) < room;
         room = max(room - __popc(same), 0);
         const unsigned mask = __ballot_sync(0xFFFFFFFFu, keep);
-        double x = keep ? (double)v : 0.0;
+        if (!keep) x = 0.0;
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
           const double o = __shfl_up_sync(0xFFFFFFFFu, x, d);
