@@ -154,6 +154,26 @@ def test_far_gates(activation):
     assert torch.isfinite(got).all() and (off <= 1e-5 * want.abs() + 1e-37).all(), off
 
 
+def test_the_curve_of_gelu():
+    """A group of one element has |y| / 448 as its scale. e = 2**-24. t = 1 / (1 + 0.3 a): 3 e, by at most 2.7 (the polynomial's t p' / p
+    at a = 0) 8 e; fit and Horner 3 e, exponential 4 e, its rounded argument a**2 / 2 * 3 e, which times |y| is below e |g|; two products
+    and the scale's division 3 e: 18 e |y| + e |g|, and 2**-120 where the exponential is flushed."""
+    g = torch.cat([torch.linspace(-14, 14, 400001), -torch.logspace(-30, 1.1, 100000), torch.logspace(-30, 30, 100000)]).cuda()[:, None]
+    q = gated_quantize(g, torch.ones_like(g), get_scheme("fp8_group128").with_(group_size=1), activation="gelu")
+    got, g = q.scale.double() * 448, g.double()
+    want = (g * torch.special.ndtr(g)).abs()
+    real = want > 1e-35
+    e = 2.0 ** -24
+    assert ((got - want).abs() <= 18 * e * want + e * g.abs() + 2.0 ** -120)[real].all()
+    ends = torch.tensor([[0.0, -0.0, -5.0, -1e30, 5.0, 1e30, -20.0]], device="cuda")
+    q = gated_quantize(ends, torch.ones_like(ends), "fp8_row", activation="gelu").values.float()
+    assert torch.signbit(q).tolist() == [[False, True, True, True, False, False, True]]
+    for inf, want in ((math.inf, math.inf), (-math.inf, math.nan), (math.nan, math.nan)):
+        s = gated_quantize(torch.full((1, 8), inf, device="cuda"), torch.ones(1, 8, device="cuda"), "fp8_row", activation="gelu").scale
+        ref = quantize(torch.full((1, 8), want, device="cuda"), "fp8_row").scale
+        assert torch.equal(s.nan_to_num(9e9), ref.nan_to_num(9e9))
+
+
 def test_strides_and_offsets():
     spec = get_scheme("mxfp8_e4m3")
     for dtype in DTYPES:
