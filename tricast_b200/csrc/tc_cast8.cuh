@@ -55,6 +55,21 @@ inline int cast8_spec(const tc_quant_spec *spec, int64_t K, const char *what, in
   return TC_OK;
 }
 
+// Eight 16-bit elements as fp32.
+template <typename T>
+__device__ __forceinline__ void widen8(uint4 w, float (&v)[8]) {
+  const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    if constexpr (Same<T, __nv_bfloat16>::value) {
+      v[2 * k] = u2f(u[k] << 16);
+      v[2 * k + 1] = u2f(u[k] & 0xFFFF0000u);
+    } else {
+      v[2 * k] = __half2float(__ushort_as_half((unsigned short)(u[k] & 0xFFFFu)));
+      v[2 * k + 1] = __half2float(__ushort_as_half((unsigned short)(u[k] >> 16)));
+    }
+  }
+}
 // Eight elements as fp32, from 16-bit or fp32 memory at a 16-byte boundary.
 template <typename T>
 __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
@@ -62,18 +77,7 @@ __device__ __forceinline__ void load8(const T *p, float (&v)[8]) {
     const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
     v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
   } else {
-    const uint4 w = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if constexpr (Same<T, __nv_bfloat16>::value) {
-        v[2 * k] = u2f(u[k] << 16);
-        v[2 * k + 1] = u2f(u[k] & 0xFFFF0000u);
-      } else {
-        v[2 * k] = __half2float(__ushort_as_half((unsigned short)(u[k] & 0xFFFFu)));
-        v[2 * k + 1] = __half2float(__ushort_as_half((unsigned short)(u[k] >> 16)));
-      }
-    }
+    widen8<T>(*reinterpret_cast<const uint4 *>(p), v);
   }
 }
 template <typename T>

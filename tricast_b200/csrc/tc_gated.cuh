@@ -4,9 +4,9 @@
 // its cancellation; gelu_tanh g / (1 + exp(-2 z)), z = sqrt(2 / pi) (g + 0.044715 g**3), which is g (1 + tanh z) / 2; relu.
 // (INT8 codes: the forms with erf and tanh, see gate8.)
 //
-// 8192 rows of 12288 gates and as many ups in fp32, to MXFP8: 156 us, 5.8 TB/s (139 for the bytes; DRAM 76% busy); with a scale a row 161;
-// in bf16 134 and 154 (77 for the bytes: 65% of issue slots, the activation and cast bound it); gelu 163. INT8 with a scale a row
-// 194, in bf16 191 (gelu 217: its functions' instructions). 333 rows of 1537 in bf16 3.4 us.
+// 8192 rows of 12288 gates and as many ups in fp32, to MXFP8: 156 us, 5.8 TB/s (139 for the bytes; DRAM 76% busy); with a scale a row 157;
+// in bf16 134 and 105 (77 for the bytes; 154 without the next row under way); gelu 163. INT8 with a scale a row
+// 184, in bf16 135 (gelu 162: its functions' instructions). 333 rows of 1537 in bf16 3.4 us.
 #pragma once
 
 #include "tc_cast8.cuh"
@@ -181,22 +181,43 @@ __global__ void __launch_bounds__(kThreads) group_kernel(Args a, int64_t width) 
   }
 }
 
-// One scale a row, which a block's registers hold: NV vectors of 8 neighbouring elements a thread.
+// One scale a row, which a block's registers hold: NV vectors of 8 neighbouring elements a thread. Vectors of 16-bit elements are small
+// enough to hold the next row's too: its loads are under way while this row's maximum is agreed on and its codes are written.
 template <typename T, int E, int NV, bool VEC, bool POW2>
 __global__ void __launch_bounds__(1024) held_kernel(Args a) {
+  constexpr bool AHEAD = VEC && sizeof(T) == 2;
   __shared__ uint32_t tops[2][32];
   const int tid = threadIdx.x, lane = tid & 31, warps = blockDim.x >> 5, threads = blockDim.x;
   int flip = 0;  // the two halves of the exchange buffer alternate, so one barrier a row suffices
+  uint4 next[AHEAD ? NV : 1][2];
+  auto ahead = [&](int64_t r) {
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const int64_t c = (int64_t)(tid + i * threads) * 8;
+        next[i][0] = next[i][1] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < a.rows && c < a.K) {
+          next[i][0] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.gate) + r * a.gate_stride + c);
+          next[i][1] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.up) + r * a.up_stride + c);
+        }
+      }
+    }
+  };
+  ahead(blockIdx.x);
   for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x, flip ^= 1) {
-    const T *gate = static_cast<const T *>(a.gate) + r * a.gate_stride, *up = static_cast<const T *>(a.up) + r * a.up_stride;
     float y[NV][8], u[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
+      if constexpr (AHEAD) {
+        widen8<T>(next[i][0], y[i]);
+        widen8<T>(next[i][1], u[i]);
+      } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) y[i][e] = u[i][e] = 0.0f;
-      const int64_t c = (int64_t)(tid + i * threads) * 8;
-      fetch8<T, VEC>(gate, c, a.K, y[i]);
-      fetch8<T, VEC>(up, c, a.K, u[i]);
+        for (int e = 0; e < 8; ++e) y[i][e] = u[i][e] = 0.0f;
+        const int64_t c = (int64_t)(tid + i * threads) * 8;
+        fetch8<T, VEC>(static_cast<const T *>(a.gate) + r * a.gate_stride, c, a.K, y[i]);
+        fetch8<T, VEC>(static_cast<const T *>(a.up) + r * a.up_stride, c, a.K, u[i]);
+      }
     }
     float m = 0.0f;
 #pragma unroll
@@ -204,6 +225,7 @@ __global__ void __launch_bounds__(1024) held_kernel(Args a) {
       gate8<E == E8_INT8>(y[i], u[i], a.act);
       m = max_abs(m, largest8(y[i]));
     }
+    ahead(r + gridDim.x);
     const uint32_t top = warp_max(abs_bits(m));
     if (lane == 0) tops[flip][tid >> 5] = top;
     __syncthreads();
@@ -267,12 +289,11 @@ static void launch_scale(const Args &a, bool lanes, cudaStream_t s) {
     group_kernel<T, E, VEC, POW2><<<(unsigned)(blocks < most ? blocks : most), kThreads, 0, s>>>(a, width);
   } else {
     const int64_t vectors = (a.K + 7) / 8;
-    int threads = 64;
-    while (threads < 512 && threads < vectors) threads *= 2;
-    while (threads < 1024 && threads * 2 < vectors) threads *= 2;
+    // One vector a thread up to 512, two beyond; whole warps, so that at most one of them is partly idle.
+    const int threads = (int)(((vectors <= 512 ? vectors : (vectors + 1) / 2) + 31) / 32 * 32);
     const int64_t most = (int64_t)sm_count() * (2048 / threads);
     const unsigned grid = (unsigned)(a.rows < most ? a.rows : most);
-    if (vectors <= threads) held_kernel<T, E, 1, VEC, POW2><<<grid, threads, 0, s>>>(a);
+    if (vectors <= 512) held_kernel<T, E, 1, VEC, POW2><<<grid, threads, 0, s>>>(a);
     else held_kernel<T, E, 2, VEC, POW2><<<grid, threads, 0, s>>>(a);
   }
   count_launch();
