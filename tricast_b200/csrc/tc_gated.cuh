@@ -105,7 +105,7 @@ __device__ __forceinline__ void gate8(float (&g)[8], const float (&u)[8], int ac
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) g[e] = g[e] > 0.0f ? g[e] : g[e] != g[e] ? g[e] : 0.0f;
+    for (int e = 0; e < 8; ++e) asm("max.NaN.f32 %0, %0, 0f00000000;" : "+f"(g[e]));
   }
 #pragma unroll
   for (int e = 0; e < 8; ++e) g[e] = __fmul_rn(g[e], u[e]);
@@ -156,28 +156,46 @@ __global__ void __launch_bounds__(kThreads) group_kernel(Args a, int64_t width) 
   const int64_t step = (int64_t)gridDim.x * kThreads, start = (int64_t)blockIdx.x * kThreads + threadIdx.x;
   const int64_t rows_a_step = step / width, rest = step - rows_a_step * width;
   int64_t r = start / width, v = start - r * width;
+  constexpr bool AHEAD = VEC && sizeof(T) == 2;  // as in held_kernel
+  uint4 next[2];
+  auto ahead = [&](int64_t r, int64_t c) {
+    if constexpr (AHEAD) {
+      next[0] = next[1] = make_uint4(0u, 0u, 0u, 0u);
+      if (r < a.rows && c < a.K) {
+        next[0] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.gate) + r * a.gate_stride + c);
+        next[1] = *reinterpret_cast<const uint4 *>(static_cast<const T *>(a.up) + r * a.up_stride + c);
+      }
+    }
+  };
+  ahead(r, v * 8);
   // A warp's lanes go on together: some may be behind the last row.
   for (int64_t base = start - (threadIdx.x & 31); base < a.rows * width; base += step) {
     const bool real = r < a.rows;
-    const int64_t c = v * 8;
+    const int64_t c = v * 8, row = r;
     float y[8], u[8];
+    if constexpr (AHEAD) {
+      widen8<T>(next[0], y);
+      widen8<T>(next[1], u);
+    } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = u[e] = 0.0f;
-    if (real) {
-      fetch8<T, VEC>(static_cast<const T *>(a.gate) + r * a.gate_stride, c, a.K, y);
-      fetch8<T, VEC>(static_cast<const T *>(a.up) + r * a.up_stride, c, a.K, u);
+      for (int e = 0; e < 8; ++e) y[e] = u[e] = 0.0f;
+      if (real) {
+        fetch8<T, VEC>(static_cast<const T *>(a.gate) + r * a.gate_stride, c, a.K, y);
+        fetch8<T, VEC>(static_cast<const T *>(a.up) + r * a.up_stride, c, a.K, u);
+      }
     }
+    r += rows_a_step;
+    v += rest;
+    if (v >= width) v -= width, ++r;
+    ahead(r, v * 8);
     gate8<E == E8_INT8>(y, u, a.act);
     uint32_t top = abs_bits(largest8(y));
     for (int k = a.group >> 4; k; k >>= 1) top = max(top, __shfl_xor_sync(0xFFFFFFFFu, top, k));
     const Scale sc = make_scale<POW2>(top, a);
     if (real && c < a.K) {
-      if ((c & (a.group - 1)) == 0) store_scale<POW2>(a, r * a.groups + (c >> a.group_shift), sc);
-      put8<VEC>(a.codes + r * a.K, c, a.K, encode_all<E, POW2>(y, sc));
+      if ((c & (a.group - 1)) == 0) store_scale<POW2>(a, row * a.groups + (c >> a.group_shift), sc);
+      put8<VEC>(a.codes + row * a.K, c, a.K, encode_all<E, POW2>(y, sc));
     }
-    r += rows_a_step;
-    v += rest;
-    if (v >= width) v -= width, ++r;
   }
 }
 
