@@ -4,9 +4,10 @@
 // its cancellation; gelu_tanh g / (1 + exp(-2 z)), z = sqrt(2 / pi) (g + 0.044715 g**3), which is g (1 + tanh z) / 2; relu.
 // (INT8 codes: the forms with erf and tanh, see gate8.)
 //
-// 8192 rows of 12288 gates and as many ups in fp32, to MXFP8: 156 us, 5.8 TB/s (139 for the bytes; DRAM 76% busy); with a scale a row 157;
-// in bf16 134 and 105 (77 for the bytes; 154 without the next row under way); gelu 163. INT8 with a scale a row
-// 184, in bf16 135 (gelu 162: its functions' instructions). 333 rows of 1537 in bf16 3.4 us.
+// 8192 rows of 12288 gates and as many ups in fp32, to MXFP8: 154 us, 5.9 TB/s (139 for the bytes; DRAM 76% busy), gelu 164; with a scale
+// a row 153, gelu 172; in bf16 116 and 103 (77 for the bytes; 134 and 154 without the loads ahead), where relu takes 82: activation
+// and cast bound it; groups of 128 with fp32 scales 135 (each lane divides for its group's). INT8 with a scale a row 184, in bf16 135
+// (gelu 202 and 162: its functions' instructions). 333 rows of 1537 in bf16 3.1 us.
 #pragma once
 
 #include "tc_cast8.cuh"
