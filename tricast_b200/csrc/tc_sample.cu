@@ -12,8 +12,12 @@ constexpr int64_t kMaxHeld = 53248;     // weights that a block's shared memory 
 template <typename T, bool HELD>
 static cudaError_t launch_as(const Args &a, cudaStream_t s) {
   const size_t bytes = HELD ? (size_t)a.part * sizeof(float) : 0;
-  cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-  if (e != cudaSuccess) return e;
+  // The attribute belongs to the kernel, which other host threads may be launching with stretches of another length: always the largest.
+  if (HELD) {
+    const cudaError_t e = cudaFuncSetAttribute(sample_kernel<T, HELD>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               (int)(kMaxHeld * sizeof(float)));
+    if (e != cudaSuccess) return e;
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(a.rows * a.blocks));
   cfg.blockDim = dim3(kThreads);
