@@ -188,7 +188,7 @@ struct Tile {
   int index[8 * NG], adapters[8 * NG];
   uint32_t members[8 * NG];  // of each distinct adapter, the groups of 8 tokens that it has
   int distinct;
-  uint32_t peak[8 * NG];     // fp16: of each token, the largest |h|
+  uint32_t peak[8 * NG];     // fp16: of each token, the largest |h| that is finite
 
   // One warp.
   __device__ __forceinline__ void fill(const Args &a, int64_t t0, int tokens) {
@@ -311,6 +311,9 @@ __device__ __forceinline__ void sum_rows(const Args &a, const Tile<NG> &tile, in
 // Floats of `part`, its splits included.
 __host__ __device__ __forceinline__ size_t part_floats(int ng, int rw, int rows) { return (size_t)(kWarps / (rows / rw)) * 8 * ng * rows; }
 
+// Of a number's magnitude the bits, 0 of what is not finite: what the power of two of fp16 parts goes by.
+__device__ __forceinline__ uint32_t finite_bits(float v) { return abs_bits(v) < 0x7F800000u ? abs_bits(v) : 0u; }
+
 // h in parts of 16 bits, each the rounded rest of the one before, `apart` elements from one another.
 template <typename T>
 __device__ __forceinline__ void split_parts(float v, int terms, uint16_t *to, int apart) {
@@ -409,14 +412,14 @@ __global__ void __launch_bounds__(kThreads, 2) tile_kernel(Args a) {
     for (int e = tid; e < kTokens * rows; e += kThreads) {
       const int t = e / rows, r = e - t * rows, who = tile.index[t];
       float x = 0.0f;
-      if (who >= 0) {
+      if (who >= 0 && r < a.rank) {  // 0 behind the rank: there A's zeros would make NaN of an infinite x
         for (int b = 0; b < blocks; ++b) x = __fadd_rn(x, *cluster.map_shared_rank(part + e, b));
         float f = a.x_scale ? a.x_scale[t0 + t] : 1.0f;
         if (a.gain) f = __fmul_rn(f, a.gain[who]);
         x = __fmul_rn(x, f);
       }
       if (kBf16) split_parts<T>(x, terms, parts + t * row_stride + r, kTokens * row_stride);
-      else full[e] = x, atomicMax(&tile.peak[t], abs_bits(x));
+      else full[e] = x, atomicMax(&tile.peak[t], finite_bits(x));
     }
     __syncthreads();
     if (!kBf16) {
@@ -498,8 +501,8 @@ __global__ void __launch_bounds__(kThreads, RW == 16 ? 4 : 3) down_kernel(Args a
 #pragma unroll
     for (int i = 0; i < kMaxRank / 32; ++i) {
       const int r = lane + 32 * i;
-      v[i] = r < rows ? sum(t * rows + r, t, who) : 0.0f;
-      if (!kBf16) top = fmaxf(top, u2f(abs_bits(v[i])));
+      v[i] = r < a.rank ? sum(t * rows + r, t, who) : 0.0f;  // as above
+      if (!kBf16) top = fmaxf(top, u2f(finite_bits(v[i])));
     }
     float factor = 1.0f;
     if (!kBf16) {
