@@ -21,7 +21,8 @@ def low_rank_add(y: torch.Tensor, x, a: torch.Tensor, b: torch.Tensor, index: to
 
     The products and the sum are fp32, rounded once to ``dtype`` (default ``y``'s). Weights of 16 bits with ``x`` of their type or 8-bit
     codes, ``y`` and ``dtype`` of their type or fp32, and ranks up to 128 go through the tensor cores, anything else element by
-    element. Any order of tokens is allowed; those of one adapter that stand together share its weights' way through the
+    element. What a token gets depends on no other token's values or adapter, to the bit, but sums are cut by how many tokens there are. Any
+    order of tokens is allowed; those of one adapter that stand together share its weights' way through the
     chip. More than some 250 tokens take scratch memory (up to 6 bytes a token and rank) while they run. No gradients pass:
     the output is detached."""
     if not y.is_cuda:

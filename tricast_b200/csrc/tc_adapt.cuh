@@ -2,10 +2,11 @@
 //   out[t] = y[t] + gain[i] * B[i] (A[i] x[t]),  i = index[t]  (out[t] = y[t] where i names no adapter)
 // x in 16 or 32 bits, or 8-bit codes with a scale a row; the products and their sum are fp32, out is rounded once.
 //
-// Measured: one token 4096 -> 6144, rank 16, fp32 to bf16 6.2 us; 64 tokens with as many adapters 4096 -> 4096, rank 32 14.5 us (5.5 for
-// the bytes: waits for loads that follow one another, index, then A, then B); 8192 tokens of E4M3 codes 4096 -> 12288 160 us (4.0 TB/s;
-// 98 for the bytes): 33 the first kernel, whose issue slots are 42% busy with widening codes and MMAs while loads are waited for, 125
-// the second, 16 warps an SM that wait for y. Rank 32 193 us, rank 64 283. Tokens whose adapters alternate cost their products each: 360 us.
+// Measured: one token 4096 -> 6144, rank 16, fp32 to bf16 6.2 us; 64 tokens with as many adapters 4096 -> 4096, rank 32 12.6 us (5.5 for
+// the bytes: waits for loads that follow one another, index, then A, then B); 8192 tokens of E4M3 codes 4096 -> 12288 157 us (4.1 TB/s;
+// 98 for the bytes): 33 the first kernel, whose issue slots are 42% busy with widening codes and MMAs while loads are waited for, 124
+// the second, 16 warps an SM that wait for y. Rank 32 194 us, rank 64 282. Tokens whose adapters alternate cost their products each: 374 us
+// (360 with sums whose order goes by the number of adapters in the tile).
 #pragma once
 
 #include <cooperative_groups.h>
@@ -224,7 +225,8 @@ struct Tile {
   }
 };
 
-// How many warps share a sum over k: as many as there are for every adapter (one at least) and block of RW rows of A.
+// How many warps share a sum over k: as many as there are for every adapter (one at least) and block of RW rows of A. The sum itself
+// is always cut into the slots that a single adapter has, which its warps take in turn: how many adapters a tile holds changes no token's bits.
 __device__ __forceinline__ int splits_of(int count, int row_blocks) {
   int splits = kWarps;
   while (splits > 1 && splits * count * row_blocks > kWarps) splits >>= 1;
@@ -242,69 +244,88 @@ __device__ __forceinline__ void sum_rows(const Args &a, const Tile<NG> &tile, in
   constexpr bool kBf16 = Same<T, __nv_bfloat16>::value;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const uint16_t *A = static_cast<const uint16_t *>(a.a);
-  const int rows = RW == 16 ? 16 : rank_rows(a.rank), row_blocks = RW == 16 ? 1 : rows / RW, count = tile.distinct, splits = splits_of(count, row_blocks);
+  const int rows = RW == 16 ? 16 : rank_rows(a.rank), row_blocks = RW == 16 ? 1 : rows / RW, count = tile.distinct;
+  const int splits = splits_of(count, row_blocks), slots = splits_of(1, row_blocks);
+  const int first = (int)c0, end = (int)c1;  // below 2**26
   for (int item = warp; item < count * row_blocks * splits; item += kWarps) {
     const int s = item % splits, rb = item / splits % row_blocks, j = item / splits / row_blocks;
     const int who = tile.adapters[j];
     const uint32_t has = tile.members[j];
     float acc[NG][kRowTiles][4];
-#pragma unroll
-    for (int i = 0; i < NG; ++i)
-#pragma unroll
-      for (int r = 0; r < kRowTiles; ++r) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.0f;
-    constexpr int kAtOnce = NG == 1 ? 4 : 2;  // steps whose loads are on their way together
-#pragma unroll kAtOnce
-    for (int64_t c = c0 + s; c < c1; c += splits) {
-      const int64_t k = c * 32 + q * 8;
-      uint32_t w[kRowTiles][2][4], x[NG][4];
-#pragma unroll
-      for (int r = 0; r < kRowTiles; ++r)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int row = rb * RW + r * 16 + h * 8 + g;
-          load16<8, VEC>(A + ((int64_t)who * a.rank + row) * a.k, k, row < a.rank ? a.k : 0, w[r][h]);
-        }
-#pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0u;
-        if ((has >> i & 1u) && i * 8 + g < tokens) load_x<CODES, VEC>(a, t0 + i * 8 + g, k, x[i]);
-      }
-      if (CODES) {  // after every load is on its way
-#pragma unroll
-        for (int i = 0; i < NG; ++i) {
-          const uint4 v = widen<T>(make_uint2(x[i][0], x[i][1]), a.x_kind);
-          x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
-        }
-      }
+    auto clear = [&] {
 #pragma unroll
       for (int i = 0; i < NG; ++i)
-        if (has >> i & 1u)
+#pragma unroll
+        for (int r = 0; r < kRowTiles; ++r) acc[i][r][0] = acc[i][r][1] = acc[i][r][2] = acc[i][r][3] = 0.0f;
+    };
+    clear();
+    constexpr int kAtOnce = !VEC ? 1 : NG == 2 ? 2 : RW == 16 ? 4 : 2;  // steps whose loads are on their way together
+    int slot = s, c = first + s;
+    while (slot < slots) {
+      uint32_t w[kAtOnce][kRowTiles][2][4], x[kAtOnce][NG][4];
+      int of[kAtOnce];     // the slot of each step, and whether it is its slot's last (an empty slot has one step, of zeros)
+      bool last[kAtOnce];
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        const int64_t k = (int64_t)c * 32 + q * 8;
+        const bool live = slot < slots && c < end;
+#pragma unroll
+        for (int r = 0; r < kRowTiles; ++r)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = rb * RW + r * 16 + h * 8 + g;
+            load16<8, VEC>(A + ((int64_t)who * a.rank + row) * a.k, k, live && row < a.rank ? a.k : 0, w[u][r][h]);
+          }
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          x[u][i][0] = x[u][i][1] = x[u][i][2] = x[u][i][3] = 0u;
+          if (live && (has >> i & 1u) && i * 8 + g < tokens) load_x<CODES, VEC>(a, t0 + i * 8 + g, k, x[u][i]);
+        }
+        of[u] = slot;
+        c += slots;
+        last[u] = c >= end;
+        if (last[u]) slot += splits, c = first + slot;
+      }
+#pragma unroll
+      for (int u = 0; u < kAtOnce; ++u) {
+        if (of[u] >= slots) break;
+#pragma unroll
+        for (int i = 0; i < NG; ++i) {
+          if (!(has >> i & 1u)) continue;
+          if (CODES) {  // after every load is on its way
+            const uint4 v = widen<T>(make_uint2(x[u][i][0], x[u][i][1]), a.x_kind);
+            x[u][i][0] = v.x, x[u][i][1] = v.y, x[u][i][2] = v.z, x[u][i][3] = v.w;
+          }
 #pragma unroll
           for (int r = 0; r < kRowTiles; ++r)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              const uint32_t f[4] = {w[r][0][2 * h], w[r][1][2 * h], w[r][0][2 * h + 1], w[r][1][2 * h + 1]};
-              mma16<kBf16>(acc[i][r], f, x[i][2 * h], x[i][2 * h + 1]);
-            }
-    }
-#pragma unroll
-    for (int i = 0; i < NG; ++i)
-      if (has >> i & 1u)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int t = i * 8 + q * 2 + e;
-          if (tile.index[t] == who)
-#pragma unroll
-            for (int r = 0; r < kRowTiles; ++r) {
-              float *to = part + ((int64_t)s * kTokens + t) * rows + rb * RW + r * 16 + g;
-              to[0] = acc[i][r][e], to[8] = acc[i][r][2 + e];
+              const uint32_t f[4] = {w[u][r][0][2 * h], w[u][r][1][2 * h], w[u][r][0][2 * h + 1], w[u][r][1][2 * h + 1]};
+              mma16<kBf16>(acc[i][r], f, x[u][i][2 * h], x[u][i][2 * h + 1]);
             }
         }
+        if (!last[u]) continue;
+#pragma unroll
+        for (int i = 0; i < NG; ++i)
+          if (has >> i & 1u)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int t = i * 8 + q * 2 + e;
+              if (tile.index[t] == who)
+#pragma unroll
+                for (int r = 0; r < kRowTiles; ++r) {
+                  float *to = part + ((int64_t)of[u] * kTokens + t) * rows + rb * RW + r * 16 + g;
+                  to[0] = acc[i][r][e], to[8] = acc[i][r][2 + e];
+                }
+            }
+        clear();
+      }
+    }
   }
   __syncthreads();
   for (int e = tid; e < kTokens * rows; e += kThreads) {
     float v = 0.0f;
-    for (int s = 0; s < splits; ++s) v = __fadd_rn(v, part[s * kTokens * rows + e]);
+    for (int s = 0; s < slots; ++s) v = __fadd_rn(v, part[s * kTokens * rows + e]);
     part[e] = v;
   }
 }
@@ -520,11 +541,13 @@ __global__ void __launch_bounds__(kThreads, RW == 16 ? 4 : 3) down_kernel(Args a
 // Then out, with tokens in the MMAs' rows and columns of out in their columns: a warp takes 32 columns and a run of tokens, a lane 8
 // neighbouring columns of two tokens of each sixteen, so that four lanes read and write a token's columns side by side (with columns in the
 // rows, as above, every quarter of a warp touched four lines at a time, and L1 was the fullest resource). The rows of B stay in
-// registers as long as the adapter does; y and the adapters of the next sixteen tokens are on their way while these are computed. Y, O: y and out have 32 bits (else 16). With 16 bits out, y is what the products are added to in the MMAs.
+// registers as long as the adapter does; y and the adapters of the next sixteen tokens are on their way while these are computed. Y, O: y and out have 32 bits (else 16). In bf16 with 16 bits out, y is
+// what the products are added to in the MMAs, whatever adapters the sixteen have; otherwise it is added in fp32 behind them.
 template <typename T, int RW, bool Y, bool O, bool VEC>
 __global__ void __launch_bounds__(kThreads, 2) up_kernel(Args a) {
   constexpr bool kBf16 = Same<T, __nv_bfloat16>::value;
   constexpr int kTerms = O ? 3 : 2, kWords = RW / 8;
+  constexpr bool kOnY = kBf16 && !O;
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int64_t columns = (a.n + 31) / 32, item = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
   const int64_t run = item / columns, base = (item - run * columns) * 32, n0 = base + q * 8, t0 = run * a.tile;
@@ -647,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 2) up_kernel(Args a) {
       loaded = i;
     };
     const int one = __shfl_sync(0xFFFFFFFFu, mine[0], 0);
-    if (!O && kBf16 && one >= 0 && __all_sync(0xFFFFFFFFu, mine[0] == one && mine[1] == one)) {
+    if (kOnY && one >= 0 && __all_sync(0xFFFFFFFFu, mine[0] == one && mine[1] == one)) {
 #pragma unroll
       for (int j = 0; j < 4; ++j) d[j][0] = y[0][2 * j], d[j][1] = y[0][2 * j + 1], d[j][2] = y[1][2 * j], d[j][3] = y[1][2 * j + 1];
       products(one);
@@ -658,11 +681,17 @@ __global__ void __launch_bounds__(kThreads, 2) up_kernel(Args a) {
       while (open[0] | open[1]) {
         const int i = open[0] ? __shfl_sync(0xFFFFFFFFu, mine[0], __ffs(open[0]) - 1) : __shfl_sync(0xFFFFFFFFu, mine[1], __ffs(open[1]) - 1);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.0f;
+        for (int j = 0; j < 4; ++j) {
+          d[j][0] = d[j][1] = d[j][2] = d[j][3] = 0.0f;
+          if (kOnY) d[j][0] = y[0][2 * j], d[j][1] = y[0][2 * j + 1], d[j][2] = y[1][2 * j], d[j][3] = y[1][2 * j + 1];
+        }
         products(i);
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          if (mine[e] == i) {
+          if (kOnY && mine[e] == i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) y[e][2 * j] = d[j][2 * e], y[e][2 * j + 1] = d[j][2 * e + 1];
+          } else if (mine[e] == i) {
             const float factor = kBf16 ? 1.0f : a.factors[token + 8 * e];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
