@@ -34,7 +34,7 @@ class Adapters(NamedTuple):
 def _project(x, operand, weight, spec, dtype, adapters, index):
     """``operand`` times ``weight`` in ``dtype``, with the adapters' products of ``x`` on top where there are some."""
     y = gemm(operand, weight, spec)
-    if adapters is None or index is None:
+    if adapters is None or index is None:  # rounded as with an index: what a token without an adapter gets does not depend on it
         return y.to(dtype)
     return low_rank_add(y, x, adapters.a, adapters.b, index, gain=adapters.gain, dtype=dtype)
 
@@ -78,7 +78,8 @@ class AttentionLayer:
 class FeedForwardLayer:
     """``w_gate_up`` ``[2 * inner, hidden]`` (the gate's rows first), ``w_down`` ``[hidden, inner]`` and the norm's ``gain``
     ``[hidden]`` on the GPU; ``activation`` as :func:`gated_quantize` names it, the rest as for :class:`AttentionLayer`. Both adapters read
-    8-bit operands, whose scales are then per row."""
+    8-bit operands, whose scales are then per row. A layer with ``gate_up_adapters`` rounds gate and up to ``gain``'s dtype before the
+    activation, for tokens without an adapter and calls without ``index`` too; one without them keeps the GEMM's fp32."""
 
     def __init__(self, w_gate_up, w_down, gain, *, activation: str = "silu", scheme: str = "fp8_row",
                  preset: str = "nvidia_hopper_fp8", eps: float = 1e-6, gate_up_adapters: Adapters | None = None,
@@ -94,8 +95,7 @@ class FeedForwardLayer:
     def __call__(self, x, residual, *, index=None):
         """``(out, h)`` for the tokens ``x`` ``[tokens, hidden]``, ``index`` and ``h`` as for :class:`AttentionLayer`."""
         normed, h = rms_norm_quantize(x, self.gain, self.scheme, residual=residual, eps=self.eps)
-        # Without adapters the activation reads the GEMM's fp32 as it is.
-        wide = torch.float32 if self.gate_up_adapters is None or index is None else self.dtype
+        wide = torch.float32 if self.gate_up_adapters is None else self.dtype
         y = _project(normed, normed, self.w_gate_up, self.spec, wide, self.gate_up_adapters, index)
         gated = gated_quantize(y[:, :self.inner], y[:, self.inner:], self.scheme, activation=self.activation)
         out = _project(gated, gated, self.w_down, self.spec, self.dtype, self.down_adapters, index)
