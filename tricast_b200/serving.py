@@ -112,10 +112,14 @@ class Decoder:
         self.head = quantize(head, scheme)
 
     def __call__(self, tokens, caches, plan, block_table, *, max_q_len: int | None = None, index=None):
-        """fp32 logits ``[batch, vocab]`` behind the last of each sequence's new ``tokens`` (int64, in the plan's order; what
-        stands behind the plan's last one does not matter). ``plan``: of :func:`plan_pages` for them. A sequence without new
-        tokens has some other's logits."""
-        x, h = self.embedding[tokens], None
+        """fp32 logits ``[batch, vocab]`` behind the last of each sequence's new ``tokens`` (int64 ``[tokens]``, as many as the plan has
+        room for, in its order; what stands behind the plan's last one does not matter, the others must lie in the vocabulary).
+        ``plan``: of :func:`plan_pages` for them. A sequence without new tokens has some other's logits."""
+        if len(caches) != len(self.layers):
+            raise ValueError("a decoder needs a cache for each of its layers")
+        if tokens.shape != plan.sequence.shape:
+            raise ValueError("tokens must be as many as the plan has room for")
+        x, h = self.embedding[torch.where(plan.sequence < 0, 0, tokens)], None
         for cache, (attention, feed_forward) in zip(caches, self.layers):
             x, h = attention(x, h, cache, plan.slots, block_table, plan.seq_lens, plan.cu_q, max_q_len=max_q_len, index=index)
             x, h = feed_forward(x, h, index=index)
