@@ -132,11 +132,19 @@ def generate(decoder: Decoder, prompts, steps: int, cache_scheme=None, *, unifor
              temperature=1.0, top_k=None, top_p=None, min_p=None):
     """int64 ``[batch, steps]``: what the decoder says after each of ``prompts`` (lists of token ids). ``uniform``: the random numbers, fp32
     ``[steps, batch]`` (torch's default generator without them); ``adapter``: int32 ``[batch]``, each request's adapter;
-    the rest as :func:`sample_tokens` takes it. Page tables, slots, positions and tokens stay on the GPU."""
+    the rest as :func:`sample_tokens` takes it. A request whose logits have no token (:func:`sample_tokens` says -1) gets no more
+    of them: -1 from there on. Page tables, slots, positions and tokens stay on the GPU."""
     device = decoder.gain.device
     batch, lens = len(prompts), [len(p) for p in prompts]
     if batch == 0 or min(lens) == 0 or steps < 1:
         raise ValueError("generate needs prompts of one token at least, and steps")
+    vocab = decoder.embedding.shape[0]
+    if any(not 0 <= t < vocab for p in prompts for t in p):
+        raise ValueError(f"prompts hold token ids from 0 to {vocab - 1}")
+    if adapter is not None and (adapter.shape != (batch,) or adapter.dtype != torch.int32 or adapter.device != device):
+        raise ValueError("adapter must be an int32 tensor [batch] on the decoder's device")
+    if uniform is not None and (uniform.ndim != 2 or uniform.shape[0] < steps or uniform.shape[1] != batch):
+        raise ValueError("uniform must be a tensor [steps, batch]")
     width = -(-(max(lens) + steps) // page_size)
     pages = sum(-(-(n + steps) // page_size) for n in lens)
     caches = [PagedKVCache(pages, page_size, attention.kv_heads, attention.head_dim, cache_scheme, dtype=attention.dtype, device=device)
@@ -149,11 +157,15 @@ def generate(decoder: Decoder, prompts, steps: int, cache_scheme=None, *, unifor
         uniform = torch.rand(steps, batch, device=device)
     said = torch.empty(steps, batch, dtype=torch.int64, device=device)
     for step in range(steps):
-        plan = plan_pages(have, new, table, free, taken, page_size=page_size, tokens=tokens.shape[0])
-        index = None if adapter is None else adapter[plan.sequence.long()]
+        plan = plan_pages(have, new, table, free, taken, page_size=page_size, tokens=tokens.shape[0] if step == 0 else batch)
+        owner = plan.sequence.clamp(min=0).long()
+        if step:
+            tokens = said[step - 1][owner]  # those that go on stand side by side
+        index = None if adapter is None else adapter[owner]
         logits = decoder(tokens, caches, plan, table, max_q_len=max(lens) if step == 0 else 1, index=index)
-        tokens = said[step] = sample_tokens(logits, uniform[step], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
-        have, taken, new = plan.seq_lens, plan.taken, torch.ones(batch, **as32)
+        got = sample_tokens(logits, uniform[step], temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+        said[step] = torch.where(new > 0, got, -1)
+        have, taken, new = plan.seq_lens, plan.taken, (said[step] >= 0).to(torch.int32)
     release_pages(table, torch.ones(batch, dtype=torch.bool, device=device), free, taken)
     return said.t()
 
