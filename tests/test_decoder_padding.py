@@ -40,3 +40,9 @@ def test_sizes_that_do_not_fit():
         decoder()(torch.tensor([1, 2, 3]), [None], plan([0, 0]), None)
     with pytest.raises(ValueError, match="cache"):
         decoder(layers=2)(torch.tensor([1, 2]), [None], plan([0, 0]), None)
+
+
+def test_a_head_of_another_vocabulary_is_refused():
+    for head in (torch.ones(12, 4), torch.ones(8, 4), torch.ones(10, 8)):
+        with pytest.raises(ValueError, match="one shape"):
+            Decoder(torch.ones(10, 4), [], torch.ones(4), head)
