@@ -70,7 +70,10 @@ __device__ __forceinline__ void gate8(float (&g)[8], const float (&u)[8], int ac
   constexpr float kLog2E = 1.44269504f;
   if (STEPS && act == ACT_SILU) {
     if (largest8(g) <= 64.0f) {
-      // The quotient by divide_fast, whose reciprocal is one Newton step from the hardware's: 1 + exp(-g) is below 2**93.
+      // The quotient by divide_fast, d = 1 + exp(-g) below 2**93. Its reciprocal has to be the correctly rounded one, and one Newton step
+      // from the hardware's gives that for every d in [1, 2**94): compared with __frcp_rn for all 2**23 significands at each exponent.
+      // The divisions are then those of the formula: a remainder is exact for quotients down to 2**-104 (g / d has multiples of its last
+      // place times d's, 2**-149 at least), and gates that small have d = 2, whose half is rounded once.
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float d = __fadd_rn(1.0f, expf(-g[e]));
