@@ -360,9 +360,10 @@ size_t tc_low_rank_add_workspace(int64_t tokens, int32_t x_kind, int32_t w_dtype
 /* Low-rank adapters beside a projection: out[t] = y[t] + gain[i] * b[i] (a[i] x[t]) with i = index[t], and out[t] = y[t] where i
  * is not in [0, adapters). y [tokens][n] and x [tokens][k] have row strides in elements, out [tokens][n] has none; a
  * [adapters][rank][k] and b [adapters][n][rank] of w_dtype; gain fp32 [adapters] or NULL (1). x_kind: a tc_dtype, or a
- * tc_x_codes; x_scale: NULL, or fp32 [tokens], a factor of each row (codes need it). Products and sums are fp32, out is rounded once. rank at most 1024. Weights of 16
- * bits with x of their type or 8-bit codes, y and out of their type or fp32, and ranks up to 128 go through the tensor cores, everything else
- * element by element. out may not alias an input. */
+ * tc_x_codes; x_scale: NULL, or fp32 [tokens], a factor of each row (codes need it). Sums are
+ * fp32, out is rounded once. rank at most 1024. Weights of 16 bits with x of their type or 8-bit codes, y and out of their type or fp32, and ranks up to 128 go through the tensor cores, everything else
+ * element by element. There a[i] x[t] enters the second product in 16-bit parts, two where out has 16 bits (bf16: 2**-16 of it is left out),
+ * three where it has 32. out may not alias an input. */
 int tc_low_rank_add(const void *y, int32_t y_dtype, int64_t y_stride, const void *x, int32_t x_kind, int64_t x_stride,
                     const float *x_scale, int64_t tokens, int64_t k, int64_t n, const void *a, const void *b, int32_t w_dtype,
                     int32_t adapters, int32_t rank, const float *gain, const int32_t *index, void *out, int32_t out_dtype,
@@ -371,7 +372,9 @@ int tc_low_rank_add(const void *y, int32_t y_dtype, int64_t y_stride, const void
 /* The activation of tc_gated_quantize. */
 typedef enum tc_activation { TC_SILU = 0, TC_GELU = 1, TC_GELU_TANH = 2, TC_RELU = 3 } tc_activation;
 
-/* y = activation(gate) * up in fp32, codes and scales as tc_quantize gives them for y. gate and up: [rows][K] of dtype with
+/* y = activation(gate) * up in fp32, codes and scales as tc_quantize gives them for y. INT8: every step of the formula is rounded by
+ * itself; else the logistic function and the normal distribution are good to some 16 halves of an fp32 step, and a scale or code
+ * follows where y lies that near a border. gate and up: [rows][K] of dtype with
  * row strides in elements (two halves of one projection's rows, say); codes, scale and spec as tc_rms_norm_quantize's. */
 int tc_gated_quantize(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, int32_t dtype, int64_t rows,
                       int64_t K, int32_t activation, const tc_quant_spec *spec, void *codes, void *scale, tc_stream stream);

@@ -20,7 +20,11 @@ def gated_quantize(gate: torch.Tensor, up: torch.Tensor, spec, *, activation: st
     ``gate`` and ``up`` ``[..., K]`` (any row strides: two halves of one projection's output, say); ``activation``: ``"silu"``,
     ``"gelu"``, ``"gelu_tanh"`` or ``"relu"``. ``spec`` as for :func:`rms_norm_quantize` (8-bit elements, row or group
     granularity, fp32 absmax or E8M0 scales), and so is the QTensor. The product is fp32, and codes and scales are those
-    :func:`quantize` gives for it. No gradients pass: the output is detached."""
+    :func:`quantize` gives for it. For INT8 codes it is that of PyTorch's operations one by one; for the others the activation's
+    exponential and reciprocal are the hardware's, which is mostly nearer to the formula (2 halves of an fp32 step of ``gate * up``, 16 of
+    the product) but not PyTorch's to the bit: a code may be the neighbouring one where the quotient lies that near the middle between two
+    (one in some 10**5 or 10**6), a power-of-two scale where the maximum lies that near a power of two (one in some 10**8). No gradients
+    pass: the output is detached."""
     if isinstance(spec, str):
         from .spec import get_scheme
 

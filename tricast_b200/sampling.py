@@ -12,7 +12,7 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     """One token (int64) for each row of ``logits`` ``[rows, vocab]`` (any row stride), chosen by ``uniform`` (fp32 ``[rows]`` in
     ``[0, 1)``).
 
-    Settings are numbers, or tensors with one a row (fp32; ``top_k`` int32); ``None`` leaves a filter out. A token weighs
+    Settings are numbers (taken as fp32), or tensors with one a row (fp32; ``top_k`` int32); ``None`` leaves a filter out. A token weighs
     ``w = exp((l - max l) / temperature)``, 0 where that is below ``2**-126``. Of the tokens with a weight the ``top_k`` largest logits
     stay (ties: the lower index; 0 or less: all), of those, in descending order, the fewest whose weights reach ``top_p`` of
     their sum (1 or more: all), of those the ones with ``w >= min_p`` (the largest always stays). The token is the first index
@@ -21,7 +21,9 @@ def sample_tokens(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
 
     A row that has no logit above ``-inf`` gives ``-1`` (log-probability ``-inf``), one with a NaN ``-1`` (NaN). Settings that
     are NaN bound nothing (a temperature: 0). With ``return_logprobs`` also the fp32 logarithms of the tokens' shares of what
-    stayed. Sums are fp64 in a fixed order: the same call gives the same tokens. No gradients pass."""
+    stayed. Weights are fp32, within 1.3e-7 of themselves (without ``top_k`` and ``top_p`` fp64, 2e-10), and their sums fp64 in a
+    fixed order: the same call gives the same tokens, and they are the definition's unless ``uniform`` or ``top_p`` lies within 1e-7 of a
+    border of the shares, or a weight within 1.3e-7 of ``min_p``. No gradients pass."""
     if not logits.is_cuda:
         raise ValueError("the B200 backend requires a CUDA tensor")
     if logits.ndim != 2 or logits.shape[1] == 0:
