@@ -332,7 +332,8 @@ size_t tc_plan_pages_workspace(int32_t batch);
 size_t tc_release_pages_workspace(int32_t batch);
 
 /* Pages and slots of a batch's new tokens. Sequence i has seq_lens[i] tokens in a paged cache and gets new_lens[i] more, the
- * batch's new tokens one after the other; those from `tokens` on are left out (the sequences they belong to get fewer). Pages of
+ * batch's new tokens one after the other; those from `tokens` on are left out (the sequences they belong to get fewer), as are those that
+ * would make a length of 2**31 or more. Pages of
  * page_size (a power of two) tokens that a sequence lacks are taken from the stack free_pages [num_free], whose entries
  * from *taken on are free, in the order of sequences and positions, and written into its row of block_table
  * [batch][max_pages] (row stride table_stride); no other entry is touched. Where the stack is empty the entry becomes -1,

@@ -58,6 +58,11 @@ __device__ __forceinline__ int64_t taken_at_start(const Args &a) {
   return t < 0 ? 0 : t < a.num_free ? t : a.num_free;
 }
 
+// A sequence's new tokens: its length stays a number of 32 bits.
+__device__ __forceinline__ int64_t wanted(const Args &a, int64_t i, int64_t len) {
+  return min((int64_t)max(a.fresh[i], 0), (int64_t)INT32_MAX - len);
+}
+
 // A sequence's pages before its new tokens, and the new ones: its table's room bounds both.
 __device__ __forceinline__ int64_t used_pages(const Args &a, int64_t len) { return (len + (1ll << a.shift) - 1) >> a.shift; }
 __device__ __forceinline__ int64_t new_pages(const Args &a, int64_t len, int64_t n) {
@@ -71,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) scan_kernel(Args a) {
   for (int64_t at = 0; at < a.batch; at += kThreads) {
     const int64_t i = at + threadIdx.x;
     const bool real = i < a.batch;
-    const int64_t len = real ? max(a.lens[i], 0) : 0, want = real ? max(a.fresh[i], 0) : 0;
+    const int64_t len = real ? max(a.lens[i], 0) : 0, want = real ? wanted(a, i, len) : 0;
     Two total;
     const int64_t start = min(tokens + block_prefix(Two{want, 0}, part, total).a, a.tokens);
     tokens += total.a;
@@ -143,7 +148,7 @@ __global__ void __launch_bounds__(kThreads) plan_kernel(Args a) {
   __shared__ int64_t first[kThreads];
   const int i = threadIdx.x, width = blockDim.x;
   const bool real = i < a.batch;
-  const int64_t len = real ? max(a.lens[i], 0) : 0, want = real ? max(a.fresh[i], 0) : 0, taken = taken_at_start(a);
+  const int64_t len = real ? max(a.lens[i], 0) : 0, want = real ? wanted(a, i, len) : 0, taken = taken_at_start(a);
   Two total;
   const int64_t at = min(block_prefix(Two{want, 0}, part, total).a, a.tokens), n = min(want, a.tokens - at);
   const int64_t need = real ? new_pages(a, len, n) : 0, lacking = used_pages(a, len + n) - used_pages(a, len) - need;
