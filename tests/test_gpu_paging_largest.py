@@ -25,3 +25,12 @@ def test_lengths_stay_in_32_bits(batch):
     assert plan.positions.tolist() == [most - 2, most - 1, 0, 1, 2, 8, 9, -1, -1, -1]
     assert plan.slots.tolist() == [-1, -1, 0, 1, 2, 8, 9, -1, -1, -1]  # the first is longer than its row
     assert table[:4].tolist() == [[-1, -1], [0, -1], [-1, -1], [9, 1]] and plan.taken.item() == 2
+
+
+@pytest.mark.parametrize("page_size", [2 ** 32 + 16, 2 ** 21, -(2 ** 32) + 16, 0, -16])
+def test_page_sizes_that_are_none(page_size):
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    table = torch.full((1, 4), -1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="page_size"):
+        plan_pages(one * 0, one, table, one, one * 0, page_size=page_size, tokens=1)
+    assert (table == -1).all()

@@ -65,6 +65,8 @@ def plan_pages(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
     _check(new_lens, (batch,), "new_lens", device)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
+    if not 1 <= page_size <= 1 << 20:  # the C entry's numbers have 32 bits
+        raise ValueError("page_size must be a power of two of at most 2**20")
     ints = torch.empty(2 * tokens + 2 * batch + 3, dtype=torch.int32, device=device)
     sequence, positions, cu, lens, out_taken, missing = ints.split((tokens, tokens, batch + 1, batch, 1, 1))
     slots = torch.empty(tokens, dtype=torch.int64, device=device)
