@@ -782,8 +782,9 @@ static cudaError_t launch_two(Args a, cudaStream_t s) {
 }
 
 // Up to this many tokens one kernel does both products: a little less than what clusters of 8 blocks with 8 tokens each hold when the
-// card is full. One and two kernels, us, 4096 -> 4096, rank 16, fp32 to bf16, runs of 6 adapters: 64 tokens 7.7 and 12.3, 160 9.0 and
-// 11.7, 256 8.7 and 11.3, 296 11.4 and 11.1.
+// card is full. One and two kernels, us, 4096 -> 4096, rank 16, fp32 to bf16: runs of 6 adapters, 64 tokens 7.4 and 7.4, 160 8.2 and 7.9,
+// 256 8.3 and 8.1, 296 13.0 and 9.0; an adapter of 64 a token, 64 tokens 8.3 and 25, 160 18 and 27, 256 19 and 31, 296 33 and 32, 400 31 and 39,
+// 600 55 and 48.
 inline int64_t few_tokens() { return (int64_t)sm_count() * 7 / 4; }
 
 template <typename T, bool CODES>
@@ -807,8 +808,9 @@ static cudaError_t launch_as(Args a, cudaStream_t s) {
   const bool codes = a.x_kind > X_F16;
   if (a.tokens > few_tokens()) return codes ? launch_two_as<T, true>(a, vec, s) : launch_two_as<T, false>(a, vec, s);
   // Tiles of at most 8 tokens, as small as the card holds clusters of 8 blocks for (two blocks an SM): tokens that share a tile
-  // wait for one another's adapters. 64 tokens with as many adapters, 4096 -> 4096, rank 32: tiles of 1, 2 and 4 in 18.5, 14.8 and
-  // 20.9 us; of one adapter 8.2 us with 2, 7.7 with 8.
+  // wait for one another's adapters. 4096 -> 4096, rank 32, us: 64 tokens with as many adapters, tiles of 1 by clusters of 4 11.0 and of
+  // 8 14.9, of 2 by 4 13.6 and by 8 10.8, of 4 by 8 15.8; of one adapter tiles of 2 by 8 8.4, of 8 by 8 7.3; 32 tokens, tiles of 1 by 4
+  // 9.5 and by 8 7.9, of 2 by 8 10.5; one token by 2, 4 and 8 9.7, 6.9 and 5.5 (rank 16).
   const int room = 2 * sm_count();
   a.tile = 1;
   while (a.tile < 8 && (a.tokens + a.tile - 1) / a.tile * 8 > room) a.tile *= 2;
