@@ -8,7 +8,8 @@ namespace adapt {
 
 constexpr int kPlainRank = 1024;
 
-// A block a token: a warp a row of A, then a thread an output.
+// A block a token: a warp a row of A, then a thread an output. 4096 -> 4096, rank 16, all fp32: one token 36 us, 64 38, 8192 1340; rank 200 in
+// bf16, 64 tokens 824: every block reads its adapter itself, in single elements. It serves what the tensor cores do not take, not speed.
 __global__ void __launch_bounds__(256) plain_kernel(Args a) {
   __shared__ float h[kPlainRank];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

@@ -4,10 +4,12 @@
 // its cancellation; gelu_tanh g / (1 + exp(-2 z)), z = sqrt(2 / pi) (g + 0.044715 g**3), which is g (1 + tanh z) / 2; relu.
 // (INT8 codes: the forms with erf and tanh, see gate8.)
 //
-// 8192 rows of 12288 gates and as many ups in fp32, to MXFP8: 154 us, 5.9 TB/s (139 for the bytes; DRAM 76% busy), gelu 164; with a scale
-// a row 153, gelu 172; in bf16 116 and 103 (77 for the bytes; 134 and 154 without the loads ahead), where relu takes 82: activation
-// and cast bound it; groups of 128 with fp32 scales 135 (each lane divides for its group's). INT8 with a scale a row 184, in bf16 135
-// (gelu 202 and 162: its functions' instructions). 333 rows of 1537 in bf16 3.1 us.
+// 8192 rows of 12288 gates and as many ups in fp32, to MXFP8: 143 us, 6.3 TB/s (139 for the bytes; DRAM 76% busy), gelu 153; with a scale
+// a row 153, gelu 172; in bf16 106 and 104 (77 for the bytes), gelu 137 and 125, where relu with a scale a row takes 82: activation
+// and cast bound it; groups of 128 with fp32 scales 135 (each lane divides for its group's). INT8 with a scale a row 181, in bf16 134
+// (gelu 202 and 162: its functions' instructions). 333 rows of 1537 in bf16 3.1 to 3.5 us. Widths
+// that no vector divides read single elements: 8192 x 12289 with a scale a row 297 us in bf16, 375 in fp32, MXFP8 160 and 235. Rows beyond
+// 16384 with a scale a row are read twice: 3500 x 28672 259 and 399 us, where groups (106 and 142) are as fast as elsewhere.
 #pragma once
 
 #include "tc_cast8.cuh"
