@@ -2,9 +2,9 @@
 //   out[t] = y[t] + gain[i] * B[i] (A[i] x[t]),  i = index[t]  (out[t] = y[t] where i names no adapter)
 // x in 16 or 32 bits, or 8-bit codes with a scale a row; the products and their sum are fp32, out is rounded once.
 //
-// Measured: one token 4096 -> 6144, rank 16, fp32 to bf16 6.2 us; 64 tokens with as many adapters 4096 -> 4096, rank 32 12.6 us (5.5 for
+// Measured: one token 4096 -> 6144, rank 16, fp32 to bf16 6.3 us; 64 tokens with as many adapters 4096 -> 4096, rank 32 12.6 us (5.5 for
 // the bytes: waits for loads that follow one another, index, then A, then B); 8192 tokens of E4M3 codes 4096 -> 12288 157 us (4.1 TB/s;
-// 98 for the bytes): 33 the first kernel, whose issue slots are 42% busy with widening codes and MMAs while loads are waited for, 124
+// 98 for the bytes): 31 the first kernel, whose issue slots are 53% busy with widening codes and MMAs while loads are waited for, 124
 // the second, 16 warps an SM that wait for y. Rank 32 194 us, rank 64 282. Tokens whose adapters alternate cost their products each: 374 us
 // (360 with sums whose order goes by the number of adapters in the tile).
 #pragma once
