@@ -107,8 +107,8 @@ class Decoder:
     and a ``head`` ``[vocab, hidden]`` behind a last norm's ``gain`` ``[hidden]``."""
 
     def __init__(self, embedding, layers, gain, head, *, scheme: str = "fp8_row", preset: str = "nvidia_hopper_fp8", eps: float = 1e-6):
-        if embedding.shape != head.shape:  # a token that the head has and the embedding lacks would be looked up outside of it
-            raise ValueError("embedding and head must have one shape [vocab, hidden]")
+        if head.shape[1:] != embedding.shape[1:] or head.shape[0] > embedding.shape[0]:  # a drawn token is looked up next
+            raise ValueError("head must be [vocab, hidden] with no more rows than the embedding")
         self.embedding, self.layers, self.gain, self.scheme, self.eps = embedding, layers, gain, scheme, eps
         self.spec = get_preset(preset).with_(out_format="fp32")
         self.head = quantize(head, scheme)
