@@ -332,15 +332,15 @@ size_t tc_plan_pages_workspace(int32_t batch);
 size_t tc_release_pages_workspace(int32_t batch);
 
 /* Pages and slots of a batch's new tokens. Sequence i has seq_lens[i] tokens in a paged cache and gets new_lens[i] more, the
- * batch's new tokens one after the other; those from `tokens` on are left out (the sequences they belong to get fewer), as are those that
- * would make a length of 2**31 or more. Pages of
- * page_size (a power of two) tokens that a sequence lacks are taken from the stack free_pages [num_free], whose entries
- * from *taken on are free, in the order of sequences and positions, and written into its row of block_table
- * [batch][max_pages] (row stride table_stride); no other entry is touched. Where the stack is empty the entry becomes -1,
- * and pages beyond max_pages are not taken. Written: out_lens [batch], the lengths with the new tokens; cu_q [batch + 1], where
- * the sequences' new tokens begin; per new token ([tokens], -1 behind the last) its slot (-1 without a page), sequence and
- * position; *out_taken, the stack's new top; *missing, pages that were lacking. Nothing else is kept: a program copies out_lens
- * and out_taken where its next call reads them. No output may alias an input. Lengths below 0 count as 0. */
+ * batch's new tokens one after the other; those from `tokens` on are left out (the sequences they belong to get fewer), as are
+ * those that would make a length of 2**31 or more. Pages of page_size (a power of two) tokens that a sequence lacks are taken
+ * from the stack free_pages [num_free], whose entries from *taken on are free, in the order of sequences and positions, and
+ * written into its row of block_table [batch][max_pages] (row stride table_stride); no other entry is touched. Where the stack
+ * is empty the entry becomes -1, and pages beyond max_pages are not taken. Written: out_lens [batch], the lengths with the new
+ * tokens; cu_q [batch + 1], where the sequences' new tokens begin; per new token ([tokens], -1 behind the last) its slot (-1
+ * without a page), sequence and position; *out_taken, the stack's new top; *missing, pages that were lacking. Nothing else is
+ * kept: a program copies out_lens and out_taken where its next call reads them. No output may alias an input. Lengths below 0
+ * count as 0. */
 int tc_plan_pages(const int32_t *seq_lens, const int32_t *new_lens, int32_t batch, int32_t *block_table, int64_t table_stride,
                   int32_t max_pages, const int32_t *free_pages, int64_t num_free, const int32_t *taken, int32_t page_size,
                   int64_t tokens, int32_t *out_lens, int32_t *cu_q, int64_t *slots, int32_t *sequence, int32_t *positions,
@@ -358,13 +358,13 @@ typedef enum tc_x_codes { TC_X_E4M3 = 3, TC_X_E5M2 = 4, TC_X_INT8 = 5 } tc_x_cod
 /* Bytes of scratch tc_low_rank_add needs for these sizes (0 when none). */
 size_t tc_low_rank_add_workspace(int64_t tokens, int32_t x_kind, int32_t w_dtype, int32_t rank, int32_t y_dtype, int32_t out_dtype);
 
-/* Low-rank adapters beside a projection: out[t] = y[t] + gain[i] * b[i] (a[i] x[t]) with i = index[t], and out[t] = y[t] where i
- * is not in [0, adapters). y [tokens][n] and x [tokens][k] have row strides in elements, out [tokens][n] has none; a
+/* Low-rank adapters beside a projection: out[t] = y[t] + gain[i] * b[i] (a[i] x[t]) with i = index[t], and out[t] = y[t] where
+ * i is not in [0, adapters). y [tokens][n] and x [tokens][k] have row strides in elements, out [tokens][n] has none; a
  * [adapters][rank][k] and b [adapters][n][rank] of w_dtype; gain fp32 [adapters] or NULL (1). x_kind: a tc_dtype, or a
- * tc_x_codes; x_scale: NULL, or fp32 [tokens], a factor of each row (codes need it). Sums are
- * fp32, out is rounded once. rank at most 1024. Weights of 16 bits with x of their type or 8-bit codes, y and out of their type or fp32, and ranks up to 128 go through the tensor cores, everything else
- * element by element. There a[i] x[t] enters the second product in 16-bit parts, two where out has 16 bits (bf16: 2**-16 of it is left out),
- * three where it has 32. out may not alias an input. */
+ * tc_x_codes; x_scale: NULL, or fp32 [tokens], a factor of each row (codes need it). Sums are fp32, out is rounded once. rank
+ * at most 1024. Weights of 16 bits with x of their type or 8-bit codes, y and out of their type or fp32, and ranks up to 128 go
+ * through the tensor cores, everything else element by element. There a[i] x[t] enters the second product in 16-bit parts, two
+ * where out has 16 bits (bf16: 2**-16 of it is left out), three where it has 32. out may not alias an input. */
 int tc_low_rank_add(const void *y, int32_t y_dtype, int64_t y_stride, const void *x, int32_t x_kind, int64_t x_stride,
                     const float *x_scale, int64_t tokens, int64_t k, int64_t n, const void *a, const void *b, int32_t w_dtype,
                     int32_t adapters, int32_t rank, const float *gain, const int32_t *index, void *out, int32_t out_dtype,
@@ -373,10 +373,10 @@ int tc_low_rank_add(const void *y, int32_t y_dtype, int64_t y_stride, const void
 /* The activation of tc_gated_quantize. */
 typedef enum tc_activation { TC_SILU = 0, TC_GELU = 1, TC_GELU_TANH = 2, TC_RELU = 3 } tc_activation;
 
-/* y = activation(gate) * up in fp32, codes and scales as tc_quantize gives them for y. INT8: every step of the formula is rounded by
- * itself; else the logistic function and the normal distribution are good to some 16 halves of an fp32 step, and a scale or code
- * follows where y lies that near a border. gate and up: [rows][K] of dtype with
- * row strides in elements (two halves of one projection's rows, say); codes, scale and spec as tc_rms_norm_quantize's. */
+/* y = activation(gate) * up in fp32, codes and scales as tc_quantize gives them for y. INT8: every step of the formula is
+ * rounded by itself; else the logistic function and the normal distribution are good to some 16 halves of an fp32 step, and a
+ * scale or code follows where y lies that near a border. gate and up: [rows][K] of dtype with row strides in elements (two
+ * halves of one projection's rows, say); codes, scale and spec as tc_rms_norm_quantize's. */
 int tc_gated_quantize(const void *gate, int64_t gate_stride, const void *up, int64_t up_stride, int32_t dtype, int64_t rows,
                       int64_t K, int32_t activation, const tc_quant_spec *spec, void *codes, void *scale, tc_stream stream);
 

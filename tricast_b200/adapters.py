@@ -20,13 +20,14 @@ def low_rank_add(y: torch.Tensor, x, a: torch.Tensor, b: torch.Tensor, index: to
     index outside the pool (``-1``) adds nothing. ``gain`` fp32 ``[adapters]``: a factor of each adapter.
 
     The sums are fp32, rounded once to ``dtype`` (default ``y``'s). Weights of 16 bits with ``x`` of their type or 8-bit
-    codes, ``y`` and ``dtype`` of their type or fp32, and ranks up to 128 go through the tensor cores, anything else element by
-    element. On the tensor cores the first product enters the second one in parts of the weights' type: two where ``dtype`` has 16
-    bits (2**-16 of it is left out in bf16, 2**-22 in fp16), three where it has 32 (2**-24, as fp32 itself). An infinite ``x`` or weight of
-    ``a`` gives what fp32 does; one of ``b``, which its column's tokens alone see, may give NaN in place of an infinity. What a token gets depends on no other token's values or adapter, to the bit, but sums are cut by how many tokens there are. Any
-    order of tokens is allowed; those of one adapter that stand together share its weights' way through the
-    chip. More than some 250 tokens take scratch memory (up to 6 bytes a token and rank) while they run. No gradients pass:
-    the output is detached."""
+    codes, ``y`` and ``dtype`` of their type or fp32, and ranks up to 128 go through the tensor cores, anything else element
+    by element. On the tensor cores the first product enters the second one in parts of the weights' type: two where
+    ``dtype`` has 16 bits (2**-16 of it is left out in bf16, 2**-22 in fp16), three where it has 32 (2**-24, as fp32
+    itself). An infinite ``x`` or weight of ``a`` gives what fp32 does; one of ``b``, which its column's tokens alone see,
+    may give NaN in place of an infinity. What a token gets depends on no other token's values or adapter, to the bit, but
+    sums are cut by how many tokens there are. Any order of tokens is allowed; those of one adapter that stand together
+    share its weights' way through the chip. More than some 250 tokens take scratch memory (up to 6 bytes a token and rank)
+    while they run. No gradients pass: the output is detached."""
     if not y.is_cuda:
         raise ValueError("the B200 backend requires a CUDA tensor")
     device, scale = y.device, None

@@ -49,13 +49,14 @@ def plan_pages(seq_lens: torch.Tensor, new_lens: torch.Tensor, block_table: torc
                taken: torch.Tensor, *, page_size: int, tokens: int) -> PagePlan:
     """Pages and slots of a batch's new tokens, without a word to the host: a decode step can be captured with it.
 
-    ``seq_lens`` (int32 ``[batch]``): the tokens each sequence has in the cache; ``new_lens`` (int32 ``[batch]``): how
-    many it gets (0: idle). The new tokens stand one after the other, sequence by sequence; ``tokens`` is the room
-    for them, those beyond it are left out (their sequences get fewer), as are those that would make a sequence longer than ``2**31 - 1``. ``free_pages`` (int32, 1-D) is a stack, of whose
-    entries those from ``taken`` (one int32 number) on are free. Pages that a sequence lacks are taken from there in
-    order and written into its row of ``block_table`` (int32 ``[batch, max_pages]``), in place; no other entry is touched.
-    Where the stack is empty the entry becomes ``-1``, and pages beyond ``max_pages`` are not taken: tokens on them get the
-    slot ``-1`` (:meth:`PagedKVCache.write` skips it) and ``missing`` counts them.
+    ``seq_lens`` (int32 ``[batch]``): the tokens each sequence has in the cache; ``new_lens`` (int32 ``[batch]``): how many
+    it gets (0: idle). The new tokens stand one after the other, sequence by sequence; ``tokens`` is the room for them,
+    those beyond it are left out (their sequences get fewer), as are those that would make a sequence longer than ``2**31 -
+    1``. ``free_pages`` (int32, 1-D) is a stack, of whose entries those from ``taken`` (one int32 number) on are free. Pages
+    that a sequence lacks are taken from there in order and written into its row of ``block_table`` (int32 ``[batch,
+    max_pages]``), in place; no other entry is touched. Where the stack is empty the entry becomes ``-1``, and pages beyond
+    ``max_pages`` are not taken: tokens on them get the slot ``-1`` (:meth:`PagedKVCache.write` skips it) and ``missing``
+    counts them.
 
     Returns a :class:`PagePlan`: its ``slots``, ``seq_lens``, ``cu_q`` go to the cache's ``write`` and
     :func:`paged_attention`; ``seq_lens`` and ``taken`` are the next call's (copy them over where a captured call reads
